@@ -66,7 +66,8 @@ LSSO_API const char* lsso_last_error(void);
 
 /* Read the kernel status word of the current device (0 = no kernel reported a
  * failure, 1 = a bounded tensor-core wait ran out, 2 = a peer rank did not reach
- * a gradient exchange in time).  Synchronizes the device.
+ * a gradient exchange in time, 3 = a token id was outside the embedding's
+ * vocabulary).  Synchronizes the device.
  * reset != 0 clears it afterwards. */
 LSSO_API int lsso_device_status(int reset);
 
@@ -353,6 +354,87 @@ LSSO_API int lsso_peer_region_destroy(void* region);
  * FP32 buffer. */
 LSSO_API int lsso_peer_allreduce(void* const* regions, int world, int rank, int64_t first, int64_t count,
                                  float scale, float* out, unsigned long long wait_limit_ns, void* stream);
+
+/* ---- Operators of the token shell around the mixer (no counterpart in the
+ * reference's native code; its experiment encoder uses PyTorch layers).
+ * Element types: */
+#define LSSO_TYPE_BF16 0
+#define LSSO_TYPE_FP16 1
+#define LSSO_TYPE_FP32 2
+
+/* Gated feed-forward block.
+ *   [g | u] = x w_in^T + b_in,  h = act(g) * u,  y = h w_out^T + b_out
+ *   x     [T, D] of `type` (BF16 or FP16);  y likewise
+ *   w_in  [2H, D] (gate rows, then up rows), w_out [D, H]: of weight_type, which
+ *         is `type`, or FP32 where lsso_ffn_streams_weights(T, D, H) is 1 and gu
+ *         is NULL (each weight is then rounded to `type` as it is read)
+ *   b_in  [2H], b_out [D] of bias_type, or NULL
+ *   gu    [T, 2H] of `type`: the pre-activations, for lsso_ffn_backward; NULL
+ *         for inference
+ *   h     [T, H] of `type`: the product, output or scratch
+ *   activation  0 = SiLU, 1 = GELU (by erf)
+ * Products accumulate in FP32; gu, h and y are rounded once.  D and H are
+ * positive multiples of 8; every matrix is row-major, contiguous and 16-byte
+ * aligned. */
+#define LSSO_FFN_SILU 0
+#define LSSO_FFN_GELU 1
+LSSO_API int lsso_ffn_streams_weights(int64_t T, int64_t D, int64_t H);
+LSSO_API int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int64_t H, const void* w_in,
+                              const void* w_out, int weight_type, const void* b_in, const void* b_out, int bias_type,
+                              int activation, void* gu, void* h, void* y, void* stream);
+
+/* Its gradients, each output optional (NULL).  x, gu, h, w_in, w_out (16-bit)
+ * as the forward had or wrote them; dy, dx [T, D] of `type`; dw_in [2H, D],
+ * dw_out [D, H], db_in [2H], db_out [D] of grad_type (BF16, FP16 or FP32).
+ * Deterministic (no atomics). */
+LSSO_API size_t lsso_ffn_backward_workspace_size(int64_t T, int64_t D, int64_t H);
+LSSO_API int lsso_ffn_backward(const void* dy, const void* x, const void* gu, const void* h, const void* w_in,
+                               const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation,
+                               int grad_type, void* dx, void* dw_in, void* dw_out, void* db_in, void* db_out,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* FP32 -> `type` (BF16 or FP16) copies of w_in and w_out in one launch
+ * (element counts multiples of 8, 16-byte aligned). */
+LSSO_API int lsso_ffn_cast(const float* w_in, void* w_in_out, int64_t w_in_count, const float* w_out,
+                           void* w_out_out, int64_t w_out_count, int type, void* stream);
+
+/* Token embedding: y[t] = scale * weight[ids[t]] (rows with row_mask[t] == 0
+ * are zero and their ids are not looked at).
+ *   ids [T] int64 (ids_int64) or int32; weight [V, D] of weight_type;
+ *   y [T, D] of out_type; row_mask uint8/bool [T] or NULL
+ * An id outside [0, V) gives a zero row and device status 3. */
+LSSO_API int lsso_embedding_forward(const void* ids, int ids_int64, const uint8_t* row_mask, int64_t T,
+                                    const void* weight, int weight_type, int64_t V, int64_t D, float scale, void* y,
+                                    int out_type, void* stream);
+
+/* Its gradient: dweight[v] = scale * sum of dy[t] over the tokens with
+ * ids[t] == v and a set mask, FP32 sums rounded once to weight_type; the row
+ * `padding` (-1: none) is zero.  dweight 16-byte aligned.  Deterministic:
+ * tokens are summed in an order that depends on ids and sizes only. */
+LSSO_API size_t lsso_embedding_backward_workspace_size(int64_t T, int64_t V, int64_t D);
+LSSO_API int lsso_embedding_backward(const void* ids, int ids_int64, const uint8_t* row_mask, int64_t T,
+                                     const void* dy, int dy_type, int64_t V, int64_t D, int64_t padding, float scale,
+                                     void* dweight, int weight_type, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
+/* Dropout with the residual sum, the mask never stored:
+ *   y = residual + branch * keep / (1 - p)   (rows with row_mask[t] == 0: zero)
+ * keep of the element with flat index 4 j + i is word i >= round(p 2^32) of
+ * Philox4x32-10 at counter (j mod 2^32, j div 2^32, site, state[1] mod 2^32)
+ * and key state[0].  A dropped element contributes exactly zero.
+ *   branch [rows, width] of branch_type; residual and y of out_type, which is
+ *   branch_type or FP32; residual may be NULL
+ *   state  int64 [2] on the device: seed, step (read by the kernel, so a
+ *          captured graph follows its updates); used_state: int64 [2] that
+ *          receives a copy of it for the backward, or NULL
+ * Backward: dbranch = dy * keep / (1 - p), dresidual = dy, both zero in masked
+ * rows; either NULL when not wanted. */
+LSSO_API int lsso_dropout_forward(const void* branch, int branch_type, const void* residual, int out_type,
+                                  const uint8_t* row_mask, int64_t rows, int64_t width, double p,
+                                  const int64_t* state, uint32_t site, int64_t* used_state, void* y, void* stream);
+LSSO_API int lsso_dropout_backward(const void* dy, int out_type, int branch_type, const uint8_t* row_mask,
+                                   int64_t rows, int64_t width, double p, const int64_t* state, uint32_t site,
+                                   void* dbranch, void* dresidual, void* stream);
 
 /* Per-kernel timing (no counterpart in the reference; instrumentation only).
  * lsso_profile_start() makes every subsequent kernel launch of the library

@@ -14,6 +14,7 @@ two autograd-key rejections.  Registration happens once per process, from
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from pathlib import Path
 
 import torch
@@ -29,7 +30,12 @@ EXPORTED_SYMBOLS = (
     "lsso_moment_elements", "lsso_forward_moments", "lsso_forward_finish", "lsso_backward_moments",
     "lsso_backward_finish", "lsso_peer_region_bytes", "lsso_peer_region_create", "lsso_peer_region_open",
     "lsso_peer_region_close", "lsso_peer_region_destroy", "lsso_peer_allreduce", "lsso_backward_with_wgrad",
+    "lsso_ffn_streams_weights", "lsso_ffn_forward", "lsso_ffn_backward_workspace_size", "lsso_ffn_backward",
+    "lsso_ffn_cast", "lsso_embedding_forward", "lsso_embedding_backward_workspace_size", "lsso_embedding_backward",
+    "lsso_dropout_forward", "lsso_dropout_backward",
 )
+# Element types of the token shell's entry points.
+ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 _LIBRARY: "NativeLibrary | None" = None
 _OPS: torch.library.Library | None = None
@@ -80,6 +86,17 @@ class NativeLibrary:
             "lsso_peer_region_close": (ci, [vp]),
             "lsso_peer_region_destroy": (ci, [vp]),
             "lsso_peer_allreduce": (ci, [c.POINTER(vp), ci, ci, i64, i64, c.c_float, vp, c.c_ulonglong, vp]),
+            "lsso_ffn_streams_weights": (ci, [i64, i64, i64]),
+            "lsso_ffn_forward": (ci, [vp, ci, i64, i64, i64, vp, vp, ci, vp, vp, ci, ci, vp, vp, vp, vp]),
+            "lsso_ffn_backward_workspace_size": (sz, [i64, i64, i64]),
+            "lsso_ffn_backward": (ci, [vp, vp, vp, vp, vp, vp, ci, i64, i64, i64, ci, ci, vp, vp, vp, vp, vp, vp, sz,
+                                       vp]),
+            "lsso_ffn_cast": (ci, [vp, vp, i64, vp, vp, i64, ci, vp]),
+            "lsso_embedding_forward": (ci, [vp, ci, vp, i64, vp, ci, i64, i64, c.c_float, vp, ci, vp]),
+            "lsso_embedding_backward_workspace_size": (sz, [i64, i64, i64]),
+            "lsso_embedding_backward": (ci, [vp, ci, vp, i64, vp, ci, i64, i64, i64, c.c_float, vp, ci, vp, sz, vp]),
+            "lsso_dropout_forward": (ci, [vp, ci, vp, ci, vp, i64, i64, c.c_double, vp, c.c_uint32, vp, vp, vp]),
+            "lsso_dropout_backward": (ci, [vp, ci, ci, vp, i64, i64, c.c_double, vp, c.c_uint32, vp, vp, vp]),
             "lsso_profile_start": (ci, []),
             "lsso_profile_stop": (ci, [ci, c.c_char_p, c.POINTER(c.c_float), c.POINTER(c.c_int)]),
         }
@@ -181,6 +198,11 @@ def _ptr(value: torch.Tensor | None):
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is current (nothing to switch when it already is)."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 # ---------------------------------------------------------------------------- operator bodies

@@ -198,7 +198,8 @@ def device_status(reset: bool = True) -> int:
 
 
 def check_device_status() -> None:
-    """Raise if a kernel of the library gave up waiting since the last check.
+    """Raise if a kernel of the library gave up waiting, or met a token id
+    outside an embedding's vocabulary, since the last check.
 
     Synchronizes the device.  A kernel whose bounded wait ran out stops,
     frees its resources and leaves its outputs undefined; this reports it
@@ -210,6 +211,10 @@ def check_device_status() -> None:
         raise RuntimeError(
             "a peer rank did not reach the LSSO gradient exchange within its wait limit (device status 2); the "
             "exchanged gradients since the last check are undefined")
+    if status == 3:
+        raise RuntimeError(
+            "a token id was outside the embedding's vocabulary (device status 3); its row was written as zero and "
+            "took no part in the gradient")
     if status != 0:
         raise RuntimeError(
             f"an LSSO CUDA kernel gave up waiting (device status {status}); the outputs of the calls since the "

@@ -19,8 +19,10 @@ ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 LIBDIR = PACKAGE / "lib"
 LIBRARY_NAME = "lsso_equilibrium_sm100.so"
-SOURCES = ("mixer.cu", "linear.cu", "tokens.cu", "solve.cu", "peer.cu", "capi.cu")
-HEADERS = ("mixer.h", "mixer_common.cuh", "tc.cuh", "linear.h", "peer.h")
+SOURCES = ("mixer.cu", "linear.cu", "tokens.cu", "solve.cu", "peer.cu", "ffn.cu", "embedding.cu",
+           "dropout.cu", "capi.cu", "capi_shell.cu")
+HEADERS = ("mixer.h", "mixer_common.cuh", "tc.cuh", "linear.h", "peer.h", "ffn.h", "shell_ops.h", "elements.cuh",
+           "capi_util.h")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 
 
@@ -71,7 +73,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     tmp = target.with_suffix(".so.tmp")
     command = [
         _nvcc(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17",
-        "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static",
+        "--threads", "0", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static",
         "-I", str(ROOT / "include"), "-o", str(tmp),
         *[str(CSRC / s) for s in SOURCES],
     ]

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "../../include/lsso_equilibrium.h"
+#include "capi_util.h"
 #include "linear.h"
 #include "mixer.h"
 #include "mixer_common.cuh"
@@ -213,6 +214,34 @@ void profile_after(const char* name, cudaStream_t stream) {
 }
 
 }  // namespace
+
+namespace lsso {
+namespace capi {
+
+void clear_error() { g_last_error.clear(); }
+
+int invalid(const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return fail(LSSO_ERR_INVALID_ARGUMENT, "%s", buf);
+}
+
+int workspace_too_small(const char* who, size_t got, size_t need) {
+  return fail(LSSO_ERR_WORKSPACE, "%s: workspace of %zu bytes is smaller than the required %zu", who, got, need);
+}
+
+int launched(cudaError_t e, const char* who) { return e == cudaSuccess ? LSSO_OK : cuda_fail(e, who); }
+
+int device(int* sms, int** status) {
+  int index = 0;
+  return device_info(&index, sms, status);
+}
+
+}  // namespace capi
+}  // namespace lsso
 
 extern "C" {
 

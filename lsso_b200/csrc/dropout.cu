@@ -1,0 +1,191 @@
+// Dropout with the residual sum, the mask regenerated instead of stored.
+//
+//   y[t, c]        = residual[t, c] + branch[t, c] * keep / (1 - p)     (0 in masked rows)
+//   dbranch[t, c]  = dy[t, c] * keep / (1 - p)                          (0 in masked rows)
+//   dresidual[t, c]= dy[t, c]                                           (0 in masked rows)
+//
+// keep of the element with flat index 4 j + i is (word i >= round(p 2^32)) of
+// Philox4x32-10 (J. K. Salmon et al., "Parallel random numbers: as easy as
+// 1, 2, 3", SC 2011) at counter (j mod 2^32, j div 2^32, site, step) and key
+// seed: a pure function of the element, so the backward recomputes it and
+// results do not depend on the launch shape.
+//
+// What bounds it: HBM traffic.  Every thread takes eight consecutive elements
+// (two counters, one 16-byte access of a 16-bit tensor), issues its loads
+// first and runs the generator while they are in flight.
+#include <type_traits>
+
+#include "elements.cuh"
+#include "mixer.h"
+#include "shell_ops.h"
+#include "tc.cuh"
+
+namespace lsso {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPer = 8;
+
+__device__ __forceinline__ uint4 philox(uint4 c, uint2 k) {
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = static_cast<uint64_t>(c.x) * 0xD2511F53u;
+    const uint64_t b = static_cast<uint64_t>(c.z) * 0xCD9E8D57u;
+    c = make_uint4(static_cast<uint32_t>(b >> 32) ^ c.y ^ k.x, static_cast<uint32_t>(b),
+                   static_cast<uint32_t>(a >> 32) ^ c.w ^ k.y, static_cast<uint32_t>(a));
+    k.x += 0x9E3779B9u;
+    k.y += 0xBB67AE85u;
+  }
+  return c;
+}
+
+// Which of eight consecutive elements starting at flat index `first` (a
+// multiple of 8) are kept.
+__device__ __forceinline__ uint32_t keep_bits(int64_t first, uint2 key, uint32_t site, uint32_t step,
+                                              uint32_t threshold) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint64_t j = (static_cast<uint64_t>(first) >> 2) + h;
+    const uint4 w = philox(make_uint4(static_cast<uint32_t>(j), static_cast<uint32_t>(j >> 32), site, step), key);
+    bits |= (w.x >= threshold ? 1u : 0u) << (4 * h);
+    bits |= (w.y >= threshold ? 2u : 0u) << (4 * h);
+    bits |= (w.z >= threshold ? 4u : 0u) << (4 * h);
+    bits |= (w.w >= threshold ? 8u : 0u) << (4 * h);
+  }
+  return bits;
+}
+
+// Which of the eight elements lie in rows whose mask is set.
+__device__ __forceinline__ uint32_t live_bits(const uint8_t* __restrict__ mask, int64_t first, int64_t total,
+                                              int64_t width) {
+  int64_t row = total <= 0xFFFFFFFFll
+                    ? static_cast<int64_t>(static_cast<uint32_t>(first) / static_cast<uint32_t>(width))
+                    : first / width;
+  int64_t left = (row + 1) * width - first;  // elements of this row from `first` on
+  uint32_t bits = 0;
+  bool live = mask[row] != 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (left == 0) {
+      left = width;
+      ++row;
+      live = first + i < total && mask[row] != 0;
+    }
+    --left;
+    bits |= live ? 1u << i : 0u;
+  }
+  return bits;
+}
+
+template <typename T>
+__device__ __forceinline__ Run<T, kPer> load8(const T* p, int64_t first, int64_t total, bool whole) {
+  if (whole) return load_run<T, kPer>(p + first);
+  Run<T, kPer> r;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) r.v[i] = first + i < total ? p[first + i] : from_float<T>(0.0f);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t first, int64_t total, bool whole, const float (&v)[kPer]) {
+  if (whole) {
+    store_run<T, kPer>(p + first, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (first + i < total) p[first + i] = from_float<T>(v[i]);
+}
+
+// kBackward: `in` is the upstream gradient (type O), `out` the branch gradient
+// (type B).  Otherwise `in` is the branch (B) and `out` is y (O).
+template <typename B, typename O, bool kBackward, bool kMasked>
+__global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutCall c, int64_t total, int vec) {
+  pdl_wait();
+  using In = typename std::conditional<kBackward, O, B>::type;
+  using Out = typename std::conditional<kBackward, B, O>::type;
+  const In* in = static_cast<const In*>(c.in);
+  const O* residual = static_cast<const O*>(c.residual);
+  Out* out = static_cast<Out*>(c.out);
+  const uint64_t seed = static_cast<uint64_t>(__ldg(reinterpret_cast<const long long*>(c.state)));
+  const uint64_t step = static_cast<uint64_t>(__ldg(reinterpret_cast<const long long*>(c.state) + 1));
+  const uint2 key = make_uint2(static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32));
+  if (!kBackward && c.used_state != nullptr && blockIdx.x == 0 && threadIdx.x < 2) {
+    c.used_state[threadIdx.x] = static_cast<int64_t>(threadIdx.x == 0 ? seed : step);
+  }
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kThreads * kPer;
+  for (int64_t first = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * kPer; first < total;
+       first += stride) {
+    const bool whole = vec && first + kPer <= total;
+    const Run<In, kPer> x = load8(in, first, total, whole);
+    Run<O, kPer> r;
+    if (!kBackward && residual != nullptr) r = load8(residual, first, total, whole);
+    uint32_t keep = c.drop_all ? 0u : keep_bits(first, key, c.site, static_cast<uint32_t>(step), c.threshold);
+    uint32_t live = 0xFFu;
+    if (kMasked) {
+      live = live_bits(c.row_mask, first, total, c.width);
+      keep &= live;
+    }
+    float v[kPer];
+    if (kBackward) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[i] = (keep >> i) & 1u ? to_float(x.v[i]) * c.scale : 0.0f;
+      if (out != nullptr) store8(out, first, total, whole, v);
+      if (c.residual_grad != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = (live >> i) & 1u ? to_float(x.v[i]) : 0.0f;
+        store8(static_cast<O*>(c.residual_grad), first, total, whole, v);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        v[i] = (keep >> i) & 1u ? to_float(x.v[i]) * c.scale : 0.0f;
+        if (residual != nullptr && ((live >> i) & 1u)) v[i] += to_float(r.v[i]);
+      }
+      store8(out, first, total, whole, v);
+    }
+  }
+}
+
+template <typename B, typename O, bool kBackward>
+cudaError_t launch_types(const DropoutCall& c, int sm_count, cudaStream_t stream) {
+  const int64_t total = c.rows * c.width;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(c.in) | reinterpret_cast<uintptr_t>(c.residual) |
+                        reinterpret_cast<uintptr_t>(c.out) | reinterpret_cast<uintptr_t>(c.residual_grad);
+  const int vec = (all & 15u) == 0 ? 1 : 0;
+  const int64_t need = (total + kThreads * kPer - 1) / (kThreads * kPer);
+  const int64_t most = static_cast<int64_t>(sm_count) * 64;
+  const unsigned grid = static_cast<unsigned>(need < most ? need : most);
+  LaunchScope scope(kBackward ? "dropout_bwd" : "dropout", stream);
+  if (c.row_mask != nullptr) {
+    launch_pdl(dropout_kernel<B, O, kBackward, true>, grid, kThreads, 0, stream, c, total, vec);
+  } else {
+    launch_pdl(dropout_kernel<B, O, kBackward, false>, grid, kThreads, 0, stream, c, total, vec);
+  }
+  return cudaGetLastError();
+}
+
+template <bool kBackward>
+cudaError_t dispatch(const DropoutCall& c, int sm_count, cudaStream_t stream) {
+  using bf = __nv_bfloat16;
+  if (c.branch_type == kFp32) return launch_types<float, float, kBackward>(c, sm_count, stream);
+  if (c.branch_type == kBf16) {
+    return c.out_type == kFp32 ? launch_types<bf, float, kBackward>(c, sm_count, stream)
+                               : launch_types<bf, bf, kBackward>(c, sm_count, stream);
+  }
+  return c.out_type == kFp32 ? launch_types<__half, float, kBackward>(c, sm_count, stream)
+                             : launch_types<__half, __half, kBackward>(c, sm_count, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_dropout_forward(const DropoutCall& c, int sm_count, cudaStream_t stream) {
+  return dispatch<false>(c, sm_count, stream);
+}
+cudaError_t launch_dropout_backward(const DropoutCall& c, int sm_count, cudaStream_t stream) {
+  return dispatch<true>(c, sm_count, stream);
+}
+
+}  // namespace lsso

@@ -1,0 +1,79 @@
+// Loads and stores of short runs of consecutive elements (FP32, BF16, FP16)
+// as FP32 values, for the element-wise kernels of the token shell.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace lsso {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// N consecutive elements held as raw bits, so that a load can be issued well
+// before its values are used.  N * sizeof(T) is 2, 4, 8, 16 or 32 bytes and
+// the address is a multiple of min(that, 16).
+template <typename T, int N>
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Run {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Run<T, N> load_run(const T* p) {
+  Run<T, N> r;
+  constexpr int kBytes = N * sizeof(T);
+  if constexpr (kBytes == 32) {
+    reinterpret_cast<uint4*>(&r)[0] = __ldg(reinterpret_cast<const uint4*>(p));
+    reinterpret_cast<uint4*>(&r)[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  } else if constexpr (kBytes == 16) {
+    *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
+  } else if constexpr (kBytes == 8) {
+    *reinterpret_cast<uint2*>(&r) = __ldg(reinterpret_cast<const uint2*>(p));
+  } else if constexpr (kBytes == 4) {
+    *reinterpret_cast<uint32_t*>(&r) = __ldg(reinterpret_cast<const uint32_t*>(p));
+  } else {
+    static_assert(N == 1, "unsupported run");
+    r.v[0] = p[0];
+  }
+  return r;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_run(T* p, const float (&x)[N]) {
+  Run<T, N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(x[i]);
+  constexpr int kBytes = N * sizeof(T);
+  if constexpr (kBytes == 32) {
+    reinterpret_cast<uint4*>(p)[0] = reinterpret_cast<uint4*>(&r)[0];
+    reinterpret_cast<uint4*>(p)[1] = reinterpret_cast<uint4*>(&r)[1];
+  } else if constexpr (kBytes == 16) {
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(&r);
+  } else if constexpr (kBytes == 8) {
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(&r);
+  } else if constexpr (kBytes == 4) {
+    *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<uint32_t*>(&r);
+  } else {
+    p[0] = r.v[0];
+  }
+}
+
+}  // namespace lsso
