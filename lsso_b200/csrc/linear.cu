@@ -736,14 +736,21 @@ CUresult encode_rows(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* map,
 }  // namespace
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (fn == nullptr) {
+  auto entry = [](const char* name) -> void* {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess) {
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }
+    const bool found = cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) == cudaSuccess;
+    return found && q == cudaDriverEntryPointSuccess ? p : nullptr;
+  };
+  static const auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(entry("cuTensorMapEncodeTiled"));
+  static const auto current = reinterpret_cast<PFN_cuCtxGetCurrent_v4000>(entry("cuCtxGetCurrent"));
+  // The encoder is a driver call and needs a current context.  The runtime
+  // makes one current on a thread's first call that needs it, so on a host
+  // thread whose first CUDA work is this call (an autograd worker) none is yet.
+  CUcontext context = nullptr;
+  if (current != nullptr && current(&context) == CUDA_SUCCESS && context == nullptr) {
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return nullptr;
   }
   return fn;
 }
