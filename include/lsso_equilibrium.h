@@ -366,14 +366,14 @@ LSSO_API int lsso_peer_allreduce(void* const* regions, int world, int rank, int6
  *   [g | u] = x w_in^T + b_in,  h = act(g) * u,  y = h w_out^T + b_out
  *   x     [T, D] of `type` (BF16 or FP16);  y likewise
  *   w_in  [2H, D] (gate rows, then up rows), w_out [D, H]: of weight_type, which
- *         is `type`, or FP32 where lsso_ffn_streams_weights(T, D, H) is 1 and gu
- *         is NULL (each weight is then rounded to `type` as it is read)
+ *         is `type`, or FP32 where lsso_ffn_streams_weights(T, D, H) is 1 and
+ *         kept is NULL (each weight is then rounded to `type` as it is read)
  *   b_in  [2H], b_out [D] of bias_type, or NULL
- *   gu    [T, 2H] of `type`: the pre-activations, for lsso_ffn_backward; NULL
- *         for inference
+ *   kept  [T, 2, H] of `type`: g and u, for lsso_ffn_backward;
+ *         NULL for inference
  *   h     [T, H] of `type`: the product, output or scratch
  *   activation  0 = SiLU, 1 = GELU (by erf)
- * Products accumulate in FP32; gu, h and y are rounded once.  D and H are
+ * Products accumulate in FP32; kept, h and y are rounded once.  D and H are
  * positive multiples of 8; every matrix is row-major, contiguous and 16-byte
  * aligned. */
 #define LSSO_FFN_SILU 0
@@ -381,14 +381,14 @@ LSSO_API int lsso_peer_allreduce(void* const* regions, int world, int rank, int6
 LSSO_API int lsso_ffn_streams_weights(int64_t T, int64_t D, int64_t H);
 LSSO_API int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int64_t H, const void* w_in,
                               const void* w_out, int weight_type, const void* b_in, const void* b_out, int bias_type,
-                              int activation, void* gu, void* h, void* y, void* stream);
+                              int activation, void* kept, void* h, void* y, void* stream);
 
-/* Its gradients, each output optional (NULL).  x, gu, h, w_in, w_out (16-bit)
+/* Its gradients, each output optional (NULL).  x, kept, h, w_in, w_out (16-bit)
  * as the forward had or wrote them; dy, dx [T, D] of `type`; dw_in [2H, D],
  * dw_out [D, H], db_in [2H], db_out [D] of grad_type (BF16, FP16 or FP32).
  * Deterministic (no atomics). */
 LSSO_API size_t lsso_ffn_backward_workspace_size(int64_t T, int64_t D, int64_t H);
-LSSO_API int lsso_ffn_backward(const void* dy, const void* x, const void* gu, const void* h, const void* w_in,
+LSSO_API int lsso_ffn_backward(const void* dy, const void* x, const void* kept, const void* h, const void* w_in,
                                const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation,
                                int grad_type, void* dx, void* dw_in, void* dw_out, void* db_in, void* db_out,
                                void* workspace, size_t workspace_bytes, void* stream);

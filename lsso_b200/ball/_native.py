@@ -14,7 +14,6 @@ two autograd-key rejections.  Registration happens once per process, from
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from pathlib import Path
 
 import torch
@@ -200,9 +199,32 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def on_device(device: torch.device):
-    """Context in which ``device`` is current (nothing to switch when it already is)."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def run(name: str, device: torch.device, *args) -> None:
+    """Call an entry point whose last argument is the stream, with ``device``
+    current and on its current stream (the raw handle: a stream object costs
+    a microsecond or two per call); raise its error."""
+    lib = library()
+    index = device.index
+    if torch.cuda.current_device() == index:
+        code = getattr(lib.lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = getattr(lib.lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        lib.check(code)
+
+
+def workspace(name: str, device: torch.device, *sizes) -> torch.Tensor:
+    """The scratch of an entry point, its bytes from the query ``name``."""
+    lib = library()
+    if torch.cuda.current_device() == device.index:
+        size = getattr(lib.lib, name)(*sizes)
+    else:
+        with torch.cuda.device(device.index):
+            size = getattr(lib.lib, name)(*sizes)
+    if size == 0:
+        lib.check(1)
+    return torch.empty((size,), dtype=torch.uint8, device=device)
 
 
 # ---------------------------------------------------------------------------- operator bodies

@@ -84,18 +84,13 @@ def _check(branch, residual, p, state, site, valid_mask) -> None:
 
 
 def _forward(branch, residual, p, state, site, mask, used):
-    lib = _native.library()
-    device = branch.device
-    out_dtype = branch.dtype if residual is None else residual.dtype
-    types = _native.ELEMENT_TYPES
-    y = torch.empty(branch.shape, dtype=out_dtype, device=device)
+    y = torch.empty_like(branch if residual is None else residual)
     if y.numel():
+        types = _native.ELEMENT_TYPES
         width = branch.shape[-1]
-        with _native.on_device(device):
-            lib.check(lib.lib.lsso_dropout_forward(
-                branch.data_ptr(), types[branch.dtype], _native._ptr(residual), types[out_dtype], _native._ptr(mask),
-                branch.numel() // width, width, p, state.data_ptr(), site, _native._ptr(used), y.data_ptr(),
-                _native._stream(device)))
+        _native.run("lsso_dropout_forward", branch.device, branch.data_ptr(), types[branch.dtype],
+                    _native._ptr(residual), types[y.dtype], _native._ptr(mask), branch.numel() // width, width, p,
+                    state.data_ptr(), site, _native._ptr(used), y.data_ptr())
     return y
 
 
@@ -115,22 +110,17 @@ class _DropoutAdd(torch.autograd.Function):
         used, mask = ctx.saved_tensors
         needs_branch, needs_residual = ctx.needs_input_grad[:2]
         dbranch = dresidual = None
-        if not (needs_branch or needs_residual):
-            return None, None, None, None, None, None
         dy = dy.contiguous()
         if needs_residual:
             dresidual = dy if mask is None else torch.empty_like(dy)
         if needs_branch:
-            dbranch = torch.empty(dy.shape, dtype=ctx.branch_dtype, device=dy.device)
-        if dy.numel() and (needs_branch or mask is not None):
-            lib = _native.library()
+            dbranch = torch.empty_like(dy, dtype=ctx.branch_dtype)
+        if dy.numel() and (needs_branch or (needs_residual and mask is not None)):
             types = _native.ELEMENT_TYPES
             width = dy.shape[-1]
-            with _native.on_device(dy.device):
-                lib.check(lib.lib.lsso_dropout_backward(
-                    dy.data_ptr(), types[dy.dtype], types[ctx.branch_dtype], _native._ptr(mask), dy.numel() // width,
-                    width, ctx.p, used.data_ptr(), ctx.site, _native._ptr(dbranch),
-                    _native._ptr(None if mask is None else dresidual), _native._stream(dy.device)))
+            _native.run("lsso_dropout_backward", dy.device, dy.data_ptr(), types[dy.dtype], types[ctx.branch_dtype],
+                        _native._ptr(mask), dy.numel() // width, width, ctx.p, used.data_ptr(), ctx.site,
+                        _native._ptr(dbranch), _native._ptr(None if mask is None else dresidual))
         return dbranch, dresidual, None, None, None, None
 
 

@@ -43,16 +43,13 @@ def token_embedding_reference(ids, weight, *, scale=1.0, valid_mask=None, paddin
 
 
 def _forward(ids, weight, scale, mask, dtype):
-    lib = _native.library()
-    device = weight.device
     types = _native.ELEMENT_TYPES
     vocab, dim = weight.shape
-    y = torch.empty((*ids.shape, dim), dtype=dtype, device=device)
-    if ids.numel():
-        with _native.on_device(device):
-            lib.check(lib.lib.lsso_embedding_forward(
-                ids.data_ptr(), int(ids.dtype == torch.int64), _native._ptr(mask), ids.numel(), weight.data_ptr(),
-                types[weight.dtype], vocab, dim, scale, y.data_ptr(), types[dtype], _native._stream(device)))
+    y = weight.new_empty((*ids.shape, dim), dtype=dtype)
+    if y.numel():
+        _native.run("lsso_embedding_forward", weight.device, ids.data_ptr(), int(ids.dtype == torch.int64),
+                    _native._ptr(mask), ids.numel(), weight.data_ptr(), types[weight.dtype], vocab, dim, scale,
+                    y.data_ptr(), types[dtype])
     return y
 
 
@@ -69,22 +66,16 @@ class _TokenEmbedding(torch.autograd.Function):
     def backward(ctx, dy):
         ids, mask = ctx.saved_tensors
         (vocab, dim), dtype = ctx.weight_meta
-        lib = _native.library()
         device = dy.device
         types = _native.ELEMENT_TYPES
         if not ids.numel():
-            return None, torch.zeros((vocab, dim), dtype=dtype, device=device), None, None, None, None
+            return None, dy.new_zeros((vocab, dim), dtype=dtype), None, None, None, None
         dy = dy.contiguous()
-        grad = torch.empty((vocab, dim), dtype=dtype, device=device)
-        with _native.on_device(device):
-            size = lib.lib.lsso_embedding_backward_workspace_size(ids.numel(), vocab, dim)
-            if size == 0:
-                lib.check(1)
-            workspace = torch.empty((size,), dtype=torch.uint8, device=device)
-            lib.check(lib.lib.lsso_embedding_backward(
-                ids.data_ptr(), int(ids.dtype == torch.int64), _native._ptr(mask), ids.numel(), dy.data_ptr(),
-                types[dy.dtype], vocab, dim, ctx.padding, ctx.scale, grad.data_ptr(), types[dtype],
-                workspace.data_ptr(), size, _native._stream(device)))
+        grad = dy.new_empty((vocab, dim), dtype=dtype)
+        scratch = _native.workspace("lsso_embedding_backward_workspace_size", device, ids.numel(), vocab, dim)
+        _native.run("lsso_embedding_backward", device, ids.data_ptr(), int(ids.dtype == torch.int64),
+                    _native._ptr(mask), ids.numel(), dy.data_ptr(), types[dy.dtype], vocab, dim, ctx.padding,
+                    ctx.scale, grad.data_ptr(), types[dtype], scratch.data_ptr(), scratch.numel())
         return None, grad, None, None, None, None
 
 

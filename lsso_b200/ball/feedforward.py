@@ -3,7 +3,7 @@
 ``gated_feed_forward(x, w_in, w_out)`` is ``(act(g) * u) w_out^T`` with
 ``[g | u] = x w_in^T``: ``w_in`` ``[2 hidden, dim]`` holds the gate rows, then
 the up rows.  Both projections, the activation and the product are one tcgen05
-kernel; the backward keeps ``[g | u]`` and the product.  Operands have x's
+kernel; a training forward keeps ``[g | u]`` and the product.  Operands have x's
 dtype (BF16 or FP16), products accumulate in FP32.  FP32 weights are rounded
 to x's dtype in the call and get FP32 gradients; weights that already have x's
 dtype (a served model's, laid out once) are used in place.
@@ -51,40 +51,36 @@ def gated_feed_forward_reference(x, w_in, w_out, b_in=None, b_out=None, *, activ
 
 
 def _forward(x, w_in, w_out, b_in, b_out, activation, keep):
-    """(y, gu, h) for x [T, D]; gu is None unless kept."""
-    lib = _native.library()
+    """(y, kept, h) for x [T, D]; kept (g and u, for the backward) is None unless ``keep``."""
     types = _native.ELEMENT_TYPES
     t, d = x.shape
     hidden = w_out.shape[1]
     bias = b_in if b_in is not None else b_out
-    h = torch.empty((t, hidden), dtype=x.dtype, device=x.device)
-    gu = torch.empty((t, 2 * hidden), dtype=x.dtype, device=x.device) if keep else None
+    h = x.new_empty((t, hidden))
+    kept = x.new_empty((t, 2, hidden)) if keep else None
     y = torch.empty_like(x)
-    lib.check(lib.lib.lsso_ffn_forward(
-        x.data_ptr(), types[x.dtype], t, d, hidden, w_in.data_ptr(), w_out.data_ptr(), types[w_in.dtype],
-        _native._ptr(b_in), _native._ptr(b_out), 2 if bias is None else types[bias.dtype], activation,
-        _native._ptr(gu), h.data_ptr(), y.data_ptr(), _native._stream(x.device)))
-    return y, gu, h
+    _native.run("lsso_ffn_forward", x.device, x.data_ptr(), types[x.dtype], t, d, hidden, w_in.data_ptr(),
+                w_out.data_ptr(), types[w_in.dtype], _native._ptr(b_in), _native._ptr(b_out),
+                2 if bias is None else types[bias.dtype], activation, _native._ptr(kept), h.data_ptr(), y.data_ptr())
+    return y, kept, h
 
 
 def _cast(w_in, w_out, dtype):
     """Both weights in ``dtype`` (one launch when they are FP32)."""
     if w_in.dtype == dtype:
         return w_in, w_out
-    lib = _native.library()
     a, b = torch.empty_like(w_in, dtype=dtype), torch.empty_like(w_out, dtype=dtype)
-    lib.check(lib.lib.lsso_ffn_cast(w_in.data_ptr(), a.data_ptr(), w_in.numel(), w_out.data_ptr(), b.data_ptr(),
-                                    w_out.numel(), _native.ELEMENT_TYPES[dtype], _native._stream(w_in.device)))
+    _native.run("lsso_ffn_cast", w_in.device, w_in.data_ptr(), a.data_ptr(), w_in.numel(), w_out.data_ptr(),
+                b.data_ptr(), w_out.numel(), _native.ELEMENT_TYPES[dtype])
     return a, b
 
 
 class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, activation):
-        with _native.on_device(x.device):
-            a, b = _cast(w_in, w_out, x.dtype)
-            y, gu, h = _forward(x, a, b, b_in, b_out, activation, True)
-        ctx.save_for_backward(x, gu, h, a, b)
+        a, b = _cast(w_in, w_out, x.dtype)
+        y, kept, h = _forward(x, a, b, b_in, b_out, activation, True)
+        ctx.save_for_backward(x, kept, h, a, b)
         ctx.activation, ctx.weight_dtype = activation, w_in.dtype
         ctx.bias_dtypes = [None if v is None else v.dtype for v in (b_in, b_out)]
         return y
@@ -92,28 +88,22 @@ class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, gu, h, w_in, w_out = ctx.saved_tensors
-        lib = _native.library()
+        x, kept, h, w_in, w_out = ctx.saved_tensors
         types = _native.ELEMENT_TYPES
         needs = ctx.needs_input_grad
         device, kind = x.device, ctx.weight_dtype
         (t, d), hidden = x.shape, h.shape[1]
         dy = _aligned(dy.contiguous())
         dx = torch.empty_like(x) if needs[0] else None
-        dw_in = torch.empty((2 * hidden, d), dtype=kind, device=device) if needs[1] else None
-        dw_out = torch.empty((d, hidden), dtype=kind, device=device) if needs[2] else None
-        db_in = torch.empty((2 * hidden,), dtype=kind, device=device) if needs[3] else None
-        db_out = torch.empty((d,), dtype=kind, device=device) if needs[4] else None
-        with _native.on_device(device):
-            size = lib.lib.lsso_ffn_backward_workspace_size(t, d, hidden)
-            if size == 0:
-                lib.check(1)
-            workspace = torch.empty((size,), dtype=torch.uint8, device=device)
-            lib.check(lib.lib.lsso_ffn_backward(
-                dy.data_ptr(), x.data_ptr(), gu.data_ptr(), h.data_ptr(), w_in.data_ptr(), w_out.data_ptr(),
-                types[x.dtype], t, d, hidden, ctx.activation, types[kind], _native._ptr(dx), _native._ptr(dw_in),
-                _native._ptr(dw_out), _native._ptr(db_in), _native._ptr(db_out), workspace.data_ptr(), size,
-                _native._stream(device)))
+        dw_in = torch.empty_like(w_in, dtype=kind) if needs[1] else None
+        dw_out = torch.empty_like(w_out, dtype=kind) if needs[2] else None
+        db_in = x.new_empty((2 * hidden,), dtype=kind) if needs[3] else None
+        db_out = x.new_empty((d,), dtype=kind) if needs[4] else None
+        scratch = _native.workspace("lsso_ffn_backward_workspace_size", device, t, d, hidden)
+        _native.run("lsso_ffn_backward", device, dy.data_ptr(), x.data_ptr(), kept.data_ptr(), h.data_ptr(),
+                    w_in.data_ptr(), w_out.data_ptr(), types[x.dtype], t, d, hidden, ctx.activation, types[kind],
+                    _native._ptr(dx), _native._ptr(dw_in), _native._ptr(dw_out), _native._ptr(db_in),
+                    _native._ptr(db_out), scratch.data_ptr(), scratch.numel())
         if db_in is not None and ctx.bias_dtypes[0] != kind:
             db_in = db_in.to(ctx.bias_dtypes[0])
         if db_out is not None and ctx.bias_dtypes[1] != kind:
@@ -146,10 +136,8 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
         if value is not None and not value.is_contiguous():
             raise RuntimeError(f"gated_feed_forward requires contiguous {name}")
     hidden, dim = w_out.shape[1], x.shape[-1]
-    lead = x.shape[:-1]
+    shape = x.shape
     rows = x.numel() // dim
-    trains = torch.is_grad_enabled() and any(
-        v is not None and v.requires_grad for v in (x, w_in, w_out, b_in, b_out))
     if rows == 0:
         # no rows: no work; gradients (zeros) through PyTorch
         return gated_feed_forward_reference(x, w_in, w_out, b_in, b_out, activation=activation)
@@ -160,21 +148,21 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
         w_out = F.pad(w_out, (0, extra_h, 0, extra_d))
         b_in = None if b_in is None else F.pad(b_in.view(2, hidden), (0, extra_h)).reshape(-1)
         b_out = None if b_out is None else F.pad(b_out, (0, extra_d))
-    flat = _aligned(x.reshape(rows, dim + extra_d).contiguous())
-    w_in, w_out = _aligned(w_in), _aligned(w_out)
+    if x.ndim != 2 or not x.is_contiguous():
+        x = x.reshape(rows, dim + extra_d).contiguous()
+    x, w_in, w_out = _aligned(x), _aligned(w_in), _aligned(w_out)
     act = _ACTIVATIONS[activation]
-    if trains:
-        y = _GatedFeedForward.apply(flat, w_in, w_out, b_in, b_out, act)
+    if torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad
+                                    or any(b is not None and b.requires_grad for b in (b_in, b_out))):
+        y = _GatedFeedForward.apply(x, w_in, w_out, b_in, b_out, act)
     else:
-        with _native.on_device(x.device):
-            a, b = w_in.detach(), w_out.detach()
-            if a.dtype != x.dtype and not _native.library().lib.lsso_ffn_streams_weights(rows, dim + extra_d,
+        if w_in.dtype != x.dtype and not _native.library().lib.lsso_ffn_streams_weights(rows, dim + extra_d,
                                                                                          hidden + extra_h):
-                a, b = _cast(a, b, x.dtype)
-            y = _forward(flat, a, b, b_in, b_out, act, False)[0]
+            w_in, w_out = _cast(w_in, w_out, x.dtype)
+        y = _forward(x, w_in, w_out, b_in, b_out, act, False)[0]
     if extra_d:
         y = y[:, :dim]
-    return y.reshape(*lead, dim)
+    return y if y.shape == shape else y.reshape(shape)
 
 
 def _aligned(value: torch.Tensor) -> torch.Tensor:

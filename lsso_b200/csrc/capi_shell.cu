@@ -61,7 +61,7 @@ int lsso_ffn_streams_weights(int64_t T, int64_t D, int64_t H) {
 }
 
 int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int64_t H, const void* w_in, const void* w_out,
-                     int weight_type, const void* b_in, const void* b_out, int bias_type, int activation, void* gu,
+                     int weight_type, const void* b_in, const void* b_out, int bias_type, int activation, void* kept,
                      void* h, void* y, void* stream) {
   lsso::capi::clear_error();
   const char* who = "lsso_ffn_forward";
@@ -72,12 +72,12 @@ int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int64_t H, c
   if (rc != LSSO_OK) return rc;
   if (!is_16bit(type)) return invalid("%s: type must be BF16 or FP16", who);
   if (weight_type != type &&
-      !(weight_type == LSSO_TYPE_FP32 && gu == nullptr && lsso::ffn_rows_usable(T, D, H))) {
+      !(weight_type == LSSO_TYPE_FP32 && kept == nullptr && lsso::ffn_rows_usable(T, D, H))) {
     return invalid("%s: the weights must have x's type (FP32 only where lsso_ffn_streams_weights says so)", who);
   }
   if ((b_in != nullptr || b_out != nullptr) && !is_type(bias_type)) return invalid("%s: unknown bias type", who);
   if (activation != LSSO_FFN_SILU && activation != LSSO_FFN_GELU) return invalid("%s: unknown activation", who);
-  if (!aligned(x, 16) || !aligned(w_in, 16) || !aligned(w_out, 16) || !aligned(gu, 16) || !aligned(h, 16) ||
+  if (!aligned(x, 16) || !aligned(w_in, 16) || !aligned(w_out, 16) || !aligned(kept, 16) || !aligned(h, 16) ||
       !aligned(y, 16)) {
     return invalid("%s: matrices must be 16-byte aligned", who);
   }
@@ -86,7 +86,7 @@ int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int64_t H, c
   rc = lsso::capi::device(&sms, &status);
   if (rc != LSSO_OK) return rc;
   const lsso::FfnForwardCall c{x,           w_in,      w_out,      b_in, b_out, T, D, H,     type,
-                               weight_type, bias_type, activation, gu,   h,     y, status};
+                               weight_type, bias_type, activation, kept, h,     y, status};
   return lsso::capi::launched(lsso::launch_ffn_forward(c, sms, static_cast<cudaStream_t>(stream)), who);
 }
 
@@ -99,13 +99,13 @@ size_t lsso_ffn_backward_workspace_size(int64_t T, int64_t D, int64_t H) {
   return lsso::ffn_backward_workspace(T, D, H, sms);
 }
 
-int lsso_ffn_backward(const void* dy, const void* x, const void* gu, const void* h, const void* w_in,
+int lsso_ffn_backward(const void* dy, const void* x, const void* kept, const void* h, const void* w_in,
                       const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation, int grad_type,
                       void* dx, void* dw_in, void* dw_out, void* db_in, void* db_out, void* workspace,
                       size_t workspace_bytes, void* stream) {
   lsso::capi::clear_error();
   const char* who = "lsso_ffn_backward";
-  if (dy == nullptr || x == nullptr || gu == nullptr || h == nullptr || w_in == nullptr || w_out == nullptr ||
+  if (dy == nullptr || x == nullptr || kept == nullptr || h == nullptr || w_in == nullptr || w_out == nullptr ||
       workspace == nullptr) {
     return invalid("%s: a required pointer is NULL", who);
   }
@@ -113,7 +113,7 @@ int lsso_ffn_backward(const void* dy, const void* x, const void* gu, const void*
   if (rc != LSSO_OK) return rc;
   if (!is_16bit(type) || !is_type(grad_type)) return invalid("%s: unknown type", who);
   if (activation != LSSO_FFN_SILU && activation != LSSO_FFN_GELU) return invalid("%s: unknown activation", who);
-  for (const void* p : {dy, x, gu, h, w_in, w_out, static_cast<const void*>(dx), static_cast<const void*>(dw_in),
+  for (const void* p : {dy, x, kept, h, w_in, w_out, static_cast<const void*>(dx), static_cast<const void*>(dw_in),
                         static_cast<const void*>(dw_out), static_cast<const void*>(db_in),
                         static_cast<const void*>(db_out), static_cast<const void*>(workspace)}) {
     if (!aligned(p, 16)) return invalid("%s: every array must be 16-byte aligned", who);
@@ -124,7 +124,7 @@ int lsso_ffn_backward(const void* dy, const void* x, const void* gu, const void*
   if (rc != LSSO_OK) return rc;
   const size_t need = lsso::ffn_backward_workspace(T, D, H, sms);
   if (workspace_bytes < need) return lsso::capi::workspace_too_small(who, workspace_bytes, need);
-  const lsso::FfnBackwardCall c{dy, x,  gu,    h,      w_in,  w_out, T, D, H, type, activation, grad_type,
+  const lsso::FfnBackwardCall c{dy, x,  kept,  h,      w_in,  w_out, T, D, H, type, activation, grad_type,
                                 dx, dw_in, dw_out, db_in, db_out, static_cast<uint8_t*>(workspace), status};
   return lsso::capi::launched(lsso::launch_ffn_backward(c, sms, static_cast<cudaStream_t>(stream)), who);
 }

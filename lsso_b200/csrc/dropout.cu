@@ -57,21 +57,36 @@ __device__ __forceinline__ uint32_t keep_bits(int64_t first, uint2 key, uint32_t
   return bits;
 }
 
-// Which of the eight elements lie in rows whose mask is set.
+// Which of the eight elements lie in rows whose mask is set.  From eight
+// columns on, eight elements touch two rows at most.
 __device__ __forceinline__ uint32_t live_bits(const uint8_t* __restrict__ mask, int64_t first, int64_t total,
-                                              int64_t width) {
-  int64_t row = total <= 0xFFFFFFFFll
-                    ? static_cast<int64_t>(static_cast<uint32_t>(first) / static_cast<uint32_t>(width))
-                    : first / width;
-  int64_t left = (row + 1) * width - first;  // elements of this row from `first` on
-  uint32_t bits = 0;
+                                              int64_t width, int64_t rows) {
+  int64_t row, left;  // left: elements of this row from `first` on
+  if (total <= 0xFFFFFFFFll) {
+    const uint32_t r = static_cast<uint32_t>(first) / static_cast<uint32_t>(width);
+    row = r;
+    left = static_cast<uint32_t>(width) - (static_cast<uint32_t>(first) - r * static_cast<uint32_t>(width));
+  } else {
+    row = first / width;
+    left = (row + 1) * width - first;
+  }
   bool live = mask[row] != 0;
+  if (width >= kPer) {
+    uint32_t bits = live ? 0xFFu : 0u;
+    if (left < kPer) {
+      const uint32_t here = (1u << left) - 1u;
+      const bool next = row + 1 < rows && mask[row + 1] != 0;
+      bits = (bits & here) | (next ? 0xFFu & ~here : 0u);
+    }
+    return bits;
+  }
+  uint32_t bits = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (left == 0) {
       left = width;
       ++row;
-      live = first + i < total && mask[row] != 0;
+      live = row < rows && mask[row] != 0;
     }
     --left;
     bits |= live ? 1u << i : 0u;
@@ -125,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutCall c, 
     uint32_t keep = c.drop_all ? 0u : keep_bits(first, key, c.site, static_cast<uint32_t>(step), c.threshold);
     uint32_t live = 0xFFu;
     if (kMasked) {
-      live = live_bits(c.row_mask, first, total, c.width);
+      live = live_bits(c.row_mask, first, total, c.width, c.rows);
       keep &= live;
     }
     float v[kPer];

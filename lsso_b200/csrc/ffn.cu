@@ -9,21 +9,28 @@
 // GELU, g P with P = (1 + erf(g / sqrt 2)) / 2 and act' = P + g phi(g).
 //
 // All operands have x's type (BF16 or FP16); products accumulate in FP32, and
-// h, [g | u], [dg | du] are rounded to that type once, because the next
-// product's tensor-core operand has it; h itself is computed from the
-// unrounded accumulators.
+// h and [dg | du] are rounded to that type once, because the next product's
+// tensor-core operand has it; h itself comes from the unrounded accumulators.
+// A training forward also keeps [g | u], rounded once to the same type, which
+// is what the backward's epilogue reads.
 //
 // Every product is one instance of one persistent, warp-specialised kernel:
 //   warp 0       TMA producer (one lane issues)
-//   warp 1       MMA issuer (one lane issues tcgen05.mma kind::f16, M = 128)
-//   warps 4-11   epilogue, two warps per TMEM sub-partition
-// A tile is 128 rows by up to 256 columns; two TMEM accumulators let the
-// epilogue of one tile run under the products of the next.  Operands are read
-// where the caller keeps them: the contraction axis may be the inner one
-// (K-major boxes) or the outer one (MN-major boxes), so no weight or
-// activation is ever transposed in memory.  The two forward projections share
-// a tile (128 rows x up to 128 gate and the same 128 up columns), so the
-// activation and the product run in its epilogue.
+//   warp 1       MMA issuer (one lane issues tcgen05.mma kind::f16)
+//   warps 4-11, 12-19  epilogue of the even and of the odd tiles, two warps per
+//                TMEM sub-partition each (all sixteen on one tile wait for the
+//                same unit at the same time: TMEM, special functions, stores)
+// CTAs work in pairs (cta_group::2): a tile is 256 rows by up to 256 columns,
+// each CTA holds 128 rows of the row operand and half of the column operand
+// and accumulates its own 128 rows, so shared memory takes 32 KB per 64-wide
+// contraction block instead of the 48 KB that one CTA needs for 128 x 256; up
+// to 128 rows run the same kernel without a partner.  Two TMEM accumulators let
+// the epilogue of one tile run under the products of the next.  Operands are
+// read where the caller keeps them: the contraction axis may be the inner one
+// (K-major boxes) or the outer one (MN-major boxes), so no weight or activation
+// is ever transposed in memory.  The two forward projections share a tile (the
+// gate and the up rows of up to 128 hidden features), so the activation and
+// the product run in its epilogue.
 //
 // Every wait is bounded and an abort flag stops all roles after a timeout.
 #include <cuda.h>
@@ -44,30 +51,30 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kBK = 64;
 constexpr int kMaxStages = 8;
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
 constexpr int kEpiWarp0 = 4;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;
 constexpr uint32_t kBox = 64 * 64 * 2;            // MN-major box: 64 contraction rows x 128 bytes
 constexpr uint32_t kABytes = kBM * kBK * 2;       // 16 KB
-constexpr uint32_t kEpiStage = 4096;              // per epilogue warp: two 32 x 32 boxes
-constexpr size_t kSmemMost = 230400;             // of 232448, the rest for the static arrays
+constexpr uint32_t kOutBox = 32 * 32 * 2;         // output box: 32 rows x 32 columns of 16 bits
+constexpr size_t kSmemMost = 230400;              // of 232448, the rest for the static arrays
 
 enum Mode : int {
-  kGate,    // h = act(x Wg^T) * (x Wu^T)
+  kGate,    // h = act(x Wg^T) * (x Wu^T), and the kept pre-activations
   kOutput,  // out = a b^T (+ bias)
   kSlope,   // [dg | du] from dh = a b, b with the contraction axis outermost
   kInput,   // out = a b, same orientation as kSlope
   kWeight,  // out = a^T b over tokens, split over tokens
 };
-
 struct GemmArgs {
   int M, N;            // output rows and columns (kGate / kSlope: N = H)
   int KB;              // 64-wide contraction blocks
   int BN;              // accumulator columns per tile (kGate: gate and up halves)
-  int ntiles, units, splits, kb_per_split, stages;
-  int activation, keep_gu, bias_type;
+  int mtiles, ntiles, units, splits, kb_per_split, stages;
+  int step_n, step_m;  // a worker's step to its next unit, in n tiles and m tiles
+  int boxes;           // output boxes of one epilogue warp
+  int keep, bias_type;
   const void* bias;    // kGate: [2N], kOutput: [N]; nullable
-  const void* gu;      // kSlope: [M, 2N]
   void* out;           // kWeight: gradient (splits == 1) or FP32 partials [splits][M][N]
   int out_type;
   int* status;
@@ -81,6 +88,88 @@ __device__ __forceinline__ bool fwait_warp(uint32_t bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, status));
 }
 
+// ---------------------------------------------------------------- CTA pairs
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+// This CTA's shared-memory address `addr` in the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void store_remote(uint32_t cluster_addr, int v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void complete_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void alloc_tmem(uint32_t dst, uint32_t ncols) {
+  if (!kPair) return tmem_alloc(dst, ncols);
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(dst), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void free_tmem(uint32_t taddr, uint32_t ncols) {
+  if (!kPair) return tmem_dealloc(taddr, ncols);
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  if (!kPair) return mma_bf16(d, adesc, bdesc, idesc, accumulate);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on the barrier at this offset in every CTA of the group when all MMAs issued so far complete.
+template <bool kPair>
+__device__ __forceinline__ void commit_all(uint32_t bar) {
+  if (!kPair) return mma_commit(bar);
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void commit_own(uint32_t bar) {
+  if (!kPair) return mma_commit(bar);
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+// Tensor loads into this CTA's shared memory that complete on `bar`: this
+// CTA's barrier, or (pairs) the leader's as a cluster address.
+template <bool kPair>
+__device__ __forceinline__ void load_2d(uint32_t dst, const void* tmap, int c0, int c1, uint32_t bar) {
+  if (!kPair) return tma_load_2d(dst, tmap, c0, c1, bar);
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];\n" ::"r"(dst),
+      "l"(tmap), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void load_3d(uint32_t dst, const void* tmap, int c0, int c1, int c2, uint32_t bar) {
+  if (!kPair) return tma_load_3d(dst, tmap, c0, c1, c2, bar);
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4}], [%5];\n" ::"r"(dst),
+      "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- element-wise parts
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if (kHalf) {
@@ -95,23 +184,58 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   return unpack_bf16(v);
 }
 
-// act(g) and act'(g).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// act(g) and act'(g) of two elements.  The special-function unit gives four
+// results per cycle and sub-partition, and two per element (an exponential and
+// a reciprocal) made it the gate epilogue's limit; one reciprocal of the two
+// denominators' product serves both (a^-1 = b (ab)^-1).  Arguments are clamped
+// where that changes nothing a 16-bit result can show, so that the product
+// stays finite and one element's infinity does not reach the other.
+//
+// GELU: Phi(-x) for x >= 0 is p(t) e^(-x^2/2) / 2 with t = 1 / (1 + 0.3275911
+// x / sqrt 2) and the degree-five p of Abramowitz and Stegun 7.1.26 (absolute
+// error of erf below 1.5e-7); the exponential is also the slope's.
 struct ActSlope {
   float act, slope;
 };
 template <int kAct>
-__device__ __forceinline__ float activate(float g) {
-  if (kAct == kSilu) return __fdividef(g, 1.0f + __expf(-g));
-  return 0.5f * g * (1.0f + erff(g * 0.70710678f));
-}
-template <int kAct>
-__device__ __forceinline__ ActSlope activate_slope(float g) {
+__device__ __forceinline__ void activate2(float g0, float g1, ActSlope& s0, ActSlope& s1) {
   if (kAct == kSilu) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-    return {g * s, s * (1.0f + g * (1.0f - s))};
+    constexpr float kLog2e = 1.44269504f;
+    const float a = 1.0f + exp2_approx(fminf(-kLog2e * g0, 58.0f)), b = 1.0f + exp2_approx(fminf(-kLog2e * g1, 58.0f));
+    const float r = reciprocal_approx(a * b);
+    const float p0 = r * b, p1 = r * a;  // the logistic function
+    s0.act = g0 * p0;
+    s1.act = g1 * p1;
+    s0.slope = fmaf(s0.act, 1.0f - p0, p0);
+    s1.slope = fmaf(s1.act, 1.0f - p1, p1);
+    return;
   }
-  const float p = 0.5f * (1.0f + erff(g * 0.70710678f));
-  return {g * p, p + g * 0.39894228f * __expf(-0.5f * g * g)};
+  const float x0 = fminf(fabsf(g0), 30.0f), x1 = fminf(fabsf(g1), 30.0f);
+  const float a = fmaf(x0, 0.23164189f, 1.0f), b = fmaf(x1, 0.23164189f, 1.0f);
+  const float r = reciprocal_approx(a * b);
+  auto finish = [](float g, float x, float t) {
+    const float e = exp2_approx(-0.72134752f * x * x);
+    float p = fmaf(t, 1.061405429f, -1.453152027f);
+    p = fmaf(t, p, 1.421413741f);
+    p = fmaf(t, p, -0.284496736f);
+    p = fmaf(t, p, 0.254829592f);
+    const float q = 0.5f * p * t * e;  // Phi(-x)
+    const float phi = g >= 0.0f ? 1.0f - q : q;
+    return ActSlope{g * phi, fmaf(g * 0.39894228f, e, phi)};
+  };
+  s0 = finish(g0, x0, r * b);
+  s1 = finish(g1, x1, r * a);
 }
 
 __device__ __forceinline__ float read_bias(const void* bias, int type, int64_t i) {
@@ -120,35 +244,41 @@ __device__ __forceinline__ float read_bias(const void* bias, int type, int64_t i
   return __bfloat162float(static_cast<const __nv_bfloat16*>(bias)[i]);
 }
 
-// One epilogue warp's output boxes: 32 rows x 32 columns of 16 bits, 64-byte
-// rows in the 64-byte swizzle, two of them so that a box fills while the
-// tensor store of the other reads.
-struct BoxWriter {
-  uint8_t* stage;
-  int buf;
-  int lane;
-
-  template <bool kHalf>
-  __device__ __forceinline__ void put(const CUtensorMap* map, const float (&v)[32], int c0, int c1, int c2) {
-    uint8_t* box = stage + buf * 2048;
-    if (lane == 0) bulk_wait_read<1>();
-    __syncwarp();
+// 16-byte piece c (0..3) of this lane's row of a box: 64-byte rows in the 64-byte swizzle.
+__device__ __forceinline__ uint4* box_piece(uint8_t* box, int lane, int c) {
+  return reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
+}
+template <bool kHalf>
+__device__ __forceinline__ void box_write(uint8_t* box, int lane, const float (&v)[32]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int j = 8 * c;
-      *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-          make_uint4(pack2<kHalf>(v[j], v[j + 1]), pack2<kHalf>(v[j + 2], v[j + 3]), pack2<kHalf>(v[j + 4], v[j + 5]),
-                     pack2<kHalf>(v[j + 6], v[j + 7]));
-    }
-    fence_proxy_async();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_3d(map, smem_u32(box), c0, c1, c2);
-      bulk_commit();
-    }
-    buf ^= 1;
+  for (int c = 0; c < 4; ++c) {
+    const int j = 8 * c;
+    *box_piece(box, lane, c) = make_uint4(pack2<kHalf>(v[j], v[j + 1]), pack2<kHalf>(v[j + 2], v[j + 3]),
+                                          pack2<kHalf>(v[j + 4], v[j + 5]), pack2<kHalf>(v[j + 6], v[j + 7]));
   }
-};
+}
+// [dg | du] from dh and the kept pre-activations, in their place.
+template <bool kHalf, int kAct>
+__device__ __forceinline__ void box_slope(uint8_t* gbox, uint8_t* ubox, int lane, const float (&dh)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint4 *pg = box_piece(gbox, lane, c), *pu = box_piece(ubox, lane, c);
+    const uint4 gq = *pg, uq = *pu;
+    const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w}, uw[4] = {uq.x, uq.y, uq.z, uq.w};
+    uint32_t dg[4], du[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 g = unpack2<kHalf>(gw[k]), u = unpack2<kHalf>(uw[k]);
+      ActSlope s0, s1;
+      activate2<kAct>(g.x, g.y, s0, s1);
+      const float d0 = dh[8 * c + 2 * k], d1 = dh[8 * c + 2 * k + 1];
+      dg[k] = pack2<kHalf>(d0 * u.x * s0.slope, d1 * u.y * s1.slope);
+      du[k] = pack2<kHalf>(d0 * s0.act, d1 * s1.act);
+    }
+    *pg = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+    *pu = make_uint4(du[0], du[1], du[2], du[3]);
+  }
+}
 
 // 32 bias values of the columns from n0 on, added to a row's accumulators
 // (through shared memory: one global load per lane, broadcast reads).
@@ -168,25 +298,81 @@ __device__ __forceinline__ void add_bias(float (&v)[32], float* scratch, const v
   }
 }
 
-template <int kMode, bool kHalf, int kAct>
+// Write one row's 32 weight-gradient values from column n0 on.
+__device__ __forceinline__ void write_gradient(const GemmArgs& a, const float (&v)[32], int split, int64_t row, int n0) {
+  const int64_t at = row * a.N + n0;
+  if (a.splits > 1 || a.out_type == kFp32) {
+    float* o = static_cast<float*>(a.out) + static_cast<int64_t>(split) * a.M * a.N + at;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4)
+      if (n0 + j < a.N) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    return;
+  }
+  uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+#pragma unroll
+  for (int j = 0; j < 32; j += 8) {
+    if (n0 + j >= a.N) continue;
+    uint4 w;
+    if (a.out_type == kFp16) {
+      w = make_uint4(pack2<true>(v[j], v[j + 1]), pack2<true>(v[j + 2], v[j + 3]), pack2<true>(v[j + 4], v[j + 5]),
+                     pack2<true>(v[j + 6], v[j + 7]));
+    } else {
+      w = make_uint4(pack2<false>(v[j], v[j + 1]), pack2<false>(v[j + 2], v[j + 3]), pack2<false>(v[j + 4], v[j + 5]),
+                     pack2<false>(v[j + 6], v[j + 7]));
+    }
+    *reinterpret_cast<uint4*>(o + j) = w;
+  }
+}
+
+// A worker's walk over its units (n tile fastest, then m tile, then split), by
+// increments: divisions per tile and warp took a sixth of the gate epilogue.
+struct UnitWalk {
+  int unit, nt, mt, split;
+
+  __device__ __forceinline__ UnitWalk(const GemmArgs& a, int first) : unit(first) {
+    nt = first % a.ntiles;
+    mt = first / a.ntiles;
+    split = mt / a.mtiles;
+    mt -= split * a.mtiles;
+  }
+  __device__ __forceinline__ void next(const GemmArgs& a, int step) {
+    unit += step;
+    nt += a.step_n;
+    mt += a.step_m;
+    if (nt >= a.ntiles) {
+      nt -= a.ntiles;
+      ++mt;
+    }
+    while (mt >= a.mtiles) {
+      mt -= a.mtiles;
+      ++split;
+    }
+  }
+};
+
+template <int kMode, bool kHalf, int kAct, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ CUtensorMap tmap_gu,
+                const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ CUtensorMap tmap_keep,
                 const GemmArgs a) {
   pdl_wait();
   constexpr bool kAmn = kMode == kWeight;
   constexpr bool kBmn = kMode == kSlope || kMode == kInput || kMode == kWeight;
+  constexpr int kCtas = kPair ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2], mdrain;
+  __shared__ __align__(8) uint64_t kept[kMode == kSlope ? kEpiWarps : 1];
   __shared__ uint32_t tmem_s;
   __shared__ int abort_flag;
+  __shared__ int peer_last[kMaxStages];  // pair leader: the partner's last use of each stage
   __shared__ __align__(16) float sbias[kEpiWarps][32];
   volatile int* abort_v = &abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = kPair ? cluster_rank() : 0u;
+  const int first_unit = static_cast<int>(blockIdx.x) / kCtas, unit_step = static_cast<int>(gridDim.x) / kCtas;
   const int S = a.stages;
-  const int BN = a.BN;
-  const uint32_t stage_bytes = kABytes + static_cast<uint32_t>(BN) * 128;
-  const int mtiles = (a.M + kBM - 1) / kBM;
+  const int BN = a.BN, BNL = BN / kCtas;  // accumulator columns; columns of the operand this CTA holds
+  const uint32_t stage_bytes = kABytes + static_cast<uint32_t>(BNL) * 128;
   const uint32_t tcols = tmem_cols_for(2 * BN);
   const int span = kMode == kGate ? BN / 2 : BN;  // output columns per tile
 
@@ -197,17 +383,22 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&tfull[b]), 1);
-      mbar_init(smem_u32(&tempty[b]), kEpiWarps);
+      mbar_init(smem_u32(&tempty[b]), kEpiWarps / 2 * kCtas);
     }
     mbar_init(smem_u32(&mdrain), 1);
+    if (kMode == kSlope) {
+      for (int i = 0; i < kEpiWarps; ++i) mbar_init(smem_u32(&kept[i]), 1);
+    }
     abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(smem_u32(&tmem_s), tcols);
+  if (warp == 1) alloc_tmem<kPair>(smem_u32(&tmem_s), tcols);
   tc_fence_before();
   __syncthreads();
+  if (kPair) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
+  int last_use[kMaxStages];  // producer's lane 0: the use of each stage whose loads were issued last
 
   if (warp == 0) {
     // ---------------- producer
@@ -217,219 +408,300 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     }
     RingPos rp;
     bool ok = true;
-    int last_use[kMaxStages];  // lane 0: the use of each stage whose loads were issued last
     for (int s = 0; s < kMaxStages; ++s) last_use[s] = -1;
-    for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x) {
-      const int nt = unit % a.ntiles, r = unit / a.ntiles;
-      const int mt = r % mtiles, split = r / mtiles;
+    for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step)) {
+      const int nt = w.nt, mt = w.mt, split = w.split;
+      const int m0 = (mt * kCtas + static_cast<int>(rank)) * kBM;
+      const int n0 = nt * BN + static_cast<int>(rank) * BNL;
       const int kb1 = min(a.KB, (split + 1) * a.kb_per_split);
       for (int kb = split * a.kb_per_split; kb < kb1 && ok; ++kb, rp.next(S)) {
         const int s = rp.s;
         ok = fwait(smem_u32(&empty[s]), (rp.u & 1) ^ 1, abort_v, a.status);
         if (ok && lane == 0) {
-          const uint32_t bar = smem_u32(&full[s]);
+          const uint32_t own_bar = smem_u32(&full[s]);
+          const uint32_t bar = kPair ? map_rank(own_bar, 0) : own_bar;
           const uint32_t dst = smem_u32(smem + s * stage_bytes);
           const uint32_t bdst = dst + kABytes;
-          mbar_arrive_expect_tx(bar, stage_bytes);
+          if (rank == 0) mbar_arrive_expect_tx(own_bar, kCtas * stage_bytes);
           if (kAmn) {
-            tma_load_2d(dst, &tmap_a, mt * kBM, kb * kBK, bar);
-            tma_load_2d(dst + kBox, &tmap_a, mt * kBM + 64, kb * kBK, bar);
+            load_2d<kPair>(dst, &tmap_a, m0, kb * kBK, bar);
+            load_2d<kPair>(dst + kBox, &tmap_a, m0 + 64, kb * kBK, bar);
           } else {
-            tma_load_2d(dst, &tmap_a, kb * kBK, mt * kBM, bar);
+            load_2d<kPair>(dst, &tmap_a, kb * kBK, m0, bar);
           }
           if (kMode == kGate) {
-            tma_load_3d(bdst, &tmap_b, kb * kBK, nt * span, 0, bar);
-            tma_load_3d(bdst + static_cast<uint32_t>(span) * 128, &tmap_b, kb * kBK, nt * span, 1, bar);
+            // columns [0, span) are the gate rows, [span, 2 span) the up rows: one plane per CTA of a pair
+            load_3d<kPair>(bdst, &tmap_b, kb * kBK, nt * span, static_cast<int>(rank), bar);
+            if (!kPair) load_3d<kPair>(bdst + static_cast<uint32_t>(span) * 128, &tmap_b, kb * kBK, nt * span, 1, bar);
           } else if (kBmn) {
-            for (int g = 0; g < BN / 64; ++g) tma_load_2d(bdst + g * kBox, &tmap_b, nt * BN + g * 64, kb * kBK, bar);
+            for (int g = 0; g < BNL / 64; ++g) load_2d<kPair>(bdst + g * kBox, &tmap_b, n0 + g * 64, kb * kBK, bar);
           } else {
-            tma_load_2d(bdst, &tmap_b, kb * kBK, nt * BN, bar);
+            load_2d<kPair>(bdst, &tmap_b, kb * kBK, n0, bar);
           }
           last_use[s] = rp.u;
         }
         __syncwarp();
       }
     }
-    if (lane == 0) {
-      // loads still in flight (only after an abort): wait for them, bounded
-      for (int s = 0; s < S; ++s) {
-        if (last_use[s] >= 0) mbar_wait(smem_u32(&full[s]), static_cast<uint32_t>(last_use[s]) & 1u, a.status);
-      }
+    if (kPair && rank == 1 && lane == 0) {
+      for (int s = 0; s < S; ++s) store_remote(map_rank(smem_u32(&peer_last[s]), 0), last_use[s]);
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ---------------- MMA issuer
-    // kind::f16 operand format bits: BF16 as set by make_idesc, FP16 as zero
-    const uint32_t idesc = make_idesc(kBM, BN, kAmn, kBmn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
-    RingPos rp;
-    bool ok = true;
-    int i = 0;
-    for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x, ++i) {
-      const int split = unit / a.ntiles / mtiles;
-      const int kb0 = split * a.kb_per_split, kb1 = min(a.KB, kb0 + a.kb_per_split);
-      const int b = i & 1;
-      ok = fwait(smem_u32(&tempty[b]), ((i >> 1) & 1) ^ 1, abort_v, a.status);
-      tc_fence_after();
-      const uint32_t d = tmem + static_cast<uint32_t>(b * BN);
-      for (int kb = kb0; kb < kb1 && ok; ++kb, rp.next(S)) {
-        const int s = rp.s;
-        ok = fwait(smem_u32(&full[s]), rp.u & 1, abort_v, a.status);
+    // ---------------- MMA issuer (of a pair: the leader's)
+    if (rank == 0) {
+      // kind::f16 operand format bits: BF16 as set by make_idesc, FP16 as zero
+      const uint32_t idesc = make_idesc(kBM * kCtas, BN, kAmn, kBmn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
+      RingPos rp;
+      bool ok = true;
+      int i = 0;
+      for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step), ++i) {
+        const int kb0 = w.split * a.kb_per_split, kb1 = min(a.KB, kb0 + a.kb_per_split);
+        const int b = i & 1;
+        ok = fwait(smem_u32(&tempty[b]), ((i >> 1) & 1) ^ 1, abort_v, a.status);
         tc_fence_after();
-        if (ok && lane == 0) {
-          const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + kABytes;
+        const uint32_t d = tmem + static_cast<uint32_t>(b * BN);
+        for (int kb = kb0; kb < kb1 && ok; ++kb, rp.next(S)) {
+          const int s = rp.s;
+          ok = fwait(smem_u32(&full[s]), rp.u & 1, abort_v, a.status);
+          tc_fence_after();
+          if (ok && lane == 0) {
+            const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + kABytes;
 #pragma unroll
-          for (int ks = 0; ks < kBK / 16; ++ks) {
-            const uint64_t ad = kAmn ? make_desc_sw128(sa + ks * 2048, kBox, 1024) : make_desc_sw128(sa + ks * 32, 16, 1024);
-            const uint64_t bd = kBmn ? make_desc_sw128(sb + ks * 2048, kBox, 1024) : make_desc_sw128(sb + ks * 32, 16, 1024);
-            mma_bf16(d, ad, bd, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
+            for (int ks = 0; ks < kBK / 16; ++ks) {
+              const uint64_t ad = kAmn ? make_desc_sw128(sa + ks * 2048, kBox, 1024) : make_desc_sw128(sa + ks * 32, 16, 1024);
+              const uint64_t bd = kBmn ? make_desc_sw128(sb + ks * 2048, kBox, 1024) : make_desc_sw128(sb + ks * 32, 16, 1024);
+              mma<kPair>(d, ad, bd, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
+            }
+            commit_all<kPair>(smem_u32(&empty[s]));
           }
-          mma_commit(smem_u32(&empty[s]));
+          __syncwarp();
         }
+        if (ok && lane == 0) commit_all<kPair>(smem_u32(&tfull[b]));
         __syncwarp();
       }
-      if (ok && lane == 0) mma_commit(smem_u32(&tfull[b]));
-      __syncwarp();
+      // no tensor-core operation still writes TMEM or reads shared memory past this point
+      if (lane == 0) {
+        commit_own<kPair>(smem_u32(&mdrain));
+        mbar_wait_bounded(smem_u32(&mdrain), 0, nullptr, a.status);
+      }
     }
-    if (lane == 0) mma_drain(smem_u32(&mdrain), a.status);
     __syncwarp();
   } else if (warp >= kEpiWarp0) {
     // ---------------- epilogue
     const int ew = warp - kEpiWarp0;
     const int sub = warp & 3;
-    const int half = ew >> 2;
-    BoxWriter box{smem + S * stage_bytes + ew * kEpiStage, 0, lane};
+    const int b = ew >> 3;                  // the tiles of this group: accumulator b
+    const int col0 = 32 * ((ew >> 2) & 1);  // first column of this warp's pieces within a tile; the next are 64 on
+    const int row_base = static_cast<int>(rank) * kBM + 32 * sub;
+    uint8_t* stage = smem + S * stage_bytes + ew * a.boxes * kOutBox;
     float* scratch = sbias[ew];
+    const uint32_t kbar = smem_u32(&kept[kMode == kSlope ? ew : 0]);
+    UnitWalk w(a, first_unit + b * unit_step), ahead = w;  // ahead, ahead_c: kSlope: the next piece whose pre-activations are loaded
+    int ahead_c = col0, loaded = 0, piece = 0;
+    // Loads the kept pre-activations of the next piece of this warp that lies in the output, if there is one.
+    auto load_kept = [&]() {
+      for (; ahead.unit < a.units; ahead.next(a, unit_step), ahead.next(a, unit_step), ahead_c = col0) {
+        const int r0 = ahead.mt * kBM * kCtas + row_base, n0 = ahead.nt * span + ahead_c;
+        if (r0 >= a.M || ahead_c >= span || n0 >= a.N) continue;
+        if (lane == 0) {
+          bulk_wait_read<0>();  // the stores from the boxes, one piece ago
+          mbar_arrive_expect_tx(kbar, 2 * kOutBox);
+          tma_load_3d(smem_u32(stage), &tmap_keep, n0, 0, r0, kbar);
+          tma_load_3d(smem_u32(stage + kOutBox), &tmap_keep, n0, 1, r0, kbar);
+        }
+        ++loaded;
+        ahead_c += 64;
+        break;
+      }
+      __syncwarp();
+    };
     if (kMode != kWeight && lane == 0) {
       prefetch_tmap(&tmap_out);
-      if (kMode == kGate) prefetch_tmap(&tmap_gu);
+      if (kMode == kGate || kMode == kSlope) prefetch_tmap(&tmap_keep);
     }
+    if (kMode == kSlope) load_kept();
+    // The boxes are free to be written again (the stores from them have read them).
+    auto boxes_free = [&]() {
+      if (lane == 0) bulk_wait_read<0>();
+      __syncwarp();
+    };
+    auto store_box = [&](const CUtensorMap* map, int box, int n0, int plane, int row0) {
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(map, smem_u32(stage + box * kOutBox), n0, plane, row0);
+        bulk_commit();
+      }
+    };
     bool ok = true;
     int i = 0;
-    for (int unit = blockIdx.x; unit < a.units && ok; unit += gridDim.x, ++i) {
-      const int nt = unit % a.ntiles, r = unit / a.ntiles;
-      const int mt = r % mtiles, split = r / mtiles;
-      const int b = i & 1;
-      ok = fwait_warp(smem_u32(&tfull[b]), (i >> 1) & 1, abort_v, a.status);
+    for (; w.unit < a.units && ok; w.next(a, unit_step), w.next(a, unit_step), ++i) {
+      ok = fwait_warp(smem_u32(&tfull[b]), i & 1, abort_v, a.status);
       tc_fence_after();
-      if (ok) {
-        const int row0 = mt * kBM + 32 * sub;
-        const int64_t row = row0 + lane;
-        const uint32_t acc = tmem + (static_cast<uint32_t>(32 * sub) << 16) + static_cast<uint32_t>(b * BN);
-        for (int c0 = 32 * half; c0 < span; c0 += 64) {
-          const int n0 = nt * span + c0;
-          if (n0 >= a.N || row0 >= a.M) break;  // warp-uniform
-          float v[32];
-          tmem_ld32(acc + c0, v);
-          if (kMode == kGate) {
-            float u[32];
-            tmem_ld32(acc + span + c0, u);
-            tmem_ld_wait();
-            if (a.bias != nullptr) {
-              add_bias(v, scratch, a.bias, a.bias_type, n0, a.N, 0, lane);
-              add_bias(u, scratch, a.bias, a.bias_type, n0, a.N, a.N, lane);
-            }
-            if (a.keep_gu) {
-              box.put<kHalf>(&tmap_gu, v, n0, 0, row0);
-              box.put<kHalf>(&tmap_gu, u, n0, 1, row0);
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = activate<kAct>(v[j]) * u[j];
-            box.put<kHalf>(&tmap_out, v, n0, 0, row0);
-          } else if (kMode == kSlope) {
-            // this row's kept pre-activations, 32 columns of each half
-            const uint16_t* src = static_cast<const uint16_t*>(a.gu) + row * 2 * a.N + n0;
-            uint4 gq[4], uq[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const bool in = row < a.M && n0 + 8 * q < a.N;
-              gq[q] = in ? __ldg(reinterpret_cast<const uint4*>(src) + q) : make_uint4(0u, 0u, 0u, 0u);
-              uq[q] = in ? __ldg(reinterpret_cast<const uint4*>(src + a.N) + q) : make_uint4(0u, 0u, 0u, 0u);
-            }
-            float du[32];
-            tmem_ld_wait();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint32_t gw[4] = {gq[q].x, gq[q].y, gq[q].z, gq[q].w};
-              const uint32_t uw[4] = {uq[q].x, uq[q].y, uq[q].z, uq[q].w};
-#pragma unroll
-              for (int p = 0; p < 4; ++p) {
-                const float2 g2 = unpack2<kHalf>(gw[p]), u2 = unpack2<kHalf>(uw[p]);
-                const int j = 8 * q + 2 * p;
-                const ActSlope s0 = activate_slope<kAct>(g2.x), s1 = activate_slope<kAct>(g2.y);
-                du[j] = v[j] * s0.act;
-                du[j + 1] = v[j + 1] * s1.act;
-                v[j] *= u2.x * s0.slope;
-                v[j + 1] *= u2.y * s1.slope;
-              }
-            }
-            box.put<kHalf>(&tmap_out, v, n0, 0, row0);
-            box.put<kHalf>(&tmap_out, du, n0, 1, row0);
-          } else if (kMode == kWeight) {
-            tmem_ld_wait();
-            if (row < a.M) {
-              const int64_t at = row * a.N + n0;
-              const int type = a.splits > 1 ? static_cast<int>(kFp32) : a.out_type;
-              if (type == kFp32) {
-                float* o = static_cast<float*>(a.out) + static_cast<int64_t>(split) * a.M * a.N + at;
-#pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                  if (n0 + j < a.N) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-              } else {
-                uint16_t* o = static_cast<uint16_t*>(a.out) + at;
-#pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                  if (n0 + j >= a.N) continue;
-                  uint4 w;
-                  if (type == kFp16) {
-                    w = make_uint4(pack2<true>(v[j], v[j + 1]), pack2<true>(v[j + 2], v[j + 3]),
-                                   pack2<true>(v[j + 4], v[j + 5]), pack2<true>(v[j + 6], v[j + 7]));
-                  } else {
-                    w = make_uint4(pack2<false>(v[j], v[j + 1]), pack2<false>(v[j + 2], v[j + 3]),
-                                   pack2<false>(v[j + 4], v[j + 5]), pack2<false>(v[j + 6], v[j + 7]));
-                  }
-                  *reinterpret_cast<uint4*>(o + j) = w;
-                }
-              }
-            }
+      const uint32_t acc = tmem + (static_cast<uint32_t>(32 * sub) << 16) + static_cast<uint32_t>(b * BN);
+      const int row0 = w.mt * kBM * kCtas + row_base;
+      const int columns = row0 < a.M ? min(span, a.N - w.nt * span) : 0;  // of this tile that lie in the output
+      // This warp's last values of the tile are in registers: its accumulator may be overwritten.
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (kPair && rank != 0) {
+            arrive_remote(map_rank(smem_u32(&tempty[b]), 0));
           } else {
-            tmem_ld_wait();
+            mbar_arrive(smem_u32(&tempty[b]));
+          }
+        }
+      };
+      if (!ok || col0 >= columns) release();
+      for (int c = col0; c < columns && ok; c += 64, ++piece) {
+        const int n0 = w.nt * span + c;
+        const bool last = c + 64 >= columns;
+        float v[32];
+        tmem_ld32(acc + c, v);
+        if (kMode == kGate) {
+          float u[32];
+          tmem_ld32(acc + span + c, u);
+          tmem_ld_wait();
+          if (last) release();
+          if (a.bias != nullptr) {
+            add_bias(v, scratch, a.bias, a.bias_type, n0, a.N, 0, lane);
+            add_bias(u, scratch, a.bias, a.bias_type, n0, a.N, a.N, lane);
+          }
+          boxes_free();
+          if (a.keep) {
+            const bool apart = a.boxes == 3;
+            box_write<kHalf>(stage + (apart ? kOutBox : 0), lane, v);
+            if (apart) box_write<kHalf>(stage + 2 * kOutBox, lane, u);
+            store_box(&tmap_keep, apart ? 1 : 0, n0, 0, row0);
+            if (!apart) {
+              boxes_free();
+              box_write<kHalf>(stage, lane, u);
+            }
+            store_box(&tmap_keep, apart ? 2 : 0, n0, 1, row0);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            ActSlope s0, s1;
+            activate2<kAct>(v[j], v[j + 1], s0, s1);
+            v[j] = s0.act * u[j];
+            v[j + 1] = s1.act * u[j + 1];
+          }
+          if (a.keep && a.boxes == 1) boxes_free();
+          box_write<kHalf>(stage, lane, v);
+          store_box(&tmap_out, 0, n0, 0, row0);
+        } else if (kMode == kSlope) {
+          tmem_ld_wait();
+          if (last) release();
+          ok = fwait_warp(kbar, piece & 1, abort_v, a.status);
+          if (!ok) {
+            if (!last) release();
+            break;
+          }
+          box_slope<kHalf, kAct>(stage, stage + kOutBox, lane, v);
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&tmap_out, smem_u32(stage), n0, 0, row0);
+            tma_store_3d(&tmap_out, smem_u32(stage + kOutBox), n0, 1, row0);
+            bulk_commit();
+          }
+          load_kept();
+        } else {
+          tmem_ld_wait();
+          if (last) release();
+          if (kMode == kWeight) {
+            const int64_t row = row0 + lane;
+            if (row < a.M) write_gradient(a, v, w.split, row, n0);
+          } else {
             if (kMode == kOutput && a.bias != nullptr) add_bias(v, scratch, a.bias, a.bias_type, n0, a.N, 0, lane);
-            box.put<kHalf>(&tmap_out, v, n0, 0, row0);
+            boxes_free();
+            box_write<kHalf>(stage, lane, v);
+            store_box(&tmap_out, 0, n0, 0, row0);
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&tempty[b]));
     }
-    if (lane == 0) bulk_wait<0>();
+    if (lane == 0) {
+      bulk_wait<0>();
+      // loads still on their way (only after an abort): wait for them, bounded
+      if (kMode == kSlope) {
+        if (piece < loaded) mbar_wait(kbar, static_cast<uint32_t>(piece) & 1u, a.status);
+      }
+    }
     __syncwarp();
   }
 
   tc_fence_before();
   __syncthreads();
+  if (kPair) cluster_sync();
+  // Loads still in flight (only after an abort): wait for them, bounded.  Both
+  // CTAs' loads complete on the leader's barriers; where one CTA issued a use
+  // of a stage that the other did not, the leader supplies the missing arrival
+  // or bytes first, so that the phase completes when the issued loads have landed.
+  if (warp == 0 && lane == 0 && rank == 0) {
+    for (int s = 0; s < S; ++s) {
+      const uint32_t bar = smem_u32(&full[s]);
+      int last = last_use[s];
+      if (kPair && peer_last[s] > last) {
+        last = peer_last[s];
+        mbar_arrive_expect_tx(bar, stage_bytes);
+      } else if (kPair && peer_last[s] < last) {
+        complete_tx(bar, stage_bytes);
+      }
+      if (last >= 0) mbar_wait(bar, static_cast<uint32_t>(last) & 1u, a.status);
+    }
+  }
+  __syncthreads();
+  if (kPair) cluster_sync();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, tcols);
+    free_tmem<kPair>(tmem, tcols);
   }
 }
 
-// Sum of the weight gradient's per-split partials, in split order.
-template <typename O>
+// Sum of per-split partials: kGroups warps take every kGroups-th split, their
+// sums are added in group order (the same order in every run).  One group for
+// few splits (a large array), eight for many.
+template <typename O, int kGroups>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ partial, int splits, int64_t count,
                                                          O* __restrict__ out) {
   pdl_wait();
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;  // count is a multiple of 8
-  if (i >= count) return;
-  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float4 p = __ldg(reinterpret_cast<const float4*>(partial + s * count + i));
-    v[0] += p.x;
-    v[1] += p.y;
-    v[2] += p.z;
-    v[3] += p.w;
+  __shared__ float4 part[kGroups][32];
+  const int group = kGroups == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * (256 / kGroups) + (kGroups == 1 ? threadIdx.x : lane)) * 4;
+  // count is a multiple of 8
+  const int64_t at = i < count ? i : 0;
+  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = group; s < splits; s += 4 * kGroups) {
+    float4 v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = __ldg(reinterpret_cast<const float4*>(partial + min(s + kGroups * q, splits - 1) * count + at));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (s + kGroups * q >= splits) continue;
+      sum.x += v[q].x;
+      sum.y += v[q].y;
+      sum.z += v[q].z;
+      sum.w += v[q].w;
+    }
   }
+  if constexpr (kGroups > 1) {
+    part[group][lane] = sum;
+    __syncthreads();
+    if (group != 0) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) {
+      const float4 p = part[g][lane];
+      sum.x += p.x;
+      sum.y += p.y;
+      sum.z += p.z;
+      sum.w += p.w;
+    }
+  }
+  if (i >= count) return;
+  const float v[4] = {sum.x, sum.y, sum.z, sum.w};
   store_run<O, 4>(out + i, v);
 }
 
@@ -540,7 +812,11 @@ __global__ void __launch_bounds__(256) ffn_rows_kernel(const S* __restrict__ x, 
   for (int t = 0; t < kRows; ++t) {
     if (t < rows && lane == t) {
       float v = g[t] + bg;
-      if constexpr (kGated) v = activate<kAct>(v) * (u[t] + bu);
+      if constexpr (kGated) {
+        ActSlope s0, s1;
+        activate2<kAct>(v, v, s0, s1);
+        v = s0.act * (u[t] + bu);
+      }
       out[t * N + n] = from_float<S>(v);
     }
   }
@@ -549,48 +825,70 @@ __global__ void __launch_bounds__(256) ffn_rows_kernel(const S* __restrict__ x, 
 // ---------------------------------------------------------------- host
 struct GemmPlan {
   GemmArgs args;
-  int grid;
+  int grid, pair;
   size_t smem;
 };
 
-// Tile width and token split.  The estimate is rounds x (columns + a fixed
-// cost per tile, in columns) x contraction blocks per unit: wide tiles reuse
-// the row operand more, narrow ones fill the SMs when there are few.
-GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count) {
+// Output boxes of one epilogue warp.  kGate with kept pre-activations: h, g and
+// u apart (96 KB, four stages) while a tile is short and its stores set the
+// pace; one box in turn for all three (32 KB, six stages) from eight
+// contraction blocks on, where loads in flight do.  kSlope: g and u in, dg and
+// du out in their place.
+int boxes_of(Mode mode, bool keep, int64_t KB) {
+  return mode == kWeight ? 0 : mode == kSlope ? 2 : mode == kGate && keep && KB < 8 ? 3 : 1;
+}
+
+// Pairs or single CTAs, tile width and token split.  The estimate counts
+// tensor-core cycles: rounds x (contraction blocks x (2 columns + a fixed cost
+// per block) + a fixed cost per tile); a single CTA's tile is held back by
+// shared-memory bandwidth.  Wide tiles reuse the row operand more, narrow ones
+// fill the SMs when there are few.
+GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, bool keep = false) {
   GemmPlan best{};
   double best_cost = 0.0;
-  const int64_t mtiles = (M + kBM - 1) / kBM;
   const int64_t KB = (K + kBK - 1) / kBK;
-  for (int bn = 256; bn >= 64; bn -= 64) {
-    const int span = mode == kGate ? bn / 2 : bn;
-    const int64_t ntiles = (N + span - 1) / span;
-    const int64_t tiles = mtiles * ntiles;
-    const int64_t most_splits = mode == kWeight ? std::min<int64_t>(KB, 64) : 1;
-    for (int64_t want = 1; want <= most_splits; ++want) {
-      const int64_t per = (KB + want - 1) / want;
-      const int64_t splits = (KB + per - 1) / per;
-      if (splits != want) continue;
-      const int64_t units = tiles * splits;
-      const int64_t rounds = (units + sm_count - 1) / sm_count;
-      double cost = static_cast<double>(rounds) * (per * (bn + 32.0) + 256.0);
-      if (splits > 1) cost += splits * static_cast<double>(M) * N / 16384.0;  // partials written and read
-      if (best.grid != 0 && cost >= best_cost) continue;
-      best_cost = cost;
-      GemmArgs a{};
-      a.M = static_cast<int>(M);
-      a.N = static_cast<int>(N);
-      a.KB = static_cast<int>(KB);
-      a.BN = bn;
-      a.ntiles = static_cast<int>(ntiles);
-      a.units = static_cast<int>(units);
-      a.splits = static_cast<int>(splits);
-      a.kb_per_split = static_cast<int>(per);
-      const size_t stage = kABytes + static_cast<size_t>(bn) * 128;
-      a.stages = static_cast<int>((kSmemMost - kEpiWarps * kEpiStage) / stage);
-      if (a.stages > kMaxStages) a.stages = kMaxStages;
-      best.args = a;
-      best.grid = static_cast<int>(units < sm_count ? units : sm_count);
-      best.smem = a.stages * stage + kEpiWarps * kEpiStage;
+  for (int pair = 1; pair >= 0; --pair) {
+    if (pair && M <= kBM) continue;
+    const int64_t rows = kBM * (pair ? 2 : 1);
+    const int64_t mtiles = (M + rows - 1) / rows;
+    const int64_t workers = pair ? sm_count / 2 : sm_count;
+    for (int bn = 256; bn >= 64; bn -= pair ? 128 : 64) {
+      const int span = mode == kGate ? bn / 2 : bn;
+      const int64_t ntiles = (N + span - 1) / span;
+      const int64_t tiles = mtiles * ntiles;
+      const int64_t most_splits = mode == kWeight ? std::min<int64_t>(KB, 64) : 1;
+      for (int64_t want = 1; want <= most_splits; ++want) {
+        const int64_t per = (KB + want - 1) / want;
+        const int64_t splits = (KB + per - 1) / per;
+        if (splits != want) continue;
+        const int64_t units = tiles * splits;
+        const int64_t rounds = (units + workers - 1) / workers;
+        double cost = static_cast<double>(rounds) * (per * ((pair ? 2.0 : 2.7) * bn + 64.0) + 1000.0);
+        if (splits > 1) cost += splits * static_cast<double>(M) * N / 512.0;  // partials written and read
+        if (best.grid != 0 && cost >= best_cost) continue;
+        best_cost = cost;
+        GemmArgs a{};
+        a.M = static_cast<int>(M);
+        a.N = static_cast<int>(N);
+        a.KB = static_cast<int>(KB);
+        a.BN = bn;
+        a.mtiles = static_cast<int>(mtiles);
+        a.ntiles = static_cast<int>(ntiles);
+        a.units = static_cast<int>(units);
+        a.splits = static_cast<int>(splits);
+        a.kb_per_split = static_cast<int>(per);
+        a.step_n = static_cast<int>(std::min(units, workers) % ntiles);
+        a.step_m = static_cast<int>(std::min(units, workers) / ntiles);
+        a.boxes = boxes_of(mode, keep, KB);
+        const size_t stage = kABytes + static_cast<size_t>(bn) * (pair ? 64 : 128);
+        const size_t staging = static_cast<size_t>(kEpiWarps) * a.boxes * kOutBox;
+        a.stages = static_cast<int>((kSmemMost - staging) / stage);
+        if (a.stages > kMaxStages) a.stages = kMaxStages;
+        best.args = a;
+        best.pair = pair;
+        best.grid = static_cast<int>(units < workers ? units : workers) * (pair ? 2 : 1);
+        best.smem = a.stages * stage + staging;
+      }
     }
   }
   return best;
@@ -631,13 +929,27 @@ bool encode_out(CUtensorMap* map, const void* ptr, bool half, int64_t rows, int6
 
 template <int kMode, int kAct>
 cudaError_t launch_gemm(const char* name, const GemmPlan& p, bool half, const CUtensorMap& ma, const CUtensorMap& mb,
-                        const CUtensorMap& mo, const CUtensorMap& mg, cudaStream_t stream) {
-  auto kernel = half ? &ffn_gemm_kernel<kMode, true, kAct> : &ffn_gemm_kernel<kMode, false, kAct>;
-  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), p.smem);
+                        const CUtensorMap& mo, const CUtensorMap& mk, cudaStream_t stream) {
+  auto kernel = p.pair ? (half ? &ffn_gemm_kernel<kMode, true, kAct, true> : &ffn_gemm_kernel<kMode, false, kAct, true>)
+                       : (half ? &ffn_gemm_kernel<kMode, true, kAct, false> : &ffn_gemm_kernel<kMode, false, kAct, false>);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), p.smem);
   if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.pair ? 2 : 1;
   LaunchScope scope(name, stream);
-  launch_pdl(kernel, p.grid, kThreads, p.smem, stream, ma, mb, mo, mg, p.args);
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, mk, p.args);
 }
 
 template <typename S, typename W, int kAct, bool kGated>
@@ -704,8 +1016,11 @@ cudaError_t reduce_partials(const char* name, const float* partial, int splits, 
   return by_type(type, [&](auto o) {
     using O = decltype(o);
     LaunchScope scope(name, stream);
-    launch_pdl(ffn_reduce_kernel<O>, static_cast<unsigned>((count / 4 + 255) / 256), 256, 0, stream, partial, splits,
-               count, static_cast<O*>(out));
+    const bool many = splits >= 8;
+    const int64_t per_block = many ? 32 : 256;
+    launch_pdl(many ? &ffn_reduce_kernel<O, 8> : &ffn_reduce_kernel<O, 1>,
+               static_cast<unsigned>((count / 4 + per_block - 1) / per_block), 256, 0, stream, partial, splits, count,
+               static_cast<O*>(out));
     return cudaGetLastError();
   });
 }
@@ -762,20 +1077,21 @@ bool ffn_rows_usable(int64_t T, int64_t D, int64_t H) {
 
 cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream_t stream) {
   const bool half = c.type == kFp16;
-  if (c.gu == nullptr && ffn_rows_usable(c.T, c.D, c.H)) {
+  if (c.kept == nullptr && ffn_rows_usable(c.T, c.D, c.H)) {
     if (c.weight_type == kFp32) return half ? forward_rows<__half, float>(c, stream) : forward_rows<__nv_bfloat16, float>(c, stream);
     return half ? forward_rows<__half, __half>(c, stream) : forward_rows<__nv_bfloat16, __nv_bfloat16>(c, stream);
   }
   if (c.weight_type == kFp32) return cudaErrorInvalidValue;
   CUtensorMap ma{}, mb{}, mo{}, mg{};
   {
-    GemmPlan p = plan_gemm(kGate, c.T, c.H, c.D, sm_count);
+    GemmPlan p = plan_gemm(kGate, c.T, c.H, c.D, sm_count, c.kept != nullptr);
     if (!encode_k(&ma, c.x, half, c.T, c.D, kBM) ||
         !encode(&mb, c.w_in, half, c.D, c.H, c.D, 2, c.H * c.D, 0, kBK, p.args.BN / 2, false) ||
-        !encode_out(&mo, c.h, half, c.T, c.H, 1) || !encode_out(&mg, c.gu != nullptr ? c.gu : c.h, half, c.T, c.H, c.gu != nullptr ? 2 : 1)) {
+        !encode_out(&mo, c.h, half, c.T, c.H, 1) ||
+        !encode_out(&mg, c.kept != nullptr ? c.kept : c.h, half, c.T, c.H, c.kept != nullptr ? 2 : 1)) {
       return cudaErrorInvalidValue;
     }
-    p.args.keep_gu = c.gu != nullptr ? 1 : 0;
+    p.args.keep = c.kept != nullptr ? 1 : 0;
     p.args.bias = c.b_in;
     p.args.bias_type = c.bias_type;
     p.args.status = c.status;
@@ -784,7 +1100,7 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
     if (e != cudaSuccess) return e;
   }
   GemmPlan p = plan_gemm(kOutput, c.T, c.D, c.H, sm_count);
-  if (!encode_k(&ma, c.h, half, c.T, c.H, kBM) || !encode_k(&mb, c.w_out, half, c.D, c.H, p.args.BN) ||
+  if (!encode_k(&ma, c.h, half, c.T, c.H, kBM) || !encode_k(&mb, c.w_out, half, c.D, c.H, p.pair ? p.args.BN / 2 : p.args.BN) ||
       !encode_out(&mo, c.y, half, c.T, c.D, 1)) {
     return cudaErrorInvalidValue;
   }
@@ -816,14 +1132,14 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
   if (c.dx == nullptr && c.dw_in == nullptr && c.db_in == nullptr) return cudaSuccess;
   {
     GemmPlan p = plan_gemm(kSlope, c.T, c.H, c.D, sm_count);
+    CUtensorMap mk{};
     if (!encode_k(&ma, c.dy, half, c.T, c.D, kBM) || !encode_mn(&mb, c.w_out, half, c.D, c.H) ||
-        !encode_out(&mo, dgu, half, c.T, c.H, 2)) {
+        !encode_out(&mo, dgu, half, c.T, c.H, 2) || !encode_out(&mk, c.kept, half, c.T, c.H, 2)) {
       return cudaErrorInvalidValue;
     }
-    p.args.gu = c.gu;
     p.args.status = c.status;
-    e = c.activation == kSilu ? launch_gemm<kSlope, kSilu>("ffn_slope", p, half, ma, mb, mo, mo, stream)
-                              : launch_gemm<kSlope, kGelu>("ffn_slope", p, half, ma, mb, mo, mo, stream);
+    e = c.activation == kSilu ? launch_gemm<kSlope, kSilu>("ffn_slope", p, half, ma, mb, mo, mk, stream)
+                              : launch_gemm<kSlope, kGelu>("ffn_slope", p, half, ma, mb, mo, mk, stream);
     if (e != cudaSuccess) return e;
   }
   if (c.dw_in != nullptr) {

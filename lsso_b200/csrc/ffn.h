@@ -21,11 +21,11 @@ struct FfnForwardCall {
   const void* b_in;   // nullable [2H]
   const void* b_out;  // nullable [D]
   int64_t T, D, H;
-  int type;           // element type of x, h, gu, y (and of 16-bit weights)
+  int type;           // element type of x, h, kept, y (and of 16-bit weights)
   int weight_type;    // `type`, or FP32 (row kernels only)
   int bias_type;
   int activation;
-  void* gu;           // nullable [T, 2H]: pre-activations kept for the backward
+  void* kept;         // nullable [T, 2, H]: g and u, for the backward
   void* h;            // [T, H]
   void* y;            // [T, D]
   int* status;
@@ -35,7 +35,7 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
 struct FfnBackwardCall {
   const void* dy;     // [T, D]
   const void* x;
-  const void* gu;
+  const void* kept;
   const void* h;
   const void* w_in;
   const void* w_out;

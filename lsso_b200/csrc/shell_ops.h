@@ -46,9 +46,10 @@ struct EmbeddingCall {
 cudaError_t launch_embedding_forward(const EmbeddingCall& c, int sm_count, cudaStream_t stream);
 
 struct EmbeddingGradPlan {
-  int blocks, tile_rounds;       // sorting blocks; sub-tiles each block takes
-  int passes, bits;              // digit passes, bits per digit
-  int chunk, chunks, slabs;      // sorted positions per warp, their count, column slabs
+  int passes, bits;                // digit passes, bits per digit
+  int items, block_tokens, blocks; // tokens per thread at a time, tokens per block, blocks of the sorting kernels
+  int chunk, chunks;               // sorted tokens summed by one group of lanes
+  size_t count_bytes;              // counts of one pass
   size_t keys[2], order[2], counts, totals, head, tail, total;  // workspace offsets
 };
 EmbeddingGradPlan make_embedding_grad_plan(int64_t tokens, int64_t vocab, int64_t width, int sm_count);
