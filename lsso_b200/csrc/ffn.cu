@@ -15,17 +15,19 @@
 // is what the backward's epilogue reads.
 //
 // Every product is one instance of one persistent, warp-specialised kernel:
-//   warp 0       TMA producer (one lane issues)
-//   warp 1       MMA issuer (one lane issues tcgen05.mma kind::f16)
-//   warps 4-11, 12-19  epilogue of the even and of the odd tiles, two warps per
-//                TMEM sub-partition each (all sixteen on one tile wait for the
-//                same unit at the same time: TMEM, special functions, stores)
+//   warps 0, 2   TMA producers of the row and of the column operand (one thread
+//                each; one thread for both took longer per block than its products)
+//   warp 1       MMA issuer (one thread issues tcgen05.mma kind::f16)
+//   warps 4-19   epilogue, in one group per accumulator (all sixteen on one tile
+//                wait for the same unit at the same time: TMEM, special
+//                functions, stores)
 // CTAs work in pairs (cta_group::2): a tile is 256 rows by up to 256 columns,
 // each CTA holds 128 rows of the row operand and half of the column operand
 // and accumulates its own 128 rows, so shared memory takes 32 KB per 64-wide
 // contraction block instead of the 48 KB that one CTA needs for 128 x 256; up
-// to 128 rows run the same kernel without a partner.  Two TMEM accumulators let
-// the epilogue of one tile run under the products of the next.  Operands are
+// to 128 rows run the same kernel without a partner.  Two TMEM
+// accumulators, or four of up to 128 columns, let the epilogues of some tiles
+// run under the products of the next.  Operands are
 // read where the caller keeps them: the contraction axis may be the inner one
 // (K-major boxes) or the outer one (MN-major boxes), so no weight or activation
 // is ever transposed in memory.  The two forward projections share a tile (the
@@ -54,6 +56,7 @@ constexpr int kMaxStages = 8;
 constexpr int kThreads = 640;
 constexpr int kEpiWarp0 = 4;
 constexpr int kEpiWarps = 16;
+constexpr int kMaxBuffers = 4;
 constexpr uint32_t kBox = 64 * 64 * 2;            // MN-major box: 64 contraction rows x 128 bytes
 constexpr uint32_t kABytes = kBM * kBK * 2;       // 16 KB
 constexpr uint32_t kOutBox = 32 * 32 * 2;         // output box: 32 rows x 32 columns of 16 bits
@@ -73,6 +76,7 @@ struct GemmArgs {
   int mtiles, ntiles, units, splits, kb_per_split, stages;
   int step_n, step_m;  // a worker's step to its next unit, in n tiles and m tiles
   int boxes;           // output boxes of one epilogue warp
+  int rev;             // m tiles from the last to the first (the rows the kernel before wrote last are in L2)
   int keep, bias_type;
   const void* bias;    // kGate: [2N], kOutput: [N]; nullable
   void* out;           // kWeight: gradient (splits == 1) or FP32 partials [splits][M][N]
@@ -104,6 +108,13 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// Without the release of this CTA's earlier stores (a wait for every
+// outstanding global store); what the partner must see is fenced by its writer.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;\n" ::: "memory"); }
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
 }
@@ -257,26 +268,15 @@ __device__ __forceinline__ void box_write(uint8_t* box, int lane, const float (&
                                           pack2<kHalf>(v[j + 4], v[j + 5]), pack2<kHalf>(v[j + 6], v[j + 7]));
   }
 }
-// [dg | du] from dh and the kept pre-activations, in their place.
-template <bool kHalf, int kAct>
-__device__ __forceinline__ void box_slope(uint8_t* gbox, uint8_t* ubox, int lane, const float (&dh)[32]) {
+template <bool kHalf>
+__device__ __forceinline__ void box_read(uint8_t* box, int lane, uint32_t (&w)[16]) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint4 *pg = box_piece(gbox, lane, c), *pu = box_piece(ubox, lane, c);
-    const uint4 gq = *pg, uq = *pu;
-    const uint32_t gw[4] = {gq.x, gq.y, gq.z, gq.w}, uw[4] = {uq.x, uq.y, uq.z, uq.w};
-    uint32_t dg[4], du[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 g = unpack2<kHalf>(gw[k]), u = unpack2<kHalf>(uw[k]);
-      ActSlope s0, s1;
-      activate2<kAct>(g.x, g.y, s0, s1);
-      const float d0 = dh[8 * c + 2 * k], d1 = dh[8 * c + 2 * k + 1];
-      dg[k] = pack2<kHalf>(d0 * u.x * s0.slope, d1 * u.y * s1.slope);
-      du[k] = pack2<kHalf>(d0 * s0.act, d1 * s1.act);
-    }
-    *pg = make_uint4(dg[0], dg[1], dg[2], dg[3]);
-    *pu = make_uint4(du[0], du[1], du[2], du[3]);
+    const uint4 q = *box_piece(box, lane, c);
+    w[4 * c] = q.x;
+    w[4 * c + 1] = q.y;
+    w[4 * c + 2] = q.z;
+    w[4 * c + 3] = q.w;
   }
 }
 
@@ -348,6 +348,10 @@ struct UnitWalk {
       ++split;
     }
   }
+  __device__ __forceinline__ int m_tile(const GemmArgs& a) const { return a.rev ? a.mtiles - 1 - mt : mt; }
+  __device__ __forceinline__ void skip(const GemmArgs& a, int step, int count) {
+    for (int i = 0; i < count; ++i) next(a, step);
+  }
 };
 
 template <int kMode, bool kHalf, int kAct, bool kPair>
@@ -360,11 +364,12 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   constexpr bool kBmn = kMode == kSlope || kMode == kInput || kMode == kWeight;
   constexpr int kCtas = kPair ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2], mdrain;
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], tfull[kMaxBuffers], tempty[kMaxBuffers], mdrain;
   __shared__ __align__(8) uint64_t kept[kMode == kSlope ? kEpiWarps : 1];
   __shared__ uint32_t tmem_s;
   __shared__ int abort_flag;
-  __shared__ int peer_last[kMaxStages];  // pair leader: the partner's last use of each stage
+  __shared__ int issued[2][kMaxStages];       // the use of each stage that a producer issued last
+  __shared__ int peer_issued[2][kMaxStages];  // pair leader: the partner's
   __shared__ __align__(16) float sbias[kEpiWarps][32];
   volatile int* abort_v = &abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -373,7 +378,8 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   const int S = a.stages;
   const int BN = a.BN, BNL = BN / kCtas;  // accumulator columns; columns of the operand this CTA holds
   const uint32_t stage_bytes = kABytes + static_cast<uint32_t>(BNL) * 128;
-  const uint32_t tcols = tmem_cols_for(2 * BN);
+  const int nbuf = BN > 128 ? 2 : kMaxBuffers;   // accumulators, and epilogue groups
+  const uint32_t tcols = tmem_cols_for(nbuf * BN);
   const int span = kMode == kGate ? BN / 2 : BN;  // output columns per tile
 
   if (threadIdx.x == 0) {
@@ -381,9 +387,9 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < nbuf; ++b) {
       mbar_init(smem_u32(&tfull[b]), 1);
-      mbar_init(smem_u32(&tempty[b]), kEpiWarps / 2 * kCtas);
+      mbar_init(smem_u32(&tempty[b]), kEpiWarps / nbuf * kCtas);
     }
     mbar_init(smem_u32(&mdrain), 1);
     if (kMode == kSlope) {
@@ -398,101 +404,105 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   if (kPair) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
-  int last_use[kMaxStages];  // producer's lane 0: the use of each stage whose loads were issued last
+  const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(full), empty_base = smem_u32(empty);
 
-  if (warp == 0) {
-    // ---------------- producer
+  if (warp == 0 || warp == 2) {
+    // ---------------- producers: warp 0 the row operand, warp 2 the column operand
     if (lane == 0) {
-      prefetch_tmap(&tmap_a);
-      prefetch_tmap(&tmap_b);
-    }
-    RingPos rp;
-    bool ok = true;
-    for (int s = 0; s < kMaxStages; ++s) last_use[s] = -1;
-    for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step)) {
-      const int nt = w.nt, mt = w.mt, split = w.split;
-      const int m0 = (mt * kCtas + static_cast<int>(rank)) * kBM;
-      const int n0 = nt * BN + static_cast<int>(rank) * BNL;
-      const int kb1 = min(a.KB, (split + 1) * a.kb_per_split);
-      for (int kb = split * a.kb_per_split; kb < kb1 && ok; ++kb, rp.next(S)) {
-        const int s = rp.s;
-        ok = fwait(smem_u32(&empty[s]), (rp.u & 1) ^ 1, abort_v, a.status);
-        if (ok && lane == 0) {
-          const uint32_t own_bar = smem_u32(&full[s]);
-          const uint32_t bar = kPair ? map_rank(own_bar, 0) : own_bar;
-          const uint32_t dst = smem_u32(smem + s * stage_bytes);
-          const uint32_t bdst = dst + kABytes;
-          if (rank == 0) mbar_arrive_expect_tx(own_bar, kCtas * stage_bytes);
-          if (kAmn) {
-            load_2d<kPair>(dst, &tmap_a, m0, kb * kBK, bar);
-            load_2d<kPair>(dst + kBox, &tmap_a, m0 + 64, kb * kBK, bar);
-          } else {
-            load_2d<kPair>(dst, &tmap_a, kb * kBK, m0, bar);
-          }
-          if (kMode == kGate) {
-            // columns [0, span) are the gate rows, [span, 2 span) the up rows: one plane per CTA of a pair
-            load_3d<kPair>(bdst, &tmap_b, kb * kBK, nt * span, static_cast<int>(rank), bar);
-            if (!kPair) load_3d<kPair>(bdst + static_cast<uint32_t>(span) * 128, &tmap_b, kb * kBK, nt * span, 1, bar);
-          } else if (kBmn) {
-            for (int g = 0; g < BNL / 64; ++g) load_2d<kPair>(bdst + g * kBox, &tmap_b, n0 + g * 64, kb * kBK, bar);
-          } else {
-            load_2d<kPair>(bdst, &tmap_b, kb * kBK, n0, bar);
-          }
-          last_use[s] = rp.u;
+      const int operand = warp >> 1;
+      prefetch_tmap(operand == 0 ? &tmap_a : &tmap_b);
+      int* mine = issued[operand];
+      for (int s = 0; s < S; ++s) mine[s] = -1;
+      const uint32_t full_bar = kPair ? map_rank(full_base, 0) : full_base;  // both CTAs' loads complete on the leader's
+      RingPos rp;
+      bool ok = true;
+      auto load_b = [&](uint32_t bdst, int nt, int kb, uint32_t bar) {
+        const int n0 = nt * BN + static_cast<int>(rank) * BNL;
+        if (kMode == kGate) {
+          // columns [0, span) are the gate rows, [span, 2 span) the up rows: one plane per CTA of a pair
+          load_3d<kPair>(bdst, &tmap_b, kb * kBK, nt * span, static_cast<int>(rank), bar);
+          if (!kPair) load_3d<kPair>(bdst + static_cast<uint32_t>(span) * 128, &tmap_b, kb * kBK, nt * span, 1, bar);
+        } else if (kBmn) {
+          for (int g = 0; g < BNL / 64; ++g) load_2d<kPair>(bdst + g * kBox, &tmap_b, n0 + g * 64, kb * kBK, bar);
+        } else {
+          load_2d<kPair>(bdst, &tmap_b, kb * kBK, n0, bar);
         }
-        __syncwarp();
+      };
+      for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step)) {
+        const int m0 = (w.m_tile(a) * kCtas + static_cast<int>(rank)) * kBM;
+        const int kb1 = min(a.KB, (w.split + 1) * a.kb_per_split);
+        for (int kb = w.split * a.kb_per_split; kb < kb1; ++kb, rp.next(S)) {
+          const int s = rp.s;
+          ok = fwait(empty_base + 8 * s, (rp.u & 1) ^ 1, abort_v, a.status);
+          if (!ok) break;
+          const uint32_t bar = full_bar + 8 * s;
+          const uint32_t dst = smem_base + s * stage_bytes;
+          if (operand == 0) {
+            if (rank == 0) mbar_arrive_expect_tx(full_base + 8 * s, kCtas * stage_bytes);
+            if (kAmn) {
+              load_2d<kPair>(dst, &tmap_a, m0, kb * kBK, bar);
+              load_2d<kPair>(dst + kBox, &tmap_a, m0 + 64, kb * kBK, bar);
+            } else {
+              load_2d<kPair>(dst, &tmap_a, kb * kBK, m0, bar);
+            }
+          } else {
+            load_b(dst + kABytes, w.nt, kb, bar);
+          }
+          mine[s] = rp.u;
+        }
       }
-    }
-    if (kPair && rank == 1 && lane == 0) {
-      for (int s = 0; s < S; ++s) store_remote(map_rank(smem_u32(&peer_last[s]), 0), last_use[s]);
+      if (kPair && rank == 1) {
+        for (int s = 0; s < S; ++s) store_remote(map_rank(smem_u32(&peer_issued[operand][s]), 0), mine[s]);
+        fence_cluster();
+      }
     }
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer (of a pair: the leader's)
-    if (rank == 0) {
+    if (rank == 0 && lane == 0) {
       // kind::f16 operand format bits: BF16 as set by make_idesc, FP16 as zero
       const uint32_t idesc = make_idesc(kBM * kCtas, BN, kAmn, kBmn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
-      RingPos rp;
+      // descriptors of stage 0; a stage and a 16-wide contraction step add to the address field (units of 16 bytes)
+      const uint64_t adesc = kAmn ? make_desc_sw128(smem_base, kBox, 1024) : make_desc_sw128(smem_base, 16, 1024);
+      const uint64_t bdesc = kBmn ? make_desc_sw128(smem_base + kABytes, kBox, 1024)
+                                  : make_desc_sw128(smem_base + kABytes, 16, 1024);
+      constexpr uint32_t kAStep = kAmn ? 2048 / 16 : 32 / 16, kBStep = kBmn ? 2048 / 16 : 32 / 16;
+      const uint32_t tfull_base = smem_u32(tfull), tempty_base = smem_u32(tempty);
+      RingPos rp, tp;  // stages, accumulators
       bool ok = true;
-      int i = 0;
-      for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step), ++i) {
+      for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step), tp.next(nbuf)) {
         const int kb0 = w.split * a.kb_per_split, kb1 = min(a.KB, kb0 + a.kb_per_split);
-        const int b = i & 1;
-        ok = fwait(smem_u32(&tempty[b]), ((i >> 1) & 1) ^ 1, abort_v, a.status);
+        ok = fwait(tempty_base + 8 * tp.s, (tp.u & 1) ^ 1, abort_v, a.status);
         tc_fence_after();
-        const uint32_t d = tmem + static_cast<uint32_t>(b * BN);
+        const uint32_t d = tmem + static_cast<uint32_t>(tp.s * BN);
         for (int kb = kb0; kb < kb1 && ok; ++kb, rp.next(S)) {
           const int s = rp.s;
-          ok = fwait(smem_u32(&full[s]), rp.u & 1, abort_v, a.status);
+          ok = fwait(full_base + 8 * s, rp.u & 1, abort_v, a.status);
+          if (!ok) break;
           tc_fence_after();
-          if (ok && lane == 0) {
-            const uint32_t sa = smem_u32(smem + s * stage_bytes), sb = sa + kABytes;
+          const uint32_t off = static_cast<uint32_t>(s) * (stage_bytes / 16);
 #pragma unroll
-            for (int ks = 0; ks < kBK / 16; ++ks) {
-              const uint64_t ad = kAmn ? make_desc_sw128(sa + ks * 2048, kBox, 1024) : make_desc_sw128(sa + ks * 32, 16, 1024);
-              const uint64_t bd = kBmn ? make_desc_sw128(sb + ks * 2048, kBox, 1024) : make_desc_sw128(sb + ks * 32, 16, 1024);
-              mma<kPair>(d, ad, bd, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
-            }
-            commit_all<kPair>(smem_u32(&empty[s]));
+          for (int ks = 0; ks < kBK / 16; ++ks) {
+            mma<kPair>(d, adesc + off + ks * kAStep, bdesc + off + ks * kBStep, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
           }
-          __syncwarp();
+          commit_all<kPair>(empty_base + 8 * s);
         }
-        if (ok && lane == 0) commit_all<kPair>(smem_u32(&tfull[b]));
-        __syncwarp();
+        if (ok) commit_all<kPair>(tfull_base + 8 * tp.s);
       }
       // no tensor-core operation still writes TMEM or reads shared memory past this point
-      if (lane == 0) {
-        commit_own<kPair>(smem_u32(&mdrain));
-        mbar_wait_bounded(smem_u32(&mdrain), 0, nullptr, a.status);
-      }
+      commit_own<kPair>(smem_u32(&mdrain));
+      mbar_wait_bounded(smem_u32(&mdrain), 0, nullptr, a.status);
     }
     __syncwarp();
   } else if (warp >= kEpiWarp0) {
     // ---------------- epilogue
     const int ew = warp - kEpiWarp0;
     const int sub = warp & 3;
-    const int b = ew >> 3;                  // the tiles of this group: accumulator b
-    const int col0 = 32 * ((ew >> 2) & 1);  // first column of this warp's pieces within a tile; the next are 64 on
+    // This warp's group takes every nbuf-th tile, in accumulator b; its pieces
+    // of a tile are 32 columns wide, from col0 on, col_step apart.
+    const int members = kEpiWarps / nbuf;
+    const int b = ew / members;
+    const int col0 = 32 * ((ew % members) >> 2), col_step = 8 * members;
     const int row_base = static_cast<int>(rank) * kBM + 32 * sub;
     uint8_t* stage = smem + S * stage_bytes + ew * a.boxes * kOutBox;
     float* scratch = sbias[ew];
@@ -501,17 +511,16 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     int ahead_c = col0, loaded = 0, piece = 0;
     // Loads the kept pre-activations of the next piece of this warp that lies in the output, if there is one.
     auto load_kept = [&]() {
-      for (; ahead.unit < a.units; ahead.next(a, unit_step), ahead.next(a, unit_step), ahead_c = col0) {
-        const int r0 = ahead.mt * kBM * kCtas + row_base, n0 = ahead.nt * span + ahead_c;
+      for (; ahead.unit < a.units; ahead.skip(a, unit_step, nbuf), ahead_c = col0) {
+        const int r0 = ahead.m_tile(a) * kBM * kCtas + row_base, n0 = ahead.nt * span + ahead_c;
         if (r0 >= a.M || ahead_c >= span || n0 >= a.N) continue;
         if (lane == 0) {
-          bulk_wait_read<0>();  // the stores from the boxes, one piece ago
           mbar_arrive_expect_tx(kbar, 2 * kOutBox);
           tma_load_3d(smem_u32(stage), &tmap_keep, n0, 0, r0, kbar);
           tma_load_3d(smem_u32(stage + kOutBox), &tmap_keep, n0, 1, r0, kbar);
         }
         ++loaded;
-        ahead_c += 64;
+        ahead_c += col_step;
         break;
       }
       __syncwarp();
@@ -536,11 +545,11 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     };
     bool ok = true;
     int i = 0;
-    for (; w.unit < a.units && ok; w.next(a, unit_step), w.next(a, unit_step), ++i) {
+    for (; w.unit < a.units && ok; w.skip(a, unit_step, nbuf), ++i) {
       ok = fwait_warp(smem_u32(&tfull[b]), i & 1, abort_v, a.status);
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(32 * sub) << 16) + static_cast<uint32_t>(b * BN);
-      const int row0 = w.mt * kBM * kCtas + row_base;
+      const int row0 = w.m_tile(a) * kBM * kCtas + row_base;
       const int columns = row0 < a.M ? min(span, a.N - w.nt * span) : 0;  // of this tile that lie in the output
       // This warp's last values of the tile are in registers: its accumulator may be overwritten.
       auto release = [&]() {
@@ -555,9 +564,9 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
       };
       if (!ok || col0 >= columns) release();
-      for (int c = col0; c < columns && ok; c += 64, ++piece) {
+      for (int c = col0; c < columns && ok; c += col_step, ++piece) {
         const int n0 = w.nt * span + c;
-        const bool last = c + 64 >= columns;
+        const bool last = c + col_step >= columns;
         float v[32];
         tmem_ld32(acc + c, v);
         if (kMode == kGate) {
@@ -571,6 +580,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           }
           boxes_free();
           if (a.keep) {
+            // stored before the activation, which runs meanwhile
             const bool apart = a.boxes == 3;
             box_write<kHalf>(stage + (apart ? kOutBox : 0), lane, v);
             if (apart) box_write<kHalf>(stage + 2 * kOutBox, lane, u);
@@ -599,15 +609,34 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             if (!last) release();
             break;
           }
-          box_slope<kHalf, kAct>(stage, stage + kOutBox, lane, v);
-          fence_proxy_async();
+          // g and u to registers, so that the next piece's loads run under this one's arithmetic
+          uint32_t g[16], u[16];
+          box_read<kHalf>(stage, lane, g);
+          box_read<kHalf>(stage + kOutBox, lane, u);
           __syncwarp();
-          if (lane == 0) {
-            tma_store_3d(&tmap_out, smem_u32(stage), n0, 0, row0);
-            tma_store_3d(&tmap_out, smem_u32(stage + kOutBox), n0, 1, row0);
-            bulk_commit();
-          }
           load_kept();
+          boxes_free();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t dg[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int j = 4 * q + k;
+              const float2 g2 = unpack2<kHalf>(g[j]), u2 = unpack2<kHalf>(u[j]);
+              ActSlope s0, s1;
+              activate2<kAct>(g2.x, g2.y, s0, s1);
+              dg[k] = pack2<kHalf>(v[2 * j] * u2.x * s0.slope, v[2 * j + 1] * u2.y * s1.slope);
+              u[j] = pack2<kHalf>(v[2 * j] * s0.act, v[2 * j + 1] * s1.act);  // du
+            }
+            *box_piece(stage + 2 * kOutBox, lane, q) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+          }
+          store_box(&tmap_out, 2, n0, 0, row0);
+          boxes_free();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            *box_piece(stage + 2 * kOutBox, lane, q) = make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
+          }
+          store_box(&tmap_out, 2, n0, 1, row0);
         } else {
           tmem_ld_wait();
           if (last) release();
@@ -624,7 +653,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       }
     }
     if (lane == 0) {
-      bulk_wait<0>();
+      bulk_wait_read<0>();  // shared memory may go; the writes complete with the grid
       // loads still on their way (only after an abort): wait for them, bounded
       if (kMode == kSlope) {
         if (piece < loaded) mbar_wait(kbar, static_cast<uint32_t>(piece) & 1u, a.status);
@@ -635,52 +664,64 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
   tc_fence_before();
   __syncthreads();
-  if (kPair) cluster_sync();
-  // Loads still in flight (only after an abort): wait for them, bounded.  Both
-  // CTAs' loads complete on the leader's barriers; where one CTA issued a use
-  // of a stage that the other did not, the leader supplies the missing arrival
-  // or bytes first, so that the phase completes when the issued loads have landed.
+  if (kPair) cluster_sync_relaxed();
+  // Loads still in flight (only after an abort): wait for them, bounded.  All
+  // loads of a stage complete on the leader's barrier; where one producer
+  // issued a use that another did not, the leader supplies the missing arrival
+  // and bytes, so that the phase completes when the issued loads have landed.
+  // (A use starts only after every producer issued the one before it.)
   if (warp == 0 && lane == 0 && rank == 0) {
     for (int s = 0; s < S; ++s) {
-      const uint32_t bar = smem_u32(&full[s]);
-      int last = last_use[s];
-      if (kPair && peer_last[s] > last) {
-        last = peer_last[s];
-        mbar_arrive_expect_tx(bar, stage_bytes);
-      } else if (kPair && peer_last[s] < last) {
-        complete_tx(bar, stage_bytes);
-      }
-      if (last >= 0) mbar_wait(bar, static_cast<uint32_t>(last) & 1u, a.status);
+      const int own_a = issued[0][s], own_b = issued[1][s];
+      const int peer_a = kPair ? peer_issued[0][s] : own_a, peer_b = kPair ? peer_issued[1][s] : own_b;
+      const int last = max(max(own_a, own_b), max(peer_a, peer_b));
+      if (last < 0) continue;
+      const uint32_t bar = full_base + 8 * s;
+      if (own_a < last) mbar_arrive_expect_tx(bar, kCtas * stage_bytes);
+      uint32_t missing = (own_a < last ? kABytes : 0u) + (own_b < last ? stage_bytes - kABytes : 0u);
+      if (kPair) missing += (peer_a < last ? kABytes : 0u) + (peer_b < last ? stage_bytes - kABytes : 0u);
+      if (missing != 0) complete_tx(bar, missing);
+      mbar_wait(bar, static_cast<uint32_t>(last) & 1u, a.status);
     }
   }
   __syncthreads();
-  if (kPair) cluster_sync();
+  if (kPair) cluster_sync_relaxed();
   if (warp == 1) {
     tc_fence_after();
     free_tmem<kPair>(tmem, tcols);
   }
 }
 
-// Sum of per-split partials: kGroups warps take every kGroups-th split, their
-// sums are added in group order (the same order in every run).  One group for
-// few splits (a large array), eight for many.
+// Sums of per-split partials, up to four arrays in one launch (both weight and
+// both bias gradients).  An array of many splits has eight warps take every
+// eighth split, their sums added in warp order; one of few has a thread take
+// all.  The order depends on the split count alone.
+struct ReduceArray {
+  const float* partial;
+  void* out;
+  int64_t count;  // a multiple of 8
+  int splits, first_block;
+};
+struct ReduceBatch {
+  ReduceArray array[4];
+  int arrays, blocks;
+};
+
 template <typename O, int kGroups>
-__global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ partial, int splits, int64_t count,
-                                                         O* __restrict__ out) {
-  pdl_wait();
-  __shared__ float4 part[kGroups][32];
+__device__ __forceinline__ void reduce_array(const ReduceArray& a, int64_t block, float4 (*part)[32]) {
   const int group = kGroups == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t i = (static_cast<int64_t>(blockIdx.x) * (256 / kGroups) + (kGroups == 1 ? threadIdx.x : lane)) * 4;
-  // count is a multiple of 8
-  const int64_t at = i < count ? i : 0;
+  const int64_t i = (block * (256 / kGroups) + (kGroups == 1 ? threadIdx.x : lane)) * 4;
+  const int64_t at = i < a.count ? i : 0;
   float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = group; s < splits; s += 4 * kGroups) {
+  for (int s = group; s < a.splits; s += 4 * kGroups) {
     float4 v[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = __ldg(reinterpret_cast<const float4*>(partial + min(s + kGroups * q, splits - 1) * count + at));
+    for (int q = 0; q < 4; ++q) {
+      v[q] = __ldg(reinterpret_cast<const float4*>(a.partial + min(s + kGroups * q, a.splits - 1) * a.count + at));
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (s + kGroups * q >= splits) continue;
+      if (s + kGroups * q >= a.splits) continue;
       sum.x += v[q].x;
       sum.y += v[q].y;
       sum.z += v[q].z;
@@ -700,41 +741,74 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict
       sum.w += p.w;
     }
   }
-  if (i >= count) return;
+  if (i >= a.count) return;
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-  store_run<O, 4>(out + i, v);
+  store_run<O, 4>(static_cast<O*>(a.out) + i, v);
 }
 
-// Column sums of a 16-bit [rows, cols] matrix (the bias gradients): each block
-// sums a run of rows for 256 columns in FP32 and the second kernel adds the
-// blocks' sums in order.
+constexpr int kManySplits = 8;
+
+template <typename O>
+__global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__ ReduceBatch batch) {
+  pdl_wait();
+  __shared__ float4 part[8][32];
+  int k = 0;
+  while (k + 1 < batch.arrays && static_cast<int>(blockIdx.x) >= batch.array[k + 1].first_block) ++k;
+  const ReduceArray& a = batch.array[k];
+  const int64_t block = static_cast<int64_t>(blockIdx.x) - a.first_block;
+  if (a.splits >= kManySplits) {
+    reduce_array<O, 8>(a, block, part);
+  } else {
+    reduce_array<O, 1>(a, block, part);
+  }
+}
+
+// Column sums of 16-bit [rows, cols] matrices (the bias gradients, up to two in
+// one launch): each block sums a run of rows for 256 columns in FP32 and the
+// reduction adds the blocks' sums in order.
+struct ColsumArray {
+  const uint16_t* in;
+  float* partial;  // [gridDim.y][cols]
+  int cols, column_blocks;
+};
+
 template <bool kHalf>
-__global__ void __launch_bounds__(256) ffn_colsum_kernel(const uint16_t* __restrict__ in, int64_t rows, int cols,
-                                                         int64_t rows_per_block, float* __restrict__ partial) {
+__global__ void __launch_bounds__(256) ffn_colsum_kernel(const ColsumArray first, const ColsumArray second, int64_t rows,
+                                                         int64_t rows_per_block) {
   pdl_wait();
   __shared__ float part[8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = blockIdx.x * 256 + lane * 8;
+  const bool in_first = static_cast<int>(blockIdx.x) < first.column_blocks;
+  const uint16_t* __restrict__ in = in_first ? first.in : second.in;
+  float* __restrict__ partial = in_first ? first.partial : second.partial;
+  const int cols = in_first ? first.cols : second.cols;
+  const int col_block = static_cast<int>(blockIdx.x) - (in_first ? 0 : first.column_blocks);
+  const int col = col_block * 256 + lane * 8;
   const int64_t begin = static_cast<int64_t>(blockIdx.y) * rows_per_block;
   const int64_t end = min(rows, begin + rows_per_block);
   float acc[8] = {};
   if (col < cols) {
-#pragma unroll 4
-    for (int64_t r = begin + warp; r < end; r += 8) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(in + r * cols + col));
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    for (int64_t r = begin + warp; r < end; r += 64) {
+      uint4 q[8];  // eight rows in flight
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float2 f = unpack2<kHalf>(w[p]);
-        acc[2 * p] += f.x;
-        acc[2 * p + 1] += f.y;
+      for (int i = 0; i < 8; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(in + min(r + 8 * i, end - 1) * cols + col));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (r + 8 * i >= end) continue;
+        const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const float2 f = unpack2<kHalf>(w[p]);
+          acc[2 * p] += f.x;
+          acc[2 * p + 1] += f.y;
+        }
       }
     }
   }
 #pragma unroll
   for (int k = 0; k < 8; ++k) part[warp][lane * 8 + k] = acc[k];
   __syncthreads();
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int c = col_block * 256 + threadIdx.x;
   if (c >= cols) return;
   float sum = 0.0f;
 #pragma unroll
@@ -829,42 +903,53 @@ struct GemmPlan {
   size_t smem;
 };
 
+constexpr int64_t kShort = 8;  // contraction blocks below which a gate tile is bound by its epilogue
+
 // Output boxes of one epilogue warp.  kGate with kept pre-activations: h, g and
 // u apart (96 KB, four stages) while a tile is short and its stores set the
 // pace; one box in turn for all three (32 KB, six stages) from eight
-// contraction blocks on, where loads in flight do.  kSlope: g and u in, dg and
-// du out in their place.
+// contraction blocks on, where loads in flight do.  kSlope: g and u in, one out
+// for dg and du in turn.
 int boxes_of(Mode mode, bool keep, int64_t KB) {
-  return mode == kWeight ? 0 : mode == kSlope ? 2 : mode == kGate && keep && KB < 8 ? 3 : 1;
+  return mode == kWeight ? 0 : mode == kSlope || (mode == kGate && keep && KB < kShort) ? 3 : 1;
 }
 
-// Pairs or single CTAs, tile width and token split.  The estimate counts
-// tensor-core cycles: rounds x (contraction blocks x (2 columns + a fixed cost
-// per block) + a fixed cost per tile); a single CTA's tile is held back by
-// shared-memory bandwidth.  Wide tiles reuse the row operand more, narrow ones
-// fill the SMs when there are few.
+// Pairs or single CTAs, tile width and token split.  The estimate is in SM
+// cycles: rounds x (contraction blocks x max(products, loads) + 2000).  Loads:
+// an SM takes in at most 62 bytes per cycle (measured; 50 assumed), so a
+// pair's 256 x 256 block takes 640 cycles against 512 of products, and a
+// narrower pair tile no fewer of products; 2000 is what a tile costs to start
+// and drain.  Token splits add the traffic of their partials.  (Keeping the
+// column operand of one n tile in shared memory, so that a short contraction
+// streams its rows only, was slower: slope kernel at 64 x 4096 tokens, 256 ->
+// 688, 295 -> 342 us; gate kernel 291 -> 287.)
 GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, bool keep = false) {
   GemmPlan best{};
   double best_cost = 0.0;
   const int64_t KB = (K + kBK - 1) / kBK;
+  const int boxes = boxes_of(mode, keep, KB);
+  const int64_t staging = kEpiWarps * boxes * static_cast<int64_t>(kOutBox);
   for (int pair = 1; pair >= 0; --pair) {
     if (pair && M <= kBM) continue;
-    const int64_t rows = kBM * (pair ? 2 : 1);
-    const int64_t mtiles = (M + rows - 1) / rows;
-    const int64_t workers = pair ? sm_count / 2 : sm_count;
+    const int ctas = pair ? 2 : 1;
+    const int64_t mtiles = (M + kBM * ctas - 1) / (kBM * ctas);
+    const int64_t workers = sm_count / ctas;
     for (int bn = 256; bn >= 64; bn -= pair ? 128 : 64) {
       const int span = mode == kGate ? bn / 2 : bn;
       const int64_t ntiles = (N + span - 1) / span;
-      const int64_t tiles = mtiles * ntiles;
+      const int64_t stage = kABytes + static_cast<int64_t>(bn) * 128 / ctas;
+      const int64_t stages = std::min<int64_t>(kMaxStages, (static_cast<int64_t>(kSmemMost) - staging) / stage);
       const int64_t most_splits = mode == kWeight ? std::min<int64_t>(KB, 64) : 1;
       for (int64_t want = 1; want <= most_splits; ++want) {
         const int64_t per = (KB + want - 1) / want;
         const int64_t splits = (KB + per - 1) / per;
         if (splits != want) continue;
-        const int64_t units = tiles * splits;
-        const int64_t rounds = (units + workers - 1) / workers;
-        double cost = static_cast<double>(rounds) * (per * ((pair ? 2.0 : 2.7) * bn + 64.0) + 1000.0);
-        if (splits > 1) cost += splits * static_cast<double>(M) * N / 512.0;  // partials written and read
+        const int64_t units = mtiles * ntiles * splits;
+        const int64_t used = std::min(units, workers);
+        const int64_t rounds = (units + used - 1) / used;
+        const double block = std::max(pair ? 512.0 : 2.0 * bn, stage / 50.0);
+        double cost = static_cast<double>(rounds) * (per * block + 2000.0);
+        if (splits > 1) cost += 4000.0 + splits * static_cast<double>(M) * N / 425.0;
         if (best.grid != 0 && cost >= best_cost) continue;
         best_cost = cost;
         GemmArgs a{};
@@ -877,17 +962,15 @@ GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, boo
         a.units = static_cast<int>(units);
         a.splits = static_cast<int>(splits);
         a.kb_per_split = static_cast<int>(per);
-        a.step_n = static_cast<int>(std::min(units, workers) % ntiles);
-        a.step_m = static_cast<int>(std::min(units, workers) / ntiles);
-        a.boxes = boxes_of(mode, keep, KB);
-        const size_t stage = kABytes + static_cast<size_t>(bn) * (pair ? 64 : 128);
-        const size_t staging = static_cast<size_t>(kEpiWarps) * a.boxes * kOutBox;
-        a.stages = static_cast<int>((kSmemMost - staging) / stage);
-        if (a.stages > kMaxStages) a.stages = kMaxStages;
+        a.step_n = static_cast<int>(used % ntiles);
+        a.step_m = static_cast<int>(used / ntiles);
+        a.boxes = boxes;
+        a.stages = static_cast<int>(stages);
+        a.rev = mode == kOutput || mode == kInput ? 1 : 0;
         best.args = a;
         best.pair = pair;
-        best.grid = static_cast<int>(units < workers ? units : workers) * (pair ? 2 : 1);
-        best.smem = a.stages * stage + staging;
+        best.grid = static_cast<int>(used) * ctas;
+        best.smem = static_cast<size_t>(stages * stage + staging);
       }
     }
   }
@@ -980,27 +1063,34 @@ cudaError_t forward_rows(const FfnForwardCall& c, cudaStream_t stream) {
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-constexpr int kColsumBlocks = 296;  // row runs of the column sums, per 256 columns at most
-
-int64_t colsum_splits(int64_t rows, int64_t cols) {
-  const int64_t column_blocks = (cols + 255) / 256;
-  return std::max<int64_t>(1, std::min<int64_t>((rows + 63) / 64, kColsumBlocks / column_blocks));
+// Row runs of the column sums: two blocks per SM over all columns.
+int64_t colsum_splits(int64_t rows, int64_t D, int64_t H, int sm_count) {
+  const int64_t column_blocks = (2 * H + 255) / 256 + (D + 255) / 256;
+  return std::max<int64_t>(1, std::min<int64_t>((rows + 63) / 64, 2 * sm_count / column_blocks));
 }
 
 struct BackwardLayout {
-  size_t dgu, partial, total;
+  GemmPlan w_in, w_out;
+  int64_t colsums;
+  size_t dgu, p_w_in, p_w_out, p_b_in, p_b_out, total;  // p_*: partials
 };
 BackwardLayout backward_layout(int64_t T, int64_t D, int64_t H, int sm_count) {
-  const GemmPlan in = plan_gemm(kWeight, 2 * H, D, T, sm_count), out = plan_gemm(kWeight, D, H, T, sm_count);
-  size_t partial = 0;
-  if (in.args.splits > 1) partial = sizeof(float) * in.args.splits * 2 * H * D;
-  if (out.args.splits > 1) partial = std::max(partial, sizeof(float) * out.args.splits * D * H);
-  partial = std::max(partial, sizeof(float) * static_cast<size_t>(colsum_splits(T, 2 * H) * 2 * H));
-  partial = std::max(partial, sizeof(float) * static_cast<size_t>(colsum_splits(T, D) * D));
   BackwardLayout l{};
-  l.dgu = 0;
-  l.partial = align256(sizeof(uint16_t) * T * 2 * H);
-  l.total = l.partial + align256(partial);
+  l.w_in = plan_gemm(kWeight, 2 * H, D, T, sm_count);
+  l.w_out = plan_gemm(kWeight, D, H, T, sm_count);
+  l.colsums = colsum_splits(T, D, H, sm_count);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = align256(off + bytes);
+    return at;
+  };
+  l.dgu = take(sizeof(uint16_t) * T * 2 * H);
+  l.p_w_in = take(l.w_in.args.splits > 1 ? sizeof(float) * l.w_in.args.splits * 2 * H * D : 0);
+  l.p_w_out = take(l.w_out.args.splits > 1 ? sizeof(float) * l.w_out.args.splits * D * H : 0);
+  l.p_b_in = take(sizeof(float) * l.colsums * 2 * H);
+  l.p_b_out = take(sizeof(float) * l.colsums * D);
+  l.total = off;
   return l;
 }
 
@@ -1011,46 +1101,22 @@ cudaError_t by_type(int type, F&& f) {
   return f(float());
 }
 
-cudaError_t reduce_partials(const char* name, const float* partial, int splits, int64_t count, void* out, int type,
-                            cudaStream_t stream) {
-  return by_type(type, [&](auto o) {
-    using O = decltype(o);
-    LaunchScope scope(name, stream);
-    const bool many = splits >= 8;
-    const int64_t per_block = many ? 32 : 256;
-    launch_pdl(many ? &ffn_reduce_kernel<O, 8> : &ffn_reduce_kernel<O, 1>,
-               static_cast<unsigned>((count / 4 + per_block - 1) / per_block), 256, 0, stream, partial, splits, count,
-               static_cast<O*>(out));
-    return cudaGetLastError();
-  });
+void add_array(ReduceBatch* batch, const float* partial, int splits, int64_t count, void* out) {
+  const int64_t per_block = splits >= kManySplits ? 32 : 256;  // quads
+  batch->array[batch->arrays++] = ReduceArray{partial, out, count, splits, batch->blocks};
+  batch->blocks += static_cast<int>((count / 4 + per_block - 1) / per_block);
 }
 
-// out [M, N] = a^T b over T tokens.
-cudaError_t weight_gradient(const void* a, const void* b, bool half, int64_t T, int64_t M, int64_t N, void* out,
-                            int type, float* partial, int* status, int sm_count, cudaStream_t stream) {
-  GemmPlan p = plan_gemm(kWeight, M, N, T, sm_count);
+// out [M, N] = a^T b over T tokens; with a token split its partials join `batch`.
+cudaError_t weight_gradient(GemmPlan p, const void* a, const void* b, bool half, int64_t T, void* out, int type,
+                            float* partial, ReduceBatch* batch, int* status, cudaStream_t stream) {
   CUtensorMap ma{}, mb{};
-  if (!encode_mn(&ma, a, half, T, M) || !encode_mn(&mb, b, half, T, N)) return cudaErrorInvalidValue;
+  if (!encode_mn(&ma, a, half, T, p.args.M) || !encode_mn(&mb, b, half, T, p.args.N)) return cudaErrorInvalidValue;
   p.args.out = p.args.splits > 1 ? static_cast<void*>(partial) : out;
   p.args.out_type = type;
   p.args.status = status;
-  const cudaError_t e = launch_gemm<kWeight, kSilu>("ffn_wgrad", p, half, ma, mb, ma, ma, stream);
-  if (e != cudaSuccess || p.args.splits == 1) return e;
-  return reduce_partials("ffn_wgrad_reduce", partial, p.args.splits, M * N, out, type, stream);
-}
-
-cudaError_t bias_gradient(const void* in, bool half, int64_t rows, int64_t cols, void* out, int type, float* partial,
-                          cudaStream_t stream) {
-  const int64_t splits = colsum_splits(rows, cols), per = (rows + splits - 1) / splits;
-  const dim3 grid(static_cast<unsigned>((cols + 255) / 256), static_cast<unsigned>(splits));
-  {
-    LaunchScope scope("ffn_colsum", stream);
-    launch_pdl(half ? &ffn_colsum_kernel<true> : &ffn_colsum_kernel<false>, grid, 256, 0, stream,
-               static_cast<const uint16_t*>(in), rows, static_cast<int>(cols), per, partial);
-  }
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  return reduce_partials("ffn_colsum_reduce", partial, static_cast<int>(splits), cols, out, type, stream);
+  if (p.args.splits > 1) add_array(batch, partial, p.args.splits, static_cast<int64_t>(p.args.M) * p.args.N, out);
+  return launch_gemm<kWeight, kSilu>("ffn_wgrad", p, half, ma, mb, ma, ma, stream);
 }
 
 }  // namespace
@@ -1118,21 +1184,12 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
   const bool half = c.type == kFp16;
   const BackwardLayout l = backward_layout(c.T, c.D, c.H, sm_count);
   void* dgu = c.workspace + l.dgu;
-  float* partial = reinterpret_cast<float*>(c.workspace + l.partial);
-  CUtensorMap ma{}, mb{}, mo{};
+  auto partial = [&](size_t offset) { return reinterpret_cast<float*>(c.workspace + offset); };
+  ReduceBatch batch{};
+  CUtensorMap ma{}, mb{}, mo{}, mk{};
   cudaError_t e = cudaSuccess;
-  if (c.dw_out != nullptr) {
-    e = weight_gradient(c.dy, c.h, half, c.T, c.D, c.H, c.dw_out, c.grad_type, partial, c.status, sm_count, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (c.db_out != nullptr) {
-    e = bias_gradient(c.dy, half, c.T, c.D, c.db_out, c.grad_type, partial, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (c.dx == nullptr && c.dw_in == nullptr && c.db_in == nullptr) return cudaSuccess;
-  {
+  if (c.dx != nullptr || c.dw_in != nullptr || c.db_in != nullptr) {
     GemmPlan p = plan_gemm(kSlope, c.T, c.H, c.D, sm_count);
-    CUtensorMap mk{};
     if (!encode_k(&ma, c.dy, half, c.T, c.D, kBM) || !encode_mn(&mb, c.w_out, half, c.D, c.H) ||
         !encode_out(&mo, dgu, half, c.T, c.H, 2) || !encode_out(&mk, c.kept, half, c.T, c.H, 2)) {
       return cudaErrorInvalidValue;
@@ -1140,14 +1197,6 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
     p.args.status = c.status;
     e = c.activation == kSilu ? launch_gemm<kSlope, kSilu>("ffn_slope", p, half, ma, mb, mo, mk, stream)
                               : launch_gemm<kSlope, kGelu>("ffn_slope", p, half, ma, mb, mo, mk, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (c.dw_in != nullptr) {
-    e = weight_gradient(dgu, c.x, half, c.T, 2 * c.H, c.D, c.dw_in, c.grad_type, partial, c.status, sm_count, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (c.db_in != nullptr) {
-    e = bias_gradient(dgu, half, c.T, 2 * c.H, c.db_in, c.grad_type, partial, stream);
     if (e != cudaSuccess) return e;
   }
   if (c.dx != nullptr) {
@@ -1158,8 +1207,42 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
     }
     p.args.status = c.status;
     e = launch_gemm<kInput, kSilu>("ffn_input", p, half, ma, mb, mo, mo, stream);
+    if (e != cudaSuccess) return e;
   }
-  return e;
+  if (c.dw_in != nullptr) {
+    e = weight_gradient(l.w_in, dgu, c.x, half, c.T, c.dw_in, c.grad_type, partial(l.p_w_in), &batch, c.status, stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (c.dw_out != nullptr) {
+    e = weight_gradient(l.w_out, c.dy, c.h, half, c.T, c.dw_out, c.grad_type, partial(l.p_w_out), &batch, c.status,
+                        stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (c.db_in != nullptr || c.db_out != nullptr) {
+    ColsumArray in{static_cast<const uint16_t*>(dgu), partial(l.p_b_in), static_cast<int>(2 * c.H),
+                   c.db_in != nullptr ? static_cast<int>((2 * c.H + 255) / 256) : 0};
+    ColsumArray out{static_cast<const uint16_t*>(c.dy), partial(l.p_b_out), static_cast<int>(c.D),
+                    c.db_out != nullptr ? static_cast<int>((c.D + 255) / 256) : 0};
+    const int64_t per = (c.T + l.colsums - 1) / l.colsums;
+    const int runs = static_cast<int>((c.T + per - 1) / per);
+    {
+      LaunchScope scope("ffn_colsum", stream);
+      launch_pdl(half ? &ffn_colsum_kernel<true> : &ffn_colsum_kernel<false>,
+                 dim3(static_cast<unsigned>(in.column_blocks + out.column_blocks), static_cast<unsigned>(runs)), 256, 0,
+                 stream, in, out, c.T, per);
+    }
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    if (c.db_in != nullptr) add_array(&batch, in.partial, runs, 2 * c.H, c.db_in);
+    if (c.db_out != nullptr) add_array(&batch, out.partial, runs, c.D, c.db_out);
+  }
+  if (batch.arrays == 0) return cudaSuccess;
+  return by_type(c.grad_type, [&](auto o) {
+    using O = decltype(o);
+    LaunchScope scope("ffn_reduce", stream);
+    launch_pdl(&ffn_reduce_kernel<O>, static_cast<unsigned>(batch.blocks), 256, 0, stream, batch);
+    return cudaGetLastError();
+  });
 }
 
 }  // namespace lsso
