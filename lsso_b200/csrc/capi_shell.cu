@@ -48,7 +48,7 @@ int check_dropout(const char* who, int branch_type, int out_type, int64_t rows, 
 void set_rate(lsso::DropoutCall* c, double p) {
   const double threshold = std::nearbyint(p * 4294967296.0);
   c->drop_all = threshold >= 4294967296.0 ? 1 : 0;
-  c->threshold = c->drop_all ? 0u : static_cast<uint32_t>(threshold);
+  c->threshold = c->drop_all ? 1u : static_cast<uint32_t>(threshold);  // p = 1: the kernel's words are zero
   c->scale = c->drop_all ? 0.0f : static_cast<float>(1.0 / (1.0 - p));
 }
 

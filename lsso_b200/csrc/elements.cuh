@@ -56,11 +56,50 @@ __device__ __forceinline__ Run<T, N> load_run(const T* p) {
   return r;
 }
 
+// Two adjacent 16-bit elements of a 32-bit word as FP32, and back, by the
+// instructions that take a pair.
+__device__ __forceinline__ float2 pair_to_float(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ float2 pair_to_float(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pair_from_float(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pair_from_float(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void run_to_float(const Run<T, N>& r, float (&x)[N]) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 f = pair_to_float(w[i], T());
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_float(r.v[i]);
+  }
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void store_run(T* p, const float (&x)[N]) {
   Run<T, N> r;
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-  for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(x[i]);
+    for (int i = 0; i < N / 2; ++i) w[i] = pair_from_float(x[2 * i], x[2 * i + 1], T());
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(x[i]);
+  }
   constexpr int kBytes = N * sizeof(T);
   if constexpr (kBytes == 32) {
     reinterpret_cast<uint4*>(p)[0] = reinterpret_cast<uint4*>(&r)[0];

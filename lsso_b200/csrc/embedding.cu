@@ -103,8 +103,9 @@ __global__ void __launch_bounds__(kThreads, 4) embed_kernel(const EmbeddingCall 
         const int i = i0 + k * side + mine;
         if (i >= count) continue;
         float v[V];
+        run_to_float(w[k], v);
 #pragma unroll
-        for (int q = 0; q < V; ++q) v[q] = row[k] >= 0 ? to_float(w[k].v[q]) * c.scale : 0.0f;
+        for (int q = 0; q < V; ++q) v[q] = row[k] >= 0 ? v[q] * c.scale : 0.0f;
         store_run<O, V>(out + i * c.width + col, v);
       }
     }
@@ -478,8 +479,10 @@ __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumArgs a,
         if (key != none) {
 #pragma unroll
           for (int i = 0; i < kAhead; ++i) {
+            float f[V];
+            run_to_float(rows[i], f);
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] += to_float(rows[i].v[k]);
+            for (int k = 0; k < V; ++k) acc[k] += f[k];
           }
         }
         continue;
@@ -497,8 +500,10 @@ __global__ void __launch_bounds__(kThreads, 4) embed_sum_kernel(const SumArgs a,
           key = next;
         }
         if (next != none) {
+          float f[V];
+          run_to_float(again, f);
 #pragma unroll
-          for (int k = 0; k < V; ++k) acc[k] += to_float(again.v[k]);
+          for (int k = 0; k < V; ++k) acc[k] += f[k];
         }
       }
     }
