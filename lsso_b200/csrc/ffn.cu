@@ -939,12 +939,16 @@ GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, boo
       const int64_t ntiles = (N + span - 1) / span;
       const int64_t stage = kABytes + static_cast<int64_t>(bn) * 128 / ctas;
       const int64_t stages = std::min<int64_t>(kMaxStages, (static_cast<int64_t>(kSmemMost) - staging) / stage);
-      const int64_t most_splits = mode == kWeight ? std::min<int64_t>(KB, 64) : 1;
-      for (int64_t want = 1; want <= most_splits; ++want) {
+      // token splits that fill one, two, .. rounds of the workers
+      const int64_t tiles = mtiles * ntiles;
+      int64_t before = 0;
+      for (int64_t fill = 0; fill <= (mode == kWeight ? 8 : 0); ++fill) {
+        const int64_t want = std::min(std::min<int64_t>(KB, 64), std::max<int64_t>(1, fill * workers / tiles));
         const int64_t per = (KB + want - 1) / want;
         const int64_t splits = (KB + per - 1) / per;
-        if (splits != want) continue;
-        const int64_t units = mtiles * ntiles * splits;
+        if (splits == before) continue;
+        before = splits;
+        const int64_t units = tiles * splits;
         const int64_t used = std::min(units, workers);
         const int64_t rounds = (units + used - 1) / used;
         const double block = std::max(pair ? 512.0 : 2.0 * bn, stage / 50.0);
