@@ -8,6 +8,13 @@ after each residual, and an optional ``x + mlp(norm2(x))`` (``mlp_ratio=0``
 leaves it out, as BASELINE config 4 does).  Tokens enter through an
 ``Embedding`` initialised N(0, 0.02).
 
+Three options replace the PyTorch layers around the mixer by the package's
+operators, on either implementation: ``gated`` (a gated feed-forward block,
+``feedforward.py``, in the MLP's place), ``dropout`` (dropout with the residual
+sum and the padding mask in one pass, ``dropout.py``, on both branches of every
+block) and ``embedding_scale`` (a scaled embedding with the mask applied and a
+deterministic gradient, ``embedding.py``).
+
 ``vision_position_ids`` is the timm adapter's position rule
 (integrations/timm.py:143-156): position 0 for the class token and centered
 one-dimensional coordinates for the patches.
@@ -19,6 +26,9 @@ import torch
 from torch import nn
 
 from .config import LSSOConfig
+from .dropout import dropout_add, dropout_add_reference, dropout_state
+from .embedding import TokenEmbedding
+from .feedforward import GatedFeedForward
 from .model import LSSO
 
 
@@ -32,53 +42,101 @@ def vision_position_ids(length: int, device: torch.device | None = None) -> torc
 
 
 class ShellBlock(nn.Module):
-    """Pre-norm residual block: x + LSSO(norm(x)), padded tokens zero (optional MLP)."""
+    """Pre-norm residual block: x + LSSO(norm(x)), padded tokens zero (optional MLP).
 
-    def __init__(self, config: LSSOConfig, *, mlp_ratio: float = 0.0) -> None:
+    ``gated`` ("silu" or "gelu"): a gated feed-forward block of ``hidden``
+    features (default ``round(dim * mlp_ratio)``) in the MLP's place.
+    ``dropout``: the rate on both branches in training mode; the block's
+    branches use the generator sites ``site`` and ``site + 1``.
+    """
+
+    def __init__(self, config: LSSOConfig, *, mlp_ratio: float = 0.0, gated: str | None = None,
+                 hidden: int | None = None, dropout: float = 0.0, site: int = 0) -> None:
         super().__init__()
         self.norm1 = nn.LayerNorm(config.dim)
         self.mixer = LSSO(config)
         self.mlp = None
-        if mlp_ratio > 0:
-            hidden = int(round(config.dim * mlp_ratio))
+        self.dropout, self.site = float(dropout), site
+        hidden = int(round(config.dim * mlp_ratio)) if hidden is None else hidden
+        if gated is not None:
+            self.norm2 = nn.LayerNorm(config.dim)
+            self.mlp = GatedFeedForward(config.dim, hidden, activation=gated, bias=config.bias)
+        elif mlp_ratio > 0:
             self.norm2 = nn.LayerNorm(config.dim)
             self.mlp = nn.Sequential(nn.Linear(config.dim, hidden, bias=config.bias), nn.GELU(),
                                      nn.Linear(hidden, config.dim, bias=config.bias))
 
-    def forward(self, x: torch.Tensor, valid_mask: torch.Tensor | None, implementation: str) -> torch.Tensor:
+    def _residual(self, x, branch, valid_mask, implementation, state, site):
+        """x + branch (with dropout in training), padded tokens zero."""
+        if self.training and self.dropout > 0:
+            if state is None:
+                raise ValueError("a block with dropout needs the generator state in training mode")
+            add = dropout_add if implementation == "cuda" else dropout_add_reference
+            return add(branch, x, p=self.dropout, state=state, site=site, valid_mask=valid_mask)
+        x = x + branch
+        if valid_mask is not None:
+            x = torch.where(valid_mask[:, :, None], x, torch.zeros_like(x))
+        return x
+
+    def forward(self, x: torch.Tensor, valid_mask: torch.Tensor | None, implementation: str,
+                state: torch.Tensor | None = None) -> torch.Tensor:
         normalized = self.norm1(x)
         if normalized.device.type == "cuda" and torch.is_autocast_enabled():
             amp = torch.get_autocast_dtype("cuda")
             if implementation == "cuda" and amp not in (torch.float16, torch.bfloat16):
                 raise TypeError("the CUDA LSSO sequence path supports FP16 or BF16 AMP")
             normalized = normalized.to(dtype=amp)
-        x = x + self.mixer(normalized, valid_mask=valid_mask, implementation=implementation)
-        if valid_mask is not None:
-            x = torch.where(valid_mask[:, :, None], x, torch.zeros_like(x))
+        branch = self.mixer(normalized, valid_mask=valid_mask, implementation=implementation)
+        x = self._residual(x, branch, valid_mask, implementation, state, self.site)
         if self.mlp is not None:
-            x = x + self.mlp(self.norm2(x))
-            if valid_mask is not None:
-                x = torch.where(valid_mask[:, :, None], x, torch.zeros_like(x))
+            if isinstance(self.mlp, GatedFeedForward):
+                branch = self.mlp(self.norm2(x).to(dtype=normalized.dtype), implementation=implementation)
+            else:
+                branch = self.mlp(self.norm2(x))
+            x = self._residual(x, branch, valid_mask, implementation, state, self.site + 1)
         return x
 
 
 class SequenceShell(nn.Module):
     """Token embedding plus ``depth`` pre-norm LSSO blocks (dim 128, 4 heads,
-    rank 48, depth 4, vocabulary 8, no MLP)."""
+    rank 48, depth 4, vocabulary 8, no MLP).
 
-    def __init__(self, config: LSSOConfig, *, depth: int = 4, vocab: int = 8, mlp_ratio: float = 0.0) -> None:
+    ``gated``, ``hidden``, ``dropout``: as in :class:`ShellBlock`, for every
+    block.  ``embedding_scale``: a :class:`TokenEmbedding` with this scale (the
+    parameter keeps the name ``embedding.weight``).  With dropout, the buffer
+    ``dropout_state`` holds ``[dropout_seed, step]`` and a training forward
+    advances the step, in a captured graph as well.
+    """
+
+    def __init__(self, config: LSSOConfig, *, depth: int = 4, vocab: int = 8, mlp_ratio: float = 0.0,
+                 gated: str | None = None, hidden: int | None = None, dropout: float = 0.0, dropout_seed: int = 0,
+                 embedding_scale: float | None = None) -> None:
         super().__init__()
-        self.embedding = nn.Embedding(vocab, config.dim)
-        nn.init.normal_(self.embedding.weight, mean=0.0, std=0.02)
-        self.blocks = nn.ModuleList(ShellBlock(config, mlp_ratio=mlp_ratio) for _ in range(depth))
+        if embedding_scale is None:
+            self.embedding = nn.Embedding(vocab, config.dim)
+            nn.init.normal_(self.embedding.weight, mean=0.0, std=0.02)
+        else:
+            self.embedding = TokenEmbedding(vocab, config.dim, scale=embedding_scale)
+        self.blocks = nn.ModuleList(
+            ShellBlock(config, mlp_ratio=mlp_ratio, gated=gated, hidden=hidden, dropout=dropout, site=2 * i)
+            for i in range(depth))
+        if dropout > 0:
+            self.register_buffer("dropout_state", dropout_state(dropout_seed))
+        else:
+            self.dropout_state = None
 
     def forward(self, token_ids: torch.Tensor, valid_mask: torch.Tensor | None = None, *,
                 implementation: str = "reference") -> torch.Tensor:
-        x = self.embedding(token_ids)
-        if valid_mask is not None:
-            x = torch.where(valid_mask[:, :, None], x, torch.zeros_like(x))
+        if isinstance(self.embedding, TokenEmbedding):
+            x = self.embedding(token_ids, valid_mask, implementation=implementation)
+        else:
+            x = self.embedding(token_ids)
+            if valid_mask is not None:
+                x = torch.where(valid_mask[:, :, None], x, torch.zeros_like(x))
         for block in self.blocks:
-            x = block(x, valid_mask, implementation)
+            x = block(x, valid_mask, implementation, self.dropout_state)
+        if self.training and self.dropout_state is not None:
+            self.dropout_state[1] += 1
         return x
 
 

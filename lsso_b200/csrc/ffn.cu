@@ -108,13 +108,11 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-// Without the release of this CTA's earlier stores (a wait for every
-// outstanding global store); what the partner must see is fenced by its writer.
+// Keeps both CTAs until each has come here; orders nothing else.
 __device__ __forceinline__ void cluster_sync_relaxed() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;\n" ::: "memory"); }
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
 }
@@ -453,7 +451,6 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       }
       if (kPair && rank == 1) {
         for (int s = 0; s < S; ++s) store_remote(map_rank(smem_u32(&peer_issued[operand][s]), 0), mine[s]);
-        fence_cluster();
       }
     }
     __syncwarp();
@@ -664,7 +661,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
   tc_fence_before();
   __syncthreads();
-  if (kPair) cluster_sync_relaxed();
+  if (kPair) cluster_sync();  // (releases the partner's arrivals on this CTA's barriers, too)
   // Loads still in flight (only after an abort): wait for them, bounded.  All
   // loads of a stage complete on the leader's barrier; where one producer
   // issued a use that another did not, the leader supplies the missing arrival

@@ -298,3 +298,33 @@ def test_cpu_refusals_and_reference() -> None:
     assert layer(x).shape == x.shape and layer.w_in.weight.shape == (40, 12)
     with pytest.raises(ValueError, match="implementation"):
         layer(x, implementation="fast")
+
+
+@pytest.mark.gpu
+def test_waits_that_run_out_leave_a_usable_library() -> None:
+    """With a one-nanosecond limit the tensor-core kernels take their abort path (nothing hangs or
+    faults), the status says so, and the next calls give the bits of the calls before."""
+    from lsso_b200.ball import _native, cuda
+    from tests.gpu_util import require_native
+
+    require_native()
+    cuda.device_status(reset=True)
+    for rows in (100, 3000):  # single CTAs and pairs
+        x, w_in, w_out, b_in, b_out, dy = _inputs(rows, 256, 688, torch.bfloat16, torch.bfloat16, True)
+        leaves = [v.requires_grad_() for v in (x, w_in, w_out, b_in, b_out)]
+
+        def step():
+            y = gated_feed_forward(*leaves)  # noqa: B023
+            return (y.detach(), *torch.autograd.grad(y, leaves, dy))  # noqa: B023
+
+        want = step()
+        torch.cuda.synchronize()
+        _native.set_wait_limit_ns(1)
+        try:
+            step()
+            torch.cuda.synchronize()
+        finally:
+            _native.set_wait_limit_ns(0)
+        assert cuda.device_status(reset=True) == 1
+        assert all(torch.equal(a, b) for a, b in zip(step(), want))
+        assert cuda.device_status(reset=True) == 0
