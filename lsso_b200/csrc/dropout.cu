@@ -101,8 +101,8 @@ __device__ __forceinline__ uint32_t live_bits(const uint8_t* __restrict__ mask, 
 }
 
 template <typename T>
-__device__ __forceinline__ Run<T, kPer> load8(const T* p, int64_t first, int64_t total, bool whole) {
-  if (whole) return load_run<T, kPer>(p + first);
+__device__ __forceinline__ Run<T, kPer> load8(const T* p, int64_t first, int64_t total, bool whole, bool wide) {
+  if (whole) return load_run<T, kPer>(p + first, wide);
   Run<T, kPer> r;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) r.v[i] = first + i < total ? p[first + i] : from_float<T>(0.0f);
@@ -110,9 +110,9 @@ __device__ __forceinline__ Run<T, kPer> load8(const T* p, int64_t first, int64_t
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int64_t first, int64_t total, bool whole, const float (&v)[kPer]) {
+__device__ __forceinline__ void store8(T* p, int64_t first, int64_t total, bool whole, bool wide, const float (&v)[kPer]) {
   if (whole) {
-    store_run<T, kPer>(p + first, v);
+    store_run<T, kPer>(p + first, v, wide);
     return;
   }
 #pragma unroll
@@ -123,7 +123,7 @@ __device__ __forceinline__ void store8(T* p, int64_t first, int64_t total, bool 
 // kBackward: `in` is the upstream gradient (type O), `out` the branch gradient
 // (type B).  Otherwise `in` is the branch (B) and `out` is y (O).
 template <typename B, typename O, bool kBackward, bool kMasked>
-__global__ void __launch_bounds__(kThreads, 6) dropout_kernel(const DropoutCall c, int64_t total, int vec) {
+__global__ void __launch_bounds__(kThreads, 6) dropout_kernel(const DropoutCall c, int64_t total, int vec, int wide) {
   pdl_wait();
   using In = typename std::conditional<kBackward, O, B>::type;
   using Out = typename std::conditional<kBackward, B, O>::type;
@@ -140,9 +140,9 @@ __global__ void __launch_bounds__(kThreads, 6) dropout_kernel(const DropoutCall 
   for (int64_t first = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * kPer; first < total;
        first += stride) {
     const bool whole = vec && first + kPer <= total;
-    const Run<In, kPer> x = load8(in, first, total, whole);
+    const Run<In, kPer> x = load8(in, first, total, whole, wide);
     Run<O, kPer> r;
-    if (!kBackward && residual != nullptr) r = load8(residual, first, total, whole);
+    if (!kBackward && residual != nullptr) r = load8(residual, first, total, whole, wide);
     // p = 1: words of zero, below the threshold of one
     Words k{};
     if (!c.drop_all) k = words_at(first, key, c.site, static_cast<uint32_t>(step));
@@ -165,14 +165,14 @@ __global__ void __launch_bounds__(kThreads, 6) dropout_kernel(const DropoutCall 
       }
     }
     if (kBackward) {
-      if (out != nullptr) store8(out, first, total, whole, v);
-      if (c.residual_grad != nullptr) store8(static_cast<O*>(c.residual_grad), first, total, whole, through);
+      if (out != nullptr) store8(out, first, total, whole, wide, v);
+      if (c.residual_grad != nullptr) store8(static_cast<O*>(c.residual_grad), first, total, whole, wide, through);
     } else {
       if (residual != nullptr) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) v[i] += through[i];
       }
-      store8(out, first, total, whole, v);
+      store8(out, first, total, whole, wide, v);
     }
   }
 }
@@ -182,13 +182,13 @@ cudaError_t launch_types(const DropoutCall& c, int sm_count, cudaStream_t stream
   const int64_t total = c.rows * c.width;
   const uintptr_t all = reinterpret_cast<uintptr_t>(c.in) | reinterpret_cast<uintptr_t>(c.residual) |
                         reinterpret_cast<uintptr_t>(c.out) | reinterpret_cast<uintptr_t>(c.residual_grad);
-  const int vec = (all & 15u) == 0 ? 1 : 0;
+  const int vec = (all & 15u) == 0 ? 1 : 0, wide = (all & 31u) == 0 ? 1 : 0;
   const int64_t need = (total + kThreads * kPer - 1) / (kThreads * kPer);
   const int64_t most = static_cast<int64_t>(sm_count) * kBlocksPerSm;
   const unsigned grid = static_cast<unsigned>(need < most ? need : most);
   auto kernel = c.row_mask != nullptr ? &dropout_kernel<B, O, kBackward, true> : &dropout_kernel<B, O, kBackward, false>;
   LaunchScope scope(kBackward ? "dropout_bwd" : "dropout", stream);
-  launch_pdl(kernel, grid, kThreads, 0, stream, c, total, vec);
+  launch_pdl(kernel, grid, kThreads, 0, stream, c, total, vec, wide);
   return cudaGetLastError();
 }
 

@@ -66,7 +66,7 @@ RowSplit split_row(int64_t width, bool aligned, int widest) {
 // ---------------------------------------------------------------- forward
 // `lanes` lanes per token, 32 / lanes tokens side by side, `per` tokens per warp.
 template <typename W, typename O, int V>
-__global__ void __launch_bounds__(kThreads, 4) embed_kernel(const EmbeddingCall c, int lanes, int slabs, int per) {
+__global__ void __launch_bounds__(kThreads, 4) embed_kernel(const EmbeddingCall c, int lanes, int slabs, int per, int wide) {
   pdl_wait();
   const W* __restrict__ weight = static_cast<const W*>(c.weight);
   O* __restrict__ out = static_cast<O*>(c.out);
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_kernel(const EmbeddingCall 
       Run<W, V> w[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        w[k] = load_run<W, V>(weight + max(row[k], 0) * c.width + col);
+        w[k] = load_run<W, V>(weight + max(row[k], 0) * c.width + col, wide);
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_kernel(const EmbeddingCall 
         run_to_float(w[k], v);
 #pragma unroll
         for (int q = 0; q < V; ++q) v[q] = row[k] >= 0 ? v[q] * c.scale : 0.0f;
-        store_run<O, V>(out + i * c.width + col, v);
+        store_run<O, V>(out + i * c.width + col, v, wide);
       }
     }
   }
@@ -116,6 +116,7 @@ template <typename W, typename O>
 cudaError_t launch_embed_types(const EmbeddingCall& c, int sm_count, cudaStream_t stream) {
   const uintptr_t both = reinterpret_cast<uintptr_t>(c.weight) | reinterpret_cast<uintptr_t>(c.out);
   const RowSplit r = split_row(c.width, (both & 15u) == 0, 8);
+  const int wide = (both & 31u) == 0 ? 1 : 0;
   // tokens per warp: 32 when that still gives every SM sixteen warps
   int per = 32;
   while (per > 32 / r.lanes && (c.tokens + per - 1) / per < 16 * static_cast<int64_t>(sm_count)) per /= 2;
@@ -123,11 +124,11 @@ cudaError_t launch_embed_types(const EmbeddingCall& c, int sm_count, cudaStream_
   const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
   LaunchScope scope("embedding", stream);
   if (r.vec == 8) {
-    launch_pdl(embed_kernel<W, O, 8>, grid, kThreads, 0, stream, c, r.lanes, r.slabs, per);
+    launch_pdl(embed_kernel<W, O, 8>, grid, kThreads, 0, stream, c, r.lanes, r.slabs, per, wide);
   } else if (r.vec == 4) {
-    launch_pdl(embed_kernel<W, O, 4>, grid, kThreads, 0, stream, c, r.lanes, r.slabs, per);
+    launch_pdl(embed_kernel<W, O, 4>, grid, kThreads, 0, stream, c, r.lanes, r.slabs, per, wide);
   } else {
-    launch_pdl(embed_kernel<W, O, 1>, grid, kThreads, 0, stream, c, r.lanes, r.slabs, per);
+    launch_pdl(embed_kernel<W, O, 1>, grid, kThreads, 0, stream, c, r.lanes, r.slabs, per, wide);
   }
   return cudaGetLastError();
 }
@@ -529,7 +530,9 @@ __device__ __forceinline__ float sum_partials(const float* __restrict__ head, in
 // Rows that cross chunks: the warp of the chunk in which such a row begins
 // adds its partials in chunk order; a row over more than 32 further chunks is
 // left to the whole block (each warp takes every eighth partial, then the
-// warps' sums are added in warp order).  Blocks: eight chunks by 32 columns.
+// warps' sums are added in warp order).  Blocks: eight chunks by 32 columns
+// (by 512 columns the few long rows of a skewed vocabulary took longer: 65536
+// tokens, 50021 x 512, 10 -> 14 us).
 template <typename W>
 __global__ void __launch_bounds__(kThreads) embed_join_kernel(const SumArgs a) {
   pdl_wait();
