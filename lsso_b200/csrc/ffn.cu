@@ -73,10 +73,10 @@ struct GemmArgs {
   int M, N;            // output rows and columns (kGate / kSlope: N = H)
   int KB;              // 64-wide contraction blocks
   int BN;              // accumulator columns per tile (kGate: gate and up halves)
-  int mtiles, ntiles, units, splits, kb_per_split, stages;
+  int mtiles, ntiles, units, splits, stages;
   int step_n, step_m;  // a worker's step to its next unit, in n tiles and m tiles
   int boxes;           // output boxes of one epilogue warp
-  int rev;             // m tiles from the last to the first (the rows the kernel before wrote last are in L2)
+  int rev;             // m tiles, or token blocks, from the last to the first (the rows written last are in L2)
   int keep, bias_type;
   const void* bias;    // kGate: [2N], kOutput: [N]; nullable
   void* out;           // kWeight: gradient (splits == 1) or FP32 partials [splits][M][N]
@@ -346,33 +346,40 @@ struct UnitWalk {
       ++split;
     }
   }
-  __device__ __forceinline__ int m_tile(const GemmArgs& a) const { return a.rev ? a.mtiles - 1 - mt : mt; }
+  // A split takes every splits-th token block, so that all workers move through the tokens together.
+  __device__ __forceinline__ int blocks(const GemmArgs& a) const { return (a.KB - split + a.splits - 1) / a.splits; }
+  __device__ __forceinline__ int token_block(const GemmArgs& a, int i) const {
+    const int kb = split + i * a.splits;
+    return a.rev ? a.KB - 1 - kb : kb;
+  }
+  __device__ __forceinline__ int m_tile(const GemmArgs& a) const { return a.rev ? a.mtiles - 1 - mt : mt; }  // (not kWeight)
   __device__ __forceinline__ void skip(const GemmArgs& a, int step, int count) {
     for (int i = 0; i < count; ++i) next(a, step);
   }
 };
 
+struct GemmShared {
+  alignas(16) float bias[kEpiWarps][32];
+  uint64_t full[kMaxStages], empty[kMaxStages], tfull[kMaxBuffers], tempty[kMaxBuffers], mdrain;
+  uint64_t kept[kEpiWarps];           // kSlope
+  int issued[2][kMaxStages];          // the use of each stage that a producer issued last
+  int peer_issued[2][kMaxStages];     // pair leader: the partner's
+  uint32_t tmem;
+  int abort_flag;
+};
+
+// One product, by worker `worker` of `workers` (a CTA or a pair).
 template <int kMode, bool kHalf, int kAct, bool kPair>
-__global__ void __launch_bounds__(kThreads, 1)
-ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ CUtensorMap tmap_keep,
-                const GemmArgs a) {
-  pdl_wait();
+__device__ __forceinline__ void gemm_body(const CUtensorMap* map_a, const CUtensorMap* map_b, const CUtensorMap* map_out,
+                                          const CUtensorMap* map_keep, const GemmArgs& a, int worker, int workers,
+                                          GemmShared& sh) {
   constexpr bool kAmn = kMode == kWeight;
   constexpr bool kBmn = kMode == kSlope || kMode == kInput || kMode == kWeight;
   constexpr int kCtas = kPair ? 2 : 1;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], tfull[kMaxBuffers], tempty[kMaxBuffers], mdrain;
-  __shared__ __align__(8) uint64_t kept[kMode == kSlope ? kEpiWarps : 1];
-  __shared__ uint32_t tmem_s;
-  __shared__ int abort_flag;
-  __shared__ int issued[2][kMaxStages];       // the use of each stage that a producer issued last
-  __shared__ int peer_issued[2][kMaxStages];  // pair leader: the partner's
-  __shared__ __align__(16) float sbias[kEpiWarps][32];
-  volatile int* abort_v = &abort_flag;
+  volatile int* abort_v = &sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = kPair ? cluster_rank() : 0u;
-  const int first_unit = static_cast<int>(blockIdx.x) / kCtas, unit_step = static_cast<int>(gridDim.x) / kCtas;
   const int S = a.stages;
   const int BN = a.BN, BNL = BN / kCtas;  // accumulator columns; columns of the operand this CTA holds
   const uint32_t stage_bytes = kABytes + static_cast<uint32_t>(BNL) * 128;
@@ -382,34 +389,34 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
-      mbar_init(smem_u32(&empty[s]), 1);
+      mbar_init(smem_u32(&sh.full[s]), 1);
+      mbar_init(smem_u32(&sh.empty[s]), 1);
     }
     for (int b = 0; b < nbuf; ++b) {
-      mbar_init(smem_u32(&tfull[b]), 1);
-      mbar_init(smem_u32(&tempty[b]), kEpiWarps / nbuf * kCtas);
+      mbar_init(smem_u32(&sh.tfull[b]), 1);
+      mbar_init(smem_u32(&sh.tempty[b]), kEpiWarps / nbuf * kCtas);
     }
-    mbar_init(smem_u32(&mdrain), 1);
+    mbar_init(smem_u32(&sh.mdrain), 1);
     if (kMode == kSlope) {
-      for (int i = 0; i < kEpiWarps; ++i) mbar_init(smem_u32(&kept[i]), 1);
+      for (int i = 0; i < kEpiWarps; ++i) mbar_init(smem_u32(&sh.kept[i]), 1);
     }
-    abort_flag = 0;
+    sh.abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) alloc_tmem<kPair>(smem_u32(&tmem_s), tcols);
+  if (warp == 1) alloc_tmem<kPair>(smem_u32(&sh.tmem), tcols);
   tc_fence_before();
   __syncthreads();
   if (kPair) cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = tmem_s;
-  const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(full), empty_base = smem_u32(empty);
+  const uint32_t tmem = sh.tmem;
+  const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(sh.full), empty_base = smem_u32(sh.empty);
 
   if (warp == 0 || warp == 2) {
     // ---------------- producers: warp 0 the row operand, warp 2 the column operand
     if (lane == 0) {
       const int operand = warp >> 1;
-      prefetch_tmap(operand == 0 ? &tmap_a : &tmap_b);
-      int* mine = issued[operand];
+      prefetch_tmap(operand == 0 ? map_a : map_b);
+      int* mine = sh.issued[operand];
       for (int s = 0; s < S; ++s) mine[s] = -1;
       const uint32_t full_bar = kPair ? map_rank(full_base, 0) : full_base;  // both CTAs' loads complete on the leader's
       RingPos rp;
@@ -418,18 +425,19 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const int n0 = nt * BN + static_cast<int>(rank) * BNL;
         if (kMode == kGate) {
           // columns [0, span) are the gate rows, [span, 2 span) the up rows: one plane per CTA of a pair
-          load_3d<kPair>(bdst, &tmap_b, kb * kBK, nt * span, static_cast<int>(rank), bar);
-          if (!kPair) load_3d<kPair>(bdst + static_cast<uint32_t>(span) * 128, &tmap_b, kb * kBK, nt * span, 1, bar);
+          load_3d<kPair>(bdst, map_b, kb * kBK, nt * span, static_cast<int>(rank), bar);
+          if (!kPair) load_3d<kPair>(bdst + static_cast<uint32_t>(span) * 128, map_b, kb * kBK, nt * span, 1, bar);
         } else if (kBmn) {
-          for (int g = 0; g < BNL / 64; ++g) load_2d<kPair>(bdst + g * kBox, &tmap_b, n0 + g * 64, kb * kBK, bar);
+          for (int g = 0; g < BNL / 64; ++g) load_2d<kPair>(bdst + g * kBox, map_b, n0 + g * 64, kb * kBK, bar);
         } else {
-          load_2d<kPair>(bdst, &tmap_b, kb * kBK, n0, bar);
+          load_2d<kPair>(bdst, map_b, kb * kBK, n0, bar);
         }
       };
-      for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step)) {
-        const int m0 = (w.m_tile(a) * kCtas + static_cast<int>(rank)) * kBM;
-        const int kb1 = min(a.KB, (w.split + 1) * a.kb_per_split);
-        for (int kb = w.split * a.kb_per_split; kb < kb1; ++kb, rp.next(S)) {
+      for (UnitWalk w(a, worker); w.unit < a.units && ok; w.next(a, workers)) {
+        const int m0 = ((kMode == kWeight ? w.mt : w.m_tile(a)) * kCtas + static_cast<int>(rank)) * kBM;
+        const int blocks = kMode == kWeight ? w.blocks(a) : a.KB;
+        for (int i = 0; i < blocks; ++i, rp.next(S)) {
+          const int kb = kMode == kWeight ? w.token_block(a, i) : i;
           const int s = rp.s;
           ok = fwait(empty_base + 8 * s, (rp.u & 1) ^ 1, abort_v, a.status);
           if (!ok) break;
@@ -438,10 +446,10 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           if (operand == 0) {
             if (rank == 0) mbar_arrive_expect_tx(full_base + 8 * s, kCtas * stage_bytes);
             if (kAmn) {
-              load_2d<kPair>(dst, &tmap_a, m0, kb * kBK, bar);
-              load_2d<kPair>(dst + kBox, &tmap_a, m0 + 64, kb * kBK, bar);
+              load_2d<kPair>(dst, map_a, m0, kb * kBK, bar);
+              load_2d<kPair>(dst + kBox, map_a, m0 + 64, kb * kBK, bar);
             } else {
-              load_2d<kPair>(dst, &tmap_a, kb * kBK, m0, bar);
+              load_2d<kPair>(dst, map_a, kb * kBK, m0, bar);
             }
           } else {
             load_b(dst + kABytes, w.nt, kb, bar);
@@ -450,7 +458,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         }
       }
       if (kPair && rank == 1) {
-        for (int s = 0; s < S; ++s) store_remote(map_rank(smem_u32(&peer_issued[operand][s]), 0), mine[s]);
+        for (int s = 0; s < S; ++s) store_remote(map_rank(smem_u32(&sh.peer_issued[operand][s]), 0), mine[s]);
       }
     }
     __syncwarp();
@@ -464,15 +472,15 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const uint64_t bdesc = kBmn ? make_desc_sw128(smem_base + kABytes, kBox, 1024)
                                   : make_desc_sw128(smem_base + kABytes, 16, 1024);
       constexpr uint32_t kAStep = kAmn ? 2048 / 16 : 32 / 16, kBStep = kBmn ? 2048 / 16 : 32 / 16;
-      const uint32_t tfull_base = smem_u32(tfull), tempty_base = smem_u32(tempty);
+      const uint32_t tfull_base = smem_u32(sh.tfull), tempty_base = smem_u32(sh.tempty);
       RingPos rp, tp;  // stages, accumulators
       bool ok = true;
-      for (UnitWalk w(a, first_unit); w.unit < a.units && ok; w.next(a, unit_step), tp.next(nbuf)) {
-        const int kb0 = w.split * a.kb_per_split, kb1 = min(a.KB, kb0 + a.kb_per_split);
+      for (UnitWalk w(a, worker); w.unit < a.units && ok; w.next(a, workers), tp.next(nbuf)) {
+        const int blocks = kMode == kWeight ? w.blocks(a) : a.KB;
         ok = fwait(tempty_base + 8 * tp.s, (tp.u & 1) ^ 1, abort_v, a.status);
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(tp.s * BN);
-        for (int kb = kb0; kb < kb1 && ok; ++kb, rp.next(S)) {
+        for (int i = 0; i < blocks && ok; ++i, rp.next(S)) {
           const int s = rp.s;
           ok = fwait(full_base + 8 * s, rp.u & 1, abort_v, a.status);
           if (!ok) break;
@@ -480,15 +488,15 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           const uint32_t off = static_cast<uint32_t>(s) * (stage_bytes / 16);
 #pragma unroll
           for (int ks = 0; ks < kBK / 16; ++ks) {
-            mma<kPair>(d, adesc + off + ks * kAStep, bdesc + off + ks * kBStep, idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
+            mma<kPair>(d, adesc + off + ks * kAStep, bdesc + off + ks * kBStep, idesc, (i > 0 || ks > 0) ? 1u : 0u);
           }
           commit_all<kPair>(empty_base + 8 * s);
         }
         if (ok) commit_all<kPair>(tfull_base + 8 * tp.s);
       }
       // no tensor-core operation still writes TMEM or reads shared memory past this point
-      commit_own<kPair>(smem_u32(&mdrain));
-      mbar_wait_bounded(smem_u32(&mdrain), 0, nullptr, a.status);
+      commit_own<kPair>(smem_u32(&sh.mdrain));
+      mbar_wait_bounded(smem_u32(&sh.mdrain), 0, nullptr, a.status);
     }
     __syncwarp();
   } else if (warp >= kEpiWarp0) {
@@ -502,19 +510,19 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     const int col0 = 32 * ((ew % members) >> 2), col_step = 8 * members;
     const int row_base = static_cast<int>(rank) * kBM + 32 * sub;
     uint8_t* stage = smem + S * stage_bytes + ew * a.boxes * kOutBox;
-    float* scratch = sbias[ew];
-    const uint32_t kbar = smem_u32(&kept[kMode == kSlope ? ew : 0]);
-    UnitWalk w(a, first_unit + b * unit_step), ahead = w;  // ahead, ahead_c: kSlope: the next piece whose pre-activations are loaded
+    float* scratch = sh.bias[ew];
+    const uint32_t kbar = smem_u32(&sh.kept[kMode == kSlope ? ew : 0]);
+    UnitWalk w(a, worker + b * workers), ahead = w;  // ahead, ahead_c: kSlope: the next piece whose pre-activations are loaded
     int ahead_c = col0, loaded = 0, piece = 0;
     // Loads the kept pre-activations of the next piece of this warp that lies in the output, if there is one.
     auto load_kept = [&]() {
-      for (; ahead.unit < a.units; ahead.skip(a, unit_step, nbuf), ahead_c = col0) {
+      for (; ahead.unit < a.units; ahead.skip(a, workers, nbuf), ahead_c = col0) {
         const int r0 = ahead.m_tile(a) * kBM * kCtas + row_base, n0 = ahead.nt * span + ahead_c;
         if (r0 >= a.M || ahead_c >= span || n0 >= a.N) continue;
         if (lane == 0) {
           mbar_arrive_expect_tx(kbar, 2 * kOutBox);
-          tma_load_3d(smem_u32(stage), &tmap_keep, n0, 0, r0, kbar);
-          tma_load_3d(smem_u32(stage + kOutBox), &tmap_keep, n0, 1, r0, kbar);
+          tma_load_3d(smem_u32(stage), map_keep, n0, 0, r0, kbar);
+          tma_load_3d(smem_u32(stage + kOutBox), map_keep, n0, 1, r0, kbar);
         }
         ++loaded;
         ahead_c += col_step;
@@ -523,8 +531,8 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       __syncwarp();
     };
     if (kMode != kWeight && lane == 0) {
-      prefetch_tmap(&tmap_out);
-      if (kMode == kGate || kMode == kSlope) prefetch_tmap(&tmap_keep);
+      prefetch_tmap(map_out);
+      if (kMode == kGate || kMode == kSlope) prefetch_tmap(map_keep);
     }
     if (kMode == kSlope) load_kept();
     // The boxes are free to be written again (the stores from them have read them).
@@ -542,11 +550,11 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     };
     bool ok = true;
     int i = 0;
-    for (; w.unit < a.units && ok; w.skip(a, unit_step, nbuf), ++i) {
-      ok = fwait_warp(smem_u32(&tfull[b]), i & 1, abort_v, a.status);
+    for (; w.unit < a.units && ok; w.skip(a, workers, nbuf), ++i) {
+      ok = fwait_warp(smem_u32(&sh.tfull[b]), i & 1, abort_v, a.status);
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(32 * sub) << 16) + static_cast<uint32_t>(b * BN);
-      const int row0 = w.m_tile(a) * kBM * kCtas + row_base;
+      const int row0 = (kMode == kWeight ? w.mt : w.m_tile(a)) * kBM * kCtas + row_base;
       const int columns = row0 < a.M ? min(span, a.N - w.nt * span) : 0;  // of this tile that lie in the output
       // This warp's last values of the tile are in registers: its accumulator may be overwritten.
       auto release = [&]() {
@@ -554,9 +562,9 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         __syncwarp();
         if (lane == 0) {
           if (kPair && rank != 0) {
-            arrive_remote(map_rank(smem_u32(&tempty[b]), 0));
+            arrive_remote(map_rank(smem_u32(&sh.tempty[b]), 0));
           } else {
-            mbar_arrive(smem_u32(&tempty[b]));
+            mbar_arrive(smem_u32(&sh.tempty[b]));
           }
         }
       };
@@ -581,12 +589,12 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             const bool apart = a.boxes == 3;
             box_write<kHalf>(stage + (apart ? kOutBox : 0), lane, v);
             if (apart) box_write<kHalf>(stage + 2 * kOutBox, lane, u);
-            store_box(&tmap_keep, apart ? 1 : 0, n0, 0, row0);
+            store_box(map_keep, apart ? 1 : 0, n0, 0, row0);
             if (!apart) {
               boxes_free();
               box_write<kHalf>(stage, lane, u);
             }
-            store_box(&tmap_keep, apart ? 2 : 0, n0, 1, row0);
+            store_box(map_keep, apart ? 2 : 0, n0, 1, row0);
           }
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
@@ -597,7 +605,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
           }
           if (a.keep && a.boxes == 1) boxes_free();
           box_write<kHalf>(stage, lane, v);
-          store_box(&tmap_out, 0, n0, 0, row0);
+          store_box(map_out, 0, n0, 0, row0);
         } else if (kMode == kSlope) {
           tmem_ld_wait();
           if (last) release();
@@ -627,13 +635,13 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             }
             *box_piece(stage + 2 * kOutBox, lane, q) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
           }
-          store_box(&tmap_out, 2, n0, 0, row0);
+          store_box(map_out, 2, n0, 0, row0);
           boxes_free();
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             *box_piece(stage + 2 * kOutBox, lane, q) = make_uint4(u[4 * q], u[4 * q + 1], u[4 * q + 2], u[4 * q + 3]);
           }
-          store_box(&tmap_out, 2, n0, 1, row0);
+          store_box(map_out, 2, n0, 1, row0);
         } else {
           tmem_ld_wait();
           if (last) release();
@@ -644,7 +652,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
             if (kMode == kOutput && a.bias != nullptr) add_bias(v, scratch, a.bias, a.bias_type, n0, a.N, 0, lane);
             boxes_free();
             box_write<kHalf>(stage, lane, v);
-            store_box(&tmap_out, 0, n0, 0, row0);
+            store_box(map_out, 0, n0, 0, row0);
           }
         }
       }
@@ -669,8 +677,8 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   // (A use starts only after every producer issued the one before it.)
   if (warp == 0 && lane == 0 && rank == 0) {
     for (int s = 0; s < S; ++s) {
-      const int own_a = issued[0][s], own_b = issued[1][s];
-      const int peer_a = kPair ? peer_issued[0][s] : own_a, peer_b = kPair ? peer_issued[1][s] : own_b;
+      const int own_a = sh.issued[0][s], own_b = sh.issued[1][s];
+      const int peer_a = kPair ? sh.peer_issued[0][s] : own_a, peer_b = kPair ? sh.peer_issued[1][s] : own_b;
       const int last = max(max(own_a, own_b), max(peer_a, peer_b));
       if (last < 0) continue;
       const uint32_t bar = full_base + 8 * s;
@@ -686,6 +694,41 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   if (warp == 1) {
     tc_fence_after();
     free_tmem<kPair>(tmem, tcols);
+  }
+}
+
+template <int kMode, bool kHalf, int kAct, bool kPair>
+__global__ void __launch_bounds__(kThreads, 1)
+ffn_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_keep,
+                const GemmArgs a) {
+  pdl_wait();
+  __shared__ __align__(16) GemmShared sh;
+  constexpr int kCtas = kPair ? 2 : 1;
+  gemm_body<kMode, kHalf, kAct, kPair>(&map_a, &map_b, &map_out, &map_keep, a, static_cast<int>(blockIdx.x) / kCtas,
+                                       static_cast<int>(gridDim.x) / kCtas, sh);
+}
+
+// The products that follow [dg | du] in one launch, side by side on the pairs:
+// the input gradient and both weight gradients, each on a share of the pairs
+// that fits its work.  They walk the tokens together, so that [dg | du] comes
+// from HBM once for the two that read it, and a short batch takes one launch.
+struct BackwardProducts {
+  CUtensorMap a[3], b[3], out;  // input gradient (out: its map), weight gradients
+  GemmArgs args[3];
+  int first[4];                 // first worker of each; first[3]: all workers
+};
+template <bool kHalf>
+__global__ void __launch_bounds__(kThreads, 1) ffn_backward_kernel(const __grid_constant__ BackwardProducts p) {
+  pdl_wait();
+  __shared__ __align__(16) GemmShared sh;
+  const int pair = static_cast<int>(blockIdx.x) / 2;
+  if (pair < p.first[1]) {
+    gemm_body<kInput, kHalf, kSilu, true>(&p.a[0], &p.b[0], &p.out, &p.out, p.args[0], pair, p.first[1], sh);
+  } else {
+    const int k = pair < p.first[2] ? 1 : 2;
+    gemm_body<kWeight, kHalf, kSilu, true>(&p.a[k], &p.b[k], &p.out, &p.out, p.args[k], pair - p.first[k],
+                                           p.first[k + 1] - p.first[k], sh);
   }
 }
 
@@ -920,31 +963,31 @@ int boxes_of(Mode mode, bool keep, int64_t KB) {
 // column operand of one n tile in shared memory, so that a short contraction
 // streams its rows only, was slower: slope kernel at 64 x 4096 tokens, 256 ->
 // 688, 295 -> 342 us; gate kernel 291 -> 287.)
-GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, bool keep = false) {
+GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, bool keep = false, int pairs_only = 0) {
   GemmPlan best{};
   double best_cost = 0.0;
   const int64_t KB = (K + kBK - 1) / kBK;
   const int boxes = boxes_of(mode, keep, KB);
   const int64_t staging = kEpiWarps * boxes * static_cast<int64_t>(kOutBox);
-  for (int pair = 1; pair >= 0; --pair) {
-    if (pair && M <= kBM) continue;
+  for (int pair = 1; pair >= (pairs_only ? 1 : 0); --pair) {
+    if (pair && M <= kBM && !pairs_only) continue;
     const int ctas = pair ? 2 : 1;
     const int64_t mtiles = (M + kBM * ctas - 1) / (kBM * ctas);
-    const int64_t workers = sm_count / ctas;
+    const int64_t workers = pairs_only ? pairs_only : sm_count / ctas;
     for (int bn = 256; bn >= 64; bn -= pair ? 128 : 64) {
       const int span = mode == kGate ? bn / 2 : bn;
       const int64_t ntiles = (N + span - 1) / span;
       const int64_t stage = kABytes + static_cast<int64_t>(bn) * 128 / ctas;
       const int64_t stages = std::min<int64_t>(kMaxStages, (static_cast<int64_t>(kSmemMost) - staging) / stage);
-      // token splits that fill one, two, .. rounds of the workers
+      // token splits that fill one to four rounds of the workers
       const int64_t tiles = mtiles * ntiles;
       int64_t before = 0;
-      for (int64_t fill = 0; fill <= (mode == kWeight ? 8 : 0); ++fill) {
-        const int64_t want = std::min(std::min<int64_t>(KB, 64), std::max<int64_t>(1, fill * workers / tiles));
-        const int64_t per = (KB + want - 1) / want;
-        const int64_t splits = (KB + per - 1) / per;
+      for (int64_t fill = 1; fill <= (mode == kWeight ? 4 : 1); ++fill) {
+        const int64_t splits =
+            mode == kWeight ? std::min(std::min<int64_t>(KB, 64), std::max<int64_t>(1, fill * workers / tiles)) : 1;
         if (splits == before) continue;
         before = splits;
+        const int64_t per = (KB + splits - 1) / splits;
         const int64_t units = tiles * splits;
         const int64_t used = std::min(units, workers);
         const int64_t rounds = (units + used - 1) / used;
@@ -962,12 +1005,11 @@ GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, boo
         a.ntiles = static_cast<int>(ntiles);
         a.units = static_cast<int>(units);
         a.splits = static_cast<int>(splits);
-        a.kb_per_split = static_cast<int>(per);
         a.step_n = static_cast<int>(used % ntiles);
         a.step_m = static_cast<int>(used / ntiles);
         a.boxes = boxes;
         a.stages = static_cast<int>(stages);
-        a.rev = mode == kOutput || mode == kInput ? 1 : 0;
+        a.rev = mode == kOutput || mode == kInput || mode == kWeight ? 1 : 0;
         best.args = a;
         best.pair = pair;
         best.grid = static_cast<int>(used) * ctas;
@@ -1011,6 +1053,27 @@ bool encode_out(CUtensorMap* map, const void* ptr, bool half, int64_t rows, int6
   return encode(map, ptr, half, cols, rows, planes * cols, planes, cols, 1, 32, 32, true);
 }
 
+template <typename... Params, typename... Args>
+cudaError_t launch_clusters(const char* name, void (*kernel)(Params...), int grid, int cluster, size_t smem,
+                            cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  LaunchScope scope(name, stream);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int kMode, int kAct>
 cudaError_t launch_gemm(const char* name, const GemmPlan& p, bool half, const CUtensorMap& ma, const CUtensorMap& mb,
                         const CUtensorMap& mo, const CUtensorMap& mk, cudaStream_t stream) {
@@ -1018,22 +1081,14 @@ cudaError_t launch_gemm(const char* name, const GemmPlan& p, bool half, const CU
                        : (half ? &ffn_gemm_kernel<kMode, true, kAct, false> : &ffn_gemm_kernel<kMode, false, kAct, false>);
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), p.smem);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.grid));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = p.smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.pair ? 2 : 1;
-  LaunchScope scope(name, stream);
-  return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, mk, p.args);
+  return launch_clusters(name, kernel, p.grid, p.pair ? 2 : 1, p.smem, stream, ma, mb, mo, mk, p.args);
+}
+
+cudaError_t launch_products(const char* name, const BackwardProducts& p, size_t smem, bool half, cudaStream_t stream) {
+  auto kernel = half ? &ffn_backward_kernel<true> : &ffn_backward_kernel<false>;
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  return launch_clusters(name, kernel, 2 * p.first[3], 2, smem, stream, p);
 }
 
 template <typename S, typename W, int kAct, bool kGated>
@@ -1070,15 +1125,59 @@ int64_t colsum_splits(int64_t rows, int64_t D, int64_t H, int sm_count) {
   return std::max<int64_t>(1, std::min<int64_t>((rows + 63) / 64, 2 * sm_count / column_blocks));
 }
 
+// The products after [dg | du] and how the pairs are shared among those that
+// are wanted: in proportion to their contraction blocks and tiles.
+struct BackwardPlan {
+  GemmPlan product[3];  // input gradient, W_in's, W_out's
+  int first[4];
+};
+BackwardPlan plan_backward(int64_t T, int64_t D, int64_t H, int sm_count, const bool (&wanted)[3]) {
+  const int64_t sizes[3][3] = {{T, D, 2 * H}, {2 * H, D, T}, {D, H, T}};  // M, N, K
+  const Mode modes[3] = {kInput, kWeight, kWeight};
+  const int pairs = sm_count / 2;
+  double work[3] = {}, total = 0.0;
+  int most = -1;
+  for (int i = 0; i < 3; ++i) {
+    if (!wanted[i]) continue;
+    const int64_t tiles = ((sizes[i][0] + 255) / 256) * ((sizes[i][1] + 255) / 256);
+    work[i] = static_cast<double>(tiles) * ((sizes[i][2] + kBK - 1) / kBK * 655.0 + 2000.0);
+    total += work[i];
+    if (most < 0 || work[i] > work[most]) most = i;
+  }
+  BackwardPlan p{};
+  if (most < 0) return p;
+  int share[3] = {}, left = pairs;
+  for (int i = 0; i < 3; ++i) {
+    if (!wanted[i] || i == most) continue;
+    share[i] = std::max(1, static_cast<int>(pairs * work[i] / total + 0.5));
+    left -= share[i];
+  }
+  share[most] = std::max(1, left);
+  for (int i = 0; i < 3; ++i) {
+    if (wanted[i]) p.product[i] = plan_gemm(modes[i], sizes[i][0], sizes[i][1], sizes[i][2], sm_count, false, share[i]);
+    p.first[i + 1] = p.first[i] + p.product[i].grid / 2;
+  }
+  return p;
+}
+
+size_t partial_bytes(const GemmPlan& p) {
+  return p.args.splits > 1 ? sizeof(float) * p.args.splits * p.args.M * p.args.N : 0;
+}
+
 struct BackwardLayout {
-  GemmPlan w_in, w_out;
   int64_t colsums;
   size_t dgu, p_w_in, p_w_out, p_b_in, p_b_out, total;  // p_*: partials
 };
+// Room for every choice of wanted gradients (it changes the shares, and so the token splits).
 BackwardLayout backward_layout(int64_t T, int64_t D, int64_t H, int sm_count) {
   BackwardLayout l{};
-  l.w_in = plan_gemm(kWeight, 2 * H, D, T, sm_count);
-  l.w_out = plan_gemm(kWeight, D, H, T, sm_count);
+  size_t w_in = 0, w_out = 0;
+  for (int choice = 2; choice < 8; ++choice) {
+    const bool wanted[3] = {(choice & 1) != 0, (choice & 2) != 0, (choice & 4) != 0};
+    const BackwardPlan p = plan_backward(T, D, H, sm_count, wanted);
+    w_in = std::max(w_in, partial_bytes(p.product[1]));
+    w_out = std::max(w_out, partial_bytes(p.product[2]));
+  }
   l.colsums = colsum_splits(T, D, H, sm_count);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -1087,8 +1186,8 @@ BackwardLayout backward_layout(int64_t T, int64_t D, int64_t H, int sm_count) {
     return at;
   };
   l.dgu = take(sizeof(uint16_t) * T * 2 * H);
-  l.p_w_in = take(l.w_in.args.splits > 1 ? sizeof(float) * l.w_in.args.splits * 2 * H * D : 0);
-  l.p_w_out = take(l.w_out.args.splits > 1 ? sizeof(float) * l.w_out.args.splits * D * H : 0);
+  l.p_w_in = take(w_in);
+  l.p_w_out = take(w_out);
   l.p_b_in = take(sizeof(float) * l.colsums * 2 * H);
   l.p_b_out = take(sizeof(float) * l.colsums * D);
   l.total = off;
@@ -1106,18 +1205,6 @@ void add_array(ReduceBatch* batch, const float* partial, int splits, int64_t cou
   const int64_t per_block = splits >= kManySplits ? 32 : 256;  // quads
   batch->array[batch->arrays++] = ReduceArray{partial, out, count, splits, batch->blocks};
   batch->blocks += static_cast<int>((count / 4 + per_block - 1) / per_block);
-}
-
-// out [M, N] = a^T b over T tokens; with a token split its partials join `batch`.
-cudaError_t weight_gradient(GemmPlan p, const void* a, const void* b, bool half, int64_t T, void* out, int type,
-                            float* partial, ReduceBatch* batch, int* status, cudaStream_t stream) {
-  CUtensorMap ma{}, mb{};
-  if (!encode_mn(&ma, a, half, T, p.args.M) || !encode_mn(&mb, b, half, T, p.args.N)) return cudaErrorInvalidValue;
-  p.args.out = p.args.splits > 1 ? static_cast<void*>(partial) : out;
-  p.args.out_type = type;
-  p.args.status = status;
-  if (p.args.splits > 1) add_array(batch, partial, p.args.splits, static_cast<int64_t>(p.args.M) * p.args.N, out);
-  return launch_gemm<kWeight, kSilu>("ffn_wgrad", p, half, ma, mb, ma, ma, stream);
 }
 
 }  // namespace
@@ -1200,23 +1287,36 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
                               : launch_gemm<kSlope, kGelu>("ffn_slope", p, half, ma, mb, mo, mk, stream);
     if (e != cudaSuccess) return e;
   }
-  if (c.dx != nullptr) {
-    GemmPlan p = plan_gemm(kInput, c.T, c.D, 2 * c.H, sm_count);
-    if (!encode_k(&ma, dgu, half, c.T, 2 * c.H, kBM) || !encode_mn(&mb, c.w_in, half, 2 * c.H, c.D) ||
-        !encode_out(&mo, c.dx, half, c.T, c.D, 1)) {
-      return cudaErrorInvalidValue;
+  const bool wanted[3] = {c.dx != nullptr, c.dw_in != nullptr, c.dw_out != nullptr};
+  if (wanted[0] || wanted[1] || wanted[2]) {
+    const BackwardPlan plan = plan_backward(c.T, c.D, c.H, sm_count, wanted);
+    BackwardProducts p{};
+    size_t smem = 0;
+    for (int i = 0; i < 4; ++i) p.first[i] = plan.first[i];
+    for (int i = 0; i < 3; ++i) {
+      if (!wanted[i]) continue;
+      p.args[i] = plan.product[i].args;
+      p.args[i].status = c.status;
+      p.args[i].out_type = c.grad_type;
+      smem = std::max(smem, plan.product[i].smem);
     }
-    p.args.status = c.status;
-    e = launch_gemm<kInput, kSilu>("ffn_input", p, half, ma, mb, mo, mo, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (c.dw_in != nullptr) {
-    e = weight_gradient(l.w_in, dgu, c.x, half, c.T, c.dw_in, c.grad_type, partial(l.p_w_in), &batch, c.status, stream);
-    if (e != cudaSuccess) return e;
-  }
-  if (c.dw_out != nullptr) {
-    e = weight_gradient(l.w_out, c.dy, c.h, half, c.T, c.dw_out, c.grad_type, partial(l.p_w_out), &batch, c.status,
-                        stream);
+    bool ok = true;
+    if (wanted[0]) {
+      ok = ok && encode_k(&p.a[0], dgu, half, c.T, 2 * c.H, kBM) && encode_mn(&p.b[0], c.w_in, half, 2 * c.H, c.D) &&
+           encode_out(&p.out, c.dx, half, c.T, c.D, 1);
+    }
+    if (wanted[1]) ok = ok && encode_mn(&p.a[1], dgu, half, c.T, 2 * c.H) && encode_mn(&p.b[1], c.x, half, c.T, c.D);
+    if (wanted[2]) ok = ok && encode_mn(&p.a[2], c.dy, half, c.T, c.D) && encode_mn(&p.b[2], c.h, half, c.T, c.H);
+    if (!ok) return cudaErrorInvalidValue;
+    void* const grads[3] = {nullptr, c.dw_in, c.dw_out};
+    float* const partials[3] = {nullptr, partial(l.p_w_in), partial(l.p_w_out)};
+    for (int i = 1; i < 3; ++i) {
+      if (!wanted[i]) continue;
+      const GemmArgs& g = p.args[i];
+      p.args[i].out = g.splits > 1 ? static_cast<void*>(partials[i]) : grads[i];
+      if (g.splits > 1) add_array(&batch, partials[i], g.splits, static_cast<int64_t>(g.M) * g.N, grads[i]);
+    }
+    e = launch_products("ffn_products", p, smem, half, stream);
     if (e != cudaSuccess) return e;
   }
   if (c.db_in != nullptr || c.db_out != nullptr) {
