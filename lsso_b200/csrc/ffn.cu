@@ -709,6 +709,189 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                                        static_cast<int>(gridDim.x) / kCtas, sh);
 }
 
+// ---------------------------------------------------------------- few tiles
+// A forward product of fewer tiles than the GPU has SMs, its contraction split
+// over the CTAs of a cluster.  An SM takes in at most 62 bytes per cycle, so one
+// CTA that walks a long contraction alone is bound by that while most SMs idle.
+// A tile is 128 rows by 64 accumulator columns; each CTA contracts its share of
+// the blocks into its own TMEM, leaves the accumulators in shared memory, and
+// after a cluster barrier sums every split's part of its own slice of the
+// columns, in split order, adds the bias, and finishes and writes that slice.
+constexpr int kSplitColumns = 64;
+constexpr int kSplitThreads = 192;  // warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 TMEM readers, all: the sums
+constexpr int kSplitStages = 7;
+constexpr int kSplitPitch = kSplitColumns + 4;  // floats per row of the accumulators in shared memory (no bank conflicts)
+constexpr uint32_t kSplitStage = kABytes + kSplitColumns * kBK * 2;
+constexpr uint32_t kSplitSums = kBM * kSplitPitch * sizeof(float);
+
+struct SplitArgs {
+  int M, N, KB, ntiles, stages;
+  int box_rows;  // rows of the row operand's box; the rows below it hold anything, and nothing reads their products
+  int bias_type;
+  const void* bias;
+  void* out;
+  int* status;
+};
+
+__device__ __forceinline__ float4 load_remote4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
+  return v;
+}
+
+template <int kMode, bool kHalf, int kAct, int kSplits>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const SplitArgs a) {
+  pdl_wait();
+  constexpr int kSpan = kMode == kGate ? kSplitColumns / 2 : kSplitColumns;  // output columns of a tile
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[kSplitStages], empty[kSplitStages], tfull, mdrain;
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_flag;
+  volatile int* abort_v = &abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_rank());
+  const int tile = static_cast<int>(blockIdx.x) / kSplits;
+  const int nt = tile % a.ntiles, m0 = tile / a.ntiles * kBM;
+  const int kb0 = a.KB * rank / kSplits, blocks = a.KB * (rank + 1) / kSplits - kb0;
+  const int S = a.stages;
+  float* sums = reinterpret_cast<float*>(smem + S * kSplitStage);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(&tfull), 1);
+    mbar_init(smem_u32(&mdrain), 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_s), kSplitColumns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(full), empty_base = smem_u32(empty);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t a_bytes = static_cast<uint32_t>(a.box_rows) * kBK * 2;
+      int issued = 0;
+      for (RingPos rp; issued < blocks; rp.next(S), ++issued) {
+        if (!fwait(empty_base + 8 * rp.s, (rp.u & 1) ^ 1, abort_v, a.status)) break;
+        const uint32_t dst = smem_base + rp.s * kSplitStage, bar = full_base + 8 * rp.s;
+        const int k = (kb0 + issued) * kBK;
+        mbar_arrive_expect_tx(bar, a_bytes + kSplitColumns * kBK * 2);
+        tma_load_2d(dst, &map_a, k, m0, bar);
+        if (kMode == kGate) {
+          tma_load_3d(dst + kABytes, &map_b, k, nt * kSpan, 0, bar);
+          tma_load_3d(dst + kABytes + kSpan * kBK * 2, &map_b, k, nt * kSpan, 1, bar);
+        } else {
+          tma_load_2d(dst + kABytes, &map_b, k, nt * kSpan, bar);
+        }
+      }
+      // no load is on its way past this point (the last use of each stage)
+      for (int i = max(0, issued - S); i < issued; ++i) {
+        mbar_wait(full_base + 8 * (i % S), static_cast<uint32_t>(i / S) & 1u, a.status);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = make_idesc(kBM, kSplitColumns, false, false) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
+      const uint64_t adesc = make_desc_sw128(smem_base, 16, 1024);
+      const uint64_t bdesc = make_desc_sw128(smem_base + kABytes, 16, 1024);
+      RingPos rp;
+      bool ok = true;
+      for (int i = 0; i < blocks && ok; ++i, rp.next(S)) {
+        ok = fwait(full_base + 8 * rp.s, rp.u & 1, abort_v, a.status);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t off = static_cast<uint32_t>(rp.s) * (kSplitStage / 16);
+#pragma unroll
+        for (int ks = 0; ks < kBK / 16; ++ks) {
+          mma<false>(tmem, adesc + off + 2 * ks, bdesc + off + 2 * ks, idesc, (i > 0 || ks > 0) ? 1u : 0u);
+        }
+        mma_commit(empty_base + 8 * rp.s);
+      }
+      if (ok) mma_commit(smem_u32(&tfull));
+      mma_commit(smem_u32(&mdrain));
+      mbar_wait_bounded(smem_u32(&mdrain), 0, nullptr, a.status);
+    }
+    __syncwarp();
+  } else {
+    const int sub = warp & 3;
+    if (fwait_warp(smem_u32(&tfull), 0, abort_v, a.status)) {
+      tc_fence_after();
+      const uint32_t acc = tmem + (static_cast<uint32_t>(32 * sub) << 16);
+      float4* row = reinterpret_cast<float4*>(sums + (32 * sub + lane) * kSplitPitch);
+#pragma unroll
+      for (int c = 0; c < kSplitColumns; c += 32) {
+        float v[32];
+        tmem_ld32(acc + c, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) row[c / 4 + j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      }
+    }
+    tc_fence_before();
+  }
+
+  __syncwarp();
+  cluster_sync();
+  constexpr int kSlice = kSpan / kSplits, kQuads = kSlice / 4;
+  const int rows = min(kBM, a.M - m0);
+  for (int item = threadIdx.x; item < rows * kQuads; item += kSplitThreads) {
+    const int r = item / kQuads, c = rank * kSlice + 4 * (item % kQuads), n = nt * kSpan + c;
+    if (n >= a.N) continue;
+    const uint32_t at = smem_u32(sums + r * kSplitPitch + c);
+    float4 part[kSplits], other[kSplits];
+#pragma unroll
+    for (int i = 0; i < kSplits; ++i) {
+      const uint32_t remote = map_rank(at, static_cast<uint32_t>(i));
+      part[i] = load_remote4(remote);
+      if (kMode == kGate) other[i] = load_remote4(remote + kSpan * sizeof(float));
+    }
+    float v[4] = {}, u[4] = {};
+    if (a.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = read_bias(a.bias, a.bias_type, n + j);
+        if (kMode == kGate) u[j] = read_bias(a.bias, a.bias_type, static_cast<int64_t>(a.N) + n + j);
+      }
+    }
+    float4 sv = part[0], su = other[0];
+#pragma unroll
+    for (int i = 1; i < kSplits; ++i) {
+      sv = make_float4(sv.x + part[i].x, sv.y + part[i].y, sv.z + part[i].z, sv.w + part[i].w);
+      if (kMode == kGate) su = make_float4(su.x + other[i].x, su.y + other[i].y, su.z + other[i].z, su.w + other[i].w);
+    }
+    v[0] += sv.x, v[1] += sv.y, v[2] += sv.z, v[3] += sv.w;
+    if (kMode == kGate) {
+      u[0] += su.x, u[1] += su.y, u[2] += su.z, u[3] += su.w;
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        ActSlope s0, s1;
+        activate2<kAct>(v[j], v[j + 1], s0, s1);
+        v[j] = s0.act * u[j];
+        v[j + 1] = s1.act * u[j + 1];
+      }
+    }
+    uint16_t* o = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(m0 + r) * a.N + n;
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<kHalf>(v[0], v[1]), pack2<kHalf>(v[2], v[3]));
+  }
+  __syncwarp();
+  cluster_sync();  // no CTA reads this one's shared memory any more
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kSplitColumns);
+  }
+}
+
 // The products that follow [dg | du] in one launch, side by side on the pairs:
 // the input gradient and both weight gradients, each on a share of the pairs
 // that fits its work.  They walk the tokens together, so that [dg | du] comes
@@ -1054,11 +1237,11 @@ bool encode_out(CUtensorMap* map, const void* ptr, bool half, int64_t rows, int6
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch_clusters(const char* name, void (*kernel)(Params...), int grid, int cluster, size_t smem,
-                            cudaStream_t stream, const Args&... args) {
+cudaError_t launch_clusters(const char* name, void (*kernel)(Params...), int grid, int cluster, int threads,
+                            size_t smem, cudaStream_t stream, const Args&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1081,14 +1264,14 @@ cudaError_t launch_gemm(const char* name, const GemmPlan& p, bool half, const CU
                        : (half ? &ffn_gemm_kernel<kMode, true, kAct, false> : &ffn_gemm_kernel<kMode, false, kAct, false>);
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), p.smem);
   if (e != cudaSuccess) return e;
-  return launch_clusters(name, kernel, p.grid, p.pair ? 2 : 1, p.smem, stream, ma, mb, mo, mk, p.args);
+  return launch_clusters(name, kernel, p.grid, p.pair ? 2 : 1, kThreads, p.smem, stream, ma, mb, mo, mk, p.args);
 }
 
 cudaError_t launch_products(const char* name, const BackwardProducts& p, size_t smem, bool half, cudaStream_t stream) {
   auto kernel = half ? &ffn_backward_kernel<true> : &ffn_backward_kernel<false>;
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
-  return launch_clusters(name, kernel, 2 * p.first[3], 2, smem, stream, p);
+  return launch_clusters(name, kernel, 2 * p.first[3], 2, kThreads, smem, stream, p);
 }
 
 template <typename S, typename W, int kAct, bool kGated>
@@ -1207,6 +1390,59 @@ void add_array(ReduceBatch* batch, const float* partial, int splits, int64_t cou
   batch->blocks += static_cast<int>((count / 4 + per_block - 1) / per_block);
 }
 
+// CTAs per tile of a forward product that has few tiles: the largest cluster
+// with which all tiles still run at once (sixteen clusters of eight fit) and
+// each CTA has two contraction blocks; 1: the persistent kernel.
+int split_of(int64_t M, int64_t N, int64_t KB, int span) {
+  const int64_t tiles = (M + kBM - 1) / kBM * ((N + span - 1) / span);
+  for (int splits = 8; splits > 1; splits /= 2) {
+    if (tiles * splits <= 128 && KB >= 2 * splits) return splits;
+  }
+  return 1;
+}
+
+template <int kMode, bool kHalf, int kAct>
+cudaError_t launch_split(const char* name, int splits, const CUtensorMap& ma, const CUtensorMap& mb, const SplitArgs& a,
+                         cudaStream_t stream) {
+  auto kernel = splits == 8   ? &ffn_split_kernel<kMode, kHalf, kAct, 8>
+                : splits == 4 ? &ffn_split_kernel<kMode, kHalf, kAct, 4>
+                              : &ffn_split_kernel<kMode, kHalf, kAct, 2>;
+  const size_t smem = a.stages * static_cast<size_t>(kSplitStage) + kSplitSums;
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  const int tiles = (a.M + kBM - 1) / kBM * a.ntiles;
+  return launch_clusters(name, kernel, tiles * splits, splits, kSplitThreads, smem, stream, ma, mb, a);
+}
+// x [T, K] times the rows of w (kGate: both planes), split over clusters.
+template <int kMode>
+cudaError_t forward_split(const char* name, int splits, const FfnForwardCall& c, const void* x, const void* w,
+                          const void* bias, void* out, int64_t N, int64_t K, cudaStream_t stream) {
+  constexpr int kSpan = kMode == kGate ? kSplitColumns / 2 : kSplitColumns;
+  const bool half = c.type == kFp16;
+  SplitArgs a{};
+  a.M = static_cast<int>(c.T);
+  a.N = static_cast<int>(N);
+  a.KB = static_cast<int>((K + kBK - 1) / kBK);
+  a.ntiles = static_cast<int>((N + kSpan - 1) / kSpan);
+  a.stages = std::min(kSplitStages, (a.KB + splits - 1) / splits);
+  a.box_rows = static_cast<int>(std::min<int64_t>(kBM, (c.T + 7) / 8 * 8));
+  a.bias = bias;
+  a.bias_type = c.bias_type;
+  a.out = out;
+  a.status = c.status;
+  CUtensorMap ma{}, mb{};
+  if (!encode_k(&ma, x, half, c.T, K, a.box_rows) ||
+      !(kMode == kGate ? encode(&mb, w, half, K, N, K, 2, N * K, 0, kBK, kSpan, false) : encode_k(&mb, w, half, N, K, kSpan))) {
+    return cudaErrorInvalidValue;
+  }
+  if (kMode == kGate && c.activation != kSilu) {
+    return half ? launch_split<kMode, true, kGelu>(name, splits, ma, mb, a, stream)
+                : launch_split<kMode, false, kGelu>(name, splits, ma, mb, a, stream);
+  }
+  return half ? launch_split<kMode, true, kSilu>(name, splits, ma, mb, a, stream)
+              : launch_split<kMode, false, kSilu>(name, splits, ma, mb, a, stream);
+}
+
 }  // namespace
 
 cudaError_t launch_ffn_cast(const float* const src[2], void* const dst[2], const int64_t count[2], int type,
@@ -1237,7 +1473,11 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
   }
   if (c.weight_type == kFp32) return cudaErrorInvalidValue;
   CUtensorMap ma{}, mb{}, mo{}, mg{};
-  {
+  const int gate_splits = c.kept != nullptr ? 1 : split_of(c.T, c.H, (c.D + kBK - 1) / kBK, kSplitColumns / 2);
+  if (gate_splits > 1) {
+    const cudaError_t e = forward_split<kGate>("ffn_gate", gate_splits, c, c.x, c.w_in, c.b_in, c.h, c.H, c.D, stream);
+    if (e != cudaSuccess) return e;
+  } else {
     GemmPlan p = plan_gemm(kGate, c.T, c.H, c.D, sm_count, c.kept != nullptr);
     if (!encode_k(&ma, c.x, half, c.T, c.D, kBM) ||
         !encode(&mb, c.w_in, half, c.D, c.H, c.D, 2, c.H * c.D, 0, kBK, p.args.BN / 2, false) ||
@@ -1252,6 +1492,10 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
     const cudaError_t e = c.activation == kSilu ? launch_gemm<kGate, kSilu>("ffn_gate", p, half, ma, mb, mo, mg, stream)
                                                 : launch_gemm<kGate, kGelu>("ffn_gate", p, half, ma, mb, mo, mg, stream);
     if (e != cudaSuccess) return e;
+  }
+  const int splits = split_of(c.T, c.D, (c.H + kBK - 1) / kBK, kSplitColumns);
+  if (splits > 1) {
+    return forward_split<kOutput>("ffn_output", splits, c, c.h, c.w_out, c.b_out, c.y, c.D, c.H, stream);
   }
   GemmPlan p = plan_gemm(kOutput, c.T, c.D, c.H, sm_count);
   if (!encode_k(&ma, c.h, half, c.T, c.H, kBM) || !encode_k(&mb, c.w_out, half, c.D, c.H, p.pair ? p.args.BN / 2 : p.args.BN) ||

@@ -328,3 +328,53 @@ def test_waits_that_run_out_leave_a_usable_library() -> None:
         assert cuda.device_status(reset=True) == 1
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
         assert cuda.device_status(reset=True) == 0
+
+
+# few rows without gradients: products of few tiles, their contraction split over two, four and eight CTAs
+FEW = [(17, 256, 688), (24, 64, 1024), (31, 1024, 64), (97, 512, 1368), (128, 1000, 4096), (129, 512, 520),
+       (250, 200, 2000), (400, 136, 344), (512, 1024, 1024)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", FEW)
+@pytest.mark.parametrize(("dtype", "activation", "bias"), [
+    (torch.bfloat16, "silu", True), (torch.float16, "gelu", False), (torch.float16, "silu", True),
+    (torch.bfloat16, "gelu", True)])
+def test_few_rows_without_gradients(shape, dtype, activation, bias) -> None:
+    from tests.gpu_util import require_native
+
+    require_native()
+    x, w_in, w_out, b_in, b_out, dy = _inputs(*shape, dtype, dtype, bias)
+    want = _exact(x, w_in, w_out, b_in, b_out, dy, activation)["y"]
+    with torch.no_grad():
+        y = gated_feed_forward(x, w_in, w_out, b_in, b_out, activation=activation)
+        _within("y", y, *want, dtype)
+        assert torch.equal(y, gated_feed_forward(x, w_in, w_out, b_in, b_out, activation=activation))
+        # a row's result depends on its own values alone, whatever the rows beside it hold
+        x[0], x[-1] = float("inf"), float("nan")
+        other = gated_feed_forward(x, w_in, w_out, b_in, b_out, activation=activation)
+    assert torch.equal(y[1:-1], other[1:-1]) and not torch.isfinite(other[[0, -1]]).any()
+
+
+@pytest.mark.gpu
+def test_split_waits_that_run_out_leave_a_usable_library() -> None:
+    """The same for the products whose contraction is split over a cluster."""
+    from lsso_b200.ball import _native, cuda
+    from tests.gpu_util import require_native
+
+    require_native()
+    cuda.device_status(reset=True)
+    for shape in ((20, 128, 512), (100, 512, 1368), (128, 1024, 4096)):
+        args = _inputs(*shape, torch.bfloat16, torch.bfloat16, True)[:5]
+        with torch.no_grad():
+            want = gated_feed_forward(*args)
+            torch.cuda.synchronize()
+            _native.set_wait_limit_ns(1)
+            try:
+                gated_feed_forward(*args)
+                torch.cuda.synchronize()
+            finally:
+                _native.set_wait_limit_ns(0)
+            assert cuda.device_status(reset=True) == 1
+            assert torch.equal(gated_feed_forward(*args), want)
+            assert cuda.device_status(reset=True) == 0
