@@ -710,16 +710,23 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 }
 
 // ---------------------------------------------------------------- few tiles
-// A forward product of fewer tiles than the GPU has SMs, its contraction split
-// over the CTAs of a cluster.  An SM takes in at most 62 bytes per cycle, so one
-// CTA that walks a long contraction alone is bound by that while most SMs idle.
-// A tile is 128 rows by 64 accumulator columns; each CTA contracts its share of
-// the blocks into its own TMEM, leaves the accumulators in shared memory, and
-// after a cluster barrier sums every split's part of its own slice of the
-// columns, in split order, adds the bias, and finishes and writes that slice.
+// A forward product of few tiles, its contraction split over the CTAs of a
+// cluster where that fills more SMs.  An SM takes in at most 62 bytes per cycle,
+// so one CTA that walks a long contraction alone is bound by that while most SMs
+// idle.  A tile is 128 rows by 64 accumulator columns; each CTA contracts its
+// share of the blocks into its own TMEM, leaves the accumulators in shared
+// memory, and after a cluster barrier sums every split's part of its own slice
+// of the columns, in split order, adds the bias, and finishes and writes that
+// slice.  Three stages, so that two CTAs fit an SM (with seven, 128 tokens 1024
+// -> 4096 took 28 us instead of 18.5: an SM holds one, and sixteen clusters of
+// eight do not all fit).  The next kernel may launch as soon as this one runs:
+// every kernel here starts by waiting for the one before it (1 us per call).
+// Both products against the persistent kernel, as a graph: 17 tokens 256 / 688:
+// 14.3 -> 6.4 us; 97 tokens 512 / 1368: 19.5 -> 10.8; 32 tokens 1024 / 4096:
+// 35 -> 13.3; 1024 tokens 256 / 688: 17.5 -> 11.7; 2048 tokens: 18.1 -> 15.0.
 constexpr int kSplitColumns = 64;
 constexpr int kSplitThreads = 192;  // warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 TMEM readers, all: the sums
-constexpr int kSplitStages = 7;
+constexpr int kSplitStages = 3;
 constexpr int kSplitPitch = kSplitColumns + 4;  // floats per row of the accumulators in shared memory (no bank conflicts)
 constexpr uint32_t kSplitStage = kABytes + kSplitColumns * kBK * 2;
 constexpr uint32_t kSplitSums = kBM * kSplitPitch * sizeof(float);
@@ -729,6 +736,7 @@ struct SplitArgs {
   int box_rows;  // rows of the row operand's box; the rows below it hold anything, and nothing reads their products
   int bias_type;
   const void* bias;
+  void* kept;  // kGate: [M, 2, N]; nullable
   void* out;
   int* status;
 };
@@ -743,9 +751,8 @@ __device__ __forceinline__ float4 load_remote4(uint32_t cluster_addr) {
 }
 
 template <int kMode, bool kHalf, int kAct, int kSplits>
-__global__ void __launch_bounds__(kSplitThreads, 1)
+__global__ void __launch_bounds__(kSplitThreads, 2)
 ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const SplitArgs a) {
-  pdl_wait();
   constexpr int kSpan = kMode == kGate ? kSplitColumns / 2 : kSplitColumns;  // output columns of a tile
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kSplitStages], empty[kSplitStages], tfull, mdrain;
@@ -776,6 +783,8 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = tmem_s;
   const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(full), empty_base = smem_u32(empty);
+  pdl_wait();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp == 0) {
     if (lane == 0) {
@@ -873,6 +882,11 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     v[0] += sv.x, v[1] += sv.y, v[2] += sv.z, v[3] += sv.w;
     if (kMode == kGate) {
       u[0] += su.x, u[1] += su.y, u[2] += su.z, u[3] += su.w;
+      if (a.kept != nullptr) {
+        uint16_t* k = static_cast<uint16_t*>(a.kept) + static_cast<int64_t>(m0 + r) * 2 * a.N + n;
+        *reinterpret_cast<uint2*>(k) = make_uint2(pack2<kHalf>(v[0], v[1]), pack2<kHalf>(v[2], v[3]));
+        *reinterpret_cast<uint2*>(k + a.N) = make_uint2(pack2<kHalf>(u[0], u[1]), pack2<kHalf>(u[2], u[3]));
+      }
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
         ActSlope s0, s1;
@@ -1390,15 +1404,19 @@ void add_array(ReduceBatch* batch, const float* partial, int splits, int64_t cou
   batch->blocks += static_cast<int>((count / 4 + per_block - 1) / per_block);
 }
 
-// CTAs per tile of a forward product that has few tiles: the largest cluster
-// with which all tiles still run at once (sixteen clusters of eight fit) and
-// each CTA has two contraction blocks; 1: the persistent kernel.
+// CTAs per tile of a forward product of few tiles; 0: the persistent kernel.
+// Four or eight only while all clusters run at once (43 gate tiles of 97 tokens
+// 512 / 1368 in two CTAs each instead of four: 10.8 us against 12.3; 22 of 256
+// tokens 256 / 688 in four each instead of eight: 9.7 against 12.8), two while
+// that is two CTAs per SM, and one up to 512 tiles (4096 tokens 256 / 688, 704
+// gate tiles: 20.8 us against the persistent kernel's 20.0; 2048 tokens, 352:
+// 15.0 against 16.4).
 int split_of(int64_t M, int64_t N, int64_t KB, int span) {
   const int64_t tiles = (M + kBM - 1) / kBM * ((N + span - 1) / span);
   for (int splits = 8; splits > 1; splits /= 2) {
-    if (tiles * splits <= 128 && KB >= 2 * splits) return splits;
+    if (tiles * splits <= (splits == 2 ? 256 : 128) && KB >= splits) return splits;
   }
-  return 1;
+  return tiles <= 512 ? 1 : 0;
 }
 
 template <int kMode, bool kHalf, int kAct>
@@ -1406,7 +1424,8 @@ cudaError_t launch_split(const char* name, int splits, const CUtensorMap& ma, co
                          cudaStream_t stream) {
   auto kernel = splits == 8   ? &ffn_split_kernel<kMode, kHalf, kAct, 8>
                 : splits == 4 ? &ffn_split_kernel<kMode, kHalf, kAct, 4>
-                              : &ffn_split_kernel<kMode, kHalf, kAct, 2>;
+                : splits == 2 ? &ffn_split_kernel<kMode, kHalf, kAct, 2>
+                              : &ffn_split_kernel<kMode, kHalf, kAct, 1>;
   const size_t smem = a.stages * static_cast<size_t>(kSplitStage) + kSplitSums;
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
@@ -1428,6 +1447,7 @@ cudaError_t forward_split(const char* name, int splits, const FfnForwardCall& c,
   a.box_rows = static_cast<int>(std::min<int64_t>(kBM, (c.T + 7) / 8 * 8));
   a.bias = bias;
   a.bias_type = c.bias_type;
+  a.kept = kMode == kGate ? c.kept : nullptr;
   a.out = out;
   a.status = c.status;
   CUtensorMap ma{}, mb{};
@@ -1473,8 +1493,8 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
   }
   if (c.weight_type == kFp32) return cudaErrorInvalidValue;
   CUtensorMap ma{}, mb{}, mo{}, mg{};
-  const int gate_splits = c.kept != nullptr ? 1 : split_of(c.T, c.H, (c.D + kBK - 1) / kBK, kSplitColumns / 2);
-  if (gate_splits > 1) {
+  const int gate_splits = split_of(c.T, c.H, (c.D + kBK - 1) / kBK, kSplitColumns / 2);
+  if (gate_splits > 0) {
     const cudaError_t e = forward_split<kGate>("ffn_gate", gate_splits, c, c.x, c.w_in, c.b_in, c.h, c.H, c.D, stream);
     if (e != cudaSuccess) return e;
   } else {
@@ -1494,7 +1514,7 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
     if (e != cudaSuccess) return e;
   }
   const int splits = split_of(c.T, c.D, (c.H + kBK - 1) / kBK, kSplitColumns);
-  if (splits > 1) {
+  if (splits > 0) {
     return forward_split<kOutput>("ffn_output", splits, c, c.h, c.w_out, c.b_out, c.y, c.D, c.H, stream);
   }
   GemmPlan p = plan_gemm(kOutput, c.T, c.D, c.H, sm_count);
