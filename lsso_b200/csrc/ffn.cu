@@ -14,7 +14,8 @@
 // A training forward also keeps [g | u], rounded once to the same type, which
 // is what the backward's epilogue reads.
 //
-// Every product is one instance of one persistent, warp-specialised kernel:
+// Every product (but those of few tiles, further down) is an instance of one
+// persistent, warp-specialised kernel:
 //   warps 0, 2   TMA producers of the row and of the column operand (one thread
 //                each; one thread for both took longer per block than its products)
 //   warp 1       MMA issuer (one thread issues tcgen05.mma kind::f16)
@@ -710,8 +711,9 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 }
 
 // ---------------------------------------------------------------- few tiles
-// A forward product of few tiles, its contraction split over the CTAs of a
-// cluster where that fills more SMs.  An SM takes in at most 62 bytes per cycle,
+// A product of few tiles, its contraction split over the CTAs of a cluster
+// where that fills more SMs (both forward products, the slopes, and the input
+// gradient).  An SM takes in at most 62 bytes per cycle,
 // so one CTA that walks a long contraction alone is bound by that while most SMs
 // idle.  A tile is 128 rows by 64 accumulator columns; each CTA contracts its
 // share of the blocks into its own TMEM, leaves the accumulators in shared
@@ -736,8 +738,8 @@ struct SplitArgs {
   int box_rows;  // rows of the row operand's box; the rows below it hold anything, and nothing reads their products
   int bias_type;
   const void* bias;
-  void* kept;  // kGate: [M, 2, N]; nullable
-  void* out;
+  void* kept;  // kGate: [M, 2, N], nullable; kSlope: the same, read
+  void* out;   // kSlope: [M, 2, N]
   int* status;
 };
 
@@ -754,6 +756,7 @@ template <int kMode, bool kHalf, int kAct, int kSplits>
 __global__ void __launch_bounds__(kSplitThreads, 2)
 ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const SplitArgs a) {
   constexpr int kSpan = kMode == kGate ? kSplitColumns / 2 : kSplitColumns;  // output columns of a tile
+  constexpr bool kBmn = kMode == kSlope || kMode == kInput;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[kSplitStages], empty[kSplitStages], tfull, mdrain;
   __shared__ uint32_t tmem_s;
@@ -799,6 +802,8 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (kMode == kGate) {
           tma_load_3d(dst + kABytes, &map_b, k, nt * kSpan, 0, bar);
           tma_load_3d(dst + kABytes + kSpan * kBK * 2, &map_b, k, nt * kSpan, 1, bar);
+        } else if (kBmn) {
+          tma_load_2d(dst + kABytes, &map_b, nt * kSpan, k, bar);
         } else {
           tma_load_2d(dst + kABytes, &map_b, k, nt * kSpan, bar);
         }
@@ -811,9 +816,10 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = make_idesc(kBM, kSplitColumns, false, false) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
+      const uint32_t idesc = make_idesc(kBM, kSplitColumns, false, kBmn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
       const uint64_t adesc = make_desc_sw128(smem_base, 16, 1024);
-      const uint64_t bdesc = make_desc_sw128(smem_base + kABytes, 16, 1024);
+      const uint64_t bdesc = make_desc_sw128(smem_base + kABytes, kBmn ? kBox : 16, 1024);
+      constexpr uint32_t kBStep = kBmn ? 2048 / 16 : 32 / 16;
       RingPos rp;
       bool ok = true;
       for (int i = 0; i < blocks && ok; ++i, rp.next(S)) {
@@ -823,7 +829,7 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const uint32_t off = static_cast<uint32_t>(rp.s) * (kSplitStage / 16);
 #pragma unroll
         for (int ks = 0; ks < kBK / 16; ++ks) {
-          mma<false>(tmem, adesc + off + 2 * ks, bdesc + off + 2 * ks, idesc, (i > 0 || ks > 0) ? 1u : 0u);
+          mma<false>(tmem, adesc + off + 2 * ks, bdesc + off + kBStep * ks, idesc, (i > 0 || ks > 0) ? 1u : 0u);
         }
         mma_commit(empty_base + 8 * rp.s);
       }
@@ -858,6 +864,13 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int r = item / kQuads, c = rank * kSlice + 4 * (item % kQuads), n = nt * kSpan + c;
     if (n >= a.N) continue;
     const uint32_t at = smem_u32(sums + r * kSplitPitch + c);
+    // kSlope: the kept pre-activations, of a pair of columns each
+    const int64_t at2 = static_cast<int64_t>(m0 + r) * 2 * a.N + n;
+    uint2 gw{}, uw{};
+    if (kMode == kSlope) {
+      gw = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.kept) + at2));
+      uw = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.kept) + at2 + a.N));
+    }
     float4 part[kSplits], other[kSplits];
 #pragma unroll
     for (int i = 0; i < kSplits; ++i) {
@@ -883,7 +896,7 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (kMode == kGate) {
       u[0] += su.x, u[1] += su.y, u[2] += su.z, u[3] += su.w;
       if (a.kept != nullptr) {
-        uint16_t* k = static_cast<uint16_t*>(a.kept) + static_cast<int64_t>(m0 + r) * 2 * a.N + n;
+        uint16_t* k = static_cast<uint16_t*>(a.kept) + at2;
         *reinterpret_cast<uint2*>(k) = make_uint2(pack2<kHalf>(v[0], v[1]), pack2<kHalf>(v[2], v[3]));
         *reinterpret_cast<uint2*>(k + a.N) = make_uint2(pack2<kHalf>(u[0], u[1]), pack2<kHalf>(u[2], u[3]));
       }
@@ -894,6 +907,22 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         v[j] = s0.act * u[j];
         v[j + 1] = s1.act * u[j + 1];
       }
+    }
+    if (kMode == kSlope) {
+      const float2 g2[2] = {unpack2<kHalf>(gw.x), unpack2<kHalf>(gw.y)};
+      const float2 u2[2] = {unpack2<kHalf>(uw.x), unpack2<kHalf>(uw.y)};
+      uint32_t dg[2], du[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        ActSlope s0, s1;
+        activate2<kAct>(g2[j].x, g2[j].y, s0, s1);
+        dg[j] = pack2<kHalf>(v[2 * j] * u2[j].x * s0.slope, v[2 * j + 1] * u2[j].y * s1.slope);
+        du[j] = pack2<kHalf>(v[2 * j] * s0.act, v[2 * j + 1] * s1.act);
+      }
+      uint16_t* o = static_cast<uint16_t*>(a.out) + at2;
+      *reinterpret_cast<uint2*>(o) = make_uint2(dg[0], dg[1]);
+      *reinterpret_cast<uint2*>(o + a.N) = make_uint2(du[0], du[1]);
+      continue;
     }
     uint16_t* o = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(m0 + r) * a.N + n;
     *reinterpret_cast<uint2*>(o) = make_uint2(pack2<kHalf>(v[0], v[1]), pack2<kHalf>(v[2], v[3]));
@@ -1404,19 +1433,19 @@ void add_array(ReduceBatch* batch, const float* partial, int splits, int64_t cou
   batch->blocks += static_cast<int>((count / 4 + per_block - 1) / per_block);
 }
 
-// CTAs per tile of a forward product of few tiles; 0: the persistent kernel.
+// CTAs per tile of a product of few tiles; 0: the persistent kernel.
 // Four or eight only while all clusters run at once (43 gate tiles of 97 tokens
 // 512 / 1368 in two CTAs each instead of four: 10.8 us against 12.3; 22 of 256
 // tokens 256 / 688 in four each instead of eight: 9.7 against 12.8), two while
 // that is two CTAs per SM, and one up to 512 tiles (4096 tokens 256 / 688, 704
 // gate tiles: 20.8 us against the persistent kernel's 20.0; 2048 tokens, 352:
-// 15.0 against 16.4).
-int split_of(int64_t M, int64_t N, int64_t KB, int span) {
+// 15.0 against 16.4), `most` of them.
+int split_of(int64_t M, int64_t N, int64_t KB, int span, int64_t most = 512) {
   const int64_t tiles = (M + kBM - 1) / kBM * ((N + span - 1) / span);
   for (int splits = 8; splits > 1; splits /= 2) {
     if (tiles * splits <= (splits == 2 ? 256 : 128) && KB >= splits) return splits;
   }
-  return tiles <= 512 ? 1 : 0;
+  return tiles <= most ? 1 : 0;
 }
 
 template <int kMode, bool kHalf, int kAct>
@@ -1432,35 +1461,38 @@ cudaError_t launch_split(const char* name, int splits, const CUtensorMap& ma, co
   const int tiles = (a.M + kBM - 1) / kBM * a.ntiles;
   return launch_clusters(name, kernel, tiles * splits, splits, kSplitThreads, smem, stream, ma, mb, a);
 }
-// x [T, K] times the rows of w (kGate: both planes), split over clusters.
+// x [T, K] times w: its rows (kGate: of both planes), or (kSlope, kInput) its columns.
 template <int kMode>
-cudaError_t forward_split(const char* name, int splits, const FfnForwardCall& c, const void* x, const void* w,
-                          const void* bias, void* out, int64_t N, int64_t K, cudaStream_t stream) {
+cudaError_t product_split(const char* name, int splits, SplitArgs a, bool half, int activation, const void* x,
+                          const void* w, int64_t K, cudaStream_t stream) {
   constexpr int kSpan = kMode == kGate ? kSplitColumns / 2 : kSplitColumns;
-  const bool half = c.type == kFp16;
-  SplitArgs a{};
-  a.M = static_cast<int>(c.T);
-  a.N = static_cast<int>(N);
   a.KB = static_cast<int>((K + kBK - 1) / kBK);
-  a.ntiles = static_cast<int>((N + kSpan - 1) / kSpan);
+  a.ntiles = (a.N + kSpan - 1) / kSpan;
   a.stages = std::min(kSplitStages, (a.KB + splits - 1) / splits);
-  a.box_rows = static_cast<int>(std::min<int64_t>(kBM, (c.T + 7) / 8 * 8));
-  a.bias = bias;
-  a.bias_type = c.bias_type;
-  a.kept = kMode == kGate ? c.kept : nullptr;
-  a.out = out;
-  a.status = c.status;
+  a.box_rows = std::min(kBM, (a.M + 7) / 8 * 8);
   CUtensorMap ma{}, mb{};
-  if (!encode_k(&ma, x, half, c.T, K, a.box_rows) ||
-      !(kMode == kGate ? encode(&mb, w, half, K, N, K, 2, N * K, 0, kBK, kSpan, false) : encode_k(&mb, w, half, N, K, kSpan))) {
-    return cudaErrorInvalidValue;
-  }
-  if (kMode == kGate && c.activation != kSilu) {
+  const bool ok = encode_k(&ma, x, half, a.M, K, a.box_rows) &&
+                  (kMode == kGate     ? encode(&mb, w, half, K, a.N, K, 2, a.N * K, 0, kBK, kSpan, false)
+                   : kMode == kOutput ? encode_k(&mb, w, half, a.N, K, kSpan)
+                                      : encode_mn(&mb, w, half, K, a.N));
+  if (!ok) return cudaErrorInvalidValue;
+  if ((kMode == kGate || kMode == kSlope) && activation != kSilu) {
     return half ? launch_split<kMode, true, kGelu>(name, splits, ma, mb, a, stream)
                 : launch_split<kMode, false, kGelu>(name, splits, ma, mb, a, stream);
   }
   return half ? launch_split<kMode, true, kSilu>(name, splits, ma, mb, a, stream)
               : launch_split<kMode, false, kSilu>(name, splits, ma, mb, a, stream);
+}
+SplitArgs split_args(int64_t M, int64_t N, const void* bias, int bias_type, void* kept, void* out, int* status) {
+  SplitArgs a{};
+  a.M = static_cast<int>(M);
+  a.N = static_cast<int>(N);
+  a.bias = bias;
+  a.bias_type = bias_type;
+  a.kept = kept;
+  a.out = out;
+  a.status = status;
+  return a;
 }
 
 }  // namespace
@@ -1495,7 +1527,9 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
   CUtensorMap ma{}, mb{}, mo{}, mg{};
   const int gate_splits = split_of(c.T, c.H, (c.D + kBK - 1) / kBK, kSplitColumns / 2);
   if (gate_splits > 0) {
-    const cudaError_t e = forward_split<kGate>("ffn_gate", gate_splits, c, c.x, c.w_in, c.b_in, c.h, c.H, c.D, stream);
+    const cudaError_t e = product_split<kGate>(
+        "ffn_gate", gate_splits, split_args(c.T, c.H, c.b_in, c.bias_type, c.kept, c.h, c.status), half, c.activation, c.x,
+        c.w_in, c.D, stream);
     if (e != cudaSuccess) return e;
   } else {
     GemmPlan p = plan_gemm(kGate, c.T, c.H, c.D, sm_count, c.kept != nullptr);
@@ -1515,7 +1549,9 @@ cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream
   }
   const int splits = split_of(c.T, c.D, (c.H + kBK - 1) / kBK, kSplitColumns);
   if (splits > 0) {
-    return forward_split<kOutput>("ffn_output", splits, c, c.h, c.w_out, c.b_out, c.y, c.D, c.H, stream);
+    return product_split<kOutput>("ffn_output", splits,
+                                  split_args(c.T, c.D, c.b_out, c.bias_type, nullptr, c.y, c.status), half, kSilu, c.h,
+                                  c.w_out, c.H, stream);
   }
   GemmPlan p = plan_gemm(kOutput, c.T, c.D, c.H, sm_count);
   if (!encode_k(&ma, c.h, half, c.T, c.H, kBM) || !encode_k(&mb, c.w_out, half, c.D, c.H, p.pair ? p.args.BN / 2 : p.args.BN) ||
@@ -1541,17 +1577,36 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
   CUtensorMap ma{}, mb{}, mo{}, mk{};
   cudaError_t e = cudaSuccess;
   if (c.dx != nullptr || c.dw_in != nullptr || c.db_in != nullptr) {
-    GemmPlan p = plan_gemm(kSlope, c.T, c.H, c.D, sm_count);
-    if (!encode_k(&ma, c.dy, half, c.T, c.D, kBM) || !encode_mn(&mb, c.w_out, half, c.D, c.H) ||
-        !encode_out(&mo, dgu, half, c.T, c.H, 2) || !encode_out(&mk, c.kept, half, c.T, c.H, 2)) {
-      return cudaErrorInvalidValue;
+    // up to 256 tiles (whole training pass, 2000 tokens 256 / 688, 176 tiles: 43 us against the
+    // persistent kernel's 49; 2000 tokens 512 / 1368, 352: 71 against 68)
+    const int splits = split_of(c.T, c.H, (c.D + kBK - 1) / kBK, kSplitColumns, 256);
+    if (splits > 0) {
+      e = product_split<kSlope>("ffn_slope", splits,
+                                split_args(c.T, c.H, nullptr, 0, const_cast<void*>(c.kept), dgu, c.status), half,
+                                c.activation, c.dy, c.w_out, c.D, stream);
+    } else {
+      GemmPlan p = plan_gemm(kSlope, c.T, c.H, c.D, sm_count);
+      if (!encode_k(&ma, c.dy, half, c.T, c.D, kBM) || !encode_mn(&mb, c.w_out, half, c.D, c.H) ||
+          !encode_out(&mo, dgu, half, c.T, c.H, 2) || !encode_out(&mk, c.kept, half, c.T, c.H, 2)) {
+        return cudaErrorInvalidValue;
+      }
+      p.args.status = c.status;
+      e = c.activation == kSilu ? launch_gemm<kSlope, kSilu>("ffn_slope", p, half, ma, mb, mo, mk, stream)
+                                : launch_gemm<kSlope, kGelu>("ffn_slope", p, half, ma, mb, mo, mk, stream);
     }
-    p.args.status = c.status;
-    e = c.activation == kSilu ? launch_gemm<kSlope, kSilu>("ffn_slope", p, half, ma, mb, mo, mk, stream)
-                              : launch_gemm<kSlope, kGelu>("ffn_slope", p, half, ma, mb, mo, mk, stream);
     if (e != cudaSuccess) return e;
   }
-  const bool wanted[3] = {c.dx != nullptr, c.dw_in != nullptr, c.dw_out != nullptr};
+  // An input gradient of few tiles and a long contraction would outlast the weight gradients beside it (256 tokens
+  // 1024 / 4096, 128 blocks: whole pass 82 us beside them, 66 split over clusters; 500 tokens 256 / 688, 22: 40, 42).
+  const int64_t dx_blocks = (2 * c.H + kBK - 1) / kBK;
+  const int dx_splits = split_of(c.T, c.D, dx_blocks, kSplitColumns);
+  const bool apart = c.dx != nullptr && dx_splits >= 4 && dx_blocks >= 32;
+  if (apart) {
+    e = product_split<kInput>("ffn_input", dx_splits, split_args(c.T, c.D, nullptr, 0, nullptr, c.dx, c.status), half,
+                              kSilu, dgu, c.w_in, 2 * c.H, stream);
+    if (e != cudaSuccess) return e;
+  }
+  const bool wanted[3] = {c.dx != nullptr && !apart, c.dw_in != nullptr, c.dw_out != nullptr};
   if (wanted[0] || wanted[1] || wanted[2]) {
     const BackwardPlan plan = plan_backward(c.T, c.D, c.H, sm_count, wanted);
     BackwardProducts p{};

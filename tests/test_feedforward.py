@@ -378,3 +378,26 @@ def test_split_waits_that_run_out_leave_a_usable_library() -> None:
             assert cuda.device_status(reset=True) == 1
             assert torch.equal(gated_feed_forward(*args), want)
             assert cuda.device_status(reset=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 64, 4096), (64, 1024, 4096), (250, 200, 2000), (520, 264, 1096), (1000, 512, 1368)])
+@pytest.mark.parametrize(("dtype", "activation"), [(torch.bfloat16, "silu"), (torch.float16, "gelu")])
+def test_few_rows_with_gradients(shape, dtype, activation) -> None:
+    """Training passes of few tiles, all gradients together, twice, and each alone."""
+    from tests.gpu_util import require_native
+
+    require_native()
+    x, w_in, w_out, b_in, b_out, dy = _inputs(*shape, dtype, dtype, True)
+    want = _exact(x, w_in, w_out, b_in, b_out, dy, activation)
+    leaves = {n: v.requires_grad_() for n, v in
+              dict(x=x, w_in=w_in, w_out=w_out, b_in=b_in, b_out=b_out).items()}
+    y = gated_feed_forward(*leaves.values(), activation=activation)
+    _within("y", y.detach(), *want["y"], dtype)
+    grads = torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)
+    for name, grad in zip(leaves, grads):
+        _within(name, grad, *want[name], dtype)
+    again = torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+    for name, leaf in leaves.items():
+        _within(name, torch.autograd.grad(y, leaf, dy, retain_graph=True)[0], *want[name], dtype)
