@@ -85,6 +85,10 @@ struct GemmArgs {
   int* status;
 };
 
+// The next kernel may launch from here on: every kernel of the library starts by waiting for the whole grid before it
+// (launch latency of a pass: 8000 tokens 256 / 688, 72.7 -> 69.4 us; forward of 4096, 20.0 -> 18.2).
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ bool fwait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
   return mbar_wait_bounded(bar, parity, abort_flag, status);
 }
@@ -704,6 +708,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_keep,
                 const GemmArgs a) {
   pdl_wait();
+  pdl_trigger();
   __shared__ __align__(16) GemmShared sh;
   constexpr int kCtas = kPair ? 2 : 1;
   gemm_body<kMode, kHalf, kAct, kPair>(&map_a, &map_b, &map_out, &map_keep, a, static_cast<int>(blockIdx.x) / kCtas,
@@ -721,8 +726,7 @@ ffn_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // of the columns, in split order, adds the bias, and finishes and writes that
 // slice.  Three stages, so that two CTAs fit an SM (with seven, 128 tokens 1024
 // -> 4096 took 28 us instead of 18.5: an SM holds one, and sixteen clusters of
-// eight do not all fit).  The next kernel may launch as soon as this one runs:
-// every kernel here starts by waiting for the one before it (1 us per call).
+// eight do not all fit).
 // Both products against the persistent kernel, as a graph: 17 tokens 256 / 688:
 // 14.3 -> 6.4 us; 97 tokens 512 / 1368: 19.5 -> 10.8; 32 tokens 1024 / 4096:
 // 35 -> 13.3; 1024 tokens 256 / 688: 17.5 -> 11.7; 2048 tokens: 18.1 -> 15.0.
@@ -787,7 +791,7 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   const uint32_t tmem = tmem_s;
   const uint32_t smem_base = smem_u32(smem), full_base = smem_u32(full), empty_base = smem_u32(empty);
   pdl_wait();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  pdl_trigger();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -947,6 +951,7 @@ struct BackwardProducts {
 template <bool kHalf>
 __global__ void __launch_bounds__(kThreads, 1) ffn_backward_kernel(const __grid_constant__ BackwardProducts p) {
   pdl_wait();
+  pdl_trigger();
   __shared__ __align__(16) GemmShared sh;
   const int pair = static_cast<int>(blockIdx.x) / 2;
   if (pair < p.first[1]) {
