@@ -57,7 +57,7 @@ void set_rate(lsso::DropoutCall* c, double p) {
 extern "C" {
 
 int lsso_ffn_streams_weights(int64_t T, int64_t D, int64_t H) {
-  return T > 0 && D > 0 && H > 0 && lsso::ffn_rows_usable(T, D, H) ? 1 : 0;
+  return T > 0 && D > 0 && H > 0 && lsso::ffn_streams_weights(T, D, H, true) ? 1 : 0;
 }
 
 int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int64_t H, const void* w_in, const void* w_out,
@@ -72,7 +72,7 @@ int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int64_t H, c
   if (rc != LSSO_OK) return rc;
   if (!is_16bit(type)) return invalid("%s: type must be BF16 or FP16", who);
   if (weight_type != type &&
-      !(weight_type == LSSO_TYPE_FP32 && kept == nullptr && lsso::ffn_rows_usable(T, D, H))) {
+      !(weight_type == LSSO_TYPE_FP32 && kept == nullptr && lsso::ffn_streams_weights(T, D, H, true))) {
     return invalid("%s: the weights must have x's type (FP32 only where lsso_ffn_streams_weights says so)", who);
   }
   if ((b_in != nullptr || b_out != nullptr) && !is_type(bias_type)) return invalid("%s: unknown bias type", who);

@@ -1101,12 +1101,11 @@ __global__ void __launch_bounds__(256) ffn_cast_kernel(const float* s0, S* d0, i
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to kFfnRows rows: the block is bound by reading the weights once, and a
-// 128-row tensor-core tile would leave most of it empty and most SMs idle.
-// One warp takes one output feature (kGate: its gate and its up row): lanes
-// walk the contraction axis with 16-byte weight loads, every row of the
-// activations (in shared memory) has an FP32 accumulator per lane, and a
-// butterfly adds the lanes.
+// A row or a few: the block is bound by reading the weights once, FP32 ones
+// without a rounded copy.  One warp takes one output feature (kGate: its gate
+// and its up row): lanes walk the contraction axis with 16-byte weight loads,
+// every row of the activations (in shared memory) has an FP32 accumulator per
+// lane, and a butterfly adds the lanes.
 template <typename S, typename W, int kRows>
 __device__ __forceinline__ void row_products(const W* __restrict__ w, const S* __restrict__ act, int64_t K, int rows,
                                              int lane, float (&acc)[kRows]) {
@@ -1326,9 +1325,10 @@ template <typename S, typename W, int kAct, bool kGated>
 cudaError_t launch_rows(const char* name, const void* x, const void* w, const void* bias, int bias_type, int rows,
                         int64_t K, int64_t N, void* out, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(rows) * K * sizeof(S);
-  auto kernel = rows == 1   ? &ffn_rows_kernel<S, W, kAct, kGated, 1>
-                : rows <= 4 ? &ffn_rows_kernel<S, W, kAct, kGated, 4>
-                            : &ffn_rows_kernel<S, W, kAct, kGated, kFfnRows>;
+  auto kernel = rows == 1 ? &ffn_rows_kernel<S, W, kAct, kGated, 1> : &ffn_rows_kernel<S, W, kAct, kGated, 4>;
+  if constexpr (sizeof(W) == 4) {
+    if (rows > 4) kernel = &ffn_rows_kernel<S, W, kAct, kGated, kFfnRows>;
+  }
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   LaunchScope scope(name, stream);
@@ -1518,13 +1518,21 @@ cudaError_t launch_ffn_cast(const float* const src[2], void* const dst[2], const
   return cudaGetLastError();
 }
 
-bool ffn_rows_usable(int64_t T, int64_t D, int64_t H) {
-  return T <= kFfnRows && T * std::max(D, H) * 2 <= 200 * 1024;  // activations in shared memory
+// 16-bit weights, as a graph, against the small-tile kernels: 1 row 1024 / 4096
+// 9.3 and 11.4 us; 2 rows 512 / 1368 7.4 and 7.7, 1024 / 4096 14.5 and 11.5; 4
+// rows 256 / 688 5.8 and 6.0, 512 / 1368 9.0 and 7.8; 8 rows 64 / 256 7.5 and 4.7.
+// FP32 weights, against a rounded copy and those: 4 rows 1024 / 4096 18 and 21;
+// 8 rows 512 / 1368 15.5 and 10.9; 16 rows 256 / 688 12.3 and 8.8, where the
+// copy's launch and allocations cost more host time than that (calls one by one).
+bool ffn_streams_weights(int64_t T, int64_t D, int64_t H, bool fp32) {
+  if (T > kFfnRows || T * std::max(D, H) * 2 > 200 * 1024) return false;  // activations in shared memory
+  if (fp32) return T <= 4 || T * D * H <= (1 << 22);
+  return T == 1 || (T <= 4 && T * D * H <= (1 << 21));
 }
 
 cudaError_t launch_ffn_forward(const FfnForwardCall& c, int sm_count, cudaStream_t stream) {
   const bool half = c.type == kFp16;
-  if (c.kept == nullptr && ffn_rows_usable(c.T, c.D, c.H)) {
+  if (c.kept == nullptr && ffn_streams_weights(c.T, c.D, c.H, c.weight_type == kFp32)) {
     if (c.weight_type == kFp32) return half ? forward_rows<__half, float>(c, stream) : forward_rows<__nv_bfloat16, float>(c, stream);
     return half ? forward_rows<__half, __half>(c, stream) : forward_rows<__nv_bfloat16, __nv_bfloat16>(c, stream);
   }

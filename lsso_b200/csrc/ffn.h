@@ -10,9 +10,9 @@ namespace lsso {
 
 enum Activation : int { kSilu = 0, kGelu = 1 };
 
-// Up to this many rows the forward may run the row kernels (weight streaming).
+// The most rows of the weight-streaming kernels, and whether a forward runs them.
 constexpr int kFfnRows = 16;
-bool ffn_rows_usable(int64_t T, int64_t D, int64_t H);
+bool ffn_streams_weights(int64_t T, int64_t D, int64_t H, bool fp32);
 
 struct FfnForwardCall {
   const void* x;      // [T, D]

@@ -401,3 +401,16 @@ def test_few_rows_with_gradients(shape, dtype, activation) -> None:
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
     for name, leaf in leaves.items():
         _within(name, torch.autograd.grad(y, leaf, dy, retain_graph=True)[0], *want[name], dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 1024, 1368), (6, 512, 1368), (16, 264, 2048)])
+def test_few_rows_with_fp32_weights(shape) -> None:
+    """Streamed or copied, FP32 weights are rounded to x's dtype first."""
+    from tests.gpu_util import require_native
+
+    require_native()
+    x, w_in, w_out, b_in, b_out, dy = _inputs(*shape, torch.bfloat16, torch.float32, True)
+    with torch.no_grad():
+        y = gated_feed_forward(x, w_in, w_out, b_in, b_out)
+    _within("y", y, *_exact(x, w_in, w_out, b_in, b_out, dy, "silu")["y"], torch.bfloat16)
