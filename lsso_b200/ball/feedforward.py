@@ -119,8 +119,8 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
     dtype, contiguous; the biases have one of these dtypes, the same for both.
     ``activation`` is ``"silu"`` or ``"gelu"`` (by erf).  Widths that are not
     multiples of 8 are padded with zeros (copies of x and the weights).
-    Without gradients, a few rows stream the weights (FP32 ones are rounded as
-    they are read); otherwise the tensor-core path runs.
+    Without gradients, one row (or a few of a small block) streams the weights,
+    FP32 ones rounded as they are read; otherwise the tensor-core path runs.
     """
     _check(x, w_in, w_out, b_in, b_out, activation)
     if not x.is_cuda:
