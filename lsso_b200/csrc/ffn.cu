@@ -1171,6 +1171,7 @@ struct GemmPlan {
   GemmArgs args;
   int grid, pair;
   size_t smem;
+  double cost;  // SM cycles, estimated
 };
 
 constexpr int64_t kShort = 8;  // contraction blocks below which a gate tile is bound by its epilogue
@@ -1242,6 +1243,7 @@ GemmPlan plan_gemm(Mode mode, int64_t M, int64_t N, int64_t K, int sm_count, boo
         a.rev = mode == kOutput || mode == kInput || mode == kWeight ? 1 : 0;
         best.args = a;
         best.pair = pair;
+        best.cost = cost;
         best.grid = static_cast<int>(used) * ctas;
         best.smem = static_cast<size_t>(stages * stage + staging);
       }
@@ -1377,17 +1379,47 @@ BackwardPlan plan_backward(int64_t T, int64_t D, int64_t H, int sm_count, const 
   }
   BackwardPlan p{};
   if (most < 0) return p;
-  int share[3] = {}, left = pairs;
+  // The largest takes the pairs that the others leave.
+  int share[3] = {};
+  auto plan = [&](int i, int workers) {
+    return plan_gemm(modes[i], sizes[i][0], sizes[i][1], sizes[i][2], sm_count, false, std::max(1, workers));
+  };
+  int others[2], count = 0, taken = 0;
   for (int i = 0; i < 3; ++i) {
     if (!wanted[i] || i == most) continue;
     share[i] = std::max(1, static_cast<int>(pairs * work[i] / total + 0.5));
-    left -= share[i];
+    taken += share[i];
+    others[count++] = i;
   }
-  share[most] = std::max(1, left);
-  for (int i = 0; i < 3; ++i) {
-    if (wanted[i]) p.product[i] = plan_gemm(modes[i], sizes[i][0], sizes[i][1], sizes[i][2], sm_count, false, share[i]);
-    p.first[i + 1] = p.first[i] + p.product[i].grid / 2;
+  if (count == 2 && total > pairs * 100000.0) {
+    // All three and 60 us or more: whole rounds of tiles and splits decide, so
+    // shares up to two pairs off are tried (64 x 4096 tokens, 256 / 688: 398 ->
+    // 364 us; 3 us of host time, which a shorter call would notice).
+    constexpr int kOff = 2;
+    GemmPlan tried[2][2 * kOff + 1], rest[4 * kOff + 1];
+    for (int d = -2 * kOff; d <= 2 * kOff; ++d) {
+      if (d >= -kOff && d <= kOff) {
+        for (int o = 0; o < 2; ++o) tried[o][d + kOff] = plan(others[o], share[others[o]] + d);
+      }
+      rest[d + 2 * kOff] = plan(most, pairs - taken - d);
+    }
+    double least = 0.0;
+    for (int d0 = -kOff; d0 <= kOff; ++d0) {
+      for (int d1 = -kOff; d1 <= kOff; ++d1) {
+        const GemmPlan &p0 = tried[0][d0 + kOff], &p1 = tried[1][d1 + kOff], &p2 = rest[d0 + d1 + 2 * kOff];
+        const double cost = std::max(std::max(p0.cost, p1.cost), p2.cost);
+        if (least != 0.0 && cost >= least) continue;
+        least = cost;
+        p.product[others[0]] = p0;
+        p.product[others[1]] = p1;
+        p.product[most] = p2;
+      }
+    }
+  } else {
+    for (int o = 0; o < count; ++o) p.product[others[o]] = plan(others[o], share[others[o]]);
+    p.product[most] = plan(most, pairs - taken);
   }
+  for (int i = 0; i < 3; ++i) p.first[i + 1] = p.first[i] + p.product[i].grid / 2;
   return p;
 }
 
