@@ -67,7 +67,8 @@ LSSO_API const char* lsso_last_error(void);
 /* Read the kernel status word of the current device (0 = no kernel reported a
  * failure, 1 = a bounded tensor-core wait ran out, 2 = a peer rank did not reach
  * a gradient exchange in time, 3 = a token id was outside the embedding's
- * vocabulary).  Synchronizes the device.
+ * vocabulary).  1 and 2, after which outputs are undefined, replace 3 and are
+ * not replaced by it.  Synchronizes the device.
  * reset != 0 clears it afterwards. */
 LSSO_API int lsso_device_status(int reset);
 

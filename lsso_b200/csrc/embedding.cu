@@ -33,7 +33,10 @@ constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = kSmallTokens / kSmallThreads;
 constexpr int kMaxBits = 9;               // digit width limit
 constexpr int kMaxBins = 1 << kMaxBits;
-constexpr int kStatusTokenRange = 3;      // an id outside [0, vocab)
+
+// An id outside [0, vocab) gives a zero row; it must not hide a report of
+// undefined outputs (any other value of the status word).
+__device__ __forceinline__ void report_token_range(int* status) { atomicCAS(status, kStatusOk, kStatusTokenRange); }
 
 __device__ __forceinline__ int64_t read_id(const void* ids, int ids64, int64_t t) {
   return ids64 ? __ldg(static_cast<const long long*>(ids) + t) : static_cast<int64_t>(__ldg(static_cast<const int*>(ids) + t));
@@ -77,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, 4) embed_kernel(const EmbeddingCall 
   if (lane < per && base + lane < c.tokens && (c.row_mask == nullptr || c.row_mask[base + lane] != 0)) {
     const int64_t id = read_id(c.ids, c.ids64, base + lane);
     if (id < 0 || id >= c.vocab) {
-      atomicExch(c.status, kStatusTokenRange);
+      report_token_range(c.status);
     } else {
       row_id = static_cast<int>(id);
     }
@@ -162,7 +165,7 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, int t) {
   if (a.row_mask != nullptr && a.row_mask[t] == 0) return static_cast<uint32_t>(a.vocab);
   const int64_t id = read_id(a.ids, a.ids64, t);
   if (id < 0 || id >= a.vocab) {
-    atomicExch(a.status, kStatusTokenRange);
+    report_token_range(a.status);
     return static_cast<uint32_t>(a.vocab);
   }
   return id == a.padding ? static_cast<uint32_t>(a.vocab) : static_cast<uint32_t>(id);

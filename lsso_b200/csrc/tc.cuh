@@ -19,6 +19,7 @@ enum DeviceStatus : int {
   kStatusOk = 0,
   kStatusMmaWaitTimeout = 1,
   kStatusPeerWaitTimeout = 2,  // a peer rank did not reach the gradient exchange in time
+  kStatusTokenRange = 3,       // an id outside an embedding's vocabulary (replaces none of the others)
 };
 
 // Time bound of a sleeping mbarrier wait: any legitimate wait inside one of
