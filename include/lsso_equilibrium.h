@@ -387,12 +387,18 @@ LSSO_API int lsso_ffn_forward(const void* x, int type, int64_t T, int64_t D, int
 /* Its gradients, each output optional (NULL).  x, kept, h, w_in, w_out (16-bit)
  * as the forward had or wrote them; dy, dx [T, D] of `type`; dw_in [2H, D],
  * dw_out [D, H], db_in [2H], db_out [D] of grad_type (BF16, FP16 or FP32).
- * Deterministic (no atomics). */
+ * Deterministic (no atomics).  lsso_ffn_backward_mixed gives db_in and db_out
+ * a type of their own, for biases that do not have the weights'. */
 LSSO_API size_t lsso_ffn_backward_workspace_size(int64_t T, int64_t D, int64_t H);
 LSSO_API int lsso_ffn_backward(const void* dy, const void* x, const void* kept, const void* h, const void* w_in,
                                const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation,
                                int grad_type, void* dx, void* dw_in, void* dw_out, void* db_in, void* db_out,
                                void* workspace, size_t workspace_bytes, void* stream);
+LSSO_API int lsso_ffn_backward_mixed(const void* dy, const void* x, const void* kept, const void* h, const void* w_in,
+                                     const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation,
+                                     int grad_type, int bias_grad_type, void* dx, void* dw_in, void* dw_out,
+                                     void* db_in, void* db_out, void* workspace, size_t workspace_bytes,
+                                     void* stream);
 
 /* FP32 -> `type` (BF16 or FP16) copies of w_in and w_out in one launch
  * (element counts multiples of 8, 16-byte aligned). */

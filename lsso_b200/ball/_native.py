@@ -30,8 +30,8 @@ EXPORTED_SYMBOLS = (
     "lsso_backward_finish", "lsso_peer_region_bytes", "lsso_peer_region_create", "lsso_peer_region_open",
     "lsso_peer_region_close", "lsso_peer_region_destroy", "lsso_peer_allreduce", "lsso_backward_with_wgrad",
     "lsso_ffn_streams_weights", "lsso_ffn_forward", "lsso_ffn_backward_workspace_size", "lsso_ffn_backward",
-    "lsso_ffn_cast", "lsso_embedding_forward", "lsso_embedding_backward_workspace_size", "lsso_embedding_backward",
-    "lsso_dropout_forward", "lsso_dropout_backward",
+    "lsso_ffn_backward_mixed", "lsso_ffn_cast", "lsso_embedding_forward", "lsso_embedding_backward_workspace_size",
+    "lsso_embedding_backward", "lsso_dropout_forward", "lsso_dropout_backward",
 )
 # Element types of the token shell's entry points.
 ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -90,6 +90,8 @@ class NativeLibrary:
             "lsso_ffn_backward_workspace_size": (sz, [i64, i64, i64]),
             "lsso_ffn_backward": (ci, [vp, vp, vp, vp, vp, vp, ci, i64, i64, i64, ci, ci, vp, vp, vp, vp, vp, vp, sz,
                                        vp]),
+            "lsso_ffn_backward_mixed": (ci, [vp, vp, vp, vp, vp, vp, ci, i64, i64, i64, ci, ci, ci, vp, vp, vp, vp, vp, vp,
+                                             sz, vp]),
             "lsso_ffn_cast": (ci, [vp, vp, i64, vp, vp, i64, ci, vp]),
             "lsso_embedding_forward": (ci, [vp, ci, vp, i64, vp, ci, i64, i64, c.c_float, vp, ci, vp]),
             "lsso_embedding_backward_workspace_size": (sz, [i64, i64, i64]),

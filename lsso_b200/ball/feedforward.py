@@ -82,7 +82,7 @@ class _GatedFeedForward(torch.autograd.Function):
         y, kept, h = _forward(x, a, b, b_in, b_out, activation, True)
         ctx.save_for_backward(x, kept, h, a, b)
         ctx.activation, ctx.weight_dtype = activation, w_in.dtype
-        ctx.bias_dtypes = [None if v is None else v.dtype for v in (b_in, b_out)]
+        ctx.bias_dtype = next((v.dtype for v in (b_in, b_out) if v is not None), w_in.dtype)
         return y
 
     @staticmethod
@@ -91,23 +91,19 @@ class _GatedFeedForward(torch.autograd.Function):
         x, kept, h, w_in, w_out = ctx.saved_tensors
         types = _native.ELEMENT_TYPES
         needs = ctx.needs_input_grad
-        device, kind = x.device, ctx.weight_dtype
+        device, kind, bias_kind = x.device, ctx.weight_dtype, ctx.bias_dtype
         (t, d), hidden = x.shape, h.shape[1]
         dy = _aligned(dy.contiguous())
         dx = torch.empty_like(x) if needs[0] else None
         dw_in = torch.empty_like(w_in, dtype=kind) if needs[1] else None
         dw_out = torch.empty_like(w_out, dtype=kind) if needs[2] else None
-        db_in = x.new_empty((2 * hidden,), dtype=kind) if needs[3] else None
-        db_out = x.new_empty((d,), dtype=kind) if needs[4] else None
+        db_in = x.new_empty((2 * hidden,), dtype=bias_kind) if needs[3] else None
+        db_out = x.new_empty((d,), dtype=bias_kind) if needs[4] else None
         scratch = _native.workspace("lsso_ffn_backward_workspace_size", device, t, d, hidden)
-        _native.run("lsso_ffn_backward", device, dy.data_ptr(), x.data_ptr(), kept.data_ptr(), h.data_ptr(),
+        _native.run("lsso_ffn_backward_mixed", device, dy.data_ptr(), x.data_ptr(), kept.data_ptr(), h.data_ptr(),
                     w_in.data_ptr(), w_out.data_ptr(), types[x.dtype], t, d, hidden, ctx.activation, types[kind],
-                    _native._ptr(dx), _native._ptr(dw_in), _native._ptr(dw_out), _native._ptr(db_in),
-                    _native._ptr(db_out), scratch.data_ptr(), scratch.numel())
-        if db_in is not None and ctx.bias_dtypes[0] != kind:
-            db_in = db_in.to(ctx.bias_dtypes[0])
-        if db_out is not None and ctx.bias_dtypes[1] != kind:
-            db_out = db_out.to(ctx.bias_dtypes[1])
+                    types[bias_kind], _native._ptr(dx), _native._ptr(dw_in), _native._ptr(dw_out),
+                    _native._ptr(db_in), _native._ptr(db_out), scratch.data_ptr(), scratch.numel())
         return dx, dw_in, dw_out, db_in, db_out, None
 
 

@@ -52,6 +52,35 @@ void set_rate(lsso::DropoutCall* c, double p) {
   c->scale = c->drop_all ? 0.0f : static_cast<float>(1.0 / (1.0 - p));
 }
 
+int ffn_backward(const char* who, const void* dy, const void* x, const void* kept, const void* h, const void* w_in,
+                 const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation, int grad_type,
+                 int bias_grad_type, void* dx, void* dw_in, void* dw_out, void* db_in, void* db_out, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  lsso::capi::clear_error();
+  if (dy == nullptr || x == nullptr || kept == nullptr || h == nullptr || w_in == nullptr || w_out == nullptr ||
+      workspace == nullptr) {
+    return invalid("%s: a required pointer is NULL", who);
+  }
+  int rc = check_ffn_sizes(who, T, D, H);
+  if (rc != LSSO_OK) return rc;
+  if (!is_16bit(type) || !is_type(grad_type) || !is_type(bias_grad_type)) return invalid("%s: unknown type", who);
+  if (activation != LSSO_FFN_SILU && activation != LSSO_FFN_GELU) return invalid("%s: unknown activation", who);
+  for (const void* p : {dy, x, kept, h, w_in, w_out, static_cast<const void*>(dx), static_cast<const void*>(dw_in),
+                        static_cast<const void*>(dw_out), static_cast<const void*>(db_in),
+                        static_cast<const void*>(db_out), static_cast<const void*>(workspace)}) {
+    if (!aligned(p, 16)) return invalid("%s: every array must be 16-byte aligned", who);
+  }
+  int sms = 0;
+  int* status = nullptr;
+  rc = lsso::capi::device(&sms, &status);
+  if (rc != LSSO_OK) return rc;
+  const size_t need = lsso::ffn_backward_workspace(T, D, H, sms);
+  if (workspace_bytes < need) return lsso::capi::workspace_too_small(who, workspace_bytes, need);
+  const lsso::FfnBackwardCall c{dy, x,  kept,  h,      w_in,  w_out, T, D, H, type, activation, grad_type, bias_grad_type,
+                                dx, dw_in, dw_out, db_in, db_out, static_cast<uint8_t*>(workspace), status};
+  return lsso::capi::launched(lsso::launch_ffn_backward(c, sms, static_cast<cudaStream_t>(stream)), who);
+}
+
 }  // namespace
 
 extern "C" {
@@ -103,30 +132,16 @@ int lsso_ffn_backward(const void* dy, const void* x, const void* kept, const voi
                       const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation, int grad_type,
                       void* dx, void* dw_in, void* dw_out, void* db_in, void* db_out, void* workspace,
                       size_t workspace_bytes, void* stream) {
-  lsso::capi::clear_error();
-  const char* who = "lsso_ffn_backward";
-  if (dy == nullptr || x == nullptr || kept == nullptr || h == nullptr || w_in == nullptr || w_out == nullptr ||
-      workspace == nullptr) {
-    return invalid("%s: a required pointer is NULL", who);
-  }
-  int rc = check_ffn_sizes(who, T, D, H);
-  if (rc != LSSO_OK) return rc;
-  if (!is_16bit(type) || !is_type(grad_type)) return invalid("%s: unknown type", who);
-  if (activation != LSSO_FFN_SILU && activation != LSSO_FFN_GELU) return invalid("%s: unknown activation", who);
-  for (const void* p : {dy, x, kept, h, w_in, w_out, static_cast<const void*>(dx), static_cast<const void*>(dw_in),
-                        static_cast<const void*>(dw_out), static_cast<const void*>(db_in),
-                        static_cast<const void*>(db_out), static_cast<const void*>(workspace)}) {
-    if (!aligned(p, 16)) return invalid("%s: every array must be 16-byte aligned", who);
-  }
-  int sms = 0;
-  int* status = nullptr;
-  rc = lsso::capi::device(&sms, &status);
-  if (rc != LSSO_OK) return rc;
-  const size_t need = lsso::ffn_backward_workspace(T, D, H, sms);
-  if (workspace_bytes < need) return lsso::capi::workspace_too_small(who, workspace_bytes, need);
-  const lsso::FfnBackwardCall c{dy, x,  kept,  h,      w_in,  w_out, T, D, H, type, activation, grad_type,
-                                dx, dw_in, dw_out, db_in, db_out, static_cast<uint8_t*>(workspace), status};
-  return lsso::capi::launched(lsso::launch_ffn_backward(c, sms, static_cast<cudaStream_t>(stream)), who);
+  return ffn_backward("lsso_ffn_backward", dy, x, kept, h, w_in, w_out, type, T, D, H, activation, grad_type, grad_type,
+                      dx, dw_in, dw_out, db_in, db_out, workspace, workspace_bytes, stream);
+}
+
+int lsso_ffn_backward_mixed(const void* dy, const void* x, const void* kept, const void* h, const void* w_in,
+                            const void* w_out, int type, int64_t T, int64_t D, int64_t H, int activation,
+                            int grad_type, int bias_grad_type, void* dx, void* dw_in, void* dw_out, void* db_in,
+                            void* db_out, void* workspace, size_t workspace_bytes, void* stream) {
+  return ffn_backward("lsso_ffn_backward_mixed", dy, x, kept, h, w_in, w_out, type, T, D, H, activation, grad_type,
+                      bias_grad_type, dx, dw_in, dw_out, db_in, db_out, workspace, workspace_bytes, stream);
 }
 
 int lsso_ffn_cast(const float* w_in, void* w_in_out, int64_t w_in_count, const float* w_out, void* w_out_out,

@@ -966,19 +966,21 @@ __global__ void __launch_bounds__(kThreads, 1) ffn_backward_kernel(const __grid_
 // Sums of per-split partials, up to four arrays in one launch (both weight and
 // both bias gradients).  An array of many splits has eight warps take every
 // eighth split, their sums added in warp order; one of few has a thread take
-// all.  The order depends on the split count alone.
+// all.  The order depends on the split count alone.  Each array has an output
+// type of its own, because the biases' may differ from the weights'.
 struct ReduceArray {
   const float* partial;
   void* out;
   int64_t count;  // a multiple of 8
   int splits, first_block;
+  int type;       // of out
 };
 struct ReduceBatch {
   ReduceArray array[4];
   int arrays, blocks;
 };
 
-template <typename O, int kGroups>
+template <int kGroups>
 __device__ __forceinline__ void reduce_array(const ReduceArray& a, int64_t block, float4 (*part)[32]) {
   const int group = kGroups == 1 ? 0 : threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t i = (block * (256 / kGroups) + (kGroups == 1 ? threadIdx.x : lane)) * 4;
@@ -1014,12 +1016,17 @@ __device__ __forceinline__ void reduce_array(const ReduceArray& a, int64_t block
   }
   if (i >= a.count) return;
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-  store_run<O, 4>(static_cast<O*>(a.out) + i, v);
+  if (a.type == kFp32) {
+    store_run<float, 4>(static_cast<float*>(a.out) + i, v);
+  } else if (a.type == kFp16) {
+    store_run<__half, 4>(static_cast<__half*>(a.out) + i, v);
+  } else {
+    store_run<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(a.out) + i, v);
+  }
 }
 
 constexpr int kManySplits = 8;
 
-template <typename O>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__ ReduceBatch batch) {
   pdl_wait();
   __shared__ float4 part[8][32];
@@ -1028,9 +1035,9 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__
   const ReduceArray& a = batch.array[k];
   const int64_t block = static_cast<int64_t>(blockIdx.x) - a.first_block;
   if (a.splits >= kManySplits) {
-    reduce_array<O, 8>(a, block, part);
+    reduce_array<8>(a, block, part);
   } else {
-    reduce_array<O, 1>(a, block, part);
+    reduce_array<1>(a, block, part);
   }
 }
 
@@ -1457,16 +1464,9 @@ BackwardLayout backward_layout(int64_t T, int64_t D, int64_t H, int sm_count) {
   return l;
 }
 
-template <typename F>
-cudaError_t by_type(int type, F&& f) {
-  if (type == kBf16) return f(__nv_bfloat16());
-  if (type == kFp16) return f(__half());
-  return f(float());
-}
-
-void add_array(ReduceBatch* batch, const float* partial, int splits, int64_t count, void* out) {
+void add_array(ReduceBatch* batch, const float* partial, int splits, int64_t count, void* out, int type) {
   const int64_t per_block = splits >= kManySplits ? 32 : 256;  // quads
-  batch->array[batch->arrays++] = ReduceArray{partial, out, count, splits, batch->blocks};
+  batch->array[batch->arrays++] = ReduceArray{partial, out, count, splits, batch->blocks, type};
   batch->blocks += static_cast<int>((count / 4 + per_block - 1) / per_block);
 }
 
@@ -1678,7 +1678,7 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
       if (!wanted[i]) continue;
       const GemmArgs& g = p.args[i];
       p.args[i].out = g.splits > 1 ? static_cast<void*>(partials[i]) : grads[i];
-      if (g.splits > 1) add_array(&batch, partials[i], g.splits, static_cast<int64_t>(g.M) * g.N, grads[i]);
+      if (g.splits > 1) add_array(&batch, partials[i], g.splits, static_cast<int64_t>(g.M) * g.N, grads[i], c.grad_type);
     }
     e = launch_products("ffn_products", p, smem, half, stream);
     if (e != cudaSuccess) return e;
@@ -1698,16 +1698,13 @@ cudaError_t launch_ffn_backward(const FfnBackwardCall& c, int sm_count, cudaStre
     }
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    if (c.db_in != nullptr) add_array(&batch, in.partial, runs, 2 * c.H, c.db_in);
-    if (c.db_out != nullptr) add_array(&batch, out.partial, runs, c.D, c.db_out);
+    if (c.db_in != nullptr) add_array(&batch, in.partial, runs, 2 * c.H, c.db_in, c.bias_grad_type);
+    if (c.db_out != nullptr) add_array(&batch, out.partial, runs, c.D, c.db_out, c.bias_grad_type);
   }
   if (batch.arrays == 0) return cudaSuccess;
-  return by_type(c.grad_type, [&](auto o) {
-    using O = decltype(o);
-    LaunchScope scope("ffn_reduce", stream);
-    launch_pdl(&ffn_reduce_kernel<O>, static_cast<unsigned>(batch.blocks), 256, 0, stream, batch);
-    return cudaGetLastError();
-  });
+  LaunchScope scope("ffn_reduce", stream);
+  launch_pdl(&ffn_reduce_kernel, static_cast<unsigned>(batch.blocks), 256, 0, stream, batch);
+  return cudaGetLastError();
 }
 
 }  // namespace lsso

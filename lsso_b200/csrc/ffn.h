@@ -41,7 +41,8 @@ struct FfnBackwardCall {
   const void* w_out;
   int64_t T, D, H;
   int type, activation;
-  int grad_type;      // weight and bias gradients: FP32, BF16 or FP16
+  int grad_type;      // weight gradients: FP32, BF16 or FP16
+  int bias_grad_type; // bias gradients, likewise
   void* dx;           // each output nullable
   void* dw_in;
   void* dw_out;
