@@ -213,8 +213,11 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
 // results per cycle and sub-partition, and two per element (an exponential and
 // a reciprocal) made it the gate epilogue's limit; one reciprocal of the two
 // denominators' product serves both (a^-1 = b (ab)^-1).  Arguments are clamped
-// where that changes nothing a 16-bit result can show, so that the product
-// stays finite and one element's infinity does not reach the other.
+// so that the product stays finite and one element's infinity does not reach
+// the other.  Past the clamp the logistic function (below 2^-58 there) is zero,
+// because g times the clamped value would grow with g again.  Its complement in
+// the slope is e^-g times itself: 1 - p would be p's rounding error, and g times
+// that a visible part of a slope of one from g = 10^4 on.
 //
 // GELU: Phi(-x) for x >= 0 is p(t) e^(-x^2/2) / 2 with t = 1 / (1 + 0.3275911
 // x / sqrt 2) and the degree-five p of Abramowitz and Stegun 7.1.26 (absolute
@@ -226,13 +229,16 @@ template <int kAct>
 __device__ __forceinline__ void activate2(float g0, float g1, ActSlope& s0, ActSlope& s1) {
   if (kAct == kSilu) {
     constexpr float kLog2e = 1.44269504f;
-    const float a = 1.0f + exp2_approx(fminf(-kLog2e * g0, 58.0f)), b = 1.0f + exp2_approx(fminf(-kLog2e * g1, 58.0f));
+    constexpr float kMost = 58.0f;
+    const float t0 = -kLog2e * g0, t1 = -kLog2e * g1;
+    const float e0 = exp2_approx(fminf(t0, kMost)), e1 = exp2_approx(fminf(t1, kMost));
+    const float a = 1.0f + e0, b = 1.0f + e1;
     const float r = reciprocal_approx(a * b);
-    const float p0 = r * b, p1 = r * a;  // the logistic function
+    const float p0 = t0 > kMost ? 0.0f : r * b, p1 = t1 > kMost ? 0.0f : r * a;  // the logistic function
     s0.act = g0 * p0;
     s1.act = g1 * p1;
-    s0.slope = fmaf(s0.act, 1.0f - p0, p0);
-    s1.slope = fmaf(s1.act, 1.0f - p1, p1);
+    s0.slope = fmaf(s0.act, e0 * p0, p0);
+    s1.slope = fmaf(s1.act, e1 * p1, p1);
     return;
   }
   const float x0 = fminf(fabsf(g0), 30.0f), x1 = fminf(fabsf(g1), 30.0f);

@@ -66,3 +66,81 @@ def test_an_unknown_type_of_bias_gradients_is_refused() -> None:
     args = [16] * 6 + [0, 4, 64, 64, 0, 2, 9] + [16] * 5 + [16, 0, None]
     assert lib.lib.lsso_ffn_backward_mixed(*args) == 1
     assert lib.last_error() == "lsso_ffn_backward_mixed: unknown type"
+
+
+# ---------------------------------------------------------------------------- large pre-activations
+def _probe(values, tokens, dtype, up=None):
+    """Operands whose pre-activations are g = ``values`` and u = ``up`` (or 1) exactly, with y[:, 0] = act(g) u and, for
+    dy = (1, 0, ..), dx[:, 0] = u act'(g) and dx[:, 1] = act(g) (times w_in's factor, which keeps operands in range).
+    The feature beside it has an ordinary pre-activation x[:, 2], and y[:, 1] is its product."""
+    hidden, dim = 512, 8
+    g = torch.tensor(values, dtype=torch.float64).repeat(-(-tokens // len(values)))[:tokens].cuda()
+    u = torch.ones_like(g) if up is None else torch.tensor(up, dtype=torch.float64).repeat(-(-tokens // len(up)))[:tokens].cuda()
+    factor = 2.0 ** 8 if up is not None else 1.0
+    x = torch.zeros(tokens, dim, dtype=torch.float64, device="cuda")
+    x[:, 0], x[:, 1] = g / factor, u / factor
+    x[:, 2] = torch.randn(tokens, generator=torch.Generator().manual_seed(tokens)).to(dtype).cuda()
+    w_in = torch.zeros(2 * hidden, dim, device="cuda")
+    w_in[0, 0], w_in[1, 2] = factor, 1.0
+    w_in[hidden:, 1] = factor
+    w_out = torch.zeros(dim, hidden, device="cuda")
+    w_out[0, 0] = w_out[1, 1] = 1.0
+    dy = torch.zeros(tokens, dim, device="cuda", dtype=dtype)
+    dy[:, 0] = 1.0
+    assert torch.equal(x.to(dtype).double(), x)
+    return g, x.to(dtype), w_in.to(dtype), w_out.to(dtype), dy
+
+
+# exact in BF16 (eight significant bits), up to 1e18 on both sides; FP16 takes those it can hold
+SATURATED = [0.0, 0.5, -0.5, 12.0, -12.0, 30.0, -30.0, 39.0, -39.0, 40.25, -40.25, 41.0, -41.0, 50.0, -50.0, 88.0, -88.0,
+             200.0, -200.0, 1000.0, -1000.0, 30080.0, -30080.0, 60160.0, -60160.0]
+BEYOND = [2.0 ** 20, -2.0 ** 20, 2.0 ** 40, -2.0 ** 40, 2.0 ** 60, -2.0 ** 60, 2.0 ** 100, -2.0 ** 100]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [3, 40, 4224])  # streamed weights, cluster-split tiles, persistent pairs
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_activation_and_slope_far_from_zero(tokens, dtype, activation) -> None:
+    """Against 64 bits.  The exponential's argument rounds to 2^-24 of up to 60, so a value is good to 2^-17 of the sum
+    of its terms' magnitudes; SiLU below -40 is smaller than 2^-52; GELU's erf polynomial is good to 1.5e-7 where
+    e^(-g^2/2) is not smaller still."""
+    from tests.gpu_util import require_native
+
+    require_native()
+    values = SATURATED + (BEYOND if dtype == torch.bfloat16 else [])
+
+    def act_and_slope(g):
+        """Values and error floors of act(g) and act'(g)."""
+        if activation == "silu":
+            p, q = torch.sigmoid(g), torch.sigmoid(-g)
+            error = 2.0 ** -17 * p * (1 + g.abs() * q) + 2.0 ** -52
+            return g * p, p * (1 + g * q), 2.0 ** -17 * g.abs() * p + 2.0 ** -52, error
+        p, tail = 0.5 * torch.erfc(-g * 0.5 ** 0.5), torch.exp(-0.5 * g * g)
+        error = tail.clamp(max=1.5e-7) + 2.0 ** -22 * p
+        slope = p + g * tail / (2 * torch.pi) ** 0.5
+        return g * p, slope, g.abs() * error, error + 2.0 ** -17 * g.abs() * tail
+
+    for start in range(0, len(values), tokens):
+        g, x, w_in, w_out, dy = _probe(values[start:] + values[:start], tokens, dtype)
+        act, slope, act_floor, slope_floor = act_and_slope(g)
+        beside, _, beside_floor, _ = act_and_slope(x[:, 2].double())
+
+        def check(name, actual, expected, floor):
+            tiny = 2.0 ** -24 if dtype == torch.float16 else 0.0
+            expected = torch.where(expected.abs() < 2.0 ** -126, 0.0, expected)  # FP32 has no such value
+            off = (actual.double() - expected).abs() - (2.1 * ROUNDOFF[dtype] * expected.abs() + floor + tiny)
+            worst = off.argmax()
+            assert off.max() <= 0, (name, g[worst].item(), actual[worst].item(), expected[worst].item())  # noqa: B023
+
+        with torch.no_grad():
+            y = gated_feed_forward(x, w_in, w_out, activation=activation)
+        check("inference", y[:, 0], act, act_floor)
+        check("inference beside", y[:, 1], beside, beside_floor)
+        x.requires_grad_()
+        y = gated_feed_forward(x, w_in, w_out, activation=activation)
+        check("y", y.detach()[:, 0], act, act_floor)
+        check("beside", y.detach()[:, 1], beside, beside_floor)
+        dx = torch.autograd.grad(y, x, dy)[0]
+        check("slope", dx[:, 0], slope, slope_floor)
+        check("du", dx[:, 1], act, act_floor)
