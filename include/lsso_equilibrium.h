@@ -370,8 +370,8 @@ LSSO_API int lsso_peer_allreduce(void* const* regions, int world, int rank, int6
  *         is `type`, or FP32 where lsso_ffn_streams_weights(T, D, H) is 1 and
  *         kept is NULL (each weight is then rounded to `type` as it is read)
  *   b_in  [2H], b_out [D] of bias_type, or NULL
- *   kept  [T, 2, H] of `type`: g and u, for lsso_ffn_backward;
- *         NULL for inference
+ *   kept  [T, 2, H] of `type`: g and u, for lsso_ffn_backward (FP16: values
+ *         beyond its range as +-65504); NULL for inference
  *   h     [T, H] of `type`: the product, output or scratch
  *   activation  0 = SiLU, 1 = GELU (by erf)
  * Products accumulate in FP32; kept, h and y are rounded once.  D and H are

@@ -3,8 +3,8 @@
 ``gated_feed_forward(x, w_in, w_out)`` is ``(act(g) * u) w_out^T`` with
 ``[g | u] = x w_in^T``: ``w_in`` ``[2 hidden, dim]`` holds the gate rows, then
 the up rows.  Both projections, the activation and the product are one tcgen05
-kernel; a training forward keeps ``[g | u]`` and the product.  Operands have x's
-dtype (BF16 or FP16), products accumulate in FP32.  FP32 weights are rounded
+kernel; a training forward keeps ``[g | u]`` (in FP16 at most +-65504) and the
+product.  Operands have x's dtype (BF16 or FP16), products accumulate in FP32.  FP32 weights are rounded
 to x's dtype in the call and get FP32 gradients; weights that already have x's
 dtype (a served model's, laid out once) are used in place.
 """

@@ -12,7 +12,10 @@
 // h and [dg | du] are rounded to that type once, because the next product's
 // tensor-core operand has it; h itself comes from the unrounded accumulators.
 // A training forward also keeps [g | u], rounded once to the same type, which
-// is what the backward's epilogue reads.
+// is what the backward's epilogue reads (already a quarter of a narrow block's
+// traffic; FP32 would double it).  FP16 cannot hold accumulators beyond 65504,
+// although h may be in range there (a closed gate, a small factor); they are
+// kept as +-65504, so that the gradients are finite where the forward is.
 //
 // Every product (but those of few tiles, further down) is an instance of one
 // persistent, warp-specialised kernel:
@@ -192,6 +195,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
   return pack_bf16(lo, hi);
 }
+// The same, FP16 values beyond its range held as its largest (NaN stays NaN).
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
+  if (!kHalf) return pack_bf16(lo, hi);
+  uint32_t v;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
+}
 template <bool kHalf>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if (kHalf) return __half22float2(*reinterpret_cast<__half2*>(&v));
@@ -268,13 +279,13 @@ __device__ __forceinline__ float read_bias(const void* bias, int type, int64_t i
 __device__ __forceinline__ uint4* box_piece(uint8_t* box, int lane, int c) {
   return reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
 }
-template <bool kHalf>
+template <bool kHalf, bool kFinite = false>
 __device__ __forceinline__ void box_write(uint8_t* box, int lane, const float (&v)[32]) {
+  auto pack = [&](int j) { return kFinite ? pack2_finite<kHalf>(v[j], v[j + 1]) : pack2<kHalf>(v[j], v[j + 1]); };
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int j = 8 * c;
-    *box_piece(box, lane, c) = make_uint4(pack2<kHalf>(v[j], v[j + 1]), pack2<kHalf>(v[j + 2], v[j + 3]),
-                                          pack2<kHalf>(v[j + 4], v[j + 5]), pack2<kHalf>(v[j + 6], v[j + 7]));
+    *box_piece(box, lane, c) = make_uint4(pack(j), pack(j + 2), pack(j + 4), pack(j + 6));
   }
 }
 template <bool kHalf>
@@ -598,12 +609,12 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap* map_a, const CUtens
           if (a.keep) {
             // stored before the activation, which runs meanwhile
             const bool apart = a.boxes == 3;
-            box_write<kHalf>(stage + (apart ? kOutBox : 0), lane, v);
-            if (apart) box_write<kHalf>(stage + 2 * kOutBox, lane, u);
+            box_write<kHalf, true>(stage + (apart ? kOutBox : 0), lane, v);
+            if (apart) box_write<kHalf, true>(stage + 2 * kOutBox, lane, u);
             store_box(map_keep, apart ? 1 : 0, n0, 0, row0);
             if (!apart) {
               boxes_free();
-              box_write<kHalf>(stage, lane, u);
+              box_write<kHalf, true>(stage, lane, u);
             }
             store_box(map_keep, apart ? 2 : 0, n0, 1, row0);
           }
@@ -907,8 +918,8 @@ ffn_split_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       u[0] += su.x, u[1] += su.y, u[2] += su.z, u[3] += su.w;
       if (a.kept != nullptr) {
         uint16_t* k = static_cast<uint16_t*>(a.kept) + at2;
-        *reinterpret_cast<uint2*>(k) = make_uint2(pack2<kHalf>(v[0], v[1]), pack2<kHalf>(v[2], v[3]));
-        *reinterpret_cast<uint2*>(k + a.N) = make_uint2(pack2<kHalf>(u[0], u[1]), pack2<kHalf>(u[2], u[3]));
+        *reinterpret_cast<uint2*>(k) = make_uint2(pack2_finite<kHalf>(v[0], v[1]), pack2_finite<kHalf>(v[2], v[3]));
+        *reinterpret_cast<uint2*>(k + a.N) = make_uint2(pack2_finite<kHalf>(u[0], u[1]), pack2_finite<kHalf>(u[2], u[3]));
       }
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {

@@ -144,3 +144,26 @@ def test_activation_and_slope_far_from_zero(tokens, dtype, activation) -> None:
         dx = torch.autograd.grad(y, x, dy)[0]
         check("slope", dx[:, 0], slope, slope_floor)
         check("du", dx[:, 1], act, act_floor)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [40, 4224])
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_fp16_preactivations_beyond_its_range_keep_finite_gradients(tokens, activation) -> None:
+    """Accumulators of 90112 do not fit the FP16 values that the backward reads; they are held as the largest FP16
+    value, which changes neither a closed gate nor an open gate's slope."""
+    from tests.gpu_util import require_native
+
+    require_native()
+    big = 90112.0  # 352 * 2^8
+    _, x, w_in, w_out, dy = _probe([-big, -64.0, big, 1.0], tokens, torch.float16, [1.0, big, 0.25, 1.0])
+    x[:, 2] = 0  # the feature beside it: act(0) = 0, so that every exact product is in range
+    x.requires_grad_()
+    w_in, w_out = w_in.float().requires_grad_(), w_out.float()  # FP32: the exact weight gradients are beyond FP16
+    y = gated_feed_forward(x, w_in, w_out, activation=activation)
+    dx, dw_in = torch.autograd.grad(y, (x, w_in), dy / 256)  # 1 / 256 takes w_in's factor back
+    assert torch.isfinite(y).all() and torch.isfinite(dx).all() and torch.isfinite(dw_in).all()
+    assert torch.count_nonzero(y[:2, 0]) == 0 and dx[:2, :2].abs().max() <= 2.0 ** -24
+    assert abs(y[2, 0].item() - 0.25 * big) <= 2.0 ** -11 * 0.25 * big
+    assert abs(dx[2, 0].item() - 0.25) <= 2.0 ** -10 * 0.25
+    assert abs(dx[2, 1].item() - 65504.0) <= 2.0 ** -10 * 65504.0
