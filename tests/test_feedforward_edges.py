@@ -167,3 +167,23 @@ def test_fp16_preactivations_beyond_its_range_keep_finite_gradients(tokens, acti
     assert abs(y[2, 0].item() - 0.25 * big) <= 2.0 ** -11 * 0.25 * big
     assert abs(dx[2, 0].item() - 0.25) <= 2.0 ** -10 * 0.25
     assert abs(dx[2, 1].item() - 65504.0) <= 2.0 ** -10 * 65504.0
+
+
+# ---------------------------------------------------------------------------- one row tile, many columns
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(100, 64, 16640), (24, 32832, 16)])
+@pytest.mark.parametrize(("dtype", "activation", "bias"), [(torch.bfloat16, "silu", True), (torch.float16, "gelu", False)])
+def test_one_row_tile_of_many_columns(shape, dtype, activation, bias) -> None:
+    """More than 512 column tiles over up to 128 rows: the persistent kernel without a partner CTA."""
+    from tests.gpu_util import require_native
+
+    require_native()
+    x, w_in, w_out, b_in, b_out, dy = _inputs(*shape, dtype, dtype, bias)
+    leaves = {n: v.requires_grad_() for n, v in
+              dict(x=x, w_in=w_in, w_out=w_out, b_in=b_in, b_out=b_out).items() if v is not None}
+    y = gated_feed_forward(x, w_in, w_out, b_in, b_out, activation=activation)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    exact = _exact(x, w_in, w_out, b_in, b_out, dy, activation)
+    _within("y", y.detach(), *exact["y"], dtype)
+    for name, grad in grads.items():
+        _within(name, grad, *exact[name], dtype)
