@@ -173,6 +173,8 @@ class GatedFeedForward(nn.Module):
         super().__init__()
         if activation not in _ACTIVATIONS:
             raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}")
+        if dim < 1 or hidden < 1:
+            raise ValueError(f"dim and hidden must be positive, got {dim} and {hidden}")
         self.activation = activation
         self.w_in = nn.Linear(dim, 2 * hidden, bias=bias)
         self.w_out = nn.Linear(hidden, dim, bias=bias)

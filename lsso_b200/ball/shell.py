@@ -45,7 +45,9 @@ class ShellBlock(nn.Module):
     """Pre-norm residual block: x + LSSO(norm(x)), padded tokens zero (optional MLP).
 
     ``gated`` ("silu" or "gelu"): a gated feed-forward block of ``hidden``
-    features (default ``round(dim * mlp_ratio)``) in the MLP's place.
+    features (default ``round(dim * mlp_ratio)``) in the MLP's place.  One of
+    ``hidden`` and ``mlp_ratio`` has to give it features; ``hidden`` alone,
+    with neither ``gated`` nor ``mlp_ratio``, is refused.
     ``dropout``: the rate on both branches in training mode; the block's
     branches use the generator sites ``site`` and ``site + 1``.
     """
@@ -57,8 +59,14 @@ class ShellBlock(nn.Module):
         self.mixer = LSSO(config)
         self.mlp = None
         self.dropout, self.site = float(dropout), site
+        if hidden is not None and hidden < 1:
+            raise ValueError(f"hidden must be positive, got {hidden}")
+        if hidden is not None and gated is None and mlp_ratio <= 0:
+            raise ValueError(f"hidden={hidden} needs a feed-forward block: set gated or mlp_ratio")
         hidden = int(round(config.dim * mlp_ratio)) if hidden is None else hidden
         if gated is not None:
+            if hidden < 1:
+                raise ValueError(f"a gated block needs features: set hidden or mlp_ratio (mlp_ratio={mlp_ratio})")
             self.norm2 = nn.LayerNorm(config.dim)
             self.mlp = GatedFeedForward(config.dim, hidden, activation=gated, bias=config.bias)
         elif mlp_ratio > 0:
