@@ -7,7 +7,9 @@ Philox4x32-10 (Salmon et al., SC 2011) at counter ``(j mod 2^32, j div 2^32,
 site, step mod 2^32)`` and key ``seed`` is at least ``round(p 2^32)``, so the
 backward computes it again.  ``state`` is an int64 CUDA tensor ``[seed,
 step]``: advance ``state[1]`` once per training step (in a captured graph,
-too) and give every dropout of a step its own ``site``.
+too) and give every dropout of a step its own ``site``.  Where activations are
+recomputed in the backward, pass a copy of the state that stays as it is until
+then.
 """
 
 from __future__ import annotations

@@ -113,7 +113,9 @@ class SequenceShell(nn.Module):
     block.  ``embedding_scale``: a :class:`TokenEmbedding` with this scale (the
     parameter keeps the name ``embedding.weight``).  With dropout, the buffer
     ``dropout_state`` holds ``[dropout_seed, step]`` and a training forward
-    advances the step, in a captured graph as well.
+    advances the step, in a captured graph as well.  Its blocks get a copy, so
+    they may be recomputed in the backward (activation checkpointing, block by
+    block); recomputing the whole shell would advance the step again.
     """
 
     def __init__(self, config: LSSOConfig, *, depth: int = 4, vocab: int = 8, mlp_ratio: float = 0.0,
@@ -141,10 +143,12 @@ class SequenceShell(nn.Module):
             x = self.embedding(token_ids)
             if valid_mask is not None:
                 x = torch.where(valid_mask[:, :, None], x, torch.zeros_like(x))
-        for block in self.blocks:
-            x = block(x, valid_mask, implementation, self.dropout_state)
-        if self.training and self.dropout_state is not None:
+        state = self.dropout_state
+        if self.training and state is not None:
+            state = state.clone()
             self.dropout_state[1] += 1
+        for block in self.blocks:
+            x = block(x, valid_mask, implementation, state)
         return x
 
 
