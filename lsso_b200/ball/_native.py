@@ -17,6 +17,7 @@ import ctypes
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 CONTRACT_VERSION = 8
 EXPORTED_SYMBOLS = (
@@ -35,6 +36,12 @@ EXPORTED_SYMBOLS = (
 )
 # Element types of the token shell's entry points.
 ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+# What refuse_transforms() asks PyTorch, bound once.
+_compiling = torch.compiler.is_dynamo_compiling
+_tracing, _dispatch_mode, _PROXY = (torch._C._get_tracing_state, torch._C._get_dispatch_mode,
+                                    torch._C._TorchDispatchModeKey.PROXY)
+_interpreter, _wrapped = torch._C._functorch.peek_interpreter_stack, torch._C._functorch.is_functorch_wrapped_tensor
 
 _LIBRARY: "NativeLibrary | None" = None
 _OPS: torch.library.Library | None = None
@@ -214,6 +221,21 @@ def run(name: str, device: torch.device, *args) -> None:
             code = getattr(lib.lib, name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if code:
         lib.check(code)
+
+
+def refuse_transforms(name: str, *tensors: torch.Tensor | None) -> None:
+    """Raise where an operator that reads data pointers would drop a transform
+    of its inputs without a word: a trace would record its output as a
+    constant, a forward-mode tangent would be lost (half a microsecond)."""
+    if _compiling():
+        return  # the compiled graph ends before the native call, which runs as it is
+    if _tracing() is not None or _dispatch_mode(_PROXY) is not None:
+        raise NotImplementedError(f"{name} cannot be traced; use {name}_reference there")
+    if _interpreter() is not None and any(t is not None and _wrapped(t) for t in tensors):
+        raise NotImplementedError(f"{name} does not support torch.func transforms; use {name}_reference there")
+    if forward_ad._current_level >= 0:
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise NotImplementedError(f"{name} does not support forward-mode derivatives; use {name}_reference there")
 
 
 def workspace(name: str, device: torch.device, *sizes) -> torch.Tensor:

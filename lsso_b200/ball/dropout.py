@@ -135,6 +135,7 @@ def dropout_add(branch: torch.Tensor, residual: torch.Tensor | None = None, *, p
     ``valid_mask`` is bool over the leading dimensions.  Non-contiguous inputs
     are copied.  A dropped element contributes exactly zero, whatever it holds.
     """
+    _native.refuse_transforms("dropout_add", branch, residual, state, valid_mask)
     _check(branch, residual, p, state, site, valid_mask)
     if not branch.is_cuda:
         raise ValueError("dropout_add requires CUDA tensors; use dropout_add_reference elsewhere")

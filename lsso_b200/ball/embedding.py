@@ -90,6 +90,7 @@ def token_embedding(ids: torch.Tensor, weight: torch.Tensor, *, scale: float = 1
     ``padding_idx`` has a zero gradient.  An id outside the table gives a zero
     row and sets the device status (``cuda.check_device_status()`` raises).
     """
+    _native.refuse_transforms("token_embedding", weight, ids, valid_mask)
     _check(ids, weight, valid_mask, padding_idx)
     if not weight.is_cuda:
         raise ValueError("token_embedding requires CUDA tensors; use token_embedding_reference elsewhere")

@@ -118,6 +118,7 @@ def gated_feed_forward(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor,
     Without gradients, one row (or a few of a small block) streams the weights,
     FP32 ones rounded as they are read; otherwise the tensor-core path runs.
     """
+    _native.refuse_transforms("gated_feed_forward", x, w_in, w_out, b_in, b_out)
     _check(x, w_in, w_out, b_in, b_out, activation)
     if not x.is_cuda:
         raise ValueError("gated_feed_forward requires CUDA tensors; use gated_feed_forward_reference elsewhere")
