@@ -9,7 +9,9 @@ backward computes it again.  ``state`` is an int64 CUDA tensor ``[seed,
 step]``: advance ``state[1]`` once per training step (in a captured graph,
 too) and give every dropout of a step its own ``site``.  Where activations are
 recomputed in the backward, pass a copy of the state that stays as it is until
-then.
+then.  The index is that of the tensor at hand: ranks that each hold a part of
+the batch or of the sequence need a seed each, or they drop the same elements
+of their parts.
 """
 
 from __future__ import annotations

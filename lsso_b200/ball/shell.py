@@ -113,9 +113,12 @@ class SequenceShell(nn.Module):
     block.  ``embedding_scale``: a :class:`TokenEmbedding` with this scale (the
     parameter keeps the name ``embedding.weight``).  With dropout, the buffer
     ``dropout_state`` holds ``[dropout_seed, step]`` and a training forward
-    advances the step, in a captured graph as well.  Its blocks get a copy, so
-    they may be recomputed in the backward (activation checkpointing, block by
-    block); recomputing the whole shell would advance the step again.
+    advances the step, in a captured graph as well.  Data-parallel ranks need a
+    ``dropout_seed`` each, which DistributedDataParallel keeps only with
+    ``broadcast_buffers=False`` and which a loaded checkpoint overwrites.  The
+    blocks get a copy of the state, so they may be recomputed in the backward
+    (activation checkpointing, block by block); recomputing the whole shell
+    would advance the step again.
     """
 
     def __init__(self, config: LSSOConfig, *, depth: int = 4, vocab: int = 8, mlp_ratio: float = 0.0,
