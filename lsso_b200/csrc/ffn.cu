@@ -88,7 +88,7 @@ struct GemmArgs {
   int* status;
 };
 
-// The next kernel may launch from here on: every kernel of the library starts by waiting for the whole grid before it
+// The next kernel may launch from here on: every kernel of the library waits for the whole grid before it (tc.cuh)
 // (launch latency of a pass: 8000 tokens 256 / 688, 72.7 -> 69.4 us; forward of 4096, 20.0 -> 18.2).
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -1060,7 +1060,9 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const __grid_constant__
 
 // Column sums of 16-bit [rows, cols] matrices (the bias gradients, up to two in
 // one launch): each block sums a run of rows for 256 columns in FP32 and the
-// reduction adds the blocks' sums in order.
+// reduction adds the blocks' sums in order.  b_in's sums [dg | du] as rounded
+// for the products: its roundings are independent, so they add up to less than
+// 2^-9 (BF16) or 2^-12 (FP16) of the root of the sum of squares.
 struct ColsumArray {
   const uint16_t* in;
   float* partial;  // [gridDim.y][cols]

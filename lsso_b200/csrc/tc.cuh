@@ -49,13 +49,23 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 // Every kernel of the library is launched with programmatic stream
 // serialisation (launch_pdl): the launch of its grid proceeds as the blocks of
 // the previous kernel on the stream exit, instead of after that kernel's
-// completion has been processed.  Each kernel therefore starts with
-// pdl_wait(), which returns once the previous grid has completed and its
-// memory operations are visible (immediately when there is no such
-// dependency), and touches no global memory before it; since every kernel
-// waits, the outputs of all earlier kernels on the stream are complete too.
-// (Triggering the next launch explicitly at the start of each kernel was
-// measured slower: the dependent grid's blocks then crowd the tail.)
+// completion has been processed.  Each kernel therefore calls pdl_wait(), which
+// returns once the previous grid has completed and its memory operations are
+// visible (immediately when there is no such dependency), and touches no global
+// memory before it; since every kernel waits, the outputs of all earlier
+// kernels on the stream are complete too.
+//
+// The feed-forward's tensor-core kernels (persistent, joint backward, few
+// tiles) trigger the next launch right after their own pdl_wait(), so blocks of
+// the next grid may be resident, up to their pdl_wait(), while all of the
+// previous grid still runs.  What a kernel does before pdl_wait() must hold
+// under that: shared memory, barriers, and what the SM has left.  The kernel of
+// few tiles also allocates its 64 TMEM columns there.  It takes them from no
+// block that still has to allocate: the persistent kernels, which allocate
+// after their trigger, leave at most 35 KB of an SM's shared memory, less than
+// that kernel needs (58 KB or more), and it triggers after its own allocation.
+// (In the mixer's kernels an explicit trigger at the start was measured slower:
+// the dependent grid's blocks then crowd the tail.)
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
 template <typename... Params, typename... Args>
