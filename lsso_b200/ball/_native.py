@@ -39,8 +39,8 @@ ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 # What refuse_transforms() asks PyTorch, bound once.
 _compiling = torch.compiler.is_dynamo_compiling
-_tracing, _dispatch_mode, _PROXY = (torch._C._get_tracing_state, torch._C._get_dispatch_mode,
-                                    torch._C._TorchDispatchModeKey.PROXY)
+_tracing, _dispatch_depth = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+_dispatch_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
 _interpreter, _wrapped = torch._C._functorch.peek_interpreter_stack, torch._C._functorch.is_functorch_wrapped_tensor
 
 _LIBRARY: "NativeLibrary | None" = None
@@ -226,10 +226,10 @@ def run(name: str, device: torch.device, *args) -> None:
 def refuse_transforms(name: str, *tensors: torch.Tensor | None) -> None:
     """Raise where an operator that reads data pointers would drop a transform
     of its inputs without a word: a trace would record its output as a
-    constant, a forward-mode tangent would be lost (half a microsecond)."""
+    constant, a forward-mode tangent would be lost (0.3 us)."""
     if _compiling():
         return  # the compiled graph ends before the native call, which runs as it is
-    if _tracing() is not None or _dispatch_mode(_PROXY) is not None:
+    if _tracing() or (_dispatch_depth() and _dispatch_mode(_PROXY) is not None):
         raise NotImplementedError(f"{name} cannot be traced; use {name}_reference there")
     if _interpreter() is not None and any(t is not None and _wrapped(t) for t in tensors):
         raise NotImplementedError(f"{name} does not support torch.func transforms; use {name}_reference there")

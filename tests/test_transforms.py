@@ -64,3 +64,7 @@ def test_tracing_is_refused(name, device) -> None:
     call, inputs = _calls(device)[name]
     with pytest.raises(NotImplementedError, match=f"{name} .*traced"):
         torch.jit.trace(call, tuple(inputs), check_trace=False)
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    with pytest.raises(NotImplementedError, match=f"{name} .*traced"):
+        make_fx(lambda *v: call(*v))(*inputs)
