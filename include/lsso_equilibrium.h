@@ -443,6 +443,65 @@ LSSO_API int lsso_dropout_backward(const void* dy, int out_type, int branch_type
                                    int64_t rows, int64_t width, double p, const int64_t* state, uint32_t site,
                                    void* dbranch, void* dresidual, void* stream);
 
+/* ---- Operators of the causal mixer (no counterpart in the reference).
+ *
+ * Linear attention with a decay per head.  Per sample and head, over the valid
+ * tokens in order (a masked token is as though absent; its output is zero):
+ *   S_t = e^log_decay S_{t-1} + k_t v_t^T     y_t = scale * S_t^T q_t
+ *   q, k [B, N, H, DK], v, y [B, N, H, DV] of `type` (BF16 or FP16), features
+ *         adjacent, 16-byte aligned; strides: batch, token and head, in
+ *         elements, positive multiples of 8
+ *   log_decay [H] FP32 (-inf: a token sees only itself; values below -1e4 count
+ *         as -1e4, whose decay is zero)
+ *   mask  uint8/bool [B, N] or NULL;  state  [B, H, DK, DV] FP32, before the
+ *         first token, or NULL for zero;  last  likewise, after the last token
+ *         (output), or NULL
+ * DK and DV are multiples of 8 from 8 to 128.  States and sums are FP32; the
+ * scores, the state as it meets q, and the output are rounded to `type`. */
+LSSO_API size_t lsso_decay_workspace_size(int64_t B, int64_t N, int64_t H, int64_t DK, int64_t DV, int backward);
+LSSO_API int lsso_decay_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                const void* v, const int64_t* v_strides, int type, const float* log_decay,
+                                const uint8_t* mask, int64_t B, int64_t N, int64_t H, int64_t DK, int64_t DV,
+                                float scale, const float* state, float* last, void* y, const int64_t* y_strides,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients dq, dk, dv (zero in masked rows) and dstate (NULL when not
+ * wanted) from dy and dlast, the gradient of the last state (NULL for zero).
+ * Deterministic (no atomics). */
+LSSO_API int lsso_decay_backward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                 const void* v, const int64_t* v_strides, const void* dy, const int64_t* dy_strides,
+                                 int type, const float* log_decay, const uint8_t* mask, int64_t B, int64_t N,
+                                 int64_t H, int64_t DK, int64_t DV, float scale, const float* state,
+                                 const float* dlast, void* dq, const int64_t* dq_strides, void* dk,
+                                 const int64_t* dk_strides, void* dv, const int64_t* dv_strides, float* dstate,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token per sample: new_state = e^log_decay state + k v^T (the same array
+ * or one apart from it), y = scale * new_state^T q.  q, k [B, H, DK], v
+ * [B, H, DV] of `type` (BF16, FP16 or FP32; strides: batch and head, in
+ * elements), y contiguous.  Samples with active[b] == 0 keep their state and
+ * give zero rows. */
+LSSO_API int lsso_decay_step(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                             const void* v, const int64_t* v_strides, int type, const float* log_decay,
+                             const uint8_t* active, int64_t B, int64_t H, int64_t DK, int64_t DV, float scale,
+                             const float* state, float* new_state, void* y, void* stream);
+
+/* Rotary positions: pair i (features 2i and 2i + 1 if interleaved, else i and
+ * i + pairs) of a head turned by position * frequencies[i] (minus that:
+ * backward) and multiplied by magnitude; features from 2 * pairs on are copied.
+ *   x [B, N, H, D] of `type` (BF16, FP16, FP32), D even, aligned to two
+ *     elements, strides (batch, token, head) even; y contiguous
+ *   frequencies [pairs] FP64 or FP32; positions [N] or [B, N] of position_type,
+ *     or NULL for 0 .. N - 1.  Angles are formed in 64 bits. */
+#define LSSO_POSITION_INT64 0
+#define LSSO_POSITION_INT32 1
+#define LSSO_POSITION_FP32 2
+#define LSSO_POSITION_FP64 3
+LSSO_API int lsso_rotary(const void* x, const int64_t* strides, int type, int64_t B, int64_t N, int64_t H, int64_t D,
+                         int64_t pairs, const void* frequencies, int frequencies_fp64, const void* positions,
+                         int position_type, int positions_batched, int interleaved, int backward, float magnitude,
+                         void* y, void* stream);
+
 /* Per-kernel timing (no counterpart in the reference; instrumentation only).
  * lsso_profile_start() makes every subsequent kernel launch of the library
  * record a CUDA event pair on its launch stream; lsso_profile_stop()

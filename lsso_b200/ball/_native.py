@@ -32,7 +32,8 @@ EXPORTED_SYMBOLS = (
     "lsso_peer_region_close", "lsso_peer_region_destroy", "lsso_peer_allreduce", "lsso_backward_with_wgrad",
     "lsso_ffn_streams_weights", "lsso_ffn_forward", "lsso_ffn_backward_workspace_size", "lsso_ffn_backward",
     "lsso_ffn_backward_mixed", "lsso_ffn_cast", "lsso_embedding_forward", "lsso_embedding_backward_workspace_size",
-    "lsso_embedding_backward", "lsso_dropout_forward", "lsso_dropout_backward",
+    "lsso_embedding_backward", "lsso_dropout_forward", "lsso_dropout_backward", "lsso_decay_workspace_size",
+    "lsso_decay_forward", "lsso_decay_backward", "lsso_decay_step", "lsso_rotary",
 )
 # Element types of the token shell's entry points.
 ELEMENT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -54,6 +55,7 @@ class NativeLibrary:
         c = ctypes
         lib = c.CDLL(str(path))
         i64, vp, sz, ci = c.c_int64, c.c_void_p, c.c_size_t, c.c_int
+        ip = c.POINTER(i64)
         signatures = {
             "lsso_contract_version": (ci, []),
             "lsso_compiled_sm": (ci, []),
@@ -105,6 +107,13 @@ class NativeLibrary:
             "lsso_embedding_backward": (ci, [vp, ci, vp, i64, vp, ci, i64, i64, i64, c.c_float, vp, ci, vp, sz, vp]),
             "lsso_dropout_forward": (ci, [vp, ci, vp, ci, vp, i64, i64, c.c_double, vp, c.c_uint32, vp, vp, vp]),
             "lsso_dropout_backward": (ci, [vp, ci, ci, vp, i64, i64, c.c_double, vp, c.c_uint32, vp, vp, vp]),
+            "lsso_decay_workspace_size": (sz, [i64, i64, i64, i64, i64, ci]),
+            "lsso_decay_forward": (ci, [vp, ip, vp, ip, vp, ip, ci, vp, vp, i64, i64, i64, i64, i64, c.c_float, vp, vp, vp,
+                                        ip, vp, sz, vp]),
+            "lsso_decay_backward": (ci, [vp, ip, vp, ip, vp, ip, vp, ip, ci, vp, vp, i64, i64, i64, i64, i64, c.c_float,
+                                         vp, vp, vp, ip, vp, ip, vp, ip, vp, vp, sz, vp]),
+            "lsso_decay_step": (ci, [vp, ip, vp, ip, vp, ip, ci, vp, vp, i64, i64, i64, i64, c.c_float, vp, vp, vp, vp]),
+            "lsso_rotary": (ci, [vp, ip, ci, i64, i64, i64, i64, i64, vp, ci, vp, ci, ci, ci, ci, c.c_float, vp, vp]),
             "lsso_profile_start": (ci, []),
             "lsso_profile_stop": (ci, [ci, c.c_char_p, c.POINTER(c.c_float), c.POINTER(c.c_int)]),
         }

@@ -20,7 +20,7 @@ CSRC = PACKAGE / "csrc"
 LIBDIR = PACKAGE / "lib"
 LIBRARY_NAME = "lsso_equilibrium_sm100.so"
 SOURCES = ("mixer.cu", "linear.cu", "tokens.cu", "solve.cu", "peer.cu", "ffn.cu", "embedding.cu",
-           "dropout.cu", "capi.cu", "capi_shell.cu")
+           "dropout.cu", "decay.cu", "decay_step.cu", "rotary.cu", "capi.cu", "capi_shell.cu", "capi_decay.cu")
 HEADERS = ("mixer.h", "mixer_common.cuh", "tc.cuh", "linear.h", "peer.h", "ffn.h", "shell_ops.h", "elements.cuh",
            "capi_util.h")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")

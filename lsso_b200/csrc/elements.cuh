@@ -131,4 +131,14 @@ __device__ __forceinline__ void store_run(T* p, const float (&x)[N], bool wide =
   }
 }
 
+// Multiplication by e^l, many times in a row.  A decay near one is rounded by up to 2^-25 when it is formed, the same way
+// every time, so n steps would be off by n 2^-25; s + s (e^l - 1) is off by the rounding of its result alone.  Below
+// e^-0.5 the difference from one would lose bits of a small decay, and e^l itself is used.
+struct Decay {
+  float factor;
+  bool near_one;
+  __device__ __forceinline__ explicit Decay(float l) : factor(l > -0.5f ? expm1f(l) : expf(l)), near_one(l > -0.5f) {}
+  __device__ __forceinline__ float apply(float s) const { return fmaf(s, factor, near_one ? s : 0.0f); }
+};
+
 }  // namespace lsso

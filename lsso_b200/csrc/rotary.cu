@@ -1,0 +1,175 @@
+// Rotary positions on sm_100a.
+//
+// Pair i of a head's first 2 f features, (a, b) = features (2i, 2i + 1) or
+// (i, i + f), becomes magnitude * (a cos t - b sin t, b cos t + a sin t) with
+// t = position * frequency_i; the other features are copied.  The backward is
+// the same kernel with -t.
+//
+// Bound by HBM: every value is read and written once.  The angle belongs to a
+// token and a pair, not to a head, so a block computes the cosines and sines of
+// its tokens once, into shared memory, and then walks its tokens' heads in
+// memory order with 16-byte runs.  Angles of far positions need more bits than
+// FP32 has (position 2^20 leaves 2^-4 of a radian), so position * frequency is
+// formed in 64 bits and reduced to a fraction of a turn there; the rest is FP32.
+#include <algorithm>
+
+#include "elements.cuh"
+#include "mixer.h"
+#include "shell_ops.h"
+#include "tc.cuh"
+
+namespace lsso {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTable = 2048;  // (cos, sin) pairs of a block: 16 KB
+
+__device__ __forceinline__ double read_position(const RotaryCall& c, int64_t sample, int64_t token) {
+  if (c.positions == nullptr) return static_cast<double>(token);
+  const int64_t at = (c.positions_batched ? sample * c.length : 0) + token;
+  switch (c.position_type) {
+    case kPosInt64: return static_cast<double>(static_cast<const int64_t*>(c.positions)[at]);
+    case kPosInt32: return static_cast<double>(static_cast<const int32_t*>(c.positions)[at]);
+    case kPosFp32: return static_cast<double>(static_cast<const float*>(c.positions)[at]);
+    default: return static_cast<const double*>(c.positions)[at];
+  }
+}
+
+// kRun pairs per thread and step; tokens [first, first + count) of the flat batch x length axis per block, heads
+// [head0, head0 + heads) per blockIdx.y.
+template <typename T, int kRun, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryCall c, int tokens_per_block, int heads_per_block) {
+  __shared__ float2 table[kMaxTable];
+  pdl_wait();
+  const int64_t total = c.batch * c.length;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * tokens_per_block;
+  const int tokens = static_cast<int>(min(static_cast<int64_t>(tokens_per_block), total - first));
+  const int f = c.pairs;
+  for (int i = threadIdx.x; i < tokens * f; i += kThreads) {
+    const int t = i / f, p = i - t * f;
+    const int64_t flat = first + t, sample = flat / c.length;
+    const double freq = c.frequency64 ? static_cast<const double*>(c.frequencies)[p]
+                                      : static_cast<double>(static_cast<const float*>(c.frequencies)[p]);
+    const double turns = read_position(c, sample, flat - sample * c.length) * freq * 0.15915494309189533577;
+    float s, co;
+    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &co);
+    table[i] = make_float2(co * c.magnitude, (c.backward ? -s : s) * c.magnitude);
+  }
+  __syncthreads();
+  const int head0 = blockIdx.y * heads_per_block;
+  const int heads = min(heads_per_block, c.heads - head0);
+  const int turned = f / kRun;                                      // runs of pairs of a head
+  const int runs = turned + (c.dim - 2 * f + 2 * kRun - 1) / (2 * kRun);  // and runs of 2 kRun copied features
+  const T* in = static_cast<const T*>(c.x);
+  T* out = static_cast<T*>(c.y);
+  // A thread's items lie kThreads apart: by increments, no division per item.
+  int run = threadIdx.x % runs, head = threadIdx.x / runs, t = head / heads;
+  head -= t * heads;
+  const int step_run = kThreads % runs, step_row = kThreads / runs, step_t = step_row / heads, step_head = step_row % heads;
+  int64_t sample = (first + t) / c.length, token = first + t - sample * c.length;
+  while (t < tokens) {
+    const int64_t flat = first + t;
+    const T* src = in + sample * c.stride_batch + token * c.stride_token + (head0 + head) * c.stride_head;
+    T* dst = out + (flat * c.heads + head0 + head) * c.dim;
+    if (run < turned) {
+      const int p = run * kRun;
+      const float2* cs = table + t * f + p;
+      if (kInterleaved) {
+        Run<T, 2 * kRun> r = load_run<T, 2 * kRun>(src + 2 * p);
+        float v[2 * kRun];
+        run_to_float(r, v);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const float a = v[2 * j], b = v[2 * j + 1];
+          v[2 * j] = a * cs[j].x - b * cs[j].y;
+          v[2 * j + 1] = b * cs[j].x + a * cs[j].y;
+        }
+        store_run(dst + 2 * p, v);
+      } else {
+        Run<T, kRun> ra = load_run<T, kRun>(src + p), rb = load_run<T, kRun>(src + f + p);
+        float a[kRun], b[kRun];
+        run_to_float(ra, a);
+        run_to_float(rb, b);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const float x = a[j];
+          a[j] = x * cs[j].x - b[j] * cs[j].y;
+          b[j] = b[j] * cs[j].x + x * cs[j].y;
+        }
+        store_run(dst + p, a);
+        store_run(dst + f + p, b);
+      }
+    } else {
+      const int at = 2 * f + (run - turned) * 2 * kRun;
+      // copied as they are, whatever they hold
+#pragma unroll
+      for (int j = 0; j < 2 * kRun; j += kRun)
+        if (at + j < c.dim) *reinterpret_cast<Run<T, kRun>*>(dst + at + j) = load_run<T, kRun>(src + at + j);
+    }
+    run += step_run;
+    head += step_head;
+    int ahead = step_t;
+    if (run >= runs) {
+      run -= runs;
+      ++head;
+    }
+    if (head >= heads) {
+      head -= heads;
+      ++ahead;
+    }
+    t += ahead;
+    token += ahead;
+    while (token >= c.length) {
+      token -= c.length;
+      ++sample;
+    }
+  }
+}
+
+template <typename T, int kRun>
+cudaError_t launch_run(const RotaryCall& c, int sm_count, cudaStream_t stream) {
+  const int64_t total = c.batch * c.length;
+  const int64_t items = static_cast<int64_t>(c.heads) * (c.dim / 2 / kRun + 1);  // of a token, about
+  // Tokens per block: sixteen items per thread where there are many tokens (the table is then shared by as many heads
+  // as there are), fewer where that leaves SMs idle, and no more than the table holds.
+  int64_t tokens = std::max<int64_t>(1, kThreads * 16 / items);
+  tokens = std::min<int64_t>(tokens, std::max<int64_t>(1, total / (4 * sm_count)));
+  tokens = std::min<int64_t>(tokens, std::max(1, kMaxTable / c.pairs));
+  const int64_t blocks = (total + tokens - 1) / tokens;
+  // Heads are split over blocks (each with its own table) where tokens alone leave SMs idle.
+  int64_t parts = std::min<int64_t>(c.heads, std::max<int64_t>(1, 2 * sm_count / blocks));
+  parts = std::min<int64_t>(parts, std::max<int64_t>(1, tokens * items / kThreads));
+  const int heads = static_cast<int>((c.heads + parts - 1) / parts);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((c.heads + heads - 1) / heads));
+  auto kernel = c.interleaved ? &rotary_kernel<T, kRun, true> : &rotary_kernel<T, kRun, false>;
+  LaunchScope scope(c.backward ? "rotary_bwd" : "rotary", stream);
+  launch_pdl(kernel, grid, kThreads, 0, stream, c, static_cast<int>(tokens), heads);
+  return cudaGetLastError();
+}
+
+// The longest run that divides every offset a run starts at, up to 16 bytes.  Interleaved runs hold both features of
+// their pairs, so they take half as many pairs.
+template <typename T>
+cudaError_t launch_type(const RotaryCall& c, int sm_count, cudaStream_t stream) {
+  const uint64_t elements = static_cast<uint64_t>(c.stride_batch) | static_cast<uint64_t>(c.stride_token) |
+                            static_cast<uint64_t>(c.stride_head) | static_cast<uint64_t>(c.dim) |
+                            (reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.y)) / sizeof(T);
+  const uint64_t starts = static_cast<uint64_t>(c.pairs) | (c.interleaved ? elements / 2 : elements);
+  const uint64_t most = 16 / sizeof(T) / (c.interleaved ? 2 : 1);
+  if constexpr (sizeof(T) == 2) {
+    if (most >= 8 && starts % 8 == 0) return launch_run<T, 8>(c, sm_count, stream);
+  }
+  if (most >= 4 && starts % 4 == 0) return launch_run<T, 4>(c, sm_count, stream);
+  if (starts % 2 == 0) return launch_run<T, 2>(c, sm_count, stream);
+  return launch_run<T, 1>(c, sm_count, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_rotary(const RotaryCall& c, int sm_count, cudaStream_t stream) {
+  if (c.type == kFp32) return launch_type<float>(c, sm_count, stream);
+  return c.type == kFp16 ? launch_type<__half>(c, sm_count, stream) : launch_type<__nv_bfloat16>(c, sm_count, stream);
+}
+
+}  // namespace lsso
