@@ -1,14 +1,35 @@
-// Linear attention with a decay per head (sm_100a), over the valid tokens of each sample and head:
+// Linear attention with a decay per head on sm_100a (tcgen05 + TMA), over the valid tokens of each sample and head:
 //   S_t = e^l S_{t-1} + k_t v_t^T        y_t = scale * S_t^T q_t
 //
 // Forward and backward are scans of one form.  With T_t the upstream gradient of S_t,
 //   dq_t = scale * S_t dy_t
 //   T_t = e^l T_{t+1} + scale * q_t dy_t^T,   dk_t = T_t v_t,   dv_t = T_t^T k_t,   dS_0 = e^l T_1
 // so y is the scan (x, y, z) = (q, k, v) forward in time, dq is (dy, v, k) forward from S_0^T, dk is (v, dy, q) and dv
-// is (k, q, dy) backward in time from the last state's gradient.
+// is (k, q, dy) backward in time from the last state's gradient.  A scan takes chunks of 128 tokens.  With n valid
+// tokens in a chunk, r the rank of a token among them in the direction of the scan, and M the state before the chunk,
+//   w_i = sum over r_j <= r_i of e^(l (r_i - r_j)) (x_i . y_j) z_j  +  e^(l (r_i + 1)) x_i M
+//   M'  = e^(l n) M + sum over j of e^(l (n - 1 - r_j)) y_j z_j^T
+// which is four matrix products of 128 tokens, and a masked token is one of weight zero.
+//
+// One CTA runs a scan of one sample and head (or a segment of it) with the state on chip, so every input is read once
+// and every output written once: 8 d values of 2 bytes per token and head in the forward, against 4 products of 128 x d
+// per token; HBM is the bound that is aimed at.  The tokens come by TMA from wherever the caller keeps them (strides of
+// a packed projection).  A token axis that is long for the number of heads is cut into segments: their states first
+// (products of y and z alone), joined in order, then all segments at once.
+//
+// Per chunk:
+//   scores P = X Y^T and X M            tcgen05, operands from shared memory, accumulators in TMEM
+//   Y' = weights * Y in place           all threads, while nothing else needs Y
+//   M change Z^T Y'                     tcgen05 (transposed, so that a thread owns a row of M^T)
+//   P' = decay * P, rounded             TMEM to registers and back, the next product's A operand
+//   P' Z                                tcgen05, A from TMEM; the threads meanwhile update M in registers
+//   w = P' Z + weight * (X M)           and out by TMA
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "elements.cuh"
+#include "linear.h"
 #include "mixer.h"
 #include "shell_ops.h"
 #include "tc.cuh"
@@ -17,111 +38,841 @@ namespace lsso {
 
 namespace {
 
-// w_t = into * x_t . M_t;  M_t = e^l M_{t-1} + from * y_t z_t^T (late = 0: decayed before the token joins; 1: after).
+constexpr int kChunk = 128;
+constexpr int kThreads = 256;
+constexpr uint32_t kBox = kChunk * 128;  // 128 tokens x 64 features of 16 bits
+constexpr uint32_t kOutBox = 32 * 64;    // 32 tokens x 32 features
+constexpr float kLog2e = 1.44269504f;
+constexpr float kLeastLog = -1e4f;       // e^-1e4 is zero, and ranks times it are finite
+
+struct ScanMaps {
+  CUtensorMap x, y, z, w;
+};
 struct ScanPass {
-  TokenTensor x, y, z, w;
-  const float* state_in;   // nullable [batch, heads, ny, nz], or [.., nz, ny] (transposed)
-  float* state_out;        // nullable [batch, heads, ny, nz]
-  int ny, nz, transposed, reverse;
-  float into, from;
+  const float* state_in;  // nullable; per sample and head [key][value], of the segment where there are several
+  float* state_out;       // nullable; likewise
+  int ny, nz;             // widths of x and y, and of z and w
+  int transposed;         // the state's axes are (z, y)
+  int reverse;            // from the last token to the first; the state then is that of before the decay
+  int exact;              // the state leaves the kernel: what joins it keeps 24 bits
+  float into, from;       // factors of the state's part of w and of what joins the state; their product is the scores'
 };
 struct ScanArgs {
+  ScanMaps maps[3];
   ScanPass pass[3];
-  const float* log_decay;
-  const uint8_t* mask;
-  int64_t batch, length;
-  int heads;
+  const float* log_decay;  // [heads]
+  const uint8_t* mask;     // nullable [batch, length]
+  int length, heads, passes, segments, segment_chunks, chunks;
+  int stages;
+  int* counts;             // state pass: valid tokens of each segment [item][segment]
+  int* status;
 };
 
-constexpr int kLanes = 8, kColumns = 16, kRows = 16;
+struct ScanShared {
+  float from[kChunk], col[kChunk];
+  float state_scale[2][kChunk];
+  uint8_t top[2 * kChunk];  // FP16: largest exponents, of score rows and of state rows in turn
+  uint64_t full[2], scores, state, out, drain;
+  uint32_t tmem;
+  int abort_flag;
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kLanes* kColumns) decay_recurrent_kernel(const ScanArgs a) {
-  pdl_wait();
-  const ScanPass& p = a.pass[blockIdx.z];
-  const int lane = threadIdx.x % kLanes, column = blockIdx.y * kColumns + threadIdx.x / kLanes;
-  if (blockIdx.y * kColumns >= p.nz) return;
-  const int head = blockIdx.x % a.heads;
-  const int64_t sample = blockIdx.x / a.heads;
-  const bool live_column = column < p.nz;
-  const int rows = p.ny / kLanes;  // of this lane
-  const T* x = static_cast<const T*>(p.x.ptr) + sample * p.x.stride_batch + head * p.x.stride_head + lane * rows;
-  const T* y = static_cast<const T*>(p.y.ptr) + sample * p.y.stride_batch + head * p.y.stride_head + lane * rows;
-  const T* z = static_cast<const T*>(p.z.ptr) + sample * p.z.stride_batch + head * p.z.stride_head + column;
-  T* w = static_cast<T*>(const_cast<void*>(p.w.ptr)) + sample * p.w.stride_batch + head * p.w.stride_head + column;
-  const Decay decay(a.log_decay[head]);
-  float s[kRows];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    s[i] = 0.0f;
-    if (p.state_in != nullptr && i < rows && live_column) {
-      const int64_t row = lane * rows + i;
-      s[i] = p.state_in[static_cast<int64_t>(blockIdx.x) * p.ny * p.nz + (p.transposed ? column * static_cast<int64_t>(p.ny) + row : row * p.nz + column)];
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (kHalf) return pair_from_float(lo, hi, __half());
+  return pair_from_float(lo, hi, __nv_bfloat16());
+}
+template <bool kHalf>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if (kHalf) return pair_to_float(v, __half());
+  return pair_to_float(v, __nv_bfloat16());
+}
+template <bool kHalf>
+__device__ __forceinline__ uint32_t idesc(int n, bool a_mn, bool b_mn) {
+  return make_idesc(128, n, a_mn, b_mn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, ScanShared& sh, int* status) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort_flag, status));
+}
+__device__ __forceinline__ void pair_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// The power of two that brings values with largest (biased) exponent e into [2^14, 2^15), and its inverse: FP16's
+// range, used in full.
+struct PowerScale {
+  float up, down;
+  __device__ __forceinline__ explicit PowerScale(uint32_t e) : up(1.0f), down(1.0f) {
+    if (e < 255) {
+      const uint32_t c = max(e, 15u);
+      up = __uint_as_float((268 - c) << 23);
+      down = __uint_as_float((c - 14) << 23);
     }
   }
-  for (int64_t n = 0; n < a.length; ++n) {
-    const int64_t t = p.reverse ? a.length - 1 - n : n;
-    if (a.mask != nullptr && a.mask[sample * a.length + t] == 0) {
-      if (lane == 0 && live_column) w[t * p.w.stride_token] = from_float<T>(0.0f);
-      continue;
-    }
-    const float zv = live_column ? to_float(z[t * p.z.stride_token]) * p.from : 0.0f;
-    float sum = 0.0f;
+};
+
+// Which of a chunk's tokens are valid, and this thread's row of it.
+struct ChunkRanks {
+  uint32_t words[4];
+  int before[4], total;  // valid tokens before each word, and in all
+
+  __device__ __forceinline__ void count() {
+    int sum = 0;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      if (i < rows) {
-        s[i] = fmaf(to_float(y[t * p.y.stride_token + i]), zv, p.reverse ? s[i] : decay.apply(s[i]));
-        sum = fmaf(to_float(x[t * p.x.stride_token + i]), s[i], sum);
-        if (p.reverse) s[i] = decay.apply(s[i]);
+    for (int w = 0; w < 4; ++w) {
+      before[w] = sum;
+      sum += __popc(words[w]);
+    }
+    total = sum;
+  }
+  // selects, not register indexing
+  __device__ __forceinline__ uint32_t word(int w) const { return w < 2 ? (w == 0 ? words[0] : words[1]) : (w == 2 ? words[2] : words[3]); }
+  __device__ __forceinline__ int sum_before(int w) const { return w < 2 ? (w == 0 ? before[0] : before[1]) : (w == 2 ? before[2] : before[3]); }
+  __device__ __forceinline__ bool live(int w, int lane) const { return (word(w) >> lane) & 1u; }
+  // rank in the direction of the scan
+  __device__ __forceinline__ int rho(int w, int lane, bool reverse) const {
+    const int r = sum_before(w) + __popc(word(w) & ((1u << lane) - 1u));
+    return reverse ? total - 1 - r : r;
+  }
+  // the largest rho of a block of 32 tokens
+  __device__ __forceinline__ int last_rho(int w, bool reverse) const {
+    return reverse ? total - 1 - sum_before(w) : sum_before(w) + __popc(word(w)) - 1;
+  }
+  __device__ __forceinline__ bool whole() const { return (words[0] & words[1] & words[2] & words[3]) == 0xffffffffu; }
+};
+
+// kKB, kVB: 64-feature boxes of x and y, and of z and w.  kStateOnly: the states of segments, no outputs.
+template <bool kHalf, int kKB, int kVB, bool kStateOnly>
+__global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_kernel(const __grid_constant__ ScanArgs a) {
+  constexpr bool kSmall = kKB + kVB == 2;
+  // TMEM columns.  P' takes the lower half of P; with single boxes P' Z takes its upper half, so that two CTAs fit an SM.
+  constexpr uint32_t kColP = 0, kColXm = 128, kColChange = kStateOnly ? 0 : kSmall ? 192 : 256, kColOut = kSmall ? 64 : 384;
+  constexpr uint32_t kCols = kStateOnly ? 64 * kKB : kSmall ? 256 : 512;
+  constexpr int kParts = kVB == 1 ? 4 : 2;         // threads that share a row of M^T (one lane quadrant or two hold it)
+  constexpr int kOwn = 64 * kKB / kParts;          // its columns held by one thread
+  constexpr uint32_t kBoxes = (kStateOnly ? 0 : kKB) + kKB + kVB;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ ScanShared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, hf = warp >> 2;
+  const int pass_index = blockIdx.x % a.passes;
+  const ScanPass& p = a.pass[pass_index];
+  const ScanMaps& maps = a.maps[pass_index];
+  const int unit = blockIdx.x / a.passes, segment = unit % a.segments, item = unit / a.segments;
+  const int head = item % a.heads, sample = item / a.heads;
+  const bool reverse = p.reverse != 0;
+  const int first = segment * a.segment_chunks, count = min(a.segment_chunks, a.chunks - first);
+  const int ny = p.ny, nz = p.nz, stages = a.stages;
+  const bool exact = p.exact != 0;
+  constexpr uint32_t kStage = kBoxes * kBox;
+  uint8_t* const state_tile = smem + stages * kStage;                                       // M^T: [kKB][64 kVB rows][128 bytes]
+  uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kVB * 64 * 128);              // exact: parts that have no other place
+
+  if (tid == 0) {
+    mbar_init(smem_u32(&sh.full[0]), 1);
+    mbar_init(smem_u32(&sh.full[1]), 1);
+    mbar_init(smem_u32(&sh.scores), 1);
+    mbar_init(smem_u32(&sh.state), 1);
+    mbar_init(smem_u32(&sh.out), 1);
+    mbar_init(smem_u32(&sh.drain), 1);
+    sh.abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tmap(&maps.y);
+    prefetch_tmap(&maps.z);
+    if (!kStateOnly) {
+      prefetch_tmap(&maps.x);
+      prefetch_tmap(&maps.w);
+    }
+  }
+  // Before the allocation, so that no block of an earlier kernel finds its TMEM taken by one that waits for it.
+  pdl_wait();
+  if (warp == 0) tmem_alloc(smem_u32(&sh.tmem), kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const uint32_t base = smem_u32(smem), full_bar = smem_u32(sh.full);
+
+  auto chunk_at = [&](int n) { return reverse ? first + count - 1 - n : first + n; };
+  auto load = [&](int n) {  // by thread 0
+    const int s = stages == 2 ? n & 1 : 0, t0 = chunk_at(n) * kChunk;
+    const uint32_t bar = full_bar + 8 * s;
+    uint32_t dst = base + s * kStage;
+    mbar_arrive_expect_tx(bar, kStage);
+    if (!kStateOnly) {
+#pragma unroll
+      for (int b = 0; b < kKB; ++b, dst += kBox) tma_load_4d(dst, &maps.x, 64 * b, head, t0, sample, bar);
+    }
+#pragma unroll
+    for (int b = 0; b < kKB; ++b, dst += kBox) tma_load_4d(dst, &maps.y, 64 * b, head, t0, sample, bar);
+#pragma unroll
+    for (int b = 0; b < kVB; ++b, dst += kBox) tma_load_4d(dst, &maps.z, 64 * b, head, t0, sample, bar);
+  };
+  int issued = 0;
+  if (tid == 0) {
+    for (; issued < min(stages, count); ++issued) load(issued);
+  }
+
+  // ---- the head's decay; valid tokens of a chunk
+  float l = a.log_decay[head];
+  if (l < kLeastLog) l = kLeastLog;  // keeps a NaN
+  const float l2 = l * kLog2e;
+  const float late = reverse ? 1.0f : 0.0f;
+  const float inside = p.into * p.from;
+  // Factor of a chunk's part of the state.  The weights of its rows leave it out, so that the largest of them is one:
+  // FP16 would lose rows whose weights are all small (a strong decay before the state of a reverse scan).
+  const float join = p.from * exp2f(l2 * late);
+  const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
+  ChunkRanks ranks;
+  uint32_t ahead = 0;  // mask bytes of a later chunk, as bits
+  auto fetch_mask = [&](int n) {
+    ahead = 0xf;
+    if (a.mask == nullptr) return;
+    ahead = 0;
+    const int t0 = chunk_at(n) * kChunk + lane;
+    const uint8_t* m = a.mask + static_cast<int64_t>(sample) * a.length;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (t0 + 32 * w < a.length && m[t0 + 32 * w] != 0) ahead |= 1u << w;
+  };
+  float row_rho = 0.0f, lambda = 0.0f, block_factor[2] = {0.0f, 0.0f};
+  bool live = false, dead_tokens = false;
+  float decay_factor = 0.0f, decay_keep = 0.0f;  // M' = M * factor + M * keep (keep is 0 or 1)
+  int decay_total = -1, tail_state = 0;
+  // Ranks and tables of chunk n from the fetched bits.  Whole chunks all have the same, and find them in place.
+  auto prepare = [&](int n) {
+    const int t0 = chunk_at(n) * kChunk;
+    if (a.mask == nullptr) {
+      const int left = a.length - t0;  // tokens
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int of_word = left - 32 * w;
+        ranks.words[w] = of_word >= 32 ? 0xffffffffu : of_word <= 0 ? 0u : (1u << of_word) - 1u;
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) ranks.words[w] = __ballot_sync(0xffffffffu, (ahead >> w) & 1u);
+    }
+    const int kind = ranks.whole() ? 1 : 2;
+    if (kind == 1 && tail_state == 1) return;
+    tail_state = kind;
+    ranks.count();
+    live = ranks.live(q, lane);
+    // tokens to be cleared: masked ones (behind the last token there are zeros)
+    dead_tokens = a.mask != nullptr && kind == 2;
+    const int rho = ranks.rho(q, lane, reverse);
+    if (hf == 0) {
+      sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : 0.0f;
+    } else if (!kStateOnly) {
+      sh.col[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.last_rho(q, reverse) - rho)) : 0.0f;
+    }
+    if (!kStateOnly) {
+      row_rho = static_cast<float>(rho);
+      lambda = p.into * exp2f(l2 * (row_rho + 1.0f - late));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(hf + 2 * i, reverse))));
       }
     }
+    if (ranks.total != decay_total) {
+      decay_total = ranks.total;
+      const Decay d(l * static_cast<float>(decay_total));
+      decay_factor = d.factor;
+      decay_keep = d.near_one ? 1.0f : 0.0f;
+    }
+  };
+
+  // ---- this thread's part of M^T: row mv, columns [mc, mc + kOwn)
+  const int mv = kVB == 1 ? 32 * (q & 1) + lane : 32 * q + lane;
+  const int part = kVB == 1 ? (q >> 1) + 2 * hf : hf;
+  const int mc = part * kOwn;
+  float m[kOwn];
+  {
+    const bool transposed = (p.transposed & 1) != 0;
+    const float* src = p.state_in == nullptr || kStateOnly
+                           ? nullptr
+                           : p.state_in + (static_cast<int64_t>(item) * a.segments + segment) * ny * nz;
 #pragma unroll
-    for (int d = kLanes / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0 && live_column) w[t * p.w.stride_token] = from_float<T>(sum * p.into);
+    for (int i = 0; i < kOwn; ++i) {
+      m[i] = 0.0f;
+      const int c = mc + i;
+      if (src != nullptr && mv < nz && c < ny) m[i] = src[transposed ? mv * ny + c : c * nz + mv];
+    }
   }
-  if (p.state_out != nullptr && live_column) {
+  // M^T as the next product's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
+  auto write_state = [&](int parity) {
+    float up = 1.0f;
+    if (kHalf) {
+      float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (i < rows) p.state_out[static_cast<int64_t>(blockIdx.x) * p.ny * p.nz + (lane * rows + i) * static_cast<int64_t>(p.nz) + column] = s[i];
+      for (int i = 0; i < kOwn; ++i) most = fmaxf(most, fabsf(m[i]));
+      uint32_t e = 0;  // the largest of the kParts threads that share the row
+      sh.top[part * (64 * kVB) + mv] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
+      pair_barrier(kVB == 1 ? 5 + (q & 1) : 1 + q, 32 * kParts);
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) e = max(e, static_cast<uint32_t>(sh.top[i * (64 * kVB) + mv]));
+      const PowerScale s(e);
+      up = s.up;
+      if (part == 0) sh.state_scale[parity][mv] = s.down;
+    }
+#pragma unroll
+    for (int i = 0; i < kOwn; i += 8) {
+      const int c = mc + i, box = c >> 6, piece = (c >> 3) & 7;
+      const uint4 v = make_uint4(pack2<kHalf>(m[i] * up, m[i + 1] * up), pack2<kHalf>(m[i + 2] * up, m[i + 3] * up),
+                                 pack2<kHalf>(m[i + 4] * up, m[i + 5] * up), pack2<kHalf>(m[i + 6] * up, m[i + 7] * up));
+      *reinterpret_cast<uint4*>(state_tile + box * (kVB * 64 * 128) + mv * 128 + ((piece ^ (mv & 7)) << 4)) = v;
+    }
+  };
+
+  fetch_mask(0);
+  prepare(0);
+  int tokens_seen = ranks.total;
+  if (!kStateOnly) write_state(0);
+  fence_proxy_async();
+  bool ok = __syncthreads_and(1) != 0;
+
+  const uint32_t quadrant = tmem + (static_cast<uint32_t>(q) << 21);  // this warp's lanes
+  const uint32_t scores_bar = smem_u32(&sh.scores), state_bar = smem_u32(&sh.state), out_bar = smem_u32(&sh.out);
+  const int y_steps = (ny + 15) / 16;
+
+  for (int n = 0; n < count; ++n) {
+    const int s = stages == 2 ? n & 1 : 0;
+    const uint32_t use = stages == 2 ? (n >> 1) & 1 : n & 1, parity = n & 1;
+    const uint32_t x_at = base + s * kStage, y_at = x_at + (kStateOnly ? 0 : kKB * kBox), z_at = y_at + kKB * kBox;
+    uint8_t* const x_tile = smem + s * kStage;
+    uint8_t* const y_tile = x_tile + (kStateOnly ? 0 : kKB * kBox);
+    uint8_t* const z_tile = y_tile + kKB * kBox;
+
+    // ---- scores and the state's part
+    ok = wait_warp(full_bar + 8 * s, use, sh, a.status) && ok;
+    if (!kStateOnly) {
+      if (tid == 0 && ok) {
+        tc_fence_after();
+        const uint32_t ip = idesc<kHalf>(128, false, false), im = idesc<kHalf>((nz + 15) & ~15, false, false);
+        for (int k = 0; k < y_steps; ++k) {
+          const uint32_t at = (k >> 2) * kBox + (k & 3) * 32;
+          const uint64_t xd = make_desc_sw128(x_at + at, 16, 1024);
+          mma_bf16(tmem + kColP, xd, make_desc_sw128(y_at + at, 16, 1024), ip, k > 0);
+          mma_bf16(tmem + kColXm, xd,
+                   make_desc_sw128(smem_u32(state_tile) + (k >> 2) * (kVB * 64 * 128) + (k & 3) * 32, 16, 1024), im, k > 0);
+        }
+        mma_commit(scores_bar);
+      }
+      __syncwarp();
+    }
+    if (n + 1 < count) fetch_mask(n + 1);
+    if (!kStateOnly) {
+      ok = wait_warp(scores_bar, parity, sh, a.status) && ok;
+      tc_fence_after();
+    }
+
+    // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
+    {
+      const int pieces = ny <= 32 ? 4 : 8;  // 16-byte pieces of a row that hold features (of each box)
+      const int shift = ny <= 32 ? 2 : 3;
+#pragma unroll 1
+      for (int b = 0; b < kKB; ++b) {
+#pragma unroll 4
+        for (int i = tid; i < kChunk * pieces; i += kThreads) {
+          const int row = i >> shift, piece = i & (pieces - 1);
+          const uint32_t at = b * kBox + row * 128 + ((piece ^ (row & 7)) << 4);
+          const float f = sh.from[row];
+          const uint4 v = *reinterpret_cast<const uint4*>(y_tile + at);
+          const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+          uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 e = unpack2<kHalf>(in[j]);
+            e.x *= f;
+            e.y *= f;
+            if (f == 0.0f) e = make_float2(0.0f, 0.0f);  // whatever a masked token holds
+            hi[j] = pack2<kHalf>(e.x, e.y);
+            if (exact) {
+              float2 h = unpack2<kHalf>(hi[j]);
+              e.x -= h.x;
+              e.y -= h.y;
+              if (kHalf) {
+                mid[j] = pack2<kHalf>(e.x * 2048.0f, e.y * 2048.0f);
+              } else {
+                mid[j] = pack2<kHalf>(e.x, e.y);
+                h = unpack2<kHalf>(mid[j]);
+                lo[j] = pack2<kHalf>(e.x - h.x, e.y - h.y);
+              }
+            }
+          }
+          *reinterpret_cast<uint4*>(y_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (exact) {
+            uint8_t* second = kStateOnly ? third + (kHalf ? 0 : kKB * kBox) : x_tile;
+            *reinterpret_cast<uint4*>(second + at) = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+            if (!kHalf) *reinterpret_cast<uint4*>(third + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        }
+      }
+      if (dead_tokens && tid < kChunk) {
+        if (!ranks.live(warp, lane)) {
+#pragma unroll
+          for (int b = 0; b < kVB; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(z_tile + b * kBox + tid * 128 + 16 * j) = make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    if (!kStateOnly && lane == 0) bulk_wait_read<0>();  // the stage before this one has been stored from
+    ok = __syncthreads_and(ok) != 0;
+    if (!ok) break;
+    if (tid == 0) {
+      tc_fence_after();
+      const uint32_t id = idesc<kHalf>((ny + 15) & ~15, true, true);
+      const uint64_t zd = make_desc_sw128(z_at, kVB == 2 ? kBox : 0, 1024);  // one box: lanes 64-127 repeat 0-63
+      const uint32_t second = kStateOnly ? smem_u32(third) + (kHalf ? 0 : kKB * kBox) : x_at;
+      const uint32_t rows[3] = {smem_u32(third), second, y_at};
+      bool more = false;
+#pragma unroll
+      for (int t = exact ? (kHalf ? 1 : 0) : 2; t < 3; ++t) {
+        const uint64_t yd = make_desc_sw128(rows[t], kBox, 1024);
+        for (int k = 0; k < kChunk / 16; ++k) {
+          if (kHalf && t == 2 && k == 0 && exact) {
+            mma_scaled_d(tmem + kColChange, zd, yd, id);  // the parts so far are 2^11 times too large
+          } else {
+            mma_bf16(tmem + kColChange, zd + k * 128, yd + k * 128, id, more);
+          }
+          more = true;
+        }
+      }
+      mma_commit(state_bar);
+      if (!kStateOnly && stages == 2 && n > 0 && n + 1 < count) {
+        load(n + 1);
+        ++issued;
+      }
+    }
+    __syncwarp();
+
+    // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns hf and hf + 2
+    float down = 1.0f;
+    if (!kStateOnly) {
+      float v[2][32];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int block = hf + 2 * i;
+        if (reverse ? block >= q : block <= q) tmem_ld32(quadrant + kColP + 32 * block, v[i]);
+      }
+      tmem_ld_wait();
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int block = hf + 2 * i;
+        const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block);
+        if (reverse ? block > q : block < q) {
+          const float f = block_factor[i];
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 c = col[j / 4];
+            if (dead_tokens) {
+              v[i][j] = c.x == 0.0f ? 0.0f : v[i][j];
+              v[i][j + 1] = c.y == 0.0f ? 0.0f : v[i][j + 1];
+              v[i][j + 2] = c.z == 0.0f ? 0.0f : v[i][j + 2];
+              v[i][j + 3] = c.w == 0.0f ? 0.0f : v[i][j + 3];
+            }
+            v[i][j] *= f * c.x;
+            v[i][j + 1] *= f * c.y;
+            v[i][j + 2] *= f * c.z;
+            v[i][j + 3] *= f * c.w;
+          }
+        } else if (block == q) {
+          // the block on the diagonal: its valid columns up to this row's token (from it on)
+          const uint32_t seen = ranks.word(q) & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane));
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 c = col[j / 4];
+            const float cs[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float w = block_factor[i] * cs[e];
+              if (!gentle) {  // tokens between the two
+                // rank distance: valid tokens seen by the row that lie on its side of token j + e
+                const uint32_t side = reverse ? (1u << (j + e)) - 1u : ~(0xffffffffu >> (31 - (j + e)));
+                w = inside * exp2f(l2 * static_cast<float>(__popc(seen & side)));
+              }
+              v[i][j + e] = (seen >> (j + e)) & 1u ? v[i][j + e] * w : 0.0f;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[i][j] = 0.0f;
+        }
+        if (kHalf) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[i][j]));
+        }
+      }
+      float up = 1.0f;
+      const uint32_t top = __float_as_uint(most) >> 23;
+      if (kHalf) sh.top[hf * kChunk + 32 * q + lane] = static_cast<uint8_t>(top);
+      tc_fence_before();
+      pair_barrier(1 + q, 64);  // both warps of these rows have read their scores
+      tc_fence_after();
+      if (kHalf) {
+        const PowerScale sc(max(top, static_cast<uint32_t>(sh.top[(hf ^ 1) * kChunk + 32 * q + lane])));
+        up = sc.up;
+        down = sc.down;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack2<kHalf>(v[i][2 * j] * up, v[i][2 * j + 1] * up);
+        tmem_st16(quadrant + kColP + 16 * (hf + 2 * i), w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      ok = __syncthreads_and(ok) != 0;
+      if (!ok) break;
+      if (tid == 0) {
+        tc_fence_after();
+        const uint32_t io = idesc<kHalf>((nz + 15) & ~15, false, true);
+        const uint64_t zd = make_desc_sw128(z_at, kBox, 1024);
+        for (int k = 0; k < kChunk / 16; ++k) mma_tmem_a(tmem + kColOut, tmem + kColP + 8 * k, zd + k * 128, io, k > 0);
+        mma_commit(out_bar);
+      }
+      __syncwarp();
+    }
+
+    // ---- the state after this chunk
+    ok = wait_warp(state_bar, parity, sh, a.status) && ok;
+    tc_fence_after();
+#pragma unroll
+    for (int i = 0; i < kOwn; i += 16) {
+      if (mc + i >= ny) break;  // no product wrote these columns
+      float d[16];
+      tmem_ld16(quadrant + kColChange + mc + i, d);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) m[i + j] = fmaf(d[j], join, fmaf(m[i + j], decay_factor, m[i + j] * decay_keep));
+    }
+    if (kStateOnly) {
+      if (n + 1 < count) {
+        prepare(n + 1);
+        tokens_seen += ranks.total;
+      }
+      tc_fence_before();
+      ok = __syncthreads_and(ok) != 0;
+      if (!ok) break;
+      if (tid == 0 && n + stages < count) {
+        load(n + stages);
+        ++issued;
+      }
+      __syncwarp();
+      continue;
+    }
+    if (n + 1 < count) write_state(parity ^ 1);
+
+    // ---- outputs
+    ok = wait_warp(out_bar, parity, sh, a.status) && ok;
+    tc_fence_after();
+    uint32_t packed[kVB][16];
+    const float row_into = lambda;
+    const bool row_live = live;
+#pragma unroll
+    for (int b = 0; b < kVB; ++b) {
+      const int col0 = 32 * (hf + 2 * b);
+      if (col0 >= nz) continue;
+      float o[32], x[32];
+      tmem_ld32(quadrant + kColOut + col0, o);
+      tmem_ld32(quadrant + kColXm + col0, x);
+      tmem_ld_wait();
+      const float4* scale = reinterpret_cast<const float4*>(sh.state_scale[parity] + col0);
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        float4 f = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        if (kHalf) f = scale[j / 4];
+        o[j] = fmaf(o[j], down, row_into * (x[j] * f.x));
+        o[j + 1] = fmaf(o[j + 1], down, row_into * (x[j + 1] * f.y));
+        o[j + 2] = fmaf(o[j + 2], down, row_into * (x[j + 2] * f.z));
+        o[j + 3] = fmaf(o[j + 3], down, row_into * (x[j + 3] * f.w));
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) packed[b][j] = row_live ? pack2<kHalf>(o[2 * j], o[2 * j + 1]) : 0u;
+    }
+    if (n + 1 < count) prepare(n + 1);
+    fence_proxy_async();
+    tc_fence_before();
+    ok = __syncthreads_and(ok) != 0;
+    if (!ok) break;
+    tc_fence_after();
+    // z's boxes have been read: the output boxes (64-byte rows and swizzle) leave from there
+    const int t0 = chunk_at(n) * kChunk + 32 * q;
+#pragma unroll
+    for (int b = 0; b < kVB; ++b) {
+      const int col0 = 32 * (hf + 2 * b);
+      if (col0 >= nz || t0 >= a.length) continue;
+      uint8_t* box = z_tile + (warp * kVB + b) * kOutBox;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+            make_uint4(packed[b][4 * c], packed[b][4 * c + 1], packed[b][4 * c + 2], packed[b][4 * c + 3]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) tma_store_4d(&maps.w, smem_u32(box), col0, head, t0, sample);
+    }
+    if (lane == 0) bulk_commit();
+    if (stages == 1) {
+      if (lane == 0) bulk_wait_read<0>();
+      __syncthreads();
+      if (tid == 0 && n + 1 < count) {
+        load(n + 1);
+        ++issued;
+      }
+      __syncwarp();
+    }
+  }
+
+  if (ok && p.state_out != nullptr && mv < nz) {
+    // a whole scan's state is the caller's; a segment's belongs to its segment
+    const bool end = reverse ? segment == 0 : segment == a.segments - 1;
+    if (kStateOnly || end) {
+      float* dst = p.state_out + (kStateOnly ? static_cast<int64_t>(item) * a.segments + segment : item) * ny * nz;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i)
+        if (mc + i < ny) dst[(mc + i) * nz + mv] = m[i];
+      if (kStateOnly && tid == 0 && pass_index == 0) a.counts[item * a.segments + segment] = tokens_seen;
+    }
+  }
+  // ---- nothing may be in flight when the CTA ends
+  if (!kStateOnly && lane == 0) bulk_wait<0>();
+  if (tid == 0) {
+    if (!ok) {
+      for (int n = max(0, issued - stages); n < issued; ++n)
+        mbar_wait_bounded(full_bar + 8 * (stages == 2 ? n & 1 : 0), stages == 2 ? (n >> 1) & 1 : n & 1, nullptr, a.status);
+    }
+    mma_drain(smem_u32(&sh.drain), a.status);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, kCols);
+}
+
+// ---------------------------------------------------------------- joining segments
+struct JoinSet {
+  float* states;         // [item][segment][values]: a segment's own part in, the state before it out
+  const float* initial;  // nullable [item][values]
+  int reverse;
+};
+struct JoinArgs {
+  JoinSet set[2];
+  const float* log_decay;
+  const int* counts;  // [item][segment]
+  int heads, segments, values;
+};
+
+// M before each segment from the segments' own parts, in scan order: a short chain of multiply-adds per element, its
+// loads in flight ahead of it.
+__global__ void __launch_bounds__(256) decay_join_kernel(const JoinArgs a) {
+  pdl_wait();
+  const JoinSet& set = a.set[blockIdx.z];
+  const int item = blockIdx.x, e = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (e >= a.values) return;
+  float l = a.log_decay[item % a.heads];
+  if (l < kLeastLog) l = kLeastLog;
+  float4* at = reinterpret_cast<float4*>(set.states + static_cast<int64_t>(item) * a.segments * a.values + e);
+  const int step = a.values / 4;
+  float4 m = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (set.initial != nullptr) m = *reinterpret_cast<const float4*>(set.initial + static_cast<int64_t>(item) * a.values + e);
+  constexpr int kAhead = 8;
+  for (int n0 = 0; n0 < a.segments; n0 += kAhead) {
+    float4 own[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int n = n0 + i;
+      if (n < a.segments) own[i] = at[static_cast<int64_t>(set.reverse ? a.segments - 1 - n : n) * step];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int n = n0 + i;
+      if (n >= a.segments) break;
+      const int seg = set.reverse ? a.segments - 1 - n : n;
+      at[static_cast<int64_t>(seg) * step] = m;
+      const Decay d(l * static_cast<float>(a.counts[item * a.segments + seg]));
+      m = make_float4(d.apply(m.x) + own[i].x, d.apply(m.y) + own[i].y, d.apply(m.z) + own[i].z, d.apply(m.w) + own[i].w);
+    }
   }
 }
 
-cudaError_t launch_scans(const ScanArgs& a, int count, int type, const char* name, cudaStream_t stream) {
-  int most = 0;
-  for (int i = 0; i < count; ++i) most = std::max(most, a.pass[i].nz);
-  const dim3 grid(static_cast<unsigned>(a.batch * a.heads), (most + kColumns - 1) / kColumns, count);
-  auto kernel = type == kFp16 ? &decay_recurrent_kernel<__half> : &decay_recurrent_kernel<__nv_bfloat16>;
-  LaunchScope scope(name, stream);
-  launch_pdl(kernel, grid, kLanes * kColumns, 0, stream, a);
-  return cudaGetLastError();
+// ---------------------------------------------------------------- plans and launches
+struct DecayPlan {
+  int chunks, segments, segment_chunks;
+  size_t counts, states[2], total;  // workspace offsets
+};
+
+DecayPlan make_plan(int64_t batch, int64_t length, int heads, int key, int value, bool backward, int sm_count) {
+  DecayPlan p{};
+  p.chunks = static_cast<int>((length + kChunk - 1) / kChunk);
+  const int64_t items = batch * heads, units = items * (backward ? 3 : 1);
+  const int per_sm = key <= 64 && value <= 64 ? 2 : 1;
+  const int64_t room = static_cast<int64_t>(per_sm) * sm_count / units;  // segments that fit in one wave
+  p.segments = 1;
+  if (room > 1 && p.chunks >= 8) p.segments = static_cast<int>(std::min<int64_t>(room, p.chunks / 2));
+  p.segment_chunks = (p.chunks + p.segments - 1) / p.segments;
+  p.segments = (p.chunks + p.segment_chunks - 1) / p.segment_chunks;
+  p.total = 16;
+  if (p.segments > 1) {
+    const size_t one = static_cast<size_t>(items) * p.segments * key * value * sizeof(float);
+    p.counts = one * (backward ? 2 : 1);
+    p.states[1] = one;
+    p.total = p.counts + (static_cast<size_t>(items) * p.segments * sizeof(int) + 15) / 16 * 16;
+  }
+  return p;
 }
 
-ScanArgs common(const DecayCall& c) {
+// Tensor map of [batch, length, heads, width] by strides: boxes of 128 tokens x 64 features (loads, 128-byte swizzle;
+// what lies outside reads as zero) or of 32 x 32 (stores, 64-byte swizzle; what lies outside is not written).
+bool encode(CUtensorMap* map, const TokenTensor& t, const DecayCall& c, int width, bool store) {
+  PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(c.heads), static_cast<cuuint64_t>(c.length),
+                        static_cast<cuuint64_t>(c.batch)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.stride_head) * 2, static_cast<cuuint64_t>(t.stride_token) * 2,
+                           static_cast<cuuint64_t>(t.stride_batch) * 2};
+  cuuint32_t box[4] = {store ? 32u : 64u, 1u, store ? 32u : static_cast<cuuint32_t>(kChunk), 1u};
+  cuuint32_t ones[4] = {1, 1, 1, 1};
+  return fn(map, c.type == kFp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+            const_cast<void*>(t.ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            store ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+ScanArgs common(const DecayCall& c, const DecayPlan& p, uint8_t* workspace) {
   ScanArgs a{};
   a.log_decay = c.log_decay;
   a.mask = c.mask;
-  a.batch = c.batch;
-  a.length = c.length;
+  a.length = static_cast<int>(c.length);
   a.heads = c.heads;
+  a.segments = p.segments;
+  a.segment_chunks = p.segment_chunks;
+  a.chunks = p.chunks;
+  a.counts = reinterpret_cast<int*>(workspace + p.counts);
+  a.status = c.status;
   return a;
+}
+
+template <bool kHalf, int kKB, int kVB, bool kStateOnly>
+cudaError_t launch_one(ScanArgs& a, int64_t items, const char* name, cudaStream_t stream) {
+  bool exact = false;
+  for (int i = 0; i < a.passes; ++i) exact = exact || a.pass[i].exact != 0;
+  // the parts of exactly weighted rows that have no other buffer
+  const int parts = !exact ? 0 : kStateOnly ? (kHalf ? 1 : 2) : (kHalf ? 0 : 1);
+  const size_t stage = ((kStateOnly ? 1 : 2) * kKB + kVB) * kBox;
+  const size_t rest = (kStateOnly ? 0 : kKB * kVB * 64 * 128) + parts * kKB * kBox;
+  // Two stages where they fit (beside a second CTA, where its TMEM leaves room for one).
+  const size_t most = kKB + kVB == 2 ? 113 * 1024 - 4096 : 232448 - 2560;
+  a.stages = 2 * stage + rest <= most ? 2 : 1;
+  auto kernel = &decay_scan_kernel<kHalf, kKB, kVB, kStateOnly>;
+  const size_t smem = a.stages * stage + rest;
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (e != cudaSuccess) return e;
+  LaunchScope scope(name, stream);
+  launch_pdl(kernel, dim3(static_cast<unsigned>(items * a.segments * a.passes)), kThreads, smem, stream, a);
+  return cudaGetLastError();
+}
+
+template <bool kStateOnly>
+cudaError_t launch_scans(ScanArgs& a, int64_t items, int type, int ny, int nz, const char* name, cudaStream_t stream) {
+  const bool half = type == kFp16;
+  if (ny <= 64 && nz <= 64)
+    return half ? launch_one<true, 1, 1, kStateOnly>(a, items, name, stream) : launch_one<false, 1, 1, kStateOnly>(a, items, name, stream);
+  if (ny <= 64)
+    return half ? launch_one<true, 1, 2, kStateOnly>(a, items, name, stream) : launch_one<false, 1, 2, kStateOnly>(a, items, name, stream);
+  if (nz <= 64)
+    return half ? launch_one<true, 2, 1, kStateOnly>(a, items, name, stream) : launch_one<false, 2, 1, kStateOnly>(a, items, name, stream);
+  return half ? launch_one<true, 2, 2, kStateOnly>(a, items, name, stream) : launch_one<false, 2, 2, kStateOnly>(a, items, name, stream);
+}
+
+struct ScanTensors {
+  const TokenTensor *x, *y, *z, *w;
+};
+bool encode_pass(ScanMaps* m, const ScanTensors& t, const DecayCall& c, int ny, int nz) {
+  if (t.x != nullptr && !(encode(&m->x, *t.x, c, ny, false) && encode(&m->w, *t.w, c, nz, true))) return false;
+  return encode(&m->y, *t.y, c, ny, false) && encode(&m->z, *t.z, c, nz, false);
 }
 
 }  // namespace
 
-size_t decay_workspace(int64_t, int64_t, int, int, int, bool, int) { return 16; }
-
-cudaError_t launch_decay_forward(const DecayCall& c, uint8_t*, int, cudaStream_t stream) {
-  ScanArgs a = common(c);
-  a.pass[0] = ScanPass{c.q, c.k, c.v, c.y, c.state, c.last, c.key, c.value, 0, 0, c.scale, 1.0f};
-  return launch_scans(a, 1, c.type, "decay", stream);
+size_t decay_workspace(int64_t batch, int64_t length, int heads, int key, int value, bool backward, int sm_count) {
+  return make_plan(batch, length, heads, key, value, backward, sm_count).total;
 }
 
-cudaError_t launch_decay_backward(const DecayCall& c, uint8_t*, int, cudaStream_t stream) {
-  ScanArgs a = common(c);
-  a.pass[0] = ScanPass{c.y, c.v, c.k, c.dq, c.state, nullptr, c.value, c.key, 1, 0, c.scale, 1.0f};
-  a.pass[1] = ScanPass{c.v, c.y, c.q, c.dk, c.dlast, nullptr, c.value, c.key, 1, 1, 1.0f, c.scale};
-  a.pass[2] = ScanPass{c.k, c.q, c.y, c.dv, c.dlast, c.dstate, c.key, c.value, 0, 1, 1.0f, c.scale};
-  return launch_scans(a, 3, c.type, "decay_bwd", stream);
+cudaError_t launch_decay_forward(const DecayCall& c, uint8_t* workspace, int sm_count, cudaStream_t stream) {
+  const DecayPlan p = make_plan(c.batch, c.length, c.heads, c.key, c.value, false, sm_count);
+  const int64_t items = c.batch * c.heads;
+  ScanArgs a = common(c, p, workspace);
+  const int exact = c.last != nullptr ? 1 : 0;
+  float* states = reinterpret_cast<float*>(workspace);
+  a.passes = 1;
+  a.pass[0] = ScanPass{nullptr, states, c.key, c.value, 0, 0, exact, 1.0f, 1.0f};
+  if (!encode_pass(&a.maps[0], ScanTensors{&c.q, &c.k, &c.v, &c.y}, c, c.key, c.value)) return cudaErrorInvalidValue;
+  if (p.segments > 1) {
+    cudaError_t e = launch_scans<true>(a, items, c.type, c.key, c.value, "decay_states", stream);
+    if (e != cudaSuccess) return e;
+    const JoinArgs j{{JoinSet{states, c.state, 0}, JoinSet{}}, c.log_decay, a.counts, c.heads, p.segments, c.key * c.value};
+    LaunchScope scope("decay_join", stream);
+    launch_pdl(&decay_join_kernel, dim3(static_cast<unsigned>(items), (c.key * c.value + 1023) / 1024, 1), 256, 0, stream, j);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  a.pass[0] = ScanPass{p.segments > 1 ? states : c.state, c.last, c.key, c.value, 0, 0, exact, c.scale, 1.0f};
+  return launch_scans<false>(a, items, c.type, c.key, c.value, "decay", stream);
+}
+
+cudaError_t launch_decay_backward(const DecayCall& c, uint8_t* workspace, int sm_count, cudaStream_t stream) {
+  const DecayPlan p = make_plan(c.batch, c.length, c.heads, c.key, c.value, true, sm_count);
+  const int64_t items = c.batch * c.heads;
+  const TokenTensor& dy = c.y;
+  const int exact = c.dstate != nullptr ? 1 : 0;
+  const float *before = c.state, *after = c.dlast;
+  if (p.segments > 1) {
+    float* sums[2] = {reinterpret_cast<float*>(workspace), reinterpret_cast<float*>(workspace + p.states[1])};
+    ScanArgs a = common(c, p, workspace);
+    a.passes = 2;
+    a.pass[0] = ScanPass{nullptr, sums[0], c.key, c.value, 0, 0, 0, 1.0f, 1.0f};
+    a.pass[1] = ScanPass{nullptr, sums[1], c.key, c.value, 0, 1, exact, 1.0f, c.scale};
+    if (!encode_pass(&a.maps[0], ScanTensors{nullptr, &c.k, &c.v, nullptr}, c, c.key, c.value) ||
+        !encode_pass(&a.maps[1], ScanTensors{nullptr, &c.q, &dy, nullptr}, c, c.key, c.value)) {
+      return cudaErrorInvalidValue;
+    }
+    cudaError_t e = launch_scans<true>(a, items, c.type, c.key, c.value, "decay_states", stream);
+    if (e != cudaSuccess) return e;
+    const JoinArgs j{{JoinSet{sums[0], c.state, 0}, JoinSet{sums[1], c.dlast, 1}}, c.log_decay, a.counts, c.heads, p.segments,
+                     c.key * c.value};
+    LaunchScope scope("decay_join", stream);
+    launch_pdl(&decay_join_kernel, dim3(static_cast<unsigned>(items), (c.key * c.value + 1023) / 1024, 2), 256, 0, stream, j);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    before = sums[0];
+    after = sums[1];
+  }
+  const ScanPass passes[3] = {ScanPass{before, nullptr, c.value, c.key, 1, 0, 0, c.scale, 1.0f},
+                              ScanPass{after, nullptr, c.value, c.key, 1, 1, 0, 1.0f, c.scale},
+                              ScanPass{after, c.dstate, c.key, c.value, 0, 1, exact, 1.0f, c.scale}};
+  const ScanTensors tensors[3] = {ScanTensors{&dy, &c.v, &c.k, &c.dq}, ScanTensors{&c.v, &dy, &c.q, &c.dk},
+                                  ScanTensors{&c.k, &c.q, &dy, &c.dv}};
+  // All three in one launch where they run the same kernel: those of a sample and head stand side by side and share
+  // their inputs in L2.
+  const bool same = (c.key <= 64) == (c.value <= 64);
+  for (int first = 0; first < 3;) {
+    ScanArgs a = common(c, p, workspace);
+    const int last = same ? 3 : first == 0 ? 2 : 3;
+    for (int i = first; i < last; ++i) {
+      a.pass[i - first] = passes[i];
+      if (!encode_pass(&a.maps[i - first], tensors[i], c, passes[i].ny, passes[i].nz)) return cudaErrorInvalidValue;
+    }
+    a.passes = last - first;
+    const cudaError_t e = launch_scans<false>(a, items, c.type, passes[first].ny, passes[first].nz, "decay_bwd", stream);
+    if (e != cudaSuccess) return e;
+    first = last;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace lsso
