@@ -94,6 +94,11 @@ __device__ __forceinline__ uint32_t idesc(int n, bool a_mn, bool b_mn) {
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, ScanShared& sh, int* status) {
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort_flag, status));
 }
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ void pair_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -425,11 +430,9 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       const uint32_t id = idesc<kHalf>((ny + 15) & ~15, true, true);
       const uint64_t zd = make_desc_sw128(z_at, kVB == 2 ? kBox : 0, 1024);  // one box: lanes 64-127 repeat 0-63
       const uint32_t second = kStateOnly ? smem_u32(third) + (kHalf ? 0 : kKB * kBox) : x_at;
-      const uint32_t rows[3] = {smem_u32(third), second, y_at};
       bool more = false;
-#pragma unroll
-      for (int t = exact ? (kHalf ? 1 : 0) : 2; t < 3; ++t) {
-        const uint64_t yd = make_desc_sw128(rows[t], kBox, 1024);
+      for (int t = exact ? (kHalf ? 1 : 0) : 2; t < 3; ++t) {  // the smallest part first
+        const uint64_t yd = make_desc_sw128(t == 0 ? smem_u32(third) : t == 1 ? second : y_at, kBox, 1024);
         for (int k = 0; k < kChunk / 16; ++k) {
           if (kHalf && t == 2 && k == 0 && exact) {
             mma_scaled_d(tmem + kColChange, zd, yd, id);  // the parts so far are 2^11 times too large
@@ -450,79 +453,90 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns hf and hf + 2
     float down = 1.0f;
     if (!kStateOnly) {
-      float v[2][32];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int block = hf + 2 * i;
-        if (reverse ? block >= q : block <= q) tmem_ld32(quadrant + kColP + 32 * block, v[i]);
-      }
-      tmem_ld_wait();
-      float most = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      // block hf + 2 i with its decay
+      auto weigh_scores = [&](int i, float (&v)[32]) {
         const int block = hf + 2 * i;
         const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block);
+        const float f = i == 0 ? block_factor[0] : block_factor[1];
         if (reverse ? block > q : block < q) {
-          const float f = block_factor[i];
+          tmem_ld32(quadrant + kColP + 32 * block, v);
+          tmem_ld_wait();
+          if (dead_tokens) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 c = col[j / 4];
-            if (dead_tokens) {
-              v[i][j] = c.x == 0.0f ? 0.0f : v[i][j];
-              v[i][j + 1] = c.y == 0.0f ? 0.0f : v[i][j + 1];
-              v[i][j + 2] = c.z == 0.0f ? 0.0f : v[i][j + 2];
-              v[i][j + 3] = c.w == 0.0f ? 0.0f : v[i][j + 3];
+            for (int j = 0; j < 32; j += 4) {
+              const float4 c = col[j / 4];
+              v[j] = c.x == 0.0f ? 0.0f : v[j] * (f * c.x);
+              v[j + 1] = c.y == 0.0f ? 0.0f : v[j + 1] * (f * c.y);
+              v[j + 2] = c.z == 0.0f ? 0.0f : v[j + 2] * (f * c.z);
+              v[j + 3] = c.w == 0.0f ? 0.0f : v[j + 3] * (f * c.w);
             }
-            v[i][j] *= f * c.x;
-            v[i][j + 1] *= f * c.y;
-            v[i][j + 2] *= f * c.z;
-            v[i][j + 3] *= f * c.w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 c = col[j / 4];
+              v[j] *= f * c.x;
+              v[j + 1] *= f * c.y;
+              v[j + 2] *= f * c.z;
+              v[j + 3] *= f * c.w;
+            }
           }
         } else if (block == q) {
           // the block on the diagonal: its valid columns up to this row's token (from it on)
+          tmem_ld32(quadrant + kColP + 32 * block, v);
+          tmem_ld_wait();
           const uint32_t seen = ranks.word(q) & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane));
+          if (gentle) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 c = col[j / 4];
-            const float cs[4] = {c.x, c.y, c.z, c.w};
+            for (int j = 0; j < 32; j += 4) {
+              const float4 c = col[j / 4];
+              v[j] = (seen >> j) & 1u ? v[j] * (f * c.x) : 0.0f;
+              v[j + 1] = (seen >> (j + 1)) & 1u ? v[j + 1] * (f * c.y) : 0.0f;
+              v[j + 2] = (seen >> (j + 2)) & 1u ? v[j + 2] * (f * c.z) : 0.0f;
+              v[j + 3] = (seen >> (j + 3)) & 1u ? v[j + 3] * (f * c.w) : 0.0f;
+            }
+          } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float w = block_factor[i] * cs[e];
-              if (!gentle) {  // tokens between the two
-                // rank distance: valid tokens seen by the row that lie on its side of token j + e
-                const uint32_t side = reverse ? (1u << (j + e)) - 1u : ~(0xffffffffu >> (31 - (j + e)));
-                w = inside * exp2f(l2 * static_cast<float>(__popc(seen & side)));
-              }
-              v[i][j + e] = (seen >> (j + e)) & 1u ? v[i][j + e] * w : 0.0f;
+            for (int j = 0; j < 32; ++j) {
+              // rank distance: valid tokens seen by the row that lie on its side of token j
+              const uint32_t side = reverse ? (1u << j) - 1u : ~(0xffffffffu >> (31 - j));
+              v[j] = (seen >> j) & 1u ? v[j] * (inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)))) : 0.0f;
             }
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[i][j] = 0.0f;
+          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
         }
-        if (kHalf) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[i][j]));
-        }
-      }
+      };
       float up = 1.0f;
-      const uint32_t top = __float_as_uint(most) >> 23;
-      if (kHalf) sh.top[hf * kChunk + 32 * q + lane] = static_cast<uint8_t>(top);
-      tc_fence_before();
-      pair_barrier(1 + q, 64);  // both warps of these rows have read their scores
-      tc_fence_after();
       if (kHalf) {
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float v[32];
+          weigh_scores(i, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
+        }
+        const uint32_t top = __float_as_uint(most) >> 23;
+        sh.top[hf * kChunk + 32 * q + lane] = static_cast<uint8_t>(top);
+        pair_barrier(1 + q, 64);
         const PowerScale sc(max(top, static_cast<uint32_t>(sh.top[(hf ^ 1) * kChunk + 32 * q + lane])));
         up = sc.up;
         down = sc.down;
       }
+      uint32_t w[2][16];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t w[16];
+        float v[32];
+        weigh_scores(i, v);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack2<kHalf>(v[i][2 * j] * up, v[i][2 * j + 1] * up);
-        tmem_st16(quadrant + kColP + 16 * (hf + 2 * i), w);
+        for (int j = 0; j < 16; ++j) w[i][j] = pack2<kHalf>(kHalf ? v[2 * j] * up : v[2 * j], kHalf ? v[2 * j + 1] * up : v[2 * j + 1]);
       }
+      tc_fence_before();
+      pair_barrier(1 + q, 64);  // both warps of these rows have read their scores
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) tmem_st16(quadrant + kColP + 16 * (hf + 2 * i), w[i]);
       tmem_st_wait();
       tc_fence_before();
       ok = __syncthreads_and(ok) != 0;
