@@ -19,11 +19,13 @@
 //
 // Per chunk:
 //   scores P = X Y^T and X M            tcgen05, operands from shared memory, accumulators in TMEM
-//   Y' = weights * Y in place           all threads, while nothing else needs Y
+//   Y' = weights * Y in place           worker warps, once P has been formed
 //   M change Z^T Y'                     tcgen05 (transposed, so that a thread owns a row of M^T)
 //   P' = decay * P, rounded             TMEM to registers and back, the next product's A operand
-//   P' Z                                tcgen05, A from TMEM; the threads meanwhile update M in registers
-//   w = P' Z + weight * (X M)           and out by TMA
+//   X M scaled by rows, + P' Z          tcgen05, A from TMEM; the workers meanwhile update M in registers
+//   w                                   out by TMA
+// The next chunk's scores are formed as soon as P' has been used.  No barrier joins all warps (but where masks change):
+// each product waits for the warps that prepare its operands, and each warp for the products that it reads.
 #include <cuda.h>
 
 #include <algorithm>
@@ -39,7 +41,7 @@ namespace lsso {
 namespace {
 
 constexpr int kChunk = 128;
-constexpr int kThreads = 256;
+constexpr int kWorkers = 256, kThreads = kWorkers + 32;
 constexpr uint32_t kBox = kChunk * 128;  // 128 tokens x 64 features of 16 bits
 constexpr uint32_t kOutBox = 32 * 64;    // 32 tokens x 32 features
 constexpr float kLog2e = 1.44269504f;
@@ -71,8 +73,10 @@ struct ScanArgs {
 struct ScanShared {
   float from[kChunk], col[kChunk];
   float state_scale[2][kChunk];
-  uint8_t top[2 * kChunk];  // FP16: largest exponents, of score rows and of state rows in turn
-  uint64_t full[2], scores, state, out, drain;
+  uint8_t row_top[2][kChunk], state_top[2 * kChunk];  // FP16: largest exponents of score rows and of state rows
+  // full: a stage has landed.  scores, xm, change, out: products done.  weighed, decayed, taken: all warps have written
+  // Y', written P' (and the state's part, scaled), read the products and written the next state; freed: stored (one stage).
+  uint64_t full[2], scores, xm, change, out, weighed, decayed, taken, freed, drain;
   uint32_t tmem;
   int abort_flag;
 };
@@ -99,7 +103,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ void pair_barrier(int id, int threads) {
+__device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 // The power of two that brings values with largest (biased) exponent e into [2^14, 2^15), and its inverse: FP16's
@@ -146,75 +150,53 @@ struct ChunkRanks {
 };
 
 // kKB, kVB: 64-feature boxes of x and y, and of z and w.  kStateOnly: the states of segments, no outputs.
+// Warps 0-7 weigh, decay, hold the state and write; one thread of warp 8 issues loads and products.
 template <bool kHalf, int kKB, int kVB, bool kStateOnly>
 __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_kernel(const __grid_constant__ ScanArgs a) {
   constexpr bool kSmall = kKB + kVB == 2;
-  // TMEM columns.  P' takes the lower half of P; with single boxes P' Z takes its upper half, so that two CTAs fit an SM.
-  constexpr uint32_t kColP = 0, kColXm = 128, kColChange = kStateOnly ? 0 : kSmall ? 192 : 256, kColOut = kSmall ? 64 : 384;
+  // TMEM columns: scores (P' of a block of 32 tokens takes the first half of the block's columns, so that no warp
+  // overwrites what another still reads), the state's part and then the output, the state's change.  Single boxes leave
+  // room for a second CTA.
+  constexpr uint32_t kColP = 0, kColOut = 128, kColChange = kStateOnly ? 0 : kSmall ? 192 : 256;
   constexpr uint32_t kCols = kStateOnly ? 64 * kKB : kSmall ? 256 : 512;
-  constexpr int kParts = kVB == 1 ? 4 : 2;         // threads that share a row of M^T (one lane quadrant or two hold it)
-  constexpr int kOwn = 64 * kKB / kParts;          // its columns held by one thread
-  constexpr uint32_t kBoxes = (kStateOnly ? 0 : kKB) + kKB + kVB;
+  constexpr int kParts = kVB == 1 ? 4 : 2;  // threads that share a row of M^T (one lane quadrant or two hold it)
+  constexpr int kOwn = 64 * kKB / kParts;   // its columns held by one thread
+  constexpr uint32_t kXBytes = kStateOnly ? 0 : kKB * kBox;
+  constexpr uint32_t kStage = kXBytes + kKB * kBox + kVB * kBox;
+  constexpr uint32_t kStateBox = kVB * 64 * 128;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ ScanShared sh;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, hf = warp >> 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int pass_index = blockIdx.x % a.passes;
   const ScanPass& p = a.pass[pass_index];
   const ScanMaps& maps = a.maps[pass_index];
   const int unit = blockIdx.x / a.passes, segment = unit % a.segments, item = unit / a.segments;
   const int head = item % a.heads, sample = item / a.heads;
-  const bool reverse = p.reverse != 0;
+  const bool reverse = p.reverse != 0, exact = p.exact != 0;
   const int first = segment * a.segment_chunks, count = min(a.segment_chunks, a.chunks - first);
   const int ny = p.ny, nz = p.nz, stages = a.stages;
-  const bool exact = p.exact != 0;
-  constexpr uint32_t kStage = kBoxes * kBox;
-  uint8_t* const state_tile = smem + stages * kStage;                                       // M^T: [kKB][64 kVB rows][128 bytes]
-  uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kVB * 64 * 128);              // exact: parts that have no other place
+  uint8_t* const state_tile = smem + stages * kStage;                                // M^T: [kKB][64 kVB rows][128 bytes]
+  uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kStateBox);            // exact: parts that have no other place
+  const uint32_t base = smem_u32(smem), full_bar = smem_u32(sh.full);
+  const uint32_t scores_bar = smem_u32(&sh.scores), xm_bar = smem_u32(&sh.xm), change_bar = smem_u32(&sh.change),
+                 out_bar = smem_u32(&sh.out), weighed_bar = smem_u32(&sh.weighed), decayed_bar = smem_u32(&sh.decayed),
+                 taken_bar = smem_u32(&sh.taken), freed_bar = smem_u32(&sh.freed);
 
   if (tid == 0) {
-    mbar_init(smem_u32(&sh.full[0]), 1);
-    mbar_init(smem_u32(&sh.full[1]), 1);
-    mbar_init(smem_u32(&sh.scores), 1);
-    mbar_init(smem_u32(&sh.state), 1);
-    mbar_init(smem_u32(&sh.out), 1);
-    mbar_init(smem_u32(&sh.drain), 1);
+    mbar_init(full_bar, 1);
+    mbar_init(full_bar + 8, 1);
+    for (uint32_t bar : {scores_bar, xm_bar, change_bar, out_bar, smem_u32(&sh.drain)}) mbar_init(bar, 1);
+    for (uint32_t bar : {weighed_bar, decayed_bar, taken_bar, freed_bar}) mbar_init(bar, kWorkers / 32);
     sh.abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&maps.y);
-    prefetch_tmap(&maps.z);
-    if (!kStateOnly) {
-      prefetch_tmap(&maps.x);
-      prefetch_tmap(&maps.w);
-    }
   }
   // Before the allocation, so that no block of an earlier kernel finds its TMEM taken by one that waits for it.
   pdl_wait();
   if (warp == 0) tmem_alloc(smem_u32(&sh.tmem), kCols);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sh.tmem;
-  const uint32_t base = smem_u32(smem), full_bar = smem_u32(sh.full);
 
   auto chunk_at = [&](int n) { return reverse ? first + count - 1 - n : first + n; };
-  auto load = [&](int n) {  // by thread 0
-    const int s = stages == 2 ? n & 1 : 0, t0 = chunk_at(n) * kChunk;
-    const uint32_t bar = full_bar + 8 * s;
-    uint32_t dst = base + s * kStage;
-    mbar_arrive_expect_tx(bar, kStage);
-    if (!kStateOnly) {
-#pragma unroll
-      for (int b = 0; b < kKB; ++b, dst += kBox) tma_load_4d(dst, &maps.x, 64 * b, head, t0, sample, bar);
-    }
-#pragma unroll
-    for (int b = 0; b < kKB; ++b, dst += kBox) tma_load_4d(dst, &maps.y, 64 * b, head, t0, sample, bar);
-#pragma unroll
-    for (int b = 0; b < kVB; ++b, dst += kBox) tma_load_4d(dst, &maps.z, 64 * b, head, t0, sample, bar);
-  };
-  int issued = 0;
-  if (tid == 0) {
-    for (; issued < min(stages, count); ++issued) load(issued);
-  }
+  auto stage_of = [&](int n) { return stages == 2 ? n & 1 : 0; };
+  auto full_parity = [&](int n) { return static_cast<uint32_t>(stages == 2 ? (n >> 1) & 1 : n & 1); };
 
   // ---- the head's decay; valid tokens of a chunk
   float l = a.log_decay[head];
@@ -226,27 +208,58 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   // FP16 would lose rows whose weights are all small (a strong decay before the state of a reverse scan).
   const float join = p.from * exp2f(l2 * late);
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
+  const int q = warp & 3, hf = (warp >> 2) & 1;
+  // this thread's part of M^T: row mv, columns [mc, mc + kOwn)
+  const int mv = kVB == 1 ? 32 * (q & 1) + lane : 32 * q + lane;
+  const int part = kVB == 1 ? (q >> 1) + 2 * hf : hf;
+  const int mc = part * kOwn;
+  float m[kOwn];
+  // M^T as the next product's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
+  auto write_state = [&](int parity) {
+    float up = 1.0f;
+    if (kHalf) {
+      float most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) most = fmaxf(most, fabsf(m[i]));
+      uint32_t e = 0;  // the largest of the kParts threads that share the row
+      sh.state_top[part * (64 * kVB) + mv] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
+      named_barrier(kVB == 1 ? 5 + (q & 1) : 1 + q, 32 * kParts);
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) e = max(e, static_cast<uint32_t>(sh.state_top[i * (64 * kVB) + mv]));
+      const PowerScale s(e);
+      up = s.up;
+      if (part == 0) sh.state_scale[parity][mv] = s.down;
+    }
+#pragma unroll
+    for (int i = 0; i < kOwn; i += 8) {
+      const int c = mc + i, box = c >> 6, piece = (c >> 3) & 7;
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = kHalf ? pack2<kHalf>(m[i + 2 * j] * up, m[i + 2 * j + 1] * up) : pack2<kHalf>(m[i + 2 * j], m[i + 2 * j + 1]);
+      *reinterpret_cast<uint4*>(state_tile + box * kStateBox + mv * 128 + ((piece ^ (mv & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  };
   ChunkRanks ranks;
   uint32_t ahead = 0;  // mask bytes of a later chunk, as bits
   auto fetch_mask = [&](int n) {
-    ahead = 0xf;
-    if (a.mask == nullptr) return;
     ahead = 0;
+    if (a.mask == nullptr) return;
     const int t0 = chunk_at(n) * kChunk + lane;
-    const uint8_t* m = a.mask + static_cast<int64_t>(sample) * a.length;
+    const uint8_t* of_sample = a.mask + static_cast<int64_t>(sample) * a.length;
 #pragma unroll
     for (int w = 0; w < 4; ++w)
-      if (t0 + 32 * w < a.length && m[t0 + 32 * w] != 0) ahead |= 1u << w;
+      if (t0 + 32 * w < a.length && of_sample[t0 + 32 * w] != 0) ahead |= 1u << w;
   };
-  float row_rho = 0.0f, lambda = 0.0f, block_factor[2] = {0.0f, 0.0f};
-  bool live = false, dead_tokens = false;
+  float lambda = 0.0f, block_factor[2] = {0.0f, 0.0f};
+  bool live = false, dead_tokens = false, was_whole = false;
   float decay_factor = 0.0f, decay_keep = 0.0f;  // M' = M * factor + M * keep (keep is 0 or 1)
-  int decay_total = -1, tail_state = 0;
+  int decay_total = -1;
   // Ranks and tables of chunk n from the fetched bits.  Whole chunks all have the same, and find them in place.
   auto prepare = [&](int n) {
-    const int t0 = chunk_at(n) * kChunk;
     if (a.mask == nullptr) {
-      const int left = a.length - t0;  // tokens
+      const int left = a.length - chunk_at(n) * kChunk;  // tokens
+      if (left >= kChunk && was_whole) return;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int of_word = left - 32 * w;
@@ -255,27 +268,26 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     } else {
 #pragma unroll
       for (int w = 0; w < 4; ++w) ranks.words[w] = __ballot_sync(0xffffffffu, (ahead >> w) & 1u);
+      if (ranks.whole() && was_whole) return;
     }
-    const int kind = ranks.whole() ? 1 : 2;
-    if (kind == 1 && tail_state == 1) return;
-    tail_state = kind;
+    was_whole = ranks.whole();
     ranks.count();
     live = ranks.live(q, lane);
     // tokens to be cleared: masked ones (behind the last token there are zeros)
-    dead_tokens = a.mask != nullptr && kind == 2;
+    dead_tokens = a.mask != nullptr && !was_whole;
     const int rho = ranks.rho(q, lane, reverse);
+    const float row_rho = static_cast<float>(rho);
+    if (n > 0) named_barrier(7, kWorkers);  // the tables have been read
     if (hf == 0) {
       sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : 0.0f;
     } else if (!kStateOnly) {
       sh.col[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.last_rho(q, reverse) - rho)) : 0.0f;
     }
+    if (n > 0) named_barrier(7, kWorkers);
     if (!kStateOnly) {
-      row_rho = static_cast<float>(rho);
       lambda = p.into * exp2f(l2 * (row_rho + 1.0f - late));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(hf + 2 * i, reverse))));
-      }
+      for (int i = 0; i < 2; ++i) block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(hf + 2 * i, reverse))));
     }
     if (ranks.total != decay_total) {
       decay_total = ranks.total;
@@ -285,13 +297,9 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     }
   };
 
-  // ---- this thread's part of M^T: row mv, columns [mc, mc + kOwn)
-  const int mv = kVB == 1 ? 32 * (q & 1) + lane : 32 * q + lane;
-  const int part = kVB == 1 ? (q >> 1) + 2 * hf : hf;
-  const int mc = part * kOwn;
-  float m[kOwn];
-  {
-    const bool transposed = (p.transposed & 1) != 0;
+  int tokens_seen = 0;
+  if (warp < kWorkers / 32) {
+    const bool transposed = p.transposed != 0;
     const float* src = p.state_in == nullptr || kStateOnly
                            ? nullptr
                            : p.state_in + (static_cast<int64_t>(item) * a.segments + segment) * ny * nz;
@@ -301,365 +309,396 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       const int c = mc + i;
       if (src != nullptr && mv < nz && c < ny) m[i] = src[transposed ? mv * ny + c : c * nz + mv];
     }
+    fetch_mask(0);
+    prepare(0);
+    tokens_seen = ranks.total;
+    if (!kStateOnly) write_state(0);
+    fence_proxy_async();
   }
-  // M^T as the next product's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
-  auto write_state = [&](int parity) {
-    float up = 1.0f;
-    if (kHalf) {
-      float most = 0.0f;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  bool ok = true;
+
+  if (warp == kWorkers / 32) {
+    // ---------------- loads and products
+    if (lane == 0) {
+      int loaded = 0;
+      auto load = [&]() {
+        const int n = loaded++, t0 = chunk_at(n) * kChunk;
+        const uint32_t bar = full_bar + 8 * stage_of(n);
+        uint32_t dst = base + stage_of(n) * kStage;
+        mbar_arrive_expect_tx(bar, kStage);
+        if (!kStateOnly) {
 #pragma unroll
-      for (int i = 0; i < kOwn; ++i) most = fmaxf(most, fabsf(m[i]));
-      uint32_t e = 0;  // the largest of the kParts threads that share the row
-      sh.top[part * (64 * kVB) + mv] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
-      pair_barrier(kVB == 1 ? 5 + (q & 1) : 1 + q, 32 * kParts);
+          for (int b = 0; b < kKB; ++b, dst += kBox) tma_load_4d(dst, &maps.x, 64 * b, head, t0, sample, bar);
+        }
 #pragma unroll
-      for (int i = 0; i < kParts; ++i) e = max(e, static_cast<uint32_t>(sh.top[i * (64 * kVB) + mv]));
-      const PowerScale s(e);
-      up = s.up;
-      if (part == 0) sh.state_scale[parity][mv] = s.down;
-    }
+        for (int b = 0; b < kKB; ++b, dst += kBox) tma_load_4d(dst, &maps.y, 64 * b, head, t0, sample, bar);
 #pragma unroll
-    for (int i = 0; i < kOwn; i += 8) {
-      const int c = mc + i, box = c >> 6, piece = (c >> 3) & 7;
-      const uint4 v = make_uint4(pack2<kHalf>(m[i] * up, m[i + 1] * up), pack2<kHalf>(m[i + 2] * up, m[i + 3] * up),
-                                 pack2<kHalf>(m[i + 4] * up, m[i + 5] * up), pack2<kHalf>(m[i + 6] * up, m[i + 7] * up));
-      *reinterpret_cast<uint4*>(state_tile + box * (kVB * 64 * 128) + mv * 128 + ((piece ^ (mv & 7)) << 4)) = v;
-    }
-  };
-
-  fetch_mask(0);
-  prepare(0);
-  int tokens_seen = ranks.total;
-  if (!kStateOnly) write_state(0);
-  fence_proxy_async();
-  bool ok = __syncthreads_and(1) != 0;
-
-  const uint32_t quadrant = tmem + (static_cast<uint32_t>(q) << 21);  // this warp's lanes
-  const uint32_t scores_bar = smem_u32(&sh.scores), state_bar = smem_u32(&sh.state), out_bar = smem_u32(&sh.out);
-  const int y_steps = (ny + 15) / 16;
-
-  for (int n = 0; n < count; ++n) {
-    const int s = stages == 2 ? n & 1 : 0;
-    const uint32_t use = stages == 2 ? (n >> 1) & 1 : n & 1, parity = n & 1;
-    const uint32_t x_at = base + s * kStage, y_at = x_at + (kStateOnly ? 0 : kKB * kBox), z_at = y_at + kKB * kBox;
-    uint8_t* const x_tile = smem + s * kStage;
-    uint8_t* const y_tile = x_tile + (kStateOnly ? 0 : kKB * kBox);
-    uint8_t* const z_tile = y_tile + kKB * kBox;
-
-    // ---- scores and the state's part
-    ok = wait_warp(full_bar + 8 * s, use, sh, a.status) && ok;
-    if (!kStateOnly) {
-      if (tid == 0 && ok) {
+        for (int b = 0; b < kVB; ++b, dst += kBox) tma_load_4d(dst, &maps.z, 64 * b, head, t0, sample, bar);
+      };
+      while (loaded < min(stages, count)) load();
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        ok = ok && mbar_wait_bounded(bar, parity, &sh.abort_flag, a.status);
         tc_fence_after();
-        const uint32_t ip = idesc<kHalf>(128, false, false), im = idesc<kHalf>((nz + 15) & ~15, false, false);
+        return ok;
+      };
+      const int y_steps = (ny + 15) / 16;
+      const uint32_t i_scores = idesc<kHalf>(128, false, false), i_xm = idesc<kHalf>((nz + 15) & ~15, false, false),
+                     i_change = idesc<kHalf>((ny + 15) & ~15, true, true), i_out = idesc<kHalf>((nz + 15) & ~15, false, true);
+      const uint64_t x0 = make_desc_sw128(base, 16, 1024), y0 = make_desc_sw128(base + kXBytes, 16, 1024),
+                     state0 = make_desc_sw128(smem_u32(state_tile), 16, 1024),
+                     x_rows = make_desc_sw128(base, kBox, 1024), y_rows = make_desc_sw128(base + kXBytes, kBox, 1024),
+                     third_rows = make_desc_sw128(smem_u32(third), kBox, 1024),
+                     // one box of z: lanes 64-127 repeat 0-63
+                     z_lanes = make_desc_sw128(base + kXBytes + kKB * kBox, kVB == 2 ? kBox : 0, 1024),
+                     z_rows = make_desc_sw128(base + kXBytes + kKB * kBox, kBox, 1024);
+      auto scores = [&](int n) {
+        const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
         for (int k = 0; k < y_steps; ++k) {
-          const uint32_t at = (k >> 2) * kBox + (k & 3) * 32;
-          const uint64_t xd = make_desc_sw128(x_at + at, 16, 1024);
-          mma_bf16(tmem + kColP, xd, make_desc_sw128(y_at + at, 16, 1024), ip, k > 0);
-          mma_bf16(tmem + kColXm, xd,
-                   make_desc_sw128(smem_u32(state_tile) + (k >> 2) * (kVB * 64 * 128) + (k & 3) * 32, 16, 1024), im, k > 0);
+          const uint64_t step = at + (k >> 2) * (kBox / 16) + (k & 3) * 2;
+          mma_bf16(tmem + kColP, x0 + step, y0 + step, i_scores, k > 0);
         }
         mma_commit(scores_bar);
-      }
-      __syncwarp();
-    }
-    if (n + 1 < count) fetch_mask(n + 1);
-    if (!kStateOnly) {
-      ok = wait_warp(scores_bar, parity, sh, a.status) && ok;
-      tc_fence_after();
-    }
-
-    // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
-    {
-      const int pieces = ny <= 32 ? 4 : 8;  // 16-byte pieces of a row that hold features (of each box)
-      const int shift = ny <= 32 ? 2 : 3;
-#pragma unroll 1
-      for (int b = 0; b < kKB; ++b) {
-#pragma unroll 4
-        for (int i = tid; i < kChunk * pieces; i += kThreads) {
-          const int row = i >> shift, piece = i & (pieces - 1);
-          const uint32_t at = b * kBox + row * 128 + ((piece ^ (row & 7)) << 4);
-          const float f = sh.from[row];
-          const uint4 v = *reinterpret_cast<const uint4*>(y_tile + at);
-          const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-          uint32_t hi[4], mid[4], lo[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float2 e = unpack2<kHalf>(in[j]);
-            e.x *= f;
-            e.y *= f;
-            if (f == 0.0f) e = make_float2(0.0f, 0.0f);  // whatever a masked token holds
-            hi[j] = pack2<kHalf>(e.x, e.y);
-            if (exact) {
-              float2 h = unpack2<kHalf>(hi[j]);
-              e.x -= h.x;
-              e.y -= h.y;
-              if (kHalf) {
-                mid[j] = pack2<kHalf>(e.x * 2048.0f, e.y * 2048.0f);
-              } else {
-                mid[j] = pack2<kHalf>(e.x, e.y);
-                h = unpack2<kHalf>(mid[j]);
-                lo[j] = pack2<kHalf>(e.x - h.x, e.y - h.y);
-              }
+      };
+      for (int n = 0; n < count; ++n) {
+        const uint32_t parity = n & 1;
+        const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
+        if (!kStateOnly) {
+          if (n == 0) {
+            if (!wait(full_bar, 0)) break;
+            scores(0);
+          }
+          if (n > 0 && !wait(taken_bar, parity ^ 1)) break;
+          for (int k = 0; k < y_steps; ++k) {
+            mma_bf16(tmem + kColOut, x0 + at + (k >> 2) * (kBox / 16) + (k & 3) * 2,
+                     state0 + (k >> 2) * (kStateBox / 16) + (k & 3) * 2, i_xm, k > 0);
+          }
+          mma_commit(xm_bar);
+        }
+        if (!wait(weighed_bar, parity)) break;
+        if (kStateOnly && n > 0 && !wait(taken_bar, parity ^ 1)) break;
+        const uint64_t zd = z_lanes + at;
+        bool more = false;
+        if (exact) {  // the smaller parts first
+          for (int t = kHalf ? 1 : 0; t < 2; ++t) {
+            const uint64_t yd = t == 0 ? third_rows : kStateOnly ? third_rows + (kHalf ? 0 : kKB * (kBox / 16)) : x_rows + at;
+            for (int k = 0; k < kChunk / 16; ++k) {
+              mma_bf16(tmem + kColChange, zd + k * 128, yd + k * 128, i_change, more);
+              more = true;
             }
           }
-          *reinterpret_cast<uint4*>(y_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (exact) {
-            uint8_t* second = kStateOnly ? third + (kHalf ? 0 : kKB * kBox) : x_tile;
-            *reinterpret_cast<uint4*>(second + at) = make_uint4(mid[0], mid[1], mid[2], mid[3]);
-            if (!kHalf) *reinterpret_cast<uint4*>(third + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        for (int k = 0; k < kChunk / 16; ++k) {
+          if (kHalf && exact && k == 0) {
+            mma_scaled_d(tmem + kColChange, zd, y_rows + at, i_change);  // the part so far is 2^11 times too large
+          } else {
+            mma_bf16(tmem + kColChange, zd + k * 128, y_rows + at + k * 128, i_change, more || k > 0);
           }
         }
+        mma_commit(change_bar);
+        if (kStateOnly) {
+          if (loaded < count) {
+            if (!wait(change_bar, parity)) break;
+            load();
+          }
+          continue;
+        }
+        // every warp's stores of the chunk before have left its stage
+        if (stages == 2 && n > 0 && loaded < count) load();
+        if (!wait(decayed_bar, parity)) break;
+        for (int k = 0; k < kChunk / 16; ++k) {
+          mma_tmem_a(tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), z_rows + at + k * 128, i_out, 1);
+        }
+        mma_commit(out_bar);
+        if (n + 1 < count) {  // the next scores as soon as these have been used
+          if (stages == 1) {
+            if (!wait(freed_bar, parity)) break;
+            load();
+          }
+          if (!wait(out_bar, parity) || !wait(full_bar + 8 * stage_of(n + 1), full_parity(n + 1))) break;
+          scores(n + 1);
+        }
       }
-      if (dead_tokens && tid < kChunk) {
-        if (!ranks.live(warp, lane)) {
+      // nothing may be in flight when the CTA ends
+      if (!ok) {
+        for (int n = max(0, loaded - stages); n < loaded; ++n)
+          mbar_wait_bounded(full_bar + 8 * stage_of(n), full_parity(n), nullptr, a.status);
+      }
+      mma_drain(smem_u32(&sh.drain), a.status);
+    }
+    __syncwarp();
+  } else {
+    // ---------------- weights, decays, states, outputs.  A wait that runs out does not leave the loop (other warps may
+    // be at a barrier with this one): the rest runs through without waiting or storing.
+    const uint32_t quadrant = tmem + (static_cast<uint32_t>(q) << 21);  // this warp's lanes
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      ok = wait_warp(bar, parity, sh, a.status) && ok;
+      tc_fence_after();
+    };
+    auto arrive = [&](uint32_t bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    for (int n = 0; n < count; ++n) {
+      const uint32_t parity = n & 1;
+      uint8_t* const x_tile = smem + stage_of(n) * kStage;
+      uint8_t* const y_tile = x_tile + kXBytes;
+      uint8_t* const z_tile = y_tile + kKB * kBox;
+      if (n + 1 < count) fetch_mask(n + 1);
+      wait(full_bar + 8 * stage_of(n), full_parity(n));
+      if (!kStateOnly) {
+        wait(scores_bar, parity);          // y's rows have been read
+        if (exact) wait(xm_bar, parity);   // x's too
+      }
+
+      // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
+      {
+        const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;  // 16-byte pieces of a row (of each box) that hold features
+        uint8_t* const second = kStateOnly ? third + (kHalf ? 0 : kKB * kBox) : x_tile;
+#pragma unroll
+        for (int b = 0; b < kKB; ++b) {
+#pragma unroll 2
+          for (int i = tid; i < kChunk * pieces; i += kWorkers) {
+            const int row = i >> shift, piece = i & (pieces - 1);
+            const uint32_t at = b * kBox + row * 128 + ((piece ^ (row & 7)) << 4);
+            const float f = sh.from[row];
+            const uint4 v = *reinterpret_cast<const uint4*>(y_tile + at);
+            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+            uint32_t hi[4];
+            float2 e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              e[j] = unpack2<kHalf>(in[j]);
+              e[j].x *= f;
+              e[j].y *= f;
+              hi[j] = pack2<kHalf>(e[j].x, e[j].y);
+            }
+            if (f == 0.0f) {  // whatever a masked token holds
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                hi[j] = 0;
+                e[j] = make_float2(0.0f, 0.0f);
+              }
+            }
+            *reinterpret_cast<uint4*>(y_tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (exact) {
+              uint32_t mid[4], lo[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 h = unpack2<kHalf>(hi[j]);
+                const float rx = e[j].x - h.x, ry = e[j].y - h.y;
+                mid[j] = kHalf ? pack2<kHalf>(rx * 2048.0f, ry * 2048.0f) : pack2<kHalf>(rx, ry);
+                const float2 g = unpack2<kHalf>(mid[j]);
+                lo[j] = pack2<kHalf>(rx - g.x, ry - g.y);
+              }
+              *reinterpret_cast<uint4*>(second + at) = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+              if (!kHalf) *reinterpret_cast<uint4*>(third + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+          }
+        }
+        if (dead_tokens && tid < kChunk && !ranks.live(warp, lane)) {
 #pragma unroll
           for (int b = 0; b < kVB; ++b)
 #pragma unroll
             for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(z_tile + b * kBox + tid * 128 + 16 * j) = make_uint4(0, 0, 0, 0);
         }
       }
-    }
-    fence_proxy_async();
-    tc_fence_before();
-    if (!kStateOnly && lane == 0) bulk_wait_read<0>();  // the stage before this one has been stored from
-    ok = __syncthreads_and(ok) != 0;
-    if (!ok) break;
-    if (tid == 0) {
-      tc_fence_after();
-      const uint32_t id = idesc<kHalf>((ny + 15) & ~15, true, true);
-      const uint64_t zd = make_desc_sw128(z_at, kVB == 2 ? kBox : 0, 1024);  // one box: lanes 64-127 repeat 0-63
-      const uint32_t second = kStateOnly ? smem_u32(third) + (kHalf ? 0 : kKB * kBox) : x_at;
-      bool more = false;
-      for (int t = exact ? (kHalf ? 1 : 0) : 2; t < 3; ++t) {  // the smallest part first
-        const uint64_t yd = make_desc_sw128(t == 0 ? smem_u32(third) : t == 1 ? second : y_at, kBox, 1024);
-        for (int k = 0; k < kChunk / 16; ++k) {
-          if (kHalf && t == 2 && k == 0 && exact) {
-            mma_scaled_d(tmem + kColChange, zd, yd, id);  // the parts so far are 2^11 times too large
-          } else {
-            mma_bf16(tmem + kColChange, zd + k * 128, yd + k * 128, id, more);
-          }
-          more = true;
-        }
-      }
-      mma_commit(state_bar);
-      if (!kStateOnly && stages == 2 && n > 0 && n + 1 < count) {
-        load(n + 1);
-        ++issued;
-      }
-    }
-    __syncwarp();
+      fence_proxy_async();
+      if (!kStateOnly && stages == 2 && lane == 0) bulk_wait_read<0>();  // the stage of the chunk before is free
+      arrive(weighed_bar);
 
-    // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns hf and hf + 2
-    float down = 1.0f;
-    if (!kStateOnly) {
-      // block hf + 2 i with its decay
-      auto weigh_scores = [&](int i, float (&v)[32]) {
-        const int block = hf + 2 * i;
-        const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block);
-        const float f = i == 0 ? block_factor[0] : block_factor[1];
-        if (reverse ? block > q : block < q) {
-          tmem_ld32(quadrant + kColP + 32 * block, v);
-          tmem_ld_wait();
-          if (dead_tokens) {
+      float down = 1.0f;
+      if (!kStateOnly) {
+        // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns hf and hf + 2
+        auto weigh_scores = [&](int i, float (&v)[32]) {
+          const int block = hf + 2 * i;
+          const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block);
+          const float f = i == 0 ? block_factor[0] : block_factor[1];
+          if (reverse ? block > q : block < q) {
+            tmem_ld32(quadrant + kColP + 32 * block, v);
+            tmem_ld_wait();
+            if (dead_tokens) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 c = col[j / 4];
-              v[j] = c.x == 0.0f ? 0.0f : v[j] * (f * c.x);
-              v[j + 1] = c.y == 0.0f ? 0.0f : v[j + 1] * (f * c.y);
-              v[j + 2] = c.z == 0.0f ? 0.0f : v[j + 2] * (f * c.z);
-              v[j + 3] = c.w == 0.0f ? 0.0f : v[j + 3] * (f * c.w);
+              for (int j = 0; j < 32; j += 4) {
+                const float4 c = col[j / 4];
+                v[j] = c.x == 0.0f ? 0.0f : v[j] * (f * c.x);
+                v[j + 1] = c.y == 0.0f ? 0.0f : v[j + 1] * (f * c.y);
+                v[j + 2] = c.z == 0.0f ? 0.0f : v[j + 2] * (f * c.z);
+                v[j + 3] = c.w == 0.0f ? 0.0f : v[j + 3] * (f * c.w);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 c = col[j / 4];
+                v[j] *= f * c.x;
+                v[j + 1] *= f * c.y;
+                v[j + 2] *= f * c.z;
+                v[j + 3] *= f * c.w;
+              }
+            }
+          } else if (block == q) {
+            // the block on the diagonal: its valid columns up to this row's token (from it on)
+            tmem_ld32(quadrant + kColP + 32 * block, v);
+            tmem_ld_wait();
+            const uint32_t seen = ranks.word(q) & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane));
+            if (gentle) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 c = col[j / 4];
+                v[j] = (seen >> j) & 1u ? v[j] * (f * c.x) : 0.0f;
+                v[j + 1] = (seen >> (j + 1)) & 1u ? v[j + 1] * (f * c.y) : 0.0f;
+                v[j + 2] = (seen >> (j + 2)) & 1u ? v[j + 2] * (f * c.z) : 0.0f;
+                v[j + 3] = (seen >> (j + 3)) & 1u ? v[j + 3] * (f * c.w) : 0.0f;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                // rank distance: valid tokens seen by the row that lie on its side of token j
+                const uint32_t side = reverse ? (1u << j) - 1u : ~(0xffffffffu >> (31 - j));
+                v[j] = (seen >> j) & 1u ? v[j] * (inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)))) : 0.0f;
+              }
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 c = col[j / 4];
-              v[j] *= f * c.x;
-              v[j + 1] *= f * c.y;
-              v[j + 2] *= f * c.z;
-              v[j + 3] *= f * c.w;
-            }
+            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
           }
-        } else if (block == q) {
-          // the block on the diagonal: its valid columns up to this row's token (from it on)
-          tmem_ld32(quadrant + kColP + 32 * block, v);
-          tmem_ld_wait();
-          const uint32_t seen = ranks.word(q) & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane));
-          if (gentle) {
+        };
+        float up = 1.0f;
+        if (kHalf) {
+          float most = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 c = col[j / 4];
-              v[j] = (seen >> j) & 1u ? v[j] * (f * c.x) : 0.0f;
-              v[j + 1] = (seen >> (j + 1)) & 1u ? v[j + 1] * (f * c.y) : 0.0f;
-              v[j + 2] = (seen >> (j + 2)) & 1u ? v[j + 2] * (f * c.z) : 0.0f;
-              v[j + 3] = (seen >> (j + 3)) & 1u ? v[j + 3] * (f * c.w) : 0.0f;
-            }
-          } else {
+          for (int i = 0; i < 2; ++i) {
+            float v[32];
+            weigh_scores(i, v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              // rank distance: valid tokens seen by the row that lie on its side of token j
-              const uint32_t side = reverse ? (1u << j) - 1u : ~(0xffffffffu >> (31 - j));
-              v[j] = (seen >> j) & 1u ? v[j] * (inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)))) : 0.0f;
-            }
+            for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          const uint32_t top = __float_as_uint(most) >> 23;
+          sh.row_top[hf][32 * q + lane] = static_cast<uint8_t>(top);
+          named_barrier(1 + q, 64);
+          const PowerScale sc(max(top, static_cast<uint32_t>(sh.row_top[hf ^ 1][32 * q + lane])));
+          up = sc.up;
+          down = sc.down;
         }
-      };
-      float up = 1.0f;
-      if (kHalf) {
-        float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float v[32];
+          uint32_t w[16];
           weigh_scores(i, v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
+          for (int j = 0; j < 16; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
+          tmem_st16(quadrant + kColP + 32 * (hf + 2 * i), w);
         }
-        const uint32_t top = __float_as_uint(most) >> 23;
-        sh.top[hf * kChunk + 32 * q + lane] = static_cast<uint8_t>(top);
-        pair_barrier(1 + q, 64);
-        const PowerScale sc(max(top, static_cast<uint32_t>(sh.top[(hf ^ 1) * kChunk + 32 * q + lane])));
-        up = sc.up;
-        down = sc.down;
-      }
-      uint32_t w[2][16];
+        // ---- the state's part, which P' Z is added to
+        wait(xm_bar, parity);
+        const float row_factor = lambda * up;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float v[32];
-        weigh_scores(i, v);
+        for (int b = 0; b < 2 * kVB; ++b) {
+          const int col0 = 32 * (hf + 2 * (b >> 1)) + 16 * (b & 1);
+          if (col0 >= nz) continue;
+          float x[16];
+          tmem_ld16(quadrant + kColOut + col0, x);
+          tmem_ld_wait();
+          uint32_t w[16];
+          const float4* scale = reinterpret_cast<const float4*>(sh.state_scale[parity] + col0);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[i][j] = pack2<kHalf>(kHalf ? v[2 * j] * up : v[2 * j], kHalf ? v[2 * j + 1] * up : v[2 * j + 1]);
+          for (int j = 0; j < 16; j += 4) {
+            float4 f = make_float4(row_factor, row_factor, row_factor, row_factor);
+            if (kHalf) {
+              const float4 c = scale[j / 4];
+              f = make_float4(row_factor * c.x, row_factor * c.y, row_factor * c.z, row_factor * c.w);
+            }
+            w[j] = __float_as_uint(x[j] * f.x);
+            w[j + 1] = __float_as_uint(x[j + 1] * f.y);
+            w[j + 2] = __float_as_uint(x[j + 2] * f.z);
+            w[j + 3] = __float_as_uint(x[j + 3] * f.w);
+          }
+          tmem_st16(quadrant + kColOut + col0, w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        arrive(decayed_bar);
       }
-      tc_fence_before();
-      pair_barrier(1 + q, 64);  // both warps of these rows have read their scores
-      tc_fence_after();
-#pragma unroll
-      for (int i = 0; i < 2; ++i) tmem_st16(quadrant + kColP + 16 * (hf + 2 * i), w[i]);
-      tmem_st_wait();
-      tc_fence_before();
-      ok = __syncthreads_and(ok) != 0;
-      if (!ok) break;
-      if (tid == 0) {
-        tc_fence_after();
-        const uint32_t io = idesc<kHalf>((nz + 15) & ~15, false, true);
-        const uint64_t zd = make_desc_sw128(z_at, kBox, 1024);
-        for (int k = 0; k < kChunk / 16; ++k) mma_tmem_a(tmem + kColOut, tmem + kColP + 8 * k, zd + k * 128, io, k > 0);
-        mma_commit(out_bar);
-      }
-      __syncwarp();
-    }
 
-    // ---- the state after this chunk
-    ok = wait_warp(state_bar, parity, sh, a.status) && ok;
-    tc_fence_after();
+      // ---- the state after this chunk
+      wait(change_bar, parity);
 #pragma unroll
-    for (int i = 0; i < kOwn; i += 16) {
-      if (mc + i >= ny) break;  // no product wrote these columns
-      float d[16];
-      tmem_ld16(quadrant + kColChange + mc + i, d);
-      tmem_ld_wait();
+      for (int i = 0; i < kOwn; i += 16) {
+        if (mc + i >= ny) break;  // no product wrote these columns
+        float d[16];
+        tmem_ld16(quadrant + kColChange + mc + i, d);
+        tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) m[i + j] = fmaf(d[j], join, fmaf(m[i + j], decay_factor, m[i + j] * decay_keep));
-    }
-    if (kStateOnly) {
-      if (n + 1 < count) {
-        prepare(n + 1);
-        tokens_seen += ranks.total;
+        for (int j = 0; j < 16; ++j) m[i + j] = fmaf(d[j], join, fmaf(m[i + j], decay_factor, m[i + j] * decay_keep));
       }
-      tc_fence_before();
-      ok = __syncthreads_and(ok) != 0;
-      if (!ok) break;
-      if (tid == 0 && n + stages < count) {
-        load(n + stages);
-        ++issued;
+      if (kStateOnly) {
+        tc_fence_before();
+        arrive(taken_bar);
+        if (n + 1 < count) {
+          prepare(n + 1);
+          tokens_seen += ranks.total;
+        }
+        continue;
       }
-      __syncwarp();
-      continue;
-    }
-    if (n + 1 < count) write_state(parity ^ 1);
-
-    // ---- outputs
-    ok = wait_warp(out_bar, parity, sh, a.status) && ok;
-    tc_fence_after();
-    uint32_t packed[kVB][16];
-    const float row_into = lambda;
-    const bool row_live = live;
-#pragma unroll
-    for (int b = 0; b < kVB; ++b) {
-      const int col0 = 32 * (hf + 2 * b);
-      if (col0 >= nz) continue;
-      float o[32], x[32];
-      tmem_ld32(quadrant + kColOut + col0, o);
-      tmem_ld32(quadrant + kColXm + col0, x);
-      tmem_ld_wait();
-      const float4* scale = reinterpret_cast<const float4*>(sh.state_scale[parity] + col0);
-#pragma unroll
-      for (int j = 0; j < 32; j += 4) {
-        float4 f = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-        if (kHalf) f = scale[j / 4];
-        o[j] = fmaf(o[j], down, row_into * (x[j] * f.x));
-        o[j + 1] = fmaf(o[j + 1], down, row_into * (x[j + 1] * f.y));
-        o[j + 2] = fmaf(o[j + 2], down, row_into * (x[j + 2] * f.z));
-        o[j + 3] = fmaf(o[j + 3], down, row_into * (x[j + 3] * f.w));
-      }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) packed[b][j] = row_live ? pack2<kHalf>(o[2 * j], o[2 * j + 1]) : 0u;
-    }
-    if (n + 1 < count) prepare(n + 1);
-    fence_proxy_async();
-    tc_fence_before();
-    ok = __syncthreads_and(ok) != 0;
-    if (!ok) break;
-    tc_fence_after();
-    // z's boxes have been read: the output boxes (64-byte rows and swizzle) leave from there
-    const int t0 = chunk_at(n) * kChunk + 32 * q;
-#pragma unroll
-    for (int b = 0; b < kVB; ++b) {
-      const int col0 = 32 * (hf + 2 * b);
-      if (col0 >= nz || t0 >= a.length) continue;
-      uint8_t* box = z_tile + (warp * kVB + b) * kOutBox;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-            make_uint4(packed[b][4 * c], packed[b][4 * c + 1], packed[b][4 * c + 2], packed[b][4 * c + 3]);
-      }
+      if (n + 1 < count) write_state(parity ^ 1);
       fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) tma_store_4d(&maps.w, smem_u32(box), col0, head, t0, sample);
-    }
-    if (lane == 0) bulk_commit();
-    if (stages == 1) {
-      if (lane == 0) bulk_wait_read<0>();
-      __syncthreads();
-      if (tid == 0 && n + 1 < count) {
-        load(n + 1);
-        ++issued;
-      }
-      __syncwarp();
-    }
-  }
 
-  if (ok && p.state_out != nullptr && mv < nz) {
-    // a whole scan's state is the caller's; a segment's belongs to its segment
-    const bool end = reverse ? segment == 0 : segment == a.segments - 1;
-    if (kStateOnly || end) {
-      float* dst = p.state_out + (kStateOnly ? static_cast<int64_t>(item) * a.segments + segment : item) * ny * nz;
+      // ---- outputs
+      wait(out_bar, parity);
+      uint32_t packed[kVB][16];
 #pragma unroll
-      for (int i = 0; i < kOwn; ++i)
-        if (mc + i < ny) dst[(mc + i) * nz + mv] = m[i];
-      if (kStateOnly && tid == 0 && pass_index == 0) a.counts[item * a.segments + segment] = tokens_seen;
+      for (int b = 0; b < 2 * kVB; ++b) {
+        const int col0 = 32 * (hf + 2 * (b >> 1)) + 16 * (b & 1);
+        if (col0 >= nz) continue;
+        float o[16];
+        tmem_ld16(quadrant + kColOut + col0, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w = kHalf ? pack2<kHalf>(o[2 * j] * down, o[2 * j + 1] * down) : pack2<kHalf>(o[2 * j], o[2 * j + 1]);
+          packed[b >> 1][8 * (b & 1) + j] = live ? w : 0u;
+        }
+      }
+      tc_fence_before();
+      arrive(taken_bar);
+      // z's boxes have been read: the output boxes (64-byte rows and swizzle) leave from there
+      const int t0 = chunk_at(n) * kChunk + 32 * q;
+#pragma unroll
+      for (int b = 0; b < kVB; ++b) {
+        const int col0 = 32 * (hf + 2 * b);
+        if (col0 >= nz || t0 >= a.length) continue;
+        uint8_t* box = z_tile + (warp * kVB + b) * kOutBox;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+              make_uint4(packed[b][4 * c], packed[b][4 * c + 1], packed[b][4 * c + 2], packed[b][4 * c + 3]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && ok) tma_store_4d(&maps.w, smem_u32(box), col0, head, t0, sample);
+      }
+      if (lane == 0) bulk_commit();
+      if (stages == 1) {
+        if (lane == 0) bulk_wait_read<0>();
+        arrive(freed_bar);
+      }
+      if (n + 1 < count) prepare(n + 1);
     }
-  }
-  // ---- nothing may be in flight when the CTA ends
-  if (!kStateOnly && lane == 0) bulk_wait<0>();
-  if (tid == 0) {
-    if (!ok) {
-      for (int n = max(0, issued - stages); n < issued; ++n)
-        mbar_wait_bounded(full_bar + 8 * (stages == 2 ? n & 1 : 0), stages == 2 ? (n >> 1) & 1 : n & 1, nullptr, a.status);
+    if (ok && p.state_out != nullptr && mv < nz) {
+      // a whole scan's state is the caller's; a segment's belongs to its segment
+      const bool end = reverse ? segment == 0 : segment == a.segments - 1;
+      if (kStateOnly || end) {
+        float* dst = p.state_out + (kStateOnly ? static_cast<int64_t>(item) * a.segments + segment : item) * ny * nz;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+          if (mc + i < ny) dst[(mc + i) * nz + mv] = m[i];
+      }
     }
-    mma_drain(smem_u32(&sh.drain), a.status);
+    if (kStateOnly && tid == 0 && pass_index == 0) a.counts[item * a.segments + segment] = tokens_seen;
+    if (!kStateOnly && lane == 0) bulk_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
