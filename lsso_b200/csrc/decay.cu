@@ -95,8 +95,15 @@ template <bool kHalf>
 __device__ __forceinline__ uint32_t idesc(int n, bool a_mn, bool b_mn) {
   return make_idesc(128, n, a_mn, b_mn) & ~(kHalf ? (1u << 7) | (1u << 10) : 0u);
 }
+// Out of line: the loop of a chunk is long, and instruction fetch is one of its limits.
+__device__ __noinline__ bool wait_late(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
+  return mbar_wait_bounded(bar, parity, abort_flag, status);
+}
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, ScanShared& sh, int* status) {
+  return mbar_try_wait(bar, parity) || wait_late(bar, parity, &sh.abort_flag, status);
+}
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, ScanShared& sh, int* status) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, &sh.abort_flag, status));
+  return __all_sync(0xffffffffu, wait_one(bar, parity, sh, status));
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       };
       while (loaded < min(stages, count)) load();
       auto wait = [&](uint32_t bar, uint32_t parity) {
-        ok = ok && mbar_wait_bounded(bar, parity, &sh.abort_flag, a.status);
+        ok = ok && wait_one(bar, parity, sh, a.status);
         tc_fence_after();
         return ok;
       };
@@ -448,11 +455,11 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       uint8_t* const y_tile = x_tile + kXBytes;
       uint8_t* const z_tile = y_tile + kKB * kBox;
       if (n + 1 < count) fetch_mask(n + 1);
-      wait(full_bar + 8 * stage_of(n), full_parity(n));
       if (!kStateOnly) {
         wait(scores_bar, parity);          // y's rows have been read
         if (exact) wait(xm_bar, parity);   // x's too
       }
+      wait(full_bar + 8 * stage_of(n), full_parity(n));
 
       // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
       {
@@ -512,92 +519,74 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
 
       float down = 1.0f;
       if (!kStateOnly) {
-        // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns hf and hf + 2
-        auto weigh_scores = [&](int i, float (&v)[32]) {
-          const int block = hf + 2 * i;
-          const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block);
-          const float f = i == 0 ? block_factor[0] : block_factor[1];
-          if (reverse ? block > q : block < q) {
-            tmem_ld32(quadrant + kColP + 32 * block, v);
+        // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns hf and hf + 2, sixteen columns
+        // at a time (a short loop: the chunk's code has to stay close to the instruction cache).  FP16 goes over them
+        // twice, first for the largest of a row.
+        float up = 1.0f, most = 0.0f;
+#pragma unroll 1
+        for (int it = kHalf ? -4 : 0; it < 4; ++it) {
+          const int block = hf + (it & 2), half = 16 * (it & 1), col0 = 32 * block + half;
+          const uint32_t whole = ranks.word(block);
+          // this row's columns: all before its block, those up to its own in it (from it on), valid ones
+          const bool on_diagonal = block == q;
+          const uint32_t seen = on_diagonal ? whole & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane))
+                                            : (reverse ? block > q : block < q) ? whole : 0u;
+          float v[16];
+          if (!on_diagonal && seen == 0u) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+          } else {
+            tmem_ld16(quadrant + kColP + col0, v);
             tmem_ld_wait();
-            if (dead_tokens) {
+            const float f = (it & 2) ? block_factor[1] : block_factor[0];
+            const float4* col = reinterpret_cast<const float4*>(sh.col + col0);
+            if (gentle || !on_diagonal) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 c = col[j / 4];
-                v[j] = c.x == 0.0f ? 0.0f : v[j] * (f * c.x);
-                v[j + 1] = c.y == 0.0f ? 0.0f : v[j + 1] * (f * c.y);
-                v[j + 2] = c.z == 0.0f ? 0.0f : v[j + 2] * (f * c.z);
-                v[j + 3] = c.w == 0.0f ? 0.0f : v[j + 3] * (f * c.w);
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
+              for (int j = 0; j < 16; j += 4) {
                 const float4 c = col[j / 4];
                 v[j] *= f * c.x;
                 v[j + 1] *= f * c.y;
                 v[j + 2] *= f * c.z;
                 v[j + 3] *= f * c.w;
               }
-            }
-          } else if (block == q) {
-            // the block on the diagonal: its valid columns up to this row's token (from it on)
-            tmem_ld32(quadrant + kColP + 32 * block, v);
-            tmem_ld_wait();
-            const uint32_t seen = ranks.word(q) & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane));
-            if (gentle) {
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 c = col[j / 4];
-                v[j] = (seen >> j) & 1u ? v[j] * (f * c.x) : 0.0f;
-                v[j + 1] = (seen >> (j + 1)) & 1u ? v[j + 1] * (f * c.y) : 0.0f;
-                v[j + 2] = (seen >> (j + 2)) & 1u ? v[j + 2] * (f * c.z) : 0.0f;
-                v[j + 3] = (seen >> (j + 3)) & 1u ? v[j + 3] * (f * c.w) : 0.0f;
-              }
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                // rank distance: valid tokens seen by the row that lie on its side of token j
-                const uint32_t side = reverse ? (1u << j) - 1u : ~(0xffffffffu >> (31 - j));
-                v[j] = (seen >> j) & 1u ? v[j] * (inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)))) : 0.0f;
+              for (int j = 0; j < 16; ++j) {
+                // rank distance: valid tokens seen by the row that lie on its side of token half + j
+                const uint32_t side = reverse ? (1u << (half + j)) - 1u : ~(0xffffffffu >> (31 - (half + j)));
+                v[j] *= inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)));
               }
             }
-          } else {
+            if (on_diagonal || seen != 0xffffffffu) {
+              const uint32_t bits = seen >> half;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+              for (int j = 0; j < 16; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.0f;
+            }
           }
-        };
-        float up = 1.0f;
-        if (kHalf) {
-          float most = 0.0f;
+          if (kHalf && it < 0) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float v[32];
-            weigh_scores(i, v);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) most = fmaxf(most, fabsf(v[j]));
+            for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[j]));
+            if (it == -1) {
+              const uint32_t top = __float_as_uint(most) >> 23;
+              sh.row_top[hf][32 * q + lane] = static_cast<uint8_t>(top);
+              named_barrier(1 + q, 64);
+              const PowerScale sc(max(top, static_cast<uint32_t>(sh.row_top[hf ^ 1][32 * q + lane])));
+              up = sc.up;
+              down = sc.down;
+            }
+            continue;
           }
-          const uint32_t top = __float_as_uint(most) >> 23;
-          sh.row_top[hf][32 * q + lane] = static_cast<uint8_t>(top);
-          named_barrier(1 + q, 64);
-          const PowerScale sc(max(top, static_cast<uint32_t>(sh.row_top[hf ^ 1][32 * q + lane])));
-          up = sc.up;
-          down = sc.down;
-        }
+          uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float v[32];
-          uint32_t w[16];
-          weigh_scores(i, v);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
-          tmem_st16(quadrant + kColP + 32 * (hf + 2 * i), w);
+          for (int j = 0; j < 8; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
+          tmem_st8(quadrant + kColP + 32 * block + half / 2, w);
         }
         // ---- the state's part, which P' Z is added to
         wait(xm_bar, parity);
         const float row_factor = lambda * up;
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < 2 * kVB; ++b) {
-          const int col0 = 32 * (hf + 2 * (b >> 1)) + 16 * (b & 1);
+          const int col0 = 32 * (hf + (b & 2)) + 16 * (b & 1);
           if (col0 >= nz) continue;
           float x[16];
           tmem_ld16(quadrant + kColOut + col0, x);
@@ -648,37 +637,34 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
 
       // ---- outputs
       wait(out_bar, parity);
-      uint32_t packed[kVB][16];
-#pragma unroll
+      // z's boxes have been read: the output boxes (32 x 32, 64-byte rows and swizzle) leave from there
+      uint8_t* const boxes = z_tile + warp * kVB * kOutBox;
+#pragma unroll 1
       for (int b = 0; b < 2 * kVB; ++b) {
-        const int col0 = 32 * (hf + 2 * (b >> 1)) + 16 * (b & 1);
+        const int col0 = 32 * (hf + (b & 2)) + 16 * (b & 1);
         if (col0 >= nz) continue;
         float o[16];
         tmem_ld16(quadrant + kColOut + col0, o);
         tmem_ld_wait();
+        uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint32_t w = kHalf ? pack2<kHalf>(o[2 * j] * down, o[2 * j + 1] * down) : pack2<kHalf>(o[2 * j], o[2 * j + 1]);
-          packed[b >> 1][8 * (b & 1) + j] = live ? w : 0u;
+          w[j] = kHalf ? pack2<kHalf>(o[2 * j] * down, o[2 * j + 1] * down) : pack2<kHalf>(o[2 * j], o[2 * j + 1]);
+          w[j] = live ? w[j] : 0u;
         }
+        uint8_t* row = boxes + (b >> 1) * kOutBox + lane * 64;
+        const int piece = 2 * (b & 1), turn = (lane >> 1) & 3;
+        *reinterpret_cast<uint4*>(row + ((piece ^ turn) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(row + (((piece + 1) ^ turn) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
       }
+      fence_proxy_async();
       tc_fence_before();
       arrive(taken_bar);
-      // z's boxes have been read: the output boxes (64-byte rows and swizzle) leave from there
       const int t0 = chunk_at(n) * kChunk + 32 * q;
+      if (lane == 0 && ok && t0 < a.length) {
 #pragma unroll
-      for (int b = 0; b < kVB; ++b) {
-        const int col0 = 32 * (hf + 2 * b);
-        if (col0 >= nz || t0 >= a.length) continue;
-        uint8_t* box = z_tile + (warp * kVB + b) * kOutBox;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          *reinterpret_cast<uint4*>(box + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-              make_uint4(packed[b][4 * c], packed[b][4 * c + 1], packed[b][4 * c + 2], packed[b][4 * c + 3]);
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0 && ok) tma_store_4d(&maps.w, smem_u32(box), col0, head, t0, sample);
+        for (int b = 0; b < kVB; ++b)
+          if (32 * (hf + 2 * b) < nz) tma_store_4d(&maps.w, smem_u32(boxes + b * kOutBox), 32 * (hf + 2 * b), head, t0, sample);
       }
       if (lane == 0) bulk_commit();
       if (stages == 1) {
