@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   const int first = segment * a.segment_chunks, count = min(a.segment_chunks, a.chunks - first);
   const int ny = p.ny, nz = p.nz, stages = a.stages;
   uint8_t* const state_tile = smem + stages * kStage;                                // M^T: [kKB][64 kVB rows][128 bytes]
-  uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kStateBox);            // exact: parts that have no other place
+  uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kStateBox);            // exact: the smaller parts of weighted rows
   const uint32_t base = smem_u32(smem), full_bar = smem_u32(sh.full);
   const uint32_t scores_bar = smem_u32(&sh.scores), xm_bar = smem_u32(&sh.xm), change_bar = smem_u32(&sh.change),
                  out_bar = smem_u32(&sh.out), weighed_bar = smem_u32(&sh.weighed), decayed_bar = smem_u32(&sh.decayed),
@@ -214,6 +214,14 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   // Factor of a chunk's part of the state.  The weights of its rows leave it out, so that the largest of them is one:
   // FP16 would lose rows whose weights are all small (a strong decay before the state of a reverse scan).
   const float join = p.from * exp2f(l2 * late);
+  // Plain chunks: with rows weighted to the chunk's last token, y'_j = e^(l (n - 1 - r_j)) y_j, and M to it as well,
+  //   w_i = a_i [ sum over j of (x_i . y'_j) z_j + kappa x_i M ],   a_i = into from e^(l (r_i - n + 1)),
+  //   kappa = e^(l (n - late)) / from,
+  // the scores need no factor of their own (only the mask of their diagonal), and the state's part and the scores' share
+  // an accumulator.  Rounding is relative, so nothing is lost while the weights stay within the type's range: e^(127 |l|)
+  // up to 2^96 in FP32 and BF16, up to 2^4 in FP16, whose small weights would become subnormal.  Other heads take the
+  // scores of raw rows and weigh every score.
+  const bool plain = l2 * 127.0f > (kHalf ? -4.0f : -96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
   const int q = warp & 3, hf = (warp >> 2) & 1;
   // this thread's part of M^T: row mv, columns [mc, mc + kOwn)
@@ -221,6 +229,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   const int part = kVB == 1 ? (q >> 1) + 2 * hf : hf;
   const int mc = part * kOwn;
   float m[kOwn];
+  float kappa = 1.0f;
   // M^T as the next product's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
   auto write_state = [&](int parity) {
     float up = 1.0f;
@@ -235,7 +244,9 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       for (int i = 0; i < kParts; ++i) e = max(e, static_cast<uint32_t>(sh.state_top[i * (64 * kVB) + mv]));
       const PowerScale s(e);
       up = s.up;
-      if (part == 0) sh.state_scale[parity][mv] = s.down;
+      if (part == 0) sh.state_scale[parity][mv] = s.down * kappa;
+    } else {
+      up = kappa;
     }
 #pragma unroll
     for (int i = 0; i < kOwn; i += 8) {
@@ -243,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        w[j] = kHalf ? pack2<kHalf>(m[i + 2 * j] * up, m[i + 2 * j + 1] * up) : pack2<kHalf>(m[i + 2 * j], m[i + 2 * j + 1]);
+        w[j] = pack2<kHalf>(m[i + 2 * j] * up, m[i + 2 * j + 1] * up);
       *reinterpret_cast<uint4*>(state_tile + box * kStateBox + mv * 128 + ((piece ^ (mv & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   };
@@ -258,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     for (int w = 0; w < 4; ++w)
       if (t0 + 32 * w < a.length && of_sample[t0 + 32 * w] != 0) ahead |= 1u << w;
   };
-  float lambda = 0.0f, block_factor[2] = {0.0f, 0.0f};
+  float lambda = 0.0f /* factor of the state's part of this row; plain: of the whole row */, block_factor[2] = {0.0f, 0.0f};
   bool live = false, dead_tokens = false, was_whole = false;
   float decay_factor = 0.0f, decay_keep = 0.0f;  // M' = M * factor + M * keep (keep is 0 or 1)
   int decay_total = -1;
@@ -287,12 +298,13 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     if (n > 0) named_barrier(7, kWorkers);  // the tables have been read
     if (hf == 0) {
       sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : 0.0f;
-    } else if (!kStateOnly) {
+    } else if (!kStateOnly && !plain) {
       sh.col[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.last_rho(q, reverse) - rho)) : 0.0f;
     }
     if (n > 0) named_barrier(7, kWorkers);
     if (!kStateOnly) {
-      lambda = p.into * exp2f(l2 * (row_rho + 1.0f - late));
+      lambda = plain ? inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.total - 1))) : p.into * exp2f(l2 * (row_rho + 1.0f - late));
+      if (plain) kappa = exp2f(l2 * (static_cast<float>(ranks.total) - late)) / p.from;
 #pragma unroll
       for (int i = 0; i < 2; ++i) block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(hf + 2 * i, reverse))));
     }
@@ -357,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
                      i_change = idesc<kHalf>((ny + 15) & ~15, true, true), i_out = idesc<kHalf>((nz + 15) & ~15, false, true);
       const uint64_t x0 = make_desc_sw128(base, 16, 1024), y0 = make_desc_sw128(base + kXBytes, 16, 1024),
                      state0 = make_desc_sw128(smem_u32(state_tile), 16, 1024),
-                     x_rows = make_desc_sw128(base, kBox, 1024), y_rows = make_desc_sw128(base + kXBytes, kBox, 1024),
+                     y_rows = make_desc_sw128(base + kXBytes, kBox, 1024),
                      third_rows = make_desc_sw128(smem_u32(third), kBox, 1024),
                      // one box of z: lanes 64-127 repeat 0-63
                      z_lanes = make_desc_sw128(base + kXBytes + kKB * kBox, kVB == 2 ? kBox : 0, 1024),
@@ -374,7 +386,12 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         const uint32_t parity = n & 1;
         const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
         if (!kStateOnly) {
-          if (n == 0) {
+          if (plain) {
+            // scores of weighted rows, once the chunk before has used its own
+            if (n > 0 && !wait(out_bar, parity ^ 1)) break;
+            if (!wait(weighed_bar, parity)) break;
+            scores(n);
+          } else if (n == 0) {
             if (!wait(full_bar, 0)) break;
             scores(0);
           }
@@ -385,13 +402,13 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
           }
           mma_commit(xm_bar);
         }
-        if (!wait(weighed_bar, parity)) break;
+        if ((kStateOnly || !plain) && !wait(weighed_bar, parity)) break;
         if (kStateOnly && n > 0 && !wait(taken_bar, parity ^ 1)) break;
         const uint64_t zd = z_lanes + at;
         bool more = false;
         if (exact) {  // the smaller parts first
           for (int t = kHalf ? 1 : 0; t < 2; ++t) {
-            const uint64_t yd = t == 0 ? third_rows : kStateOnly ? third_rows + (kHalf ? 0 : kKB * (kBox / 16)) : x_rows + at;
+            const uint64_t yd = third_rows + (t == 0 || kHalf ? 0 : kKB * (kBox / 16));
             for (int k = 0; k < kChunk / 16; ++k) {
               mma_bf16(tmem + kColChange, zd + k * 128, yd + k * 128, i_change, more);
               more = true;
@@ -420,13 +437,16 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
           mma_tmem_a(tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), z_rows + at + k * 128, i_out, 1);
         }
         mma_commit(out_bar);
-        if (n + 1 < count) {  // the next scores as soon as these have been used
+        if (n + 1 < count) {
           if (stages == 1) {
             if (!wait(freed_bar, parity)) break;
             load();
           }
-          if (!wait(out_bar, parity) || !wait(full_bar + 8 * stage_of(n + 1), full_parity(n + 1))) break;
-          scores(n + 1);
+          // the next scores as soon as these have been used
+          if (!plain) {
+            if (!wait(out_bar, parity) || !wait(full_bar + 8 * stage_of(n + 1), full_parity(n + 1))) break;
+            scores(n + 1);
+          }
         }
       }
       // nothing may be in flight when the CTA ends
@@ -451,20 +471,16 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     };
     for (int n = 0; n < count; ++n) {
       const uint32_t parity = n & 1;
-      uint8_t* const x_tile = smem + stage_of(n) * kStage;
-      uint8_t* const y_tile = x_tile + kXBytes;
+      uint8_t* const y_tile = smem + stage_of(n) * kStage + kXBytes;
       uint8_t* const z_tile = y_tile + kKB * kBox;
       if (n + 1 < count) fetch_mask(n + 1);
-      if (!kStateOnly) {
-        wait(scores_bar, parity);          // y's rows have been read
-        if (exact) wait(xm_bar, parity);   // x's too
-      }
+      if (!kStateOnly && !plain) wait(scores_bar, parity);  // y's rows have been read
       wait(full_bar + 8 * stage_of(n), full_parity(n));
 
       // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
       {
         const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;  // 16-byte pieces of a row (of each box) that hold features
-        uint8_t* const second = kStateOnly ? third + (kHalf ? 0 : kKB * kBox) : x_tile;
+        uint8_t* const second = third + (kHalf ? 0 : kKB * kBox);
 #pragma unroll
         for (int b = 0; b < kKB; ++b) {
 #pragma unroll 2
@@ -523,10 +539,11 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         // at a time (a short loop: the chunk's code has to stay close to the instruction cache).  FP16 goes over them
         // twice, first for the largest of a row.
         float up = 1.0f, most = 0.0f;
+        if (plain) wait(scores_bar, parity);
 #pragma unroll 1
         for (int it = kHalf ? -4 : 0; it < 4; ++it) {
           const int block = hf + (it & 2), half = 16 * (it & 1), col0 = 32 * block + half;
-          const uint32_t whole = ranks.word(block);
+          const uint32_t whole = plain ? 0xffffffffu : ranks.word(block);  // plain: masked rows of y are zero
           // this row's columns: all before its block, those up to its own in it (from it on), valid ones
           const bool on_diagonal = block == q;
           const uint32_t seen = on_diagonal ? whole & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane))
@@ -540,7 +557,8 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
             tmem_ld_wait();
             const float f = (it & 2) ? block_factor[1] : block_factor[0];
             const float4* col = reinterpret_cast<const float4*>(sh.col + col0);
-            if (gentle || !on_diagonal) {
+            if (plain) {
+            } else if (gentle || !on_diagonal) {
 #pragma unroll
               for (int j = 0; j < 16; j += 4) {
                 const float4 c = col[j / 4];
@@ -581,9 +599,11 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
           for (int j = 0; j < 8; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
           tmem_st8(quadrant + kColP + 32 * block + half / 2, w);
         }
-        // ---- the state's part, which P' Z is added to
+        // ---- the state's part, which P' Z is added to, by the row's factor (plain chunks have it in M already, and FP16
+        // that of its rows)
+        if (kHalf || !plain) {
         wait(xm_bar, parity);
-        const float row_factor = lambda * up;
+        const float row_factor = plain ? up : lambda * up;
 #pragma unroll 1
         for (int b = 0; b < 2 * kVB; ++b) {
           const int col0 = 32 * (hf + (b & 2)) + 16 * (b & 1);
@@ -606,6 +626,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
             w[j + 3] = __float_as_uint(x[j + 3] * f.w);
           }
           tmem_st16(quadrant + kColOut + col0, w);
+        }
         }
         tmem_st_wait();
         tc_fence_before();
@@ -632,7 +653,12 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         }
         continue;
       }
-      if (n + 1 < count) write_state(parity ^ 1);
+      const float row_out = plain ? lambda * down : down;
+      const bool row_live = live;
+      if (n + 1 < count) {
+        prepare(n + 1);
+        write_state(parity ^ 1);
+      }
       fence_proxy_async();
 
       // ---- outputs
@@ -649,8 +675,8 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          w[j] = kHalf ? pack2<kHalf>(o[2 * j] * down, o[2 * j + 1] * down) : pack2<kHalf>(o[2 * j], o[2 * j + 1]);
-          w[j] = live ? w[j] : 0u;
+          w[j] = pack2<kHalf>(o[2 * j] * row_out, o[2 * j + 1] * row_out);
+          w[j] = row_live ? w[j] : 0u;
         }
         uint8_t* row = boxes + (b >> 1) * kOutBox + lane * 64;
         const int piece = 2 * (b & 1), turn = (lane >> 1) & 3;
@@ -671,7 +697,6 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         if (lane == 0) bulk_wait_read<0>();
         arrive(freed_bar);
       }
-      if (n + 1 < count) prepare(n + 1);
     }
     if (ok && p.state_out != nullptr && mv < nz) {
       // a whole scan's state is the caller's; a segment's belongs to its segment
@@ -800,8 +825,8 @@ template <bool kHalf, int kKB, int kVB, bool kStateOnly>
 cudaError_t launch_one(ScanArgs& a, int64_t items, const char* name, cudaStream_t stream) {
   bool exact = false;
   for (int i = 0; i < a.passes; ++i) exact = exact || a.pass[i].exact != 0;
-  // the parts of exactly weighted rows that have no other buffer
-  const int parts = !exact ? 0 : kStateOnly ? (kHalf ? 1 : 2) : (kHalf ? 0 : 1);
+  // the smaller parts of exactly weighted rows
+  const int parts = !exact ? 0 : kHalf ? 1 : 2;
   const size_t stage = ((kStateOnly ? 1 : 2) * kKB + kVB) * kBox;
   const size_t rest = (kStateOnly ? 0 : kKB * kVB * 64 * 128) + parts * kKB * kBox;
   // Two stages where they fit (beside a second CTA, where its TMEM leaves room for one).
