@@ -81,6 +81,8 @@ struct ScanShared {
   int abort_flag;
 };
 
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[16]) { tmem_ld16(taddr, v); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if (kHalf) return pair_from_float(lo, hi, __half());
@@ -168,6 +170,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   constexpr uint32_t kCols = kStateOnly ? 64 * kKB : kSmall ? 256 : 512;
   constexpr int kParts = kVB == 1 ? 4 : 2;  // threads that share a row of M^T (one lane quadrant or two hold it)
   constexpr int kOwn = 64 * kKB / kParts;   // its columns held by one thread
+  constexpr int kPiece = kOwn > 16 ? 32 : 16;  // of them per TMEM load
   constexpr uint32_t kXBytes = kStateOnly ? 0 : kKB * kBox;
   constexpr uint32_t kStage = kXBytes + kKB * kBox + kVB * kBox;
   constexpr uint32_t kStateBox = kVB * 64 * 128;
@@ -341,11 +344,12 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   bool ok = true;
 
   if (warp == kWorkers / 32) {
-    // ---------------- loads and products
-    if (lane == 0) {
-      int loaded = 0;
-      auto load = [&]() {
-        const int n = loaded++, t0 = chunk_at(n) * kChunk;
+    // ---------------- loads and products: the warp walks them together, one lane issues
+    const bool leader = elect_leader();
+    int loaded = 0;
+    auto load = [&]() {
+      const int n = loaded++, t0 = chunk_at(n) * kChunk;
+      if (leader) {
         const uint32_t bar = full_bar + 8 * stage_of(n);
         uint32_t dst = base + stage_of(n) * kStage;
         mbar_arrive_expect_tx(bar, kStage);
@@ -357,99 +361,108 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         for (int b = 0; b < kKB; ++b, dst += kBox) tma_load_4d(dst, &maps.y, 64 * b, head, t0, sample, bar);
 #pragma unroll
         for (int b = 0; b < kVB; ++b, dst += kBox) tma_load_4d(dst, &maps.z, 64 * b, head, t0, sample, bar);
-      };
-      while (loaded < min(stages, count)) load();
-      auto wait = [&](uint32_t bar, uint32_t parity) {
-        ok = ok && wait_one(bar, parity, sh, a.status);
-        tc_fence_after();
-        return ok;
-      };
-      const int y_steps = (ny + 15) / 16;
-      const uint32_t i_scores = idesc<kHalf>(128, false, false), i_xm = idesc<kHalf>((nz + 15) & ~15, false, false),
-                     i_change = idesc<kHalf>((ny + 15) & ~15, true, true), i_out = idesc<kHalf>((nz + 15) & ~15, false, true);
-      const uint64_t x0 = make_desc_sw128(base, 16, 1024), y0 = make_desc_sw128(base + kXBytes, 16, 1024),
-                     state0 = make_desc_sw128(smem_u32(state_tile), 16, 1024),
-                     y_rows = make_desc_sw128(base + kXBytes, kBox, 1024),
-                     third_rows = make_desc_sw128(smem_u32(third), kBox, 1024),
-                     // one box of z: lanes 64-127 repeat 0-63
-                     z_lanes = make_desc_sw128(base + kXBytes + kKB * kBox, kVB == 2 ? kBox : 0, 1024),
-                     z_rows = make_desc_sw128(base + kXBytes + kKB * kBox, kBox, 1024);
-      auto scores = [&](int n) {
-        const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
-        for (int k = 0; k < y_steps; ++k) {
-          const uint64_t step = at + (k >> 2) * (kBox / 16) + (k & 3) * 2;
-          mma_bf16(tmem + kColP, x0 + step, y0 + step, i_scores, k > 0);
+      }
+      __syncwarp();
+    };
+    while (loaded < min(stages, count)) load();
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      ok = ok && wait_warp(bar, parity, sh, a.status);
+      tc_fence_after();
+      return ok;
+    };
+    const int y_steps = (ny + 15) / 16;
+    const uint32_t i_scores = idesc<kHalf>(128, false, false), i_xm = idesc<kHalf>((nz + 15) & ~15, false, false),
+                   i_change = idesc<kHalf>((ny + 15) & ~15, true, true), i_out = idesc<kHalf>((nz + 15) & ~15, false, true);
+    const uint64_t x0 = make_desc_sw128(base, 16, 1024), y0 = make_desc_sw128(base + kXBytes, 16, 1024),
+                   state0 = make_desc_sw128(smem_u32(state_tile), 16, 1024),
+                   y_rows = make_desc_sw128(base + kXBytes, kBox, 1024),
+                   third_rows = make_desc_sw128(smem_u32(third), kBox, 1024),
+                   // one box of z: lanes 64-127 repeat 0-63
+                   z_lanes = make_desc_sw128(base + kXBytes + kKB * kBox, kVB == 2 ? kBox : 0, 1024),
+                   z_rows = make_desc_sw128(base + kXBytes + kKB * kBox, kBox, 1024);
+    auto scores = [&](int n) {
+      const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
+      const uint64_t xd = x0 + at, yd = y0 + at;
+#pragma unroll
+      for (int k = 0; k < 4 * kKB; ++k) {
+        const int step = (k >> 2) * (kBox / 16) + (k & 3) * 2;
+        if (k < y_steps) mma_led(leader, tmem + kColP, xd + step, yd + step, i_scores, k > 0);
+      }
+      mma_led_commit(leader, scores_bar);
+    };
+    for (int n = 0; n < count; ++n) {
+      const uint32_t parity = n & 1;
+      const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
+      if (!kStateOnly) {
+        if (plain) {
+          // scores of weighted rows, once the chunk before has used its own
+          if (n > 0 && !wait(out_bar, parity ^ 1)) break;
+          if (!wait(weighed_bar, parity)) break;
+          scores(n);
+        } else if (n == 0) {
+          if (!wait(full_bar, 0)) break;
+          scores(0);
         }
-        mma_commit(scores_bar);
-      };
-      for (int n = 0; n < count; ++n) {
-        const uint32_t parity = n & 1;
-        const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
-        if (!kStateOnly) {
-          if (plain) {
-            // scores of weighted rows, once the chunk before has used its own
-            if (n > 0 && !wait(out_bar, parity ^ 1)) break;
-            if (!wait(weighed_bar, parity)) break;
-            scores(n);
-          } else if (n == 0) {
-            if (!wait(full_bar, 0)) break;
-            scores(0);
-          }
-          if (n > 0 && !wait(taken_bar, parity ^ 1)) break;
-          for (int k = 0; k < y_steps; ++k) {
-            mma_bf16(tmem + kColOut, x0 + at + (k >> 2) * (kBox / 16) + (k & 3) * 2,
-                     state0 + (k >> 2) * (kStateBox / 16) + (k & 3) * 2, i_xm, k > 0);
-          }
-          mma_commit(xm_bar);
-        }
-        if ((kStateOnly || !plain) && !wait(weighed_bar, parity)) break;
-        if (kStateOnly && n > 0 && !wait(taken_bar, parity ^ 1)) break;
-        const uint64_t zd = z_lanes + at;
-        bool more = false;
-        if (exact) {  // the smaller parts first
-          for (int t = kHalf ? 1 : 0; t < 2; ++t) {
-            const uint64_t yd = third_rows + (t == 0 || kHalf ? 0 : kKB * (kBox / 16));
-            for (int k = 0; k < kChunk / 16; ++k) {
-              mma_bf16(tmem + kColChange, zd + k * 128, yd + k * 128, i_change, more);
-              more = true;
-            }
+        if (n > 0 && !wait(taken_bar, parity ^ 1)) break;
+        const uint64_t xd = x0 + at;
+#pragma unroll
+        for (int k = 0; k < 4 * kKB; ++k) {
+          if (k < y_steps) {
+            mma_led(leader, tmem + kColOut, xd + (k >> 2) * (kBox / 16) + (k & 3) * 2,
+                    state0 + (k >> 2) * (kStateBox / 16) + (k & 3) * 2, i_xm, k > 0);
           }
         }
-        for (int k = 0; k < kChunk / 16; ++k) {
-          if (kHalf && exact && k == 0) {
-            mma_scaled_d(tmem + kColChange, zd, y_rows + at, i_change);  // the part so far is 2^11 times too large
-          } else {
-            mma_bf16(tmem + kColChange, zd + k * 128, y_rows + at + k * 128, i_change, more || k > 0);
-          }
-        }
-        mma_commit(change_bar);
-        if (kStateOnly) {
-          if (loaded < count) {
-            if (!wait(change_bar, parity)) break;
-            load();
-          }
-          continue;
-        }
-        // every warp's stores of the chunk before have left its stage
-        if (stages == 2 && n > 0 && loaded < count) load();
-        if (!wait(decayed_bar, parity)) break;
-        for (int k = 0; k < kChunk / 16; ++k) {
-          mma_tmem_a(tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), z_rows + at + k * 128, i_out, 1);
-        }
-        mma_commit(out_bar);
-        if (n + 1 < count) {
-          if (stages == 1) {
-            if (!wait(freed_bar, parity)) break;
-            load();
-          }
-          // the next scores as soon as these have been used
-          if (!plain) {
-            if (!wait(out_bar, parity) || !wait(full_bar + 8 * stage_of(n + 1), full_parity(n + 1))) break;
-            scores(n + 1);
-          }
+        mma_led_commit(leader, xm_bar);
+      }
+      if ((kStateOnly || !plain) && !wait(weighed_bar, parity)) break;
+      if (kStateOnly && n > 0 && !wait(taken_bar, parity ^ 1)) break;
+      const uint64_t zd = z_lanes + at, yd = y_rows + at;
+      if (exact) {  // the smaller parts first
+#pragma unroll 1
+        for (int t = kHalf ? 1 : 0; t < 2; ++t) {
+          const uint64_t rows = third_rows + (t == 0 || kHalf ? 0 : kKB * (kBox / 16));
+#pragma unroll
+          for (int k = 0; k < kChunk / 16; ++k)
+            mma_led(leader, tmem + kColChange, zd + k * 128, rows + k * 128, i_change, k > 0 || (!kHalf && t == 1));
         }
       }
-      // nothing may be in flight when the CTA ends
+      if (kHalf && exact) {
+        mma_led_scaled_d(leader, tmem + kColChange, zd, yd, i_change);  // the part so far is 2^11 times too large
+      } else {
+        mma_led(leader, tmem + kColChange, zd, yd, i_change, exact);
+      }
+#pragma unroll
+      for (int k = 1; k < kChunk / 16; ++k) mma_led(leader, tmem + kColChange, zd + k * 128, yd + k * 128, i_change, 1);
+      mma_led_commit(leader, change_bar);
+      if (kStateOnly) {
+        if (loaded < count) {
+          if (!wait(change_bar, parity)) break;
+          load();
+        }
+        continue;
+      }
+      // every warp's stores of the chunk before have left its stage
+      if (stages == 2 && n > 0 && loaded < count) load();
+      if (!wait(decayed_bar, parity)) break;
+      const uint64_t zr = z_rows + at;
+#pragma unroll
+      for (int k = 0; k < kChunk / 16; ++k)
+        mma_led_tmem_a(leader, tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), zr + k * 128, i_out, 1);
+      mma_led_commit(leader, out_bar);
+      if (n + 1 < count) {
+        if (stages == 1) {
+          if (!wait(freed_bar, parity)) break;
+          load();
+        }
+        // the next scores as soon as these have been used
+        if (!plain) {
+          if (!wait(out_bar, parity) || !wait(full_bar + 8 * stage_of(n + 1), full_parity(n + 1))) break;
+          scores(n + 1);
+        }
+      }
+    }
+    // nothing may be in flight when the CTA ends
+    if (leader) {
       if (!ok) {
         for (int n = max(0, loaded - stages); n < loaded; ++n)
           mbar_wait_bounded(full_bar + 8 * stage_of(n), full_parity(n), nullptr, a.status);
@@ -483,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         uint8_t* const second = third + (kHalf ? 0 : kKB * kBox);
 #pragma unroll
         for (int b = 0; b < kKB; ++b) {
-#pragma unroll 2
+#pragma unroll 4
           for (int i = tid; i < kChunk * pieces; i += kWorkers) {
             const int row = i >> shift, piece = i & (pieces - 1);
             const uint32_t at = b * kBox + row * 128 + ((piece ^ (row & 7)) << 4);
@@ -636,13 +649,15 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       // ---- the state after this chunk
       wait(change_bar, parity);
 #pragma unroll
-      for (int i = 0; i < kOwn; i += 16) {
-        if (mc + i >= ny) break;  // no product wrote these columns
-        float d[16];
-        tmem_ld16(quadrant + kColChange + mc + i, d);
+      for (int i = 0; i < kOwn; i += kPiece) {
+        if (mc + i >= ny) break;  // no product wrote these columns (or those of a piece's second half, which are unused)
+        float d[kPiece];
+        tmem_ld(quadrant + kColChange + mc + i, d);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) m[i + j] = fmaf(d[j], join, fmaf(m[i + j], decay_factor, m[i + j] * decay_keep));
+        for (int j = 0; j < kPiece; ++j) {
+          if (j < 16 || mc + i + 16 < ny) m[i + j] = fmaf(d[j], join, fmaf(m[i + j], decay_factor, m[i + j] * decay_keep));
+        }
       }
       if (kStateOnly) {
         tc_fence_before();
