@@ -18,14 +18,14 @@
 // (products of y and z alone), joined in order, then all segments at once.
 //
 // Per chunk:
-//   scores P = X Y^T and X M            tcgen05, operands from shared memory, accumulators in TMEM
-//   Y' = weights * Y in place           worker warps, once P has been formed
+//   Y' = weights * Y in place           worker warps
+//   scores P = X Y'^T, X M              tcgen05, operands from shared memory, accumulators in TMEM
 //   M change Z^T Y'                     tcgen05 (transposed, so that a thread owns a row of M^T)
-//   P' = decay * P, rounded             TMEM to registers and back, the next product's A operand
-//   X M scaled by rows, + P' Z          tcgen05, A from TMEM; the workers meanwhile update M in registers
-//   w                                   out by TMA
-// The next chunk's scores are formed as soon as P' has been used.  No barrier joins all warps (but where masks change):
-// each product waits for the warps that prepare its operands, and each warp for the products that it reads.
+//   P' = masked P, rounded              TMEM to registers and back, the next product's A operand
+//   X M + P' Z                          tcgen05, A from TMEM
+//   M in registers, w                   worker warps, while the next chunk's scores are formed
+// Strong decays take the scores of raw rows and weigh every score instead.  No barrier joins all warps (but where masks
+// change): each product waits for the warps that prepare its operands, and each warp for the products that it reads.
 #include <cuda.h>
 
 #include <algorithm>
@@ -41,16 +41,16 @@ namespace lsso {
 namespace {
 
 constexpr int kChunk = 128;
-constexpr int kWorkers = 256, kThreads = kWorkers + 32;
 constexpr uint32_t kBox = kChunk * 128;  // 128 tokens x 64 features of 16 bits
-constexpr uint32_t kOutBox = 32 * 64;    // 32 tokens x 32 features
 constexpr float kLog2e = 1.44269504f;
 constexpr float kLeastLog = -1e4f;       // e^-1e4 is zero, and ranks times it are finite
 
 struct ScanMaps {
-  CUtensorMap x, y, z, w;
+  CUtensorMap x, y, z;
 };
 struct ScanPass {
+  TokenTensor w;
+  int wide;               // w's rows start on 32 bytes
   const float* state_in;  // nullable; per sample and head [key][value], of the segment where there are several
   float* state_out;       // nullable; likewise
   int ny, nz;             // widths of x and y, and of z and w
@@ -72,16 +72,18 @@ struct ScanArgs {
 
 struct ScanShared {
   float from[kChunk], col[kChunk];
-  float state_scale[2][kChunk];
-  uint8_t row_top[2][kChunk], state_top[2 * kChunk];  // FP16: largest exponents of score rows and of state rows
-  // full: a stage has landed.  scores, xm, change, out: products done.  weighed, decayed, taken: all warps have written
-  // Y', written P' (and the state's part, scaled), read the products and written the next state; freed: stored (one stage).
-  uint64_t full[2], scores, xm, change, out, weighed, decayed, taken, freed, drain;
+  uint8_t row_top[4 * kChunk], state_top[4 * kChunk];  // FP16: largest exponents of score rows and of state rows
+  uint8_t state_exponent[2][kChunk];                   // FP16: of the state rows as the product has them
+  // full: a stage has landed.  scores, xm, change, out: products done.  weighed, decayed, taken: all workers have written
+  // Y', written P' (and scaled the state's part), and read the products of a chunk and written the next one's state.
+  uint64_t full[2], scores, xm, change, out, weighed, decayed, taken, drain;
   uint32_t tmem;
   int abort_flag;
 };
 
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[16]) { tmem_ld16(taddr, v); }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[8]) { tmem_st8(taddr, r); }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -107,6 +109,11 @@ __device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, ScanShar
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, ScanShared& sh, int* status) {
   return __all_sync(0xffffffffu, wait_one(bar, parity, sh, status));
 }
+__device__ __forceinline__ void store_32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -120,7 +127,7 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
 struct PowerScale {
   float up, down;
   __device__ __forceinline__ explicit PowerScale(uint32_t e) : up(1.0f), down(1.0f) {
-    if (e < 255) {
+    if (e < 255) {  // infinities and NaN as they are
       const uint32_t c = max(e, 15u);
       up = __uint_as_float((268 - c) << 23);
       down = __uint_as_float((c - 14) << 23);
@@ -159,18 +166,26 @@ struct ChunkRanks {
 };
 
 // kKB, kVB: 64-feature boxes of x and y, and of z and w.  kStateOnly: the states of segments, no outputs.
-// Warps 0-7 weigh, decay, hold the state and write; one thread of warp 8 issues loads and products.
+// The worker warps weigh, decay, hold the state and write; the warp after them issues loads and products.  With single
+// boxes eight workers and two CTAs per SM, else sixteen and one.
+template <int kKB, int kVB>
+constexpr int kWorkerWarps = kKB + kVB == 2 ? 8 : 16;
+
 template <bool kHalf, int kKB, int kVB, bool kStateOnly>
-__global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_kernel(const __grid_constant__ ScanArgs a) {
+__global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB> + 32, kKB + kVB == 2 ? 2 : 1)
+    decay_scan_kernel(const __grid_constant__ ScanArgs a) {
   constexpr bool kSmall = kKB + kVB == 2;
+  constexpr int kWarps = kWorkerWarps<kKB, kVB>, kWorkers = 32 * kWarps;
+  constexpr int kGroups = kWarps / 4;              // workers of a lane quadrant
+  constexpr int kBlocks = 4 / kGroups;             // of 32 score columns, per worker
   // TMEM columns: scores (P' of a block of 32 tokens takes the first half of the block's columns, so that no warp
   // overwrites what another still reads), the state's part and then the output, the state's change.  Single boxes leave
   // room for a second CTA.
   constexpr uint32_t kColP = 0, kColOut = 128, kColChange = kStateOnly ? 0 : kSmall ? 192 : 256;
   constexpr uint32_t kCols = kStateOnly ? 64 * kKB : kSmall ? 256 : 512;
-  constexpr int kParts = kVB == 1 ? 4 : 2;  // threads that share a row of M^T (one lane quadrant or two hold it)
-  constexpr int kOwn = 64 * kKB / kParts;   // its columns held by one thread
-  constexpr int kPiece = kOwn > 16 ? 32 : 16;  // of them per TMEM load
+  constexpr int kParts = kVB == 1 ? 2 * kGroups : kGroups;  // threads that share a row of M^T (two quadrants or one hold it)
+  constexpr int kOwn = 64 * kKB / kParts;                   // its columns held by one thread: 16 or 32
+  constexpr int kPiece = kOwn == 16 ? 32 : 16;              // score and output columns at a time, as registers allow
   constexpr uint32_t kXBytes = kStateOnly ? 0 : kKB * kBox;
   constexpr uint32_t kStage = kXBytes + kKB * kBox + kVB * kBox;
   constexpr uint32_t kStateBox = kVB * 64 * 128;
@@ -185,18 +200,16 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   const bool reverse = p.reverse != 0, exact = p.exact != 0;
   const int first = segment * a.segment_chunks, count = min(a.segment_chunks, a.chunks - first);
   const int ny = p.ny, nz = p.nz, stages = a.stages;
-  uint8_t* const state_tile = smem + stages * kStage;                                // M^T: [kKB][64 kVB rows][128 bytes]
-  uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kStateBox);            // exact: the smaller parts of weighted rows
+  uint8_t* const state_tile = smem + stages * kStage;                      // M^T: [kKB][64 kVB rows][128 bytes]
+  uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kStateBox);  // exact: the smaller parts of weighted rows
   const uint32_t base = smem_u32(smem), full_bar = smem_u32(sh.full);
   const uint32_t scores_bar = smem_u32(&sh.scores), xm_bar = smem_u32(&sh.xm), change_bar = smem_u32(&sh.change),
                  out_bar = smem_u32(&sh.out), weighed_bar = smem_u32(&sh.weighed), decayed_bar = smem_u32(&sh.decayed),
-                 taken_bar = smem_u32(&sh.taken), freed_bar = smem_u32(&sh.freed);
+                 taken_bar = smem_u32(&sh.taken);
 
   if (tid == 0) {
-    mbar_init(full_bar, 1);
-    mbar_init(full_bar + 8, 1);
-    for (uint32_t bar : {scores_bar, xm_bar, change_bar, out_bar, smem_u32(&sh.drain)}) mbar_init(bar, 1);
-    for (uint32_t bar : {weighed_bar, decayed_bar, taken_bar, freed_bar}) mbar_init(bar, kWorkers / 32);
+    for (uint32_t bar : {full_bar, full_bar + 8, scores_bar, xm_bar, change_bar, out_bar, smem_u32(&sh.drain)}) mbar_init(bar, 1);
+    for (uint32_t bar : {weighed_bar, decayed_bar, taken_bar}) mbar_init(bar, kWarps);
     sh.abort_flag = 0;
     fence_mbar_init();
   }
@@ -226,16 +239,16 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   // scores of raw rows and weigh every score.
   const bool plain = l2 * 127.0f > (kHalf ? -4.0f : -96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
-  const int q = warp & 3, hf = (warp >> 2) & 1;
+  const int q = warp & 3, group = warp >> 2;
   // this thread's part of M^T: row mv, columns [mc, mc + kOwn)
   const int mv = kVB == 1 ? 32 * (q & 1) + lane : 32 * q + lane;
-  const int part = kVB == 1 ? (q >> 1) + 2 * hf : hf;
+  const int part = kVB == 1 ? (q >> 1) + 2 * group : group;
   const int mc = part * kOwn;
   float m[kOwn];
   float kappa = 1.0f;
-  // M^T as the next product's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
-  auto write_state = [&](int parity) {
-    float up = 1.0f;
+  // M^T as chunk n's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
+  auto write_state = [&](int n) {
+    float up = kappa;
     if (kHalf) {
       float most = 0.0f;
 #pragma unroll
@@ -245,19 +258,15 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       named_barrier(kVB == 1 ? 5 + (q & 1) : 1 + q, 32 * kParts);
 #pragma unroll
       for (int i = 0; i < kParts; ++i) e = max(e, static_cast<uint32_t>(sh.state_top[i * (64 * kVB) + mv]));
-      const PowerScale s(e);
-      up = s.up;
-      if (part == 0) sh.state_scale[parity][mv] = s.down * kappa;
-    } else {
-      up = kappa;
+      up = PowerScale(e).up;
+      if (part == 0) sh.state_exponent[n & 1][mv] = static_cast<uint8_t>(e);
     }
 #pragma unroll
     for (int i = 0; i < kOwn; i += 8) {
       const int c = mc + i, box = c >> 6, piece = (c >> 3) & 7;
       uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = pack2<kHalf>(m[i + 2 * j] * up, m[i + 2 * j + 1] * up);
+      for (int j = 0; j < 4; ++j) w[j] = pack2<kHalf>(m[i + 2 * j] * up, m[i + 2 * j + 1] * up);
       *reinterpret_cast<uint4*>(state_tile + box * kStateBox + mv * 128 + ((piece ^ (mv & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   };
@@ -272,7 +281,8 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     for (int w = 0; w < 4; ++w)
       if (t0 + 32 * w < a.length && of_sample[t0 + 32 * w] != 0) ahead |= 1u << w;
   };
-  float lambda = 0.0f /* factor of the state's part of this row; plain: of the whole row */, block_factor[2] = {0.0f, 0.0f};
+  float lambda = 0.0f;  // factor of the state's part of this row; plain: of the whole row
+  float block_factor[kBlocks];
   bool live = false, dead_tokens = false, was_whole = false;
   float decay_factor = 0.0f, decay_keep = 0.0f;  // M' = M * factor + M * keep (keep is 0 or 1)
   int decay_total = -1;
@@ -299,28 +309,27 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     const int rho = ranks.rho(q, lane, reverse);
     const float row_rho = static_cast<float>(rho);
     if (n > 0) named_barrier(7, kWorkers);  // the tables have been read
-    if (hf == 0) {
+    if (group == 0) {
       sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : 0.0f;
-    } else if (!kStateOnly && !plain) {
+    } else if (group == 1 && !kStateOnly && !plain) {
       sh.col[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.last_rho(q, reverse) - rho)) : 0.0f;
     }
     if (n > 0) named_barrier(7, kWorkers);
     if (!kStateOnly) {
-      lambda = plain ? inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.total - 1))) : p.into * exp2f(l2 * (row_rho + 1.0f - late));
-      if (plain) kappa = exp2f(l2 * (static_cast<float>(ranks.total) - late)) / p.from;
+      if (plain) {
+        lambda = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.total - 1)));
+        kappa = exp2f(l2 * (static_cast<float>(ranks.total) - late)) / p.from;
+      } else {
+        lambda = p.into * exp2f(l2 * (row_rho + 1.0f - late));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(hf + 2 * i, reverse))));
-    }
-    if (ranks.total != decay_total) {
-      decay_total = ranks.total;
-      const Decay d(l * static_cast<float>(decay_total));
-      decay_factor = d.factor;
-      decay_keep = d.near_one ? 1.0f : 0.0f;
+        for (int i = 0; i < kBlocks; ++i)
+          block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(group + kGroups * i, reverse))));
+      }
     }
   };
 
   int tokens_seen = 0;
-  if (warp < kWorkers / 32) {
+  if (warp < kWarps) {
     const bool transposed = p.transposed != 0;
     const float* src = p.state_in == nullptr || kStateOnly
                            ? nullptr
@@ -333,7 +342,6 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
     }
     fetch_mask(0);
     prepare(0);
-    tokens_seen = ranks.total;
     if (!kStateOnly) write_state(0);
     fence_proxy_async();
   }
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
   const uint32_t tmem = sh.tmem;
   bool ok = true;
 
-  if (warp == kWorkers / 32) {
+  if (warp == kWarps) {
     // ---------------- loads and products: the warp walks them together, one lane issues
     const bool leader = elect_leader();
     int loaded = 0;
@@ -380,31 +388,27 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
                    // one box of z: lanes 64-127 repeat 0-63
                    z_lanes = make_desc_sw128(base + kXBytes + kKB * kBox, kVB == 2 ? kBox : 0, 1024),
                    z_rows = make_desc_sw128(base + kXBytes + kKB * kBox, kBox, 1024);
-    auto scores = [&](int n) {
-      const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
-      const uint64_t xd = x0 + at, yd = y0 + at;
-#pragma unroll
-      for (int k = 0; k < 4 * kKB; ++k) {
-        const int step = (k >> 2) * (kBox / 16) + (k & 3) * 2;
-        if (k < y_steps) mma_led(leader, tmem + kColP, xd + step, yd + step, i_scores, k > 0);
-      }
-      mma_led_commit(leader, scores_bar);
-    };
     for (int n = 0; n < count; ++n) {
       const uint32_t parity = n & 1;
       const uint64_t at = static_cast<uint64_t>(stage_of(n) * (kStage / 16));
+      const uint64_t xd = x0 + at;
+      if (n > 0) {
+        // the chunk before is done with its stage and its scores
+        if (!wait(kStateOnly ? change_bar : out_bar, parity ^ 1)) break;
+        if (loaded < count) load();
+      }
       if (!kStateOnly) {
-        if (plain) {
-          // scores of weighted rows, once the chunk before has used its own
-          if (n > 0 && !wait(out_bar, parity ^ 1)) break;
-          if (!wait(weighed_bar, parity)) break;
-          scores(n);
-        } else if (n == 0) {
-          if (!wait(full_bar, 0)) break;
-          scores(0);
+        if (!(plain ? wait(weighed_bar, parity) : wait(full_bar + 8 * stage_of(n), full_parity(n)))) break;
+        const uint64_t yd = y0 + at;
+#pragma unroll
+        for (int k = 0; k < 4 * kKB; ++k) {
+          const int step = (k >> 2) * (kBox / 16) + (k & 3) * 2;
+          if (k < y_steps) mma_led(leader, tmem + kColP, xd + step, yd + step, i_scores, k > 0);
         }
-        if (n > 0 && !wait(taken_bar, parity ^ 1)) break;
-        const uint64_t xd = x0 + at;
+        mma_led_commit(leader, scores_bar);
+      }
+      if (n > 0 && !wait(taken_bar, parity ^ 1)) break;
+      if (!kStateOnly) {
 #pragma unroll
         for (int k = 0; k < 4 * kKB; ++k) {
           if (k < y_steps) {
@@ -415,7 +419,6 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         mma_led_commit(leader, xm_bar);
       }
       if ((kStateOnly || !plain) && !wait(weighed_bar, parity)) break;
-      if (kStateOnly && n > 0 && !wait(taken_bar, parity ^ 1)) break;
       const uint64_t zd = z_lanes + at, yd = y_rows + at;
       if (exact) {  // the smaller parts first
 #pragma unroll 1
@@ -434,32 +437,13 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
 #pragma unroll
       for (int k = 1; k < kChunk / 16; ++k) mma_led(leader, tmem + kColChange, zd + k * 128, yd + k * 128, i_change, 1);
       mma_led_commit(leader, change_bar);
-      if (kStateOnly) {
-        if (loaded < count) {
-          if (!wait(change_bar, parity)) break;
-          load();
-        }
-        continue;
-      }
-      // every warp's stores of the chunk before have left its stage
-      if (stages == 2 && n > 0 && loaded < count) load();
+      if (kStateOnly) continue;
       if (!wait(decayed_bar, parity)) break;
       const uint64_t zr = z_rows + at;
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k)
         mma_led_tmem_a(leader, tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), zr + k * 128, i_out, 1);
       mma_led_commit(leader, out_bar);
-      if (n + 1 < count) {
-        if (stages == 1) {
-          if (!wait(freed_bar, parity)) break;
-          load();
-        }
-        // the next scores as soon as these have been used
-        if (!plain) {
-          if (!wait(out_bar, parity) || !wait(full_bar + 8 * stage_of(n + 1), full_parity(n + 1))) break;
-          scores(n + 1);
-        }
-      }
     }
     // nothing may be in flight when the CTA ends
     if (leader) {
@@ -482,12 +466,72 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
+    // what the products of chunk n - 1 left to do while those of chunk n run: its state, its output
+    float row_out = 0.0f;
+    bool row_live = false;
+    auto take = [&](int n, bool more) {
+      wait(change_bar, (n - 1) & 1);
+#pragma unroll
+      for (int i = 0; i < kOwn; i += 16) {
+        if (mc + i >= ny) break;  // no product wrote these columns
+        float d[16];
+        tmem_ld16(quadrant + kColChange + mc + i, d);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) m[i + j] = fmaf(d[j], join, fmaf(m[i + j], decay_factor, m[i + j] * decay_keep));
+      }
+      if (!kStateOnly && more) {
+        write_state(n);
+        fence_proxy_async();
+      }
+      if (kStateOnly) {
+        tc_fence_before();
+        arrive(taken_bar);
+        return;
+      }
+      wait(out_bar, (n - 1) & 1);
+      const int col0 = 32 * group, t = chunk_at(n - 1) * kChunk + 32 * q + lane;
+      uint32_t w[16];
+      if (col0 < nz) {
+#pragma unroll
+        for (int i = 0; i < 32; i += kPiece) {
+          float o[kPiece];
+          tmem_ld(quadrant + kColOut + col0 + i, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < kPiece / 2; ++j) {
+            w[i / 2 + j] = pack2<kHalf>(o[2 * j] * row_out, o[2 * j + 1] * row_out);
+            w[i / 2 + j] = row_live ? w[i / 2 + j] : 0u;
+          }
+        }
+      }
+      tc_fence_before();
+      arrive(taken_bar);
+      if (col0 < nz && ok && t < a.length) {
+        uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(p.w.ptr)) + sample * p.w.stride_batch +
+                        t * p.w.stride_token + head * p.w.stride_head + col0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (p.wide && col0 + 16 * c + 16 <= nz) {
+            store_32(dst + 16 * c, &w[8 * c]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (col0 + 16 * c + 8 * h < nz)
+                *reinterpret_cast<uint4*>(dst + 16 * c + 8 * h) =
+                    make_uint4(w[8 * c + 4 * h], w[8 * c + 4 * h + 1], w[8 * c + 4 * h + 2], w[8 * c + 4 * h + 3]);
+          }
+        }
+      }
+    };
     for (int n = 0; n < count; ++n) {
       const uint32_t parity = n & 1;
       uint8_t* const y_tile = smem + stage_of(n) * kStage + kXBytes;
       uint8_t* const z_tile = y_tile + kKB * kBox;
       if (n + 1 < count) fetch_mask(n + 1);
+      tokens_seen += ranks.total;
       if (!kStateOnly && !plain) wait(scores_bar, parity);  // y's rows have been read
+      if (exact && n > 0) wait(change_bar, parity ^ 1);     // the small parts have been, too
       wait(full_bar + 8 * stage_of(n), full_parity(n));
 
       // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
@@ -543,176 +587,116 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
         }
       }
       fence_proxy_async();
-      if (!kStateOnly && stages == 2 && lane == 0) bulk_wait_read<0>();  // the stage of the chunk before is free
       arrive(weighed_bar);
+      if (n > 0) take(n, true);
+      if (ranks.total != decay_total) {  // of this chunk, for its state
+        decay_total = ranks.total;
+        const Decay d(l * static_cast<float>(decay_total));
+        decay_factor = d.factor;
+        decay_keep = d.near_one ? 1.0f : 0.0f;
+      }
 
       float down = 1.0f;
       if (!kStateOnly) {
-        // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns hf and hf + 2, sixteen columns
-        // at a time (a short loop: the chunk's code has to stay close to the instruction cache).  FP16 goes over them
-        // twice, first for the largest of a row.
+        // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns (a short loop: the chunk's code has
+        // to stay close to the instruction cache).  FP16 goes over them twice, first for the largest of a row.
+        constexpr int kPieces = kBlocks * 32 / kPiece;
         float up = 1.0f, most = 0.0f;
         if (plain) wait(scores_bar, parity);
 #pragma unroll 1
-        for (int it = kHalf ? -4 : 0; it < 4; ++it) {
-          const int block = hf + (it & 2), half = 16 * (it & 1), col0 = 32 * block + half;
+        for (int it = kHalf ? -kPieces : 0; it < kPieces; ++it) {
+          const int i = (it & (kPieces - 1)) * kPiece / 32, half = ((it & (kPieces - 1)) * kPiece) & 31;
+          const int block = group + kGroups * i;
           const uint32_t whole = plain ? 0xffffffffu : ranks.word(block);  // plain: masked rows of y are zero
           // this row's columns: all before its block, those up to its own in it (from it on), valid ones
           const bool on_diagonal = block == q;
           const uint32_t seen = on_diagonal ? whole & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane))
                                             : (reverse ? block > q : block < q) ? whole : 0u;
-          float v[16];
+          float v[kPiece];
           if (!on_diagonal && seen == 0u) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+            for (int j = 0; j < kPiece; ++j) v[j] = 0.0f;
           } else {
-            tmem_ld16(quadrant + kColP + col0, v);
+            tmem_ld(quadrant + kColP + 32 * block + half, v);
             tmem_ld_wait();
-            const float f = (it & 2) ? block_factor[1] : block_factor[0];
-            const float4* col = reinterpret_cast<const float4*>(sh.col + col0);
-            if (plain) {
-            } else if (gentle || !on_diagonal) {
+            if (!plain) {
+              const float f = kBlocks > 1 && i == 1 ? block_factor[kBlocks - 1] : block_factor[0];
+              const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block + half);
+              if (gentle || !on_diagonal) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 c = col[j / 4];
-                v[j] *= f * c.x;
-                v[j + 1] *= f * c.y;
-                v[j + 2] *= f * c.z;
-                v[j + 3] *= f * c.w;
-              }
-            } else {
+                for (int j = 0; j < kPiece; j += 4) {
+                  const float4 c = col[j / 4];
+                  v[j] *= f * c.x;
+                  v[j + 1] *= f * c.y;
+                  v[j + 2] *= f * c.z;
+                  v[j + 3] *= f * c.w;
+                }
+              } else {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                // rank distance: valid tokens seen by the row that lie on its side of token half + j
-                const uint32_t side = reverse ? (1u << (half + j)) - 1u : ~(0xffffffffu >> (31 - (half + j)));
-                v[j] *= inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)));
+                for (int j = 0; j < kPiece; ++j) {
+                  // rank distance: valid tokens seen by the row that lie on its side of token half + j
+                  const uint32_t side = reverse ? (1u << (half + j)) - 1u : ~(0xffffffffu >> (31 - half - j));
+                  v[j] *= inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)));
+                }
               }
             }
             if (on_diagonal || seen != 0xffffffffu) {
               const uint32_t bits = seen >> half;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.0f;
+              for (int j = 0; j < kPiece; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.0f;
             }
           }
           if (kHalf && it < 0) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[j]));
+            for (int j = 0; j < kPiece; ++j) most = fmaxf(most, fabsf(v[j]));
             if (it == -1) {
-              const uint32_t top = __float_as_uint(most) >> 23;
-              sh.row_top[hf][32 * q + lane] = static_cast<uint8_t>(top);
-              named_barrier(1 + q, 64);
-              const PowerScale sc(max(top, static_cast<uint32_t>(sh.row_top[hf ^ 1][32 * q + lane])));
+              sh.row_top[group * kChunk + 32 * q + lane] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
+              named_barrier(1 + q, 32 * kGroups);
+              uint32_t e = 0;
+#pragma unroll
+              for (int g = 0; g < kGroups; ++g) e = max(e, static_cast<uint32_t>(sh.row_top[g * kChunk + 32 * q + lane]));
+              const PowerScale sc(e);
               up = sc.up;
               down = sc.down;
             }
             continue;
           }
-          uint32_t w[8];
+          uint32_t w[kPiece / 2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
-          tmem_st8(quadrant + kColP + 32 * block + half / 2, w);
+          for (int j = 0; j < kPiece / 2; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
+          tmem_st(quadrant + kColP + 32 * block + half / 2, w);
         }
-        // ---- the state's part, which P' Z is added to, by the row's factor (plain chunks have it in M already, and FP16
-        // that of its rows)
+        // ---- the state's part, which P' Z is added to, by the row's factor (plain chunks have it in M already) and, in
+        // FP16, those of P' and of M's rows
         if (kHalf || !plain) {
-        wait(xm_bar, parity);
-        const float row_factor = plain ? up : lambda * up;
+          wait(xm_bar, parity);
+          const float row_factor = plain ? up * kappa : lambda * up;
 #pragma unroll 1
-        for (int b = 0; b < 2 * kVB; ++b) {
-          const int col0 = 32 * (hf + (b & 2)) + 16 * (b & 1);
-          if (col0 >= nz) continue;
-          float x[16];
-          tmem_ld16(quadrant + kColOut + col0, x);
-          tmem_ld_wait();
-          uint32_t w[16];
-          const float4* scale = reinterpret_cast<const float4*>(sh.state_scale[parity] + col0);
+          for (int c = 0; c < 2; ++c) {
+            const int col0 = 32 * group + 16 * c;
+            if (col0 >= nz) break;
+            float x[16];
+            tmem_ld16(quadrant + kColOut + col0, x);
+            tmem_ld_wait();
+            uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            float4 f = make_float4(row_factor, row_factor, row_factor, row_factor);
-            if (kHalf) {
-              const float4 c = scale[j / 4];
-              f = make_float4(row_factor * c.x, row_factor * c.y, row_factor * c.z, row_factor * c.w);
+            for (int j = 0; j < 16; ++j) {
+              float f = row_factor;
+              if (kHalf) f *= PowerScale(sh.state_exponent[parity][col0 + j]).down;
+              w[j] = __float_as_uint(x[j] * f);
             }
-            w[j] = __float_as_uint(x[j] * f.x);
-            w[j + 1] = __float_as_uint(x[j + 1] * f.y);
-            w[j + 2] = __float_as_uint(x[j + 2] * f.z);
-            w[j + 3] = __float_as_uint(x[j + 3] * f.w);
+            tmem_st16(quadrant + kColOut + col0, w);
           }
-          tmem_st16(quadrant + kColOut + col0, w);
-        }
         }
         tmem_st_wait();
         tc_fence_before();
         arrive(decayed_bar);
       }
-
-      // ---- the state after this chunk
-      wait(change_bar, parity);
-#pragma unroll
-      for (int i = 0; i < kOwn; i += kPiece) {
-        if (mc + i >= ny) break;  // no product wrote these columns (or those of a piece's second half, which are unused)
-        float d[kPiece];
-        tmem_ld(quadrant + kColChange + mc + i, d);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < kPiece; ++j) {
-          if (j < 16 || mc + i + 16 < ny) m[i + j] = fmaf(d[j], join, fmaf(m[i + j], decay_factor, m[i + j] * decay_keep));
-        }
-      }
-      if (kStateOnly) {
-        tc_fence_before();
-        arrive(taken_bar);
-        if (n + 1 < count) {
-          prepare(n + 1);
-          tokens_seen += ranks.total;
-        }
-        continue;
-      }
-      const float row_out = plain ? lambda * down : down;
-      const bool row_live = live;
-      if (n + 1 < count) {
-        prepare(n + 1);
-        write_state(parity ^ 1);
-      }
-      fence_proxy_async();
-
-      // ---- outputs
-      wait(out_bar, parity);
-      // z's boxes have been read: the output boxes (32 x 32, 64-byte rows and swizzle) leave from there
-      uint8_t* const boxes = z_tile + warp * kVB * kOutBox;
-#pragma unroll 1
-      for (int b = 0; b < 2 * kVB; ++b) {
-        const int col0 = 32 * (hf + (b & 2)) + 16 * (b & 1);
-        if (col0 >= nz) continue;
-        float o[16];
-        tmem_ld16(quadrant + kColOut + col0, o);
-        tmem_ld_wait();
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          w[j] = pack2<kHalf>(o[2 * j] * row_out, o[2 * j + 1] * row_out);
-          w[j] = row_live ? w[j] : 0u;
-        }
-        uint8_t* row = boxes + (b >> 1) * kOutBox + lane * 64;
-        const int piece = 2 * (b & 1), turn = (lane >> 1) & 3;
-        *reinterpret_cast<uint4*>(row + ((piece ^ turn) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4*>(row + (((piece + 1) ^ turn) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-      fence_proxy_async();
-      tc_fence_before();
-      arrive(taken_bar);
-      const int t0 = chunk_at(n) * kChunk + 32 * q;
-      if (lane == 0 && ok && t0 < a.length) {
-#pragma unroll
-        for (int b = 0; b < kVB; ++b)
-          if (32 * (hf + 2 * b) < nz) tma_store_4d(&maps.w, smem_u32(boxes + b * kOutBox), 32 * (hf + 2 * b), head, t0, sample);
-      }
-      if (lane == 0) bulk_commit();
-      if (stages == 1) {
-        if (lane == 0) bulk_wait_read<0>();
-        arrive(freed_bar);
-      }
+      row_out = plain ? lambda * down : down;
+      row_live = live;
+      if (n + 1 < count) prepare(n + 1);
     }
+    take(count, false);
     if (ok && p.state_out != nullptr && mv < nz) {
       // a whole scan's state is the caller's; a segment's belongs to its segment
       const bool end = reverse ? segment == 0 : segment == a.segments - 1;
@@ -724,7 +708,6 @@ __global__ void __launch_bounds__(kThreads, kKB + kVB == 2 ? 2 : 1) decay_scan_k
       }
     }
     if (kStateOnly && tid == 0 && pass_index == 0) a.counts[item * a.segments + segment] = tokens_seen;
-    if (!kStateOnly && lane == 0) bulk_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -745,37 +728,49 @@ struct JoinArgs {
   int heads, segments, values;
 };
 
-// M before each segment from the segments' own parts, in scan order: a short chain of multiply-adds per element, its
-// loads in flight ahead of it.
-__global__ void __launch_bounds__(256) decay_join_kernel(const JoinArgs a) {
+constexpr int kJoinThreads = 128, kJoinAhead = 16, kMostSegments = 512;
+
+// M before each segment from the segments' own parts, in scan order: a chain of multiply-adds per element, its loads in
+// flight ahead of it.
+__global__ void __launch_bounds__(kJoinThreads) decay_join_kernel(const JoinArgs a) {
+  __shared__ float factor[kMostSegments], keep[kMostSegments];
   pdl_wait();
   const JoinSet& set = a.set[blockIdx.z];
-  const int item = blockIdx.x, e = (blockIdx.y * 256 + threadIdx.x) * 4;
-  if (e >= a.values) return;
+  const int item = blockIdx.x, e = blockIdx.y * kJoinThreads + threadIdx.x;
   float l = a.log_decay[item % a.heads];
   if (l < kLeastLog) l = kLeastLog;
-  float4* at = reinterpret_cast<float4*>(set.states + static_cast<int64_t>(item) * a.segments * a.values + e);
-  const int step = a.values / 4;
-  float4 m = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (set.initial != nullptr) m = *reinterpret_cast<const float4*>(set.initial + static_cast<int64_t>(item) * a.values + e);
-  constexpr int kAhead = 8;
-  for (int n0 = 0; n0 < a.segments; n0 += kAhead) {
-    float4 own[kAhead];
+  for (int s = threadIdx.x; s < a.segments; s += kJoinThreads) {
+    const Decay d(l * static_cast<float>(a.counts[item * a.segments + s]));
+    factor[s] = d.factor;
+    keep[s] = d.near_one ? 1.0f : 0.0f;
+  }
+  __syncthreads();
+  if (e >= a.values) return;
+  float* at = set.states + static_cast<int64_t>(item) * a.segments * a.values + e;
+  float m = set.initial != nullptr ? set.initial[static_cast<int64_t>(item) * a.values + e] : 0.0f;
+  for (int n0 = 0; n0 < a.segments; n0 += kJoinAhead) {
+    float own[kJoinAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kJoinAhead; ++i) {
       const int n = n0 + i;
-      if (n < a.segments) own[i] = at[static_cast<int64_t>(set.reverse ? a.segments - 1 - n : n) * step];
+      if (n < a.segments) own[i] = at[static_cast<int64_t>(set.reverse ? a.segments - 1 - n : n) * a.values];
     }
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kJoinAhead; ++i) {
       const int n = n0 + i;
       if (n >= a.segments) break;
-      const int seg = set.reverse ? a.segments - 1 - n : n;
-      at[static_cast<int64_t>(seg) * step] = m;
-      const Decay d(l * static_cast<float>(a.counts[item * a.segments + seg]));
-      m = make_float4(d.apply(m.x) + own[i].x, d.apply(m.y) + own[i].y, d.apply(m.z) + own[i].z, d.apply(m.w) + own[i].w);
+      const int s = set.reverse ? a.segments - 1 - n : n;
+      at[static_cast<int64_t>(s) * a.values] = m;
+      m = fmaf(m, factor[s], m * keep[s]) + own[i];
     }
   }
+}
+
+cudaError_t launch_join(const JoinArgs& j, int64_t items, int sets, cudaStream_t stream) {
+  LaunchScope scope("decay_join", stream);
+  launch_pdl(&decay_join_kernel, dim3(static_cast<unsigned>(items), (j.values + kJoinThreads - 1) / kJoinThreads, sets),
+             kJoinThreads, 0, stream, j);
+  return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------- plans and launches
@@ -791,7 +786,7 @@ DecayPlan make_plan(int64_t batch, int64_t length, int heads, int key, int value
   const int per_sm = key <= 64 && value <= 64 ? 2 : 1;
   const int64_t room = static_cast<int64_t>(per_sm) * sm_count / units;  // segments that fit in one wave
   p.segments = 1;
-  if (room > 1 && p.chunks >= 8) p.segments = static_cast<int>(std::min<int64_t>(room, p.chunks / 2));
+  if (room > 1 && p.chunks >= 8) p.segments = static_cast<int>(std::min<int64_t>({room, p.chunks / 2, kMostSegments}));
   p.segment_chunks = (p.chunks + p.segments - 1) / p.segments;
   p.segments = (p.chunks + p.segment_chunks - 1) / p.segment_chunks;
   p.total = 16;
@@ -804,22 +799,20 @@ DecayPlan make_plan(int64_t batch, int64_t length, int heads, int key, int value
   return p;
 }
 
-// Tensor map of [batch, length, heads, width] by strides: boxes of 128 tokens x 64 features (loads, 128-byte swizzle;
-// what lies outside reads as zero) or of 32 x 32 (stores, 64-byte swizzle; what lies outside is not written).
-bool encode(CUtensorMap* map, const TokenTensor& t, const DecayCall& c, int width, bool store) {
+// Tensor map of [batch, length, heads, width] by strides: boxes of 128 tokens x 64 features, 128-byte swizzle; what lies
+// outside reads as zero.
+bool encode(CUtensorMap* map, const TokenTensor& t, const DecayCall& c, int width) {
   PFN_cuTensorMapEncodeTiled_v12000 fn = tensor_map_encoder();
   if (fn == nullptr) return false;
   cuuint64_t dims[4] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(c.heads), static_cast<cuuint64_t>(c.length),
                         static_cast<cuuint64_t>(c.batch)};
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.stride_head) * 2, static_cast<cuuint64_t>(t.stride_token) * 2,
                            static_cast<cuuint64_t>(t.stride_batch) * 2};
-  cuuint32_t box[4] = {store ? 32u : 64u, 1u, store ? 32u : static_cast<cuuint32_t>(kChunk), 1u};
+  cuuint32_t box[4] = {64u, 1u, static_cast<cuuint32_t>(kChunk), 1u};
   cuuint32_t ones[4] = {1, 1, 1, 1};
   return fn(map, c.type == kFp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
             const_cast<void*>(t.ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-            store ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 ScanArgs common(const DecayCall& c, const DecayPlan& p, uint8_t* workspace) {
@@ -852,7 +845,7 @@ cudaError_t launch_one(ScanArgs& a, int64_t items, const char* name, cudaStream_
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   LaunchScope scope(name, stream);
-  launch_pdl(kernel, dim3(static_cast<unsigned>(items * a.segments * a.passes)), kThreads, smem, stream, a);
+  launch_pdl(kernel, dim3(static_cast<unsigned>(items * a.segments * a.passes)), 32 * kWorkerWarps<kKB, kVB> + 32, smem, stream, a);
   return cudaGetLastError();
 }
 
@@ -868,12 +861,17 @@ cudaError_t launch_scans(ScanArgs& a, int64_t items, int type, int ny, int nz, c
   return half ? launch_one<true, 2, 2, kStateOnly>(a, items, name, stream) : launch_one<false, 2, 2, kStateOnly>(a, items, name, stream);
 }
 
-struct ScanTensors {
-  const TokenTensor *x, *y, *z, *w;
-};
-bool encode_pass(ScanMaps* m, const ScanTensors& t, const DecayCall& c, int ny, int nz) {
-  if (t.x != nullptr && !(encode(&m->x, *t.x, c, ny, false) && encode(&m->w, *t.w, c, nz, true))) return false;
-  return encode(&m->y, *t.y, c, ny, false) && encode(&m->z, *t.z, c, nz, false);
+// A pass over x (null: states only), y and z, and its maps.
+bool set_pass(ScanArgs* a, int i, const DecayCall& c, const TokenTensor* x, const TokenTensor& y, const TokenTensor& z,
+              const TokenTensor* w, const ScanPass& pass) {
+  a->pass[i] = pass;
+  ScanMaps& m = a->maps[i];
+  if (w != nullptr) {
+    a->pass[i].w = *w;
+    a->pass[i].wide = (reinterpret_cast<uintptr_t>(w->ptr) % 32 == 0 &&
+                       (w->stride_batch | w->stride_token | w->stride_head) % 16 == 0) ? 1 : 0;
+  }
+  return (x == nullptr || encode(&m.x, *x, c, pass.ny)) && encode(&m.y, y, c, pass.ny) && encode(&m.z, z, c, pass.nz);
 }
 
 }  // namespace
@@ -889,18 +887,17 @@ cudaError_t launch_decay_forward(const DecayCall& c, uint8_t* workspace, int sm_
   const int exact = c.last != nullptr ? 1 : 0;
   float* states = reinterpret_cast<float*>(workspace);
   a.passes = 1;
-  a.pass[0] = ScanPass{nullptr, states, c.key, c.value, 0, 0, exact, 1.0f, 1.0f};
-  if (!encode_pass(&a.maps[0], ScanTensors{&c.q, &c.k, &c.v, &c.y}, c, c.key, c.value)) return cudaErrorInvalidValue;
+  const ScanPass pass{{}, 0, p.segments > 1 ? states : c.state, c.last, c.key, c.value, 0, 0, exact, c.scale, 1.0f};
   if (p.segments > 1) {
+    const ScanPass own{{}, 0, nullptr, states, c.key, c.value, 0, 0, exact, 1.0f, 1.0f};
+    if (!set_pass(&a, 0, c, nullptr, c.k, c.v, nullptr, own)) return cudaErrorInvalidValue;
     cudaError_t e = launch_scans<true>(a, items, c.type, c.key, c.value, "decay_states", stream);
     if (e != cudaSuccess) return e;
-    const JoinArgs j{{JoinSet{states, c.state, 0}, JoinSet{}}, c.log_decay, a.counts, c.heads, p.segments, c.key * c.value};
-    LaunchScope scope("decay_join", stream);
-    launch_pdl(&decay_join_kernel, dim3(static_cast<unsigned>(items), (c.key * c.value + 1023) / 1024, 1), 256, 0, stream, j);
-    e = cudaGetLastError();
+    e = launch_join(JoinArgs{{JoinSet{states, c.state, 0}, JoinSet{}}, c.log_decay, a.counts, c.heads, p.segments, c.key * c.value},
+                    items, 1, stream);
     if (e != cudaSuccess) return e;
   }
-  a.pass[0] = ScanPass{p.segments > 1 ? states : c.state, c.last, c.key, c.value, 0, 0, exact, c.scale, 1.0f};
+  if (!set_pass(&a, 0, c, &c.q, c.k, c.v, &c.y, pass)) return cudaErrorInvalidValue;
   return launch_scans<false>(a, items, c.type, c.key, c.value, "decay", stream);
 }
 
@@ -914,28 +911,24 @@ cudaError_t launch_decay_backward(const DecayCall& c, uint8_t* workspace, int sm
     float* sums[2] = {reinterpret_cast<float*>(workspace), reinterpret_cast<float*>(workspace + p.states[1])};
     ScanArgs a = common(c, p, workspace);
     a.passes = 2;
-    a.pass[0] = ScanPass{nullptr, sums[0], c.key, c.value, 0, 0, 0, 1.0f, 1.0f};
-    a.pass[1] = ScanPass{nullptr, sums[1], c.key, c.value, 0, 1, exact, 1.0f, c.scale};
-    if (!encode_pass(&a.maps[0], ScanTensors{nullptr, &c.k, &c.v, nullptr}, c, c.key, c.value) ||
-        !encode_pass(&a.maps[1], ScanTensors{nullptr, &c.q, &dy, nullptr}, c, c.key, c.value)) {
+    const ScanPass own[2] = {ScanPass{{}, 0, nullptr, sums[0], c.key, c.value, 0, 0, 0, 1.0f, 1.0f},
+                             ScanPass{{}, 0, nullptr, sums[1], c.key, c.value, 0, 1, exact, 1.0f, c.scale}};
+    if (!set_pass(&a, 0, c, nullptr, c.k, c.v, nullptr, own[0]) || !set_pass(&a, 1, c, nullptr, c.q, dy, nullptr, own[1])) {
       return cudaErrorInvalidValue;
     }
     cudaError_t e = launch_scans<true>(a, items, c.type, c.key, c.value, "decay_states", stream);
     if (e != cudaSuccess) return e;
-    const JoinArgs j{{JoinSet{sums[0], c.state, 0}, JoinSet{sums[1], c.dlast, 1}}, c.log_decay, a.counts, c.heads, p.segments,
-                     c.key * c.value};
-    LaunchScope scope("decay_join", stream);
-    launch_pdl(&decay_join_kernel, dim3(static_cast<unsigned>(items), (c.key * c.value + 1023) / 1024, 2), 256, 0, stream, j);
-    e = cudaGetLastError();
+    e = launch_join(JoinArgs{{JoinSet{sums[0], c.state, 0}, JoinSet{sums[1], c.dlast, 1}}, c.log_decay, a.counts, c.heads,
+                             p.segments, c.key * c.value},
+                    items, 2, stream);
     if (e != cudaSuccess) return e;
     before = sums[0];
     after = sums[1];
   }
-  const ScanPass passes[3] = {ScanPass{before, nullptr, c.value, c.key, 1, 0, 0, c.scale, 1.0f},
-                              ScanPass{after, nullptr, c.value, c.key, 1, 1, 0, 1.0f, c.scale},
-                              ScanPass{after, c.dstate, c.key, c.value, 0, 1, exact, 1.0f, c.scale}};
-  const ScanTensors tensors[3] = {ScanTensors{&dy, &c.v, &c.k, &c.dq}, ScanTensors{&c.v, &dy, &c.q, &c.dk},
-                                  ScanTensors{&c.k, &c.q, &dy, &c.dv}};
+  const ScanPass passes[3] = {ScanPass{{}, 0, before, nullptr, c.value, c.key, 1, 0, 0, c.scale, 1.0f},
+                              ScanPass{{}, 0, after, nullptr, c.value, c.key, 1, 1, 0, 1.0f, c.scale},
+                              ScanPass{{}, 0, after, c.dstate, c.key, c.value, 0, 1, exact, 1.0f, c.scale}};
+  const TokenTensor* tensors[3][4] = {{&dy, &c.v, &c.k, &c.dq}, {&c.v, &dy, &c.q, &c.dk}, {&c.k, &c.q, &dy, &c.dv}};
   // All three in one launch where they run the same kernel: those of a sample and head stand side by side and share
   // their inputs in L2.
   const bool same = (c.key <= 64) == (c.value <= 64);
@@ -943,8 +936,8 @@ cudaError_t launch_decay_backward(const DecayCall& c, uint8_t* workspace, int sm
     ScanArgs a = common(c, p, workspace);
     const int last = same ? 3 : first == 0 ? 2 : 3;
     for (int i = first; i < last; ++i) {
-      a.pass[i - first] = passes[i];
-      if (!encode_pass(&a.maps[i - first], tensors[i], c, passes[i].ny, passes[i].nz)) return cudaErrorInvalidValue;
+      const TokenTensor* const* t = tensors[i];
+      if (!set_pass(&a, i - first, c, t[0], *t[1], *t[2], t[3], passes[i])) return cudaErrorInvalidValue;
     }
     a.passes = last - first;
     const cudaError_t e = launch_scans<false>(a, items, c.type, passes[first].ny, passes[first].nz, "decay_bwd", stream);
