@@ -190,12 +190,15 @@ struct ChunkRanks {
 // With single boxes eight warps and two CTAs per SM, else sixteen and one.
 template <int kKB, int kVB>
 constexpr int kWorkerWarps = kKB + kVB == 2 ? 8 : 16;
+template <int kKB, int kVB>
+constexpr int kScanThreads = 32 * kWorkerWarps<kKB, kVB> + (kKB + kVB == 2 ? 0 : 32);
 
 template <bool kHalf, int kKB, int kVB, bool kStateOnly>
-__global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 2 : 1)
+__global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1)
     decay_scan_kernel(const __grid_constant__ ScanArgs a) {
   constexpr bool kSmall = kKB + kVB == 2;
   constexpr int kWarps = kWorkerWarps<kKB, kVB>, kWorkers = 32 * kWarps;
+  constexpr bool kOwnIssuer = !kSmall;             // a warp of its own for loads and products
   constexpr int kGroups = kWarps / 4;              // workers of a lane quadrant
   constexpr int kBlocks = 4 / kGroups;             // of 32 score columns, per worker
   // TMEM columns: scores (P' of a block of 32 tokens takes the first half of the block's columns, so that no warp
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
   constexpr uint32_t kCols = kStateOnly ? 64 * kKB : kSmall ? 256 : 512;
   constexpr int kParts = kVB == 1 ? 2 * kGroups : kGroups;  // threads that share a row of M^T (two quadrants or one hold it)
   constexpr int kOwn = 64 * kKB / kParts;                   // its columns held by one thread: 16 or 32
-  constexpr int kPiece = 16;                                // score and output columns at a time, as registers allow
+  constexpr int kPiece = kSmall ? 32 : 16;                  // score and output columns at a time, as registers allow
   constexpr uint32_t kXBytes = kStateOnly ? 0 : kKB * kBox;
   constexpr uint32_t kStage = kXBytes + kKB * kBox + kVB * kBox;
   constexpr uint32_t kStateBox = kVB * 64 * 128;
@@ -260,10 +263,10 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
   const bool plain = l2 * 127.0f > (kHalf ? -4.0f : -96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
   bool ok = true;
-  // Weights, decays, states, outputs by all warps; loads and products by warp 0 as well (a warp of its own for them would
-  // cost every warp a quarter of its registers), which walks them together while one lane issues.  A wait that runs out
-  // does not leave the loop (other warps may be at a barrier with this one): the rest runs through without waiting,
-  // issuing or storing.
+  // Weights, decays, states, outputs by the workers.  Loads and products by a warp of its own, or (single boxes) by warp 0
+  // as well, because a ninth warp would cost every warp a quarter of its registers; that warp walks them together while
+  // one lane issues.  A wait that runs out does not leave the loop (other warps may be at a barrier with this one): the
+  // rest runs through without waiting, issuing or storing.
   const bool leader = elect_leader();
   int loaded = 0;
   auto load = [&]() {
@@ -379,22 +382,24 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
         }
       };
 
-      {
-        const bool transposed = p.transposed != 0;
-        const float* src = p.state_in == nullptr || kStateOnly
-                               ? nullptr
-                               : p.state_in + (static_cast<int64_t>(item) * a.segments + segment) * ny * nz;
+      if (!kOwnIssuer || warp < kWarps) {
+        {
+          const bool transposed = p.transposed != 0;
+          const float* src = p.state_in == nullptr || kStateOnly
+                                 ? nullptr
+                                 : p.state_in + (static_cast<int64_t>(item) * a.segments + segment) * ny * nz;
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-          m[i] = 0.0f;
-          const int c = mc + i;
-          if (src != nullptr && mv < nz && c < ny) m[i] = src[transposed ? mv * ny + c : c * nz + mv];
+          for (int i = 0; i < kOwn; ++i) {
+            m[i] = 0.0f;
+            const int c = mc + i;
+            if (src != nullptr && mv < nz && c < ny) m[i] = src[transposed ? mv * ny + c : c * nz + mv];
+          }
         }
+        fetch_mask(0);
+        prepare(0);
+        if (!kStateOnly) write_state(0);
+        fence_proxy_async();
       }
-      fetch_mask(0);
-      prepare(0);
-      if (!kStateOnly) write_state(0);
-      fence_proxy_async();
       tc_fence_before();
       __syncthreads();
       tc_fence_after();
@@ -454,14 +459,58 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
           mma_led_tmem_a(leader, tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), zd + k * 128, i_out, 1);
         mma_led_commit(leader, out_bar);
       };
-      if (warp == 0) {
-        while (loaded < min(stages, count)) load();
-      }
-      const uint32_t quadrant = tmem + (static_cast<uint32_t>(q) << 21);  // this warp's lanes
       auto wait = [&](uint32_t bar, uint32_t parity) {
         ok = wait_warp(bar, parity, sh, a.status) && ok;
         tc_fence_after();
       };
+      const bool issuer = warp == (kOwnIssuer ? kWarps : 0);
+      if (issuer) {
+        while (loaded < min(stages, count)) load();
+      }
+      // The issuing warp's part of chunk n, up to its weighing, after it, before its scores' use, and after that.
+      // The next load goes out once the chunk before is done with its stage (and its scores).
+      auto move_on = [&](int n) {
+        if (n > 0) {
+          wait(kStateOnly ? change_bar : out_bar, (n & 1) ^ 1);
+          if (loaded < count) load();
+        }
+      };
+      auto issue_first = [&](int n) {
+        if (!kStateOnly && !kPlain) {
+          move_on(n);
+          wait(full_bar + 8 * stage_of(n), full_parity(n));
+          if (ok) issue_scores(n);
+        } else if (stages == 1) {
+          move_on(n);
+        }
+      };
+      auto issue_weighed = [&](int n) {
+        if (kStateOnly || kPlain) {
+          if (stages == 2) move_on(n);
+          wait(weighed_bar, n & 1);
+          if (!kStateOnly && ok) issue_scores(n);
+        }
+      };
+      auto issue_taken = [&](int n) {
+        if (n > 0) wait(taken_bar, (n & 1) ^ 1);
+        if (!kStateOnly && !kPlain) wait(weighed_bar, n & 1);
+        if (!kStateOnly && ok) issue_state(n);
+        if (ok) issue_change(n);
+      };
+      auto issue_decayed = [&](int n) {
+        wait(decayed_bar, n & 1);
+        if (ok) issue_out(n);
+      };
+      if (kOwnIssuer && issuer) {
+        for (int n = 0; n < count; ++n) {
+          issue_first(n);
+          issue_weighed(n);
+          issue_taken(n);
+          if (!kStateOnly) issue_decayed(n);
+        }
+        return;
+      }
+      const uint32_t quadrant = tmem + (static_cast<uint32_t>(q) << 21);  // this warp's lanes
       auto arrive = [&](uint32_t bar) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
@@ -470,7 +519,8 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
       float row_out = 0.0f;
       bool row_live = false;
       auto take = [&](int n, bool more) {
-        wait(change_bar, (n - 1) & 1);
+        // (the output's product is issued after the change's and completes after it)
+        wait(kStateOnly ? change_bar : out_bar, (n - 1) & 1);
 #pragma unroll
         for (int i = 0; i < kOwn; i += 16) {
           if (mc + i >= ny) break;  // no product wrote these columns
@@ -495,7 +545,6 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
           arrive(taken_bar);
           return;
         }
-        wait(out_bar, (n - 1) & 1);
         const int col0 = 32 * group, t = chunk_at(n - 1) * kChunk + 32 * q + lane;
         uint32_t w[16];
         if (col0 < nz) {
@@ -540,23 +589,8 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
         uint8_t* const z_tile = y_tile + kKB * kBox;
         if (n + 1 < count) fetch_mask(n + 1);
         tokens_seen += ranks.total;
-        // loads of the next chunk, once the one before is done with its stage (and its scores)
-        auto move_on = [&]() {
-          if (n > 0) {
-            wait(kStateOnly ? change_bar : out_bar, parity ^ 1);
-            if (loaded < count) load();
-          }
-        };
-        if (!kStateOnly && !kPlain) {
-          if (warp == 0) {
-            move_on();
-            wait(full_bar + 8 * stage_of(n), full_parity(n));
-            if (ok) issue_scores(n);
-          }
-          wait(scores_bar, parity);  // y's rows have been read
-        } else if (stages == 1 && warp == 0) {
-          move_on();
-        }
+        if (!kOwnIssuer && issuer) issue_first(n);
+        if (!kStateOnly && !kPlain) wait(scores_bar, parity);  // y's rows have been read
         if (kExact && n > 0) wait(change_bar, parity ^ 1);     // the small parts have been, too
         wait(full_bar + 8 * stage_of(n), full_parity(n));
 
@@ -629,18 +663,9 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
         }
         fence_proxy_async();
         arrive(weighed_bar);
-        if (warp == 0 && (kStateOnly || kPlain)) {
-          if (stages == 2) move_on();
-          wait(weighed_bar, parity);
-          if (!kStateOnly && ok) issue_scores(n);
-        }
+        if (!kOwnIssuer && issuer) issue_weighed(n);
         if (n > 0) take(n, true);
-        if (warp == 0) {
-          if (n > 0) wait(taken_bar, parity ^ 1);
-          if (!kStateOnly && !kPlain) wait(weighed_bar, parity);
-          if (!kStateOnly && ok) issue_state(n);
-          if (ok) issue_change(n);
-        }
+        if (!kOwnIssuer && issuer) issue_taken(n);
         if (ranks.total != decay_total) {  // of this chunk, for its state
           decay_total = ranks.total;
           const Decay d(l * static_cast<float>(decay_total));
@@ -743,10 +768,7 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
           tmem_st_wait();
           tc_fence_before();
           arrive(decayed_bar);
-          if (warp == 0) {
-            wait(decayed_bar, parity);
-            if (ok) issue_out(n);
-          }
+          if (!kOwnIssuer && issuer) issue_decayed(n);
         }
         row_out = kPlain ? lambda * down : down;
         row_live = live;
@@ -777,7 +799,7 @@ __global__ void __launch_bounds__(32 * kWorkerWarps<kKB, kVB>, kKB + kVB == 2 ? 
     work(std::false_type(), std::false_type());
   }
   // nothing may be in flight when the CTA ends
-  if (warp == 0 && leader) {
+  if (warp == (kOwnIssuer ? kWarps : 0) && leader) {
     if (!ok) {
       for (int n = max(0, loaded - stages); n < loaded; ++n)
         mbar_wait_bounded(full_bar + 8 * stage_of(n), full_parity(n), nullptr, a.status);
@@ -920,7 +942,7 @@ cudaError_t launch_one(ScanArgs& a, int64_t items, const char* name, cudaStream_
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
   LaunchScope scope(name, stream);
-  launch_pdl(kernel, dim3(static_cast<unsigned>(items * a.segments * a.passes)), 32 * kWorkerWarps<kKB, kVB>, smem, stream, a);
+  launch_pdl(kernel, dim3(static_cast<unsigned>(items * a.segments * a.passes)), kScanThreads<kKB, kVB>, smem, stream, a);
   return cudaGetLastError();
 }
 
