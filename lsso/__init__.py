@@ -8,6 +8,7 @@ import sys as _sys
 
 import lsso_b200 as _impl
 import lsso_b200.ball as _ball
+import lsso_b200.ball.causal as _causal
 import lsso_b200.ball.config as _config
 import lsso_b200.ball.cuda as _cuda
 import lsso_b200.ball.decay as _decay
@@ -19,6 +20,7 @@ import lsso_b200.ball.reference as _reference
 import lsso_b200.ball.rotary as _rotary
 
 _sys.modules[__name__ + ".ball"] = _ball
+_sys.modules[__name__ + ".ball.causal"] = _causal
 _sys.modules[__name__ + ".ball.config"] = _config
 _sys.modules[__name__ + ".ball.cuda"] = _cuda
 _sys.modules[__name__ + ".ball.decay"] = _decay

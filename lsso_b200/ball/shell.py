@@ -15,6 +15,10 @@ sum and the padding mask in one pass, ``dropout.py``, on both branches of every
 block) and ``embedding_scale`` (a scaled embedding with the mask applied and a
 deterministic gradient, ``embedding.py``).
 
+``mixer="causal"`` puts the causal mixer (``causal.py``: decay attention with
+rotary positions) in LSSO's place.  Such a shell can continue a sequence:
+``new_state`` and the ``state`` argument run prompts and then single tokens.
+
 ``vision_position_ids`` is the timm adapter's position rule
 (integrations/timm.py:143-156): position 0 for the class token and centered
 one-dimensional coordinates for the patches.
@@ -25,6 +29,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from .causal import CausalMixer, CausalState
 from .config import LSSOConfig
 from .dropout import dropout_add, dropout_add_reference, dropout_state
 from .embedding import TokenEmbedding
@@ -50,13 +55,20 @@ class ShellBlock(nn.Module):
     with neither ``gated`` nor ``mlp_ratio``, is refused.
     ``dropout``: the rate on both branches in training mode; the block's
     branches use the generator sites ``site`` and ``site + 1``.
+    ``mixer``: "lsso", or "causal" for a :class:`CausalMixer` with
+    ``mixer_options``.
     """
 
     def __init__(self, config: LSSOConfig, *, mlp_ratio: float = 0.0, gated: str | None = None,
-                 hidden: int | None = None, dropout: float = 0.0, site: int = 0) -> None:
+                 hidden: int | None = None, dropout: float = 0.0, site: int = 0, mixer: str = "lsso",
+                 mixer_options: dict | None = None) -> None:
         super().__init__()
+        if mixer not in ("lsso", "causal"):
+            raise ValueError(f"mixer must be 'lsso' or 'causal', got {mixer!r}")
+        if mixer == "lsso" and mixer_options:
+            raise ValueError("mixer_options are the causal mixer's: set mixer='causal'")
         self.norm1 = nn.LayerNorm(config.dim)
-        self.mixer = LSSO(config)
+        self.mixer = LSSO(config) if mixer == "lsso" else CausalMixer(config, **(mixer_options or {}))
         self.mlp = None
         self.dropout, self.site = float(dropout), site
         if hidden is not None and hidden < 1:
@@ -87,14 +99,16 @@ class ShellBlock(nn.Module):
         return x
 
     def forward(self, x: torch.Tensor, valid_mask: torch.Tensor | None, implementation: str,
-                state: torch.Tensor | None = None) -> torch.Tensor:
+                state: torch.Tensor | None = None, memory: CausalState | None = None) -> torch.Tensor:
+        """``state``: the dropout generator's; ``memory``: the causal mixer's."""
         normalized = self.norm1(x)
         if normalized.device.type == "cuda" and torch.is_autocast_enabled():
             amp = torch.get_autocast_dtype("cuda")
             if implementation == "cuda" and amp not in (torch.float16, torch.bfloat16):
                 raise TypeError("the CUDA LSSO sequence path supports FP16 or BF16 AMP")
             normalized = normalized.to(dtype=amp)
-        branch = self.mixer(normalized, valid_mask=valid_mask, implementation=implementation)
+        options = {} if memory is None else {"state": memory}
+        branch = self.mixer(normalized, valid_mask=valid_mask, implementation=implementation, **options)
         x = self._residual(x, branch, valid_mask, implementation, state, self.site)
         if self.mlp is not None:
             if isinstance(self.mlp, GatedFeedForward):
@@ -118,12 +132,13 @@ class SequenceShell(nn.Module):
     ``broadcast_buffers=False`` and which a loaded checkpoint overwrites.  The
     blocks get a copy of the state, so they may be recomputed in the backward
     (activation checkpointing, block by block); recomputing the whole shell
-    would advance the step again.
+    would advance the step again.  ``mixer``, ``mixer_options``: as in
+    :class:`ShellBlock`, for every block.
     """
 
     def __init__(self, config: LSSOConfig, *, depth: int = 4, vocab: int = 8, mlp_ratio: float = 0.0,
                  gated: str | None = None, hidden: int | None = None, dropout: float = 0.0, dropout_seed: int = 0,
-                 embedding_scale: float | None = None) -> None:
+                 embedding_scale: float | None = None, mixer: str = "lsso", mixer_options: dict | None = None) -> None:
         super().__init__()
         if embedding_scale is None:
             self.embedding = nn.Embedding(vocab, config.dim)
@@ -131,27 +146,47 @@ class SequenceShell(nn.Module):
         else:
             self.embedding = TokenEmbedding(vocab, config.dim, scale=embedding_scale)
         self.blocks = nn.ModuleList(
-            ShellBlock(config, mlp_ratio=mlp_ratio, gated=gated, hidden=hidden, dropout=dropout, site=2 * i)
+            ShellBlock(config, mlp_ratio=mlp_ratio, gated=gated, hidden=hidden, dropout=dropout, site=2 * i, mixer=mixer,
+                       mixer_options=mixer_options)
             for i in range(depth))
         if dropout > 0:
             self.register_buffer("dropout_state", dropout_state(dropout_seed))
         else:
             self.dropout_state = None
 
+    def new_state(self, batch: int) -> list[CausalState]:
+        """The state of ``batch`` sequences before their first token (``mixer="causal"``), one entry per block."""
+        if not all(isinstance(block.mixer, CausalMixer) for block in self.blocks):
+            raise RuntimeError("only a shell with mixer='causal' has a state")
+        return [block.mixer.new_state(batch) for block in self.blocks]
+
     def forward(self, token_ids: torch.Tensor, valid_mask: torch.Tensor | None = None, *,
-                implementation: str = "reference") -> torch.Tensor:
+                implementation: str = "reference", state: list[CausalState] | None = None) -> torch.Tensor:
+        """Hidden states ``[batch, length, dim]``.
+
+        ``state`` (from :meth:`new_state`, under ``torch.no_grad()``, in
+        evaluation mode): the tokens continue the sequences it stands for, and
+        it moves on behind them, in a captured graph as well.
+        """
+        if state is not None:
+            if not all(isinstance(block.mixer, CausalMixer) for block in self.blocks):
+                raise RuntimeError("only a shell with mixer='causal' has a state")
+            if len(state) != len(self.blocks):
+                raise ValueError(f"the state must have an entry for each of the {len(self.blocks)} blocks, got {len(state)}")
+            if self.training and self.dropout_state is not None:
+                raise RuntimeError("a state is for evaluation: call eval() first")
         if isinstance(self.embedding, TokenEmbedding):
             x = self.embedding(token_ids, valid_mask, implementation=implementation)
         else:
             x = self.embedding(token_ids)
             if valid_mask is not None:
                 x = torch.where(valid_mask[:, :, None], x, torch.zeros_like(x))
-        state = self.dropout_state
-        if self.training and state is not None:
-            state = state.clone()
+        generator = self.dropout_state
+        if self.training and generator is not None:
+            generator = generator.clone()
             self.dropout_state[1] += 1
-        for block in self.blocks:
-            x = block(x, valid_mask, implementation, state)
+        for i, block in enumerate(self.blocks):
+            x = block(x, valid_mask, implementation, generator, None if state is None else state[i])
         return x
 
 
