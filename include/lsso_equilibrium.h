@@ -456,8 +456,9 @@ LSSO_API int lsso_dropout_backward(const void* dy, int out_type, int branch_type
  *   mask  uint8/bool [B, N] or NULL;  state  [B, H, DK, DV] FP32, before the
  *         first token, or NULL for zero;  last  likewise, after the last token
  *         (output), or NULL
- * DK and DV are multiples of 8 from 8 to 128.  States and sums are FP32; the
- * scores, the state as it meets q, and the output are rounded to `type`. */
+ * DK and DV are multiples of 8 from 8 to 128.  The workspace may be NULL where
+ * its size is at most 16 (sequences that are not cut into segments).  States
+ * and sums are FP32; weighted keys, the scores, the state as it meets q, and the output are rounded to `type`. */
 LSSO_API size_t lsso_decay_workspace_size(int64_t B, int64_t N, int64_t H, int64_t DK, int64_t DV, int backward);
 LSSO_API int lsso_decay_forward(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                 const void* v, const int64_t* v_strides, int type, const float* log_decay,

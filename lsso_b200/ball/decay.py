@@ -67,6 +67,23 @@ def _check_cuda(name, q, k, v, log_decay, dtypes) -> None:
             raise ValueError(f"{name} supports {label} widths that are multiples of 8 from 8 to 128, got {width}")
 
 
+_HALVES = frozenset((torch.bfloat16, torch.float16))
+
+
+def _usual(q, k, v, log_decay, state, valid_mask, lead: int) -> bool:
+    """Whether all of _check and _check_cuda but the types holds, in one expression (2 us less than asking one by one)."""
+    shape, values, kind, device = q.shape, v.shape, q.dtype, q.device
+    if len(shape) != lead + 2 or len(values) != lead + 2 or k.shape != shape or not q.is_cuda:
+        return False
+    batch, heads, key, value = shape[0], shape[-2], shape[-1], values[-1]
+    return (values[:-1] == shape[:-1] and k.dtype is kind and v.dtype is kind and log_decay.dtype is torch.float32
+            and log_decay.shape == (heads,) and 8 <= key <= 128 and 8 <= value <= 128 and not (key | value) % 8
+            and k.device == device and v.device == device and log_decay.device == device
+            and (state is None or (state.shape == (batch, heads, key, value) and state.device == device))
+            and (valid_mask is None or (valid_mask.shape == shape[:lead] and valid_mask.dtype is torch.bool
+                                        and valid_mask.device == device)))
+
+
 def decay_attention_reference(q, k, v, log_decay, *, scale=None, state=None, valid_mask=None, return_state=False):
     """The same operator in PyTorch (any device; first-order autograd by PyTorch, the decay's gradient included)."""
     _check(q, k, v, log_decay, state, valid_mask, 2)
@@ -121,31 +138,61 @@ def decay_attention_step_reference(q, k, v, log_decay, state, *, scale=None, val
 
 
 # ---------------------------------------------------------------------------- the native calls
-_Strides3, _Strides2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
+_arrays: dict[tuple, ctypes.Array] = {}
+_sizes: dict[tuple, int] = {}
+
+
+def _array(strides: tuple) -> ctypes.Array:
+    """Strides as the library takes them (made once per set of strides: 0.6 us each)."""
+    found = _arrays.get(strides)
+    if found is None:
+        if len(_arrays) >= 4096:
+            _arrays.clear()
+        found = _arrays[strides] = (ctypes.c_int64 * len(strides))(*strides)
+    return found
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
     """``t`` (copied if a tensor map cannot describe it) and its strides."""
+    strides = t.stride()
+    sb, sn, sh, sd = strides
+    if sd == 1 and not (sb | sn | sh) % 8 and sb > 0 and sn > 0 and sh > 0 and not t.data_ptr() % 16:
+        return t, _array(strides[:3])
     b, n, h, d = t.shape
-    for again in (False, True):
+    for _ in range(2):
         sb, sn, sh, sd = t.stride()
         # the stride of an axis of one is never used: any allowed value
         sh = d if h == 1 else sh
         sn = h * d if n == 1 else sn
         sb = n * h * d if b == 1 else sb
         if sd == 1 and min(sb, sn, sh) > 0 and not (sb | sn | sh) % 8 and not t.data_ptr() % 16:
-            return t, _Strides3(sb, sn, sh)
+            return t, _array((sb, sn, sh))
         t = t.clone(memory_format=torch.contiguous_format)
     raise RuntimeError("a fresh tensor was not aligned to 16 bytes")
 
 
-def _workspace(device, sizes, backward):
-    return _native.workspace("lsso_decay_workspace_size", device, *sizes, int(backward))
+def _workspace(device: torch.device, sizes: tuple, backward: bool) -> tuple[int | None, int, torch.Tensor | None]:
+    """Pointer, bytes and owner of a call's scratch (none where the sequences are not cut)."""
+    key = (device.index, *sizes, backward)
+    size = _sizes.get(key)
+    if size is None:
+        lib = _native.library()
+        with torch.cuda.device(device):
+            size = lib.lib.lsso_decay_workspace_size(*sizes, int(backward))
+        if size == 0:
+            lib.check(1)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        _sizes[key] = size
+    if size <= 16:
+        return None, 0, None
+    scratch = torch.empty((size,), dtype=torch.uint8, device=device)
+    return scratch.data_ptr(), size, scratch
 
 
 def _forward(q, k, v, log_decay, scale, state, mask, return_state):
     batch, length, heads, key = q.shape
-    value = v.shape[-1]
+    value = v.shape[3]
     y = q.new_empty((batch, length, heads, value))
     last = None
     if return_state:
@@ -154,12 +201,13 @@ def _forward(q, k, v, log_decay, scale, state, mask, return_state):
         if last is not None:
             last.zero_() if state is None else last.copy_(state)
         return y, last
-    (q, qs), (k, ks), (v, vs), (y, ys) = _rows(q), _rows(k), _rows(v), _rows(y)
+    (q, qs), (k, ks), (v, vs), (_, ys) = _rows(q), _rows(k), _rows(v), _rows(y)
     sizes = (batch, length, heads, key, value)
-    scratch = _workspace(q.device, sizes, False)
-    _native.run("lsso_decay_forward", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+    device = q.device
+    scratch, scratch_bytes, _owner = _workspace(device, sizes, False)
+    _native.run("lsso_decay_forward", device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
                 _native.ELEMENT_TYPES[q.dtype], log_decay.data_ptr(), _native._ptr(mask), *sizes, scale,
-                _native._ptr(state), _native._ptr(last), y.data_ptr(), ys, scratch.data_ptr(), scratch.numel())
+                _native._ptr(state), _native._ptr(last), y.data_ptr(), ys, scratch, scratch_bytes)
     return y, last
 
 
@@ -192,11 +240,11 @@ class _DecayAttention(torch.autograd.Function):
         (q, qs), (k, ks), (v, vs), (dy, ys) = _rows(q), _rows(k), _rows(v), _rows(dy)
         (dq, dqs), (dk, dks), (dv, dvs) = _rows(dq), _rows(dk), _rows(dv)
         sizes = (batch, length, heads, key, value)
-        scratch = _workspace(q.device, sizes, True)
+        scratch, scratch_bytes, _owner = _workspace(q.device, sizes, True)
         _native.run("lsso_decay_backward", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, dy.data_ptr(),
                     ys, _native.ELEMENT_TYPES[q.dtype], log_decay.data_ptr(), _native._ptr(mask), *sizes, ctx.scale,
                     _native._ptr(state), _native._ptr(dlast), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dvs,
-                    _native._ptr(dstate), scratch.data_ptr(), scratch.numel())
+                    _native._ptr(dstate), scratch, scratch_bytes)
         return dq, dk, dv, None, None, dstate, None, None
 
 
@@ -217,8 +265,11 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     Gradients: q, k, v and state.
     """
     _native.refuse_transforms("decay_attention", q, k, v, log_decay, state, valid_mask)
-    _check(q, k, v, log_decay, state, valid_mask, 2)
-    _check_cuda("decay_attention", q, k, v, log_decay, (torch.bfloat16, torch.float16))
+    if not _usual(q, k, v, log_decay, state, valid_mask, 2):
+        _check(q, k, v, log_decay, state, valid_mask, 2)
+        _check_cuda("decay_attention", q, k, v, log_decay, (torch.bfloat16, torch.float16))
+    elif q.dtype not in _HALVES or (log_decay.requires_grad and torch.is_grad_enabled()):
+        _check_cuda("decay_attention", q, k, v, log_decay, (torch.bfloat16, torch.float16))
     if state is not None and state.dtype != torch.float32:
         raise TypeError(f"state must use torch.float32, got {state.dtype}")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
@@ -250,29 +301,38 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     Not differentiable: train with :func:`decay_attention`.
     """
     _native.refuse_transforms("decay_attention_step", q, k, v, log_decay, state, valid_mask)
-    _check(q, k, v, log_decay, state, valid_mask, 1)
-    _check_cuda("decay_attention_step", q, k, v, log_decay, (torch.bfloat16, torch.float16, torch.float32))
+    kind, device = q.dtype, q.device
+    if not _usual(q, k, v, log_decay, state, valid_mask, 1) or kind not in _native.ELEMENT_TYPES or log_decay.requires_grad:
+        _check(q, k, v, log_decay, state, valid_mask, 1)
+        _check_cuda("decay_attention_step", q, k, v, log_decay, (torch.bfloat16, torch.float16, torch.float32))
     target = state if new_state is None else new_state
-    for name, value in (("state", state), ("new_state", target)):
-        if value.dtype != torch.float32 or value.shape != state.shape or value.device != q.device:
-            raise ValueError(f"{name} must be FP32 {tuple(state.shape)} on {q.device}, got {value.dtype} "
+    for name, value in (("state", state),) if new_state is None else (("state", state), ("new_state", new_state)):
+        if value.dtype is not torch.float32 or value.shape != state.shape or value.device != device:
+            raise ValueError(f"{name} must be FP32 {tuple(state.shape)} on {device}, got {value.dtype} "
                              f"{tuple(value.shape)} on {value.device}")
         if not value.is_contiguous():
             raise RuntimeError(f"decay_attention_step requires a contiguous {name}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state, target)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad
+                                    or target.requires_grad):
         raise ValueError("decay_attention_step has no gradient; call it under torch.no_grad() or use decay_attention")
     batch, heads, key = q.shape
-    y = q.new_empty((batch, heads, v.shape[-1]))
+    value = v.shape[2]
+    y = q.new_empty((batch, heads, value))
     if not y.numel():
         return y
-    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
-    log_decay = log_decay.contiguous()
-    mask = None if valid_mask is None else valid_mask.contiguous()
-    scale = key ** -0.5 if scale is None else float(scale)
-    _native.run("lsso_decay_step", q.device, q.data_ptr(), _Strides2(q.stride(0), q.stride(1)), k.data_ptr(),
-                _Strides2(k.stride(0), k.stride(1)), v.data_ptr(), _Strides2(v.stride(0), v.stride(1)),
-                _native.ELEMENT_TYPES[q.dtype], log_decay.data_ptr(), _native._ptr(mask), batch, heads, key, v.shape[-1],
-                scale, state.data_ptr(), target.data_ptr(), y.data_ptr())
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if qs[2] != 1 or ks[2] != 1 or vs[2] != 1:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if not log_decay.is_contiguous():
+        log_decay = log_decay.contiguous()
+    if valid_mask is not None and not valid_mask.is_contiguous():
+        valid_mask = valid_mask.contiguous()
+    at = state.data_ptr()
+    _native.run("lsso_decay_step", device, q.data_ptr(), _array(qs[:2]), k.data_ptr(), _array(ks[:2]), v.data_ptr(),
+                _array(vs[:2]), _native.ELEMENT_TYPES[kind], log_decay.data_ptr(), _native._ptr(valid_mask), batch, heads,
+                key, value, key ** -0.5 if scale is None else scale, at, at if new_state is None else new_state.data_ptr(),
+                y.data_ptr())
     return y
 
 

@@ -59,7 +59,7 @@ int lsso_decay_forward(const void* q, const int64_t* q_strides, const void* k, c
   if (rc == LSSO_OK) rc = check_tensor(who, "v", v, v_strides);
   if (rc == LSSO_OK) rc = check_tensor(who, "y", y, y_strides);
   if (rc != LSSO_OK) return rc;
-  if (log_decay == nullptr || workspace == nullptr) return invalid("%s: a required pointer is NULL", who);
+  if (log_decay == nullptr) return invalid("%s: a required pointer is NULL", who);
   if (type != LSSO_TYPE_BF16 && type != LSSO_TYPE_FP16) return invalid("%s: type must be BF16 or FP16", who);
   if (!aligned(log_decay, 4) || !aligned(state, 16) || !aligned(last, 16) || !aligned(workspace, 16)) {
     return invalid("%s: states and workspace must be 16-byte aligned", who);
@@ -69,7 +69,9 @@ int lsso_decay_forward(const void* q, const int64_t* q_strides, const void* k, c
   rc = lsso::capi::device(&sms, &c.status);
   if (rc != LSSO_OK) return rc;
   const size_t need = lsso::decay_workspace(B, N, static_cast<int>(H), static_cast<int>(DK), static_cast<int>(DV), false, sms);
-  if (workspace_bytes < need) return lsso::capi::workspace_too_small(who, workspace_bytes, need);
+  if (need > 16 && (workspace == nullptr || workspace_bytes < need)) {
+    return lsso::capi::workspace_too_small(who, workspace == nullptr ? 0 : workspace_bytes, need);
+  }
   c.q = tensor(q, q_strides);
   c.k = tensor(k, k_strides);
   c.v = tensor(v, v_strides);
@@ -107,7 +109,7 @@ int lsso_decay_backward(const void* q, const int64_t* q_strides, const void* k, 
   if (rc == LSSO_OK) rc = check_tensor(who, "dk", dk, dk_strides);
   if (rc == LSSO_OK) rc = check_tensor(who, "dv", dv, dv_strides);
   if (rc != LSSO_OK) return rc;
-  if (log_decay == nullptr || workspace == nullptr) return invalid("%s: a required pointer is NULL", who);
+  if (log_decay == nullptr) return invalid("%s: a required pointer is NULL", who);
   if (type != LSSO_TYPE_BF16 && type != LSSO_TYPE_FP16) return invalid("%s: type must be BF16 or FP16", who);
   if (!aligned(log_decay, 4) || !aligned(state, 16) || !aligned(dlast, 16) || !aligned(dstate, 16) || !aligned(workspace, 16)) {
     return invalid("%s: states and workspace must be 16-byte aligned", who);
@@ -117,7 +119,9 @@ int lsso_decay_backward(const void* q, const int64_t* q_strides, const void* k, 
   rc = lsso::capi::device(&sms, &c.status);
   if (rc != LSSO_OK) return rc;
   const size_t need = lsso::decay_workspace(B, N, static_cast<int>(H), static_cast<int>(DK), static_cast<int>(DV), true, sms);
-  if (workspace_bytes < need) return lsso::capi::workspace_too_small(who, workspace_bytes, need);
+  if (need > 16 && (workspace == nullptr || workspace_bytes < need)) {
+    return lsso::capi::workspace_too_small(who, workspace == nullptr ? 0 : workspace_bytes, need);
+  }
   c.q = tensor(q, q_strides);
   c.k = tensor(k, k_strides);
   c.v = tensor(v, v_strides);
