@@ -82,10 +82,6 @@ struct ScanShared {
   int abort_flag;
 };
 
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[16]) { tmem_ld16(taddr, v); }
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[8]) { tmem_st8(taddr, r); }
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[32]) { tmem_ld32(taddr, v); }
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if (kHalf) return pair_from_float(lo, hi, __half());
@@ -191,14 +187,13 @@ struct ChunkRanks {
 template <int kKB, int kVB>
 constexpr int kWorkerWarps = kKB + kVB == 2 ? 8 : 16;
 template <int kKB, int kVB>
-constexpr int kScanThreads = 32 * kWorkerWarps<kKB, kVB> + (kKB + kVB == 2 ? 0 : 32);
+constexpr int kScanThreads = 32 * kWorkerWarps<kKB, kVB> + 32;
 
-template <bool kHalf, int kKB, int kVB, bool kStateOnly>
+template <bool kHalf, int kKB, int kVB, bool kStateOnly, bool kMayExact>
 __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1)
     decay_scan_kernel(const __grid_constant__ ScanArgs a) {
   constexpr bool kSmall = kKB + kVB == 2;
   constexpr int kWarps = kWorkerWarps<kKB, kVB>, kWorkers = 32 * kWarps;
-  constexpr bool kOwnIssuer = !kSmall;             // a warp of its own for loads and products
   constexpr int kGroups = kWarps / 4;              // workers of a lane quadrant
   constexpr int kBlocks = 4 / kGroups;             // of 32 score columns, per worker
   // TMEM columns: scores (P' of a block of 32 tokens takes the first half of the block's columns, so that no warp
@@ -208,7 +203,6 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   constexpr uint32_t kCols = kStateOnly ? 64 * kKB : kSmall ? 256 : 512;
   constexpr int kParts = kVB == 1 ? 2 * kGroups : kGroups;  // threads that share a row of M^T (two quadrants or one hold it)
   constexpr int kOwn = 64 * kKB / kParts;                   // its columns held by one thread: 16 or 32
-  constexpr int kPiece = kSmall ? 32 : 16;                  // score and output columns at a time, as registers allow
   constexpr uint32_t kXBytes = kStateOnly ? 0 : kKB * kBox;
   constexpr uint32_t kStage = kXBytes + kKB * kBox + kVB * kBox;
   constexpr uint32_t kStateBox = kVB * 64 * 128;
@@ -263,10 +257,10 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   const bool plain = l2 * 127.0f > (kHalf ? -4.0f : -96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
   bool ok = true;
-  // Weights, decays, states, outputs by the workers.  Loads and products by a warp of its own, or (single boxes) by warp 0
-  // as well, because a ninth warp would cost every warp a quarter of its registers; that warp walks them together while
-  // one lane issues.  A wait that runs out does not leave the loop (other warps may be at a barrier with this one): the
-  // rest runs through without waiting, issuing or storing.
+  // Weights, decays, states, outputs by the workers; loads and products by a warp of its own, which walks them together
+  // while one lane issues (warp 0 doing both had a third more registers and took 196 against 174 us, forward of 64 x 4096
+  // tokens, 8 heads of 32).  A wait that runs out does not leave the loop (other warps may be at a barrier with this one):
+  // the rest runs through without waiting, issuing or storing.
   const bool leader = elect_leader();
   int loaded = 0;
   auto load = [&]() {
@@ -288,518 +282,481 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
     __syncwarp();
   };
   auto work = [&](auto plain_heads, auto exact_states) {
-      constexpr bool kPlain = decltype(plain_heads)::value, kExact = decltype(exact_states)::value;
-      const int q = warp & 3, group = warp >> 2;
-      // this thread's part of M^T: row mv, columns [mc, mc + kOwn)
-      const int mv = kVB == 1 ? 32 * (q & 1) + lane : 32 * q + lane;
-      const int part = kVB == 1 ? (q >> 1) + 2 * group : group;
-      const int mc = part * kOwn;
-      float m[kOwn];
-      float kappa = 1.0f;
-      // M^T as chunk n's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
-      auto write_state = [&](int n) {
-        float up = kappa;
-        if (kHalf) {
-          float most = 0.0f;
+    constexpr bool kPlain = decltype(plain_heads)::value, kExact = decltype(exact_states)::value;
+    const int q = warp & 3, group = warp >> 2;
+    // this thread's part of M^T: row mv, columns [mc, mc + kOwn)
+    const int mv = kVB == 1 ? 32 * (q & 1) + lane : 32 * q + lane;
+    const int part = kVB == 1 ? (q >> 1) + 2 * group : group;
+    const int mc = part * kOwn;
+    float m[kOwn];
+    float kappa = 1.0f;
+    // M^T as chunk n's B operand, rounded to the type; FP16 by rows that are brought into range by powers of two.
+    auto write_state = [&](int n) {
+      float up = kappa;
+      if (kHalf) {
+        float most = 0.0f;
 #pragma unroll
-          for (int i = 0; i < kOwn; ++i) most = fmaxf(most, fabsf(m[i]));
-          uint32_t e = 0;  // the largest of the kParts threads that share the row
-          sh.state_top[part * (64 * kVB) + mv] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
-          named_barrier(kVB == 1 ? 5 + (q & 1) : 1 + q, 32 * kParts);
+        for (int i = 0; i < kOwn; ++i) most = fmaxf(most, fabsf(m[i]));
+        uint32_t e = 0;  // the largest of the kParts threads that share the row
+        sh.state_top[part * (64 * kVB) + mv] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
+        named_barrier(kVB == 1 ? 5 + (q & 1) : 1 + q, 32 * kParts);
 #pragma unroll
-          for (int i = 0; i < kParts; ++i) e = max(e, static_cast<uint32_t>(sh.state_top[i * (64 * kVB) + mv]));
-          up = PowerScale(e).up;
-          if (part == 0) sh.state_exponent[n & 1][mv] = static_cast<uint8_t>(e);
+        for (int i = 0; i < kParts; ++i) e = max(e, static_cast<uint32_t>(sh.state_top[i * (64 * kVB) + mv]));
+        up = PowerScale(e).up;
+        if (part == 0) sh.state_exponent[n & 1][mv] = static_cast<uint8_t>(e);
+      }
+#pragma unroll
+      for (int i = 0; i < kOwn; i += 8) {
+        const int c = mc + i, box = c >> 6, piece = (c >> 3) & 7;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 v = mul2(make_float2(m[i + 2 * j], m[i + 2 * j + 1]), make_float2(up, up));
+          w[j] = pack2<kHalf>(v.x, v.y);
         }
+        *reinterpret_cast<uint4*>(state_tile + box * kStateBox + mv * 128 + ((piece ^ (mv & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    };
+    uint32_t words[4] = {0, 0, 0, 0};  // general heads: valid tokens of the chunk
+    int total = 0;                     // how many
+    uint32_t ahead = 0;  // mask bytes of a later chunk, as bits
+    auto fetch_mask = [&](int n) {
+      ahead = 0;
+      if (a.mask == nullptr) return;
+      const int t0 = chunk_at(n) * kChunk + lane;
+      const uint8_t* of_sample = a.mask + static_cast<int64_t>(sample) * a.length;
 #pragma unroll
-        for (int i = 0; i < kOwn; i += 8) {
-          const int c = mc + i, box = c >> 6, piece = (c >> 3) & 7;
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 v = mul2(make_float2(m[i + 2 * j], m[i + 2 * j + 1]), make_float2(up, up));
-            w[j] = pack2<kHalf>(v.x, v.y);
-          }
-          *reinterpret_cast<uint4*>(state_tile + box * kStateBox + mv * 128 + ((piece ^ (mv & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      };
+      for (int w = 0; w < 4; ++w)
+        if (t0 + 32 * w < a.length && of_sample[t0 + 32 * w] != 0) ahead |= 1u << w;
+    };
+    float lambda = 0.0f;  // factor of the state's part of this row; plain: of the whole row
+    float block_factor[kBlocks];
+    bool live = false, live_token = false, dead_tokens = false, was_whole = false;  // of this thread's row, and of token tid
+    float decay_factor = 0.0f, decay_keep = 0.0f;  // M' = M * factor + M * keep (keep is 0 or 1)
+    int decay_total = -1;
+    // Ranks and tables of chunk n from the fetched bits.  Whole chunks all have the same, and find them in place.
+    auto prepare = [&](int n) {
       ChunkRanks ranks;
-      uint32_t ahead = 0;  // mask bytes of a later chunk, as bits
-      auto fetch_mask = [&](int n) {
-        ahead = 0;
-        if (a.mask == nullptr) return;
-        const int t0 = chunk_at(n) * kChunk + lane;
-        const uint8_t* of_sample = a.mask + static_cast<int64_t>(sample) * a.length;
+      if (a.mask == nullptr) {
+        const int left = a.length - chunk_at(n) * kChunk;  // tokens
+        if (left >= kChunk && was_whole) return;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-          if (t0 + 32 * w < a.length && of_sample[t0 + 32 * w] != 0) ahead |= 1u << w;
-      };
-      float lambda = 0.0f;  // factor of the state's part of this row; plain: of the whole row
-      float block_factor[kBlocks];
-      bool live = false, live_token = false, dead_tokens = false, was_whole = false;  // of this thread's row, and of token tid
-      float decay_factor = 0.0f, decay_keep = 0.0f;  // M' = M * factor + M * keep (keep is 0 or 1)
-      int decay_total = -1;
-      // Ranks and tables of chunk n from the fetched bits.  Whole chunks all have the same, and find them in place.
-      auto prepare = [&](int n) {
-        if (a.mask == nullptr) {
-          const int left = a.length - chunk_at(n) * kChunk;  // tokens
-          if (left >= kChunk && was_whole) return;
+        for (int w = 0; w < 4; ++w) {
+          const int of_word = left - 32 * w;
+          ranks.words[w] = of_word >= 32 ? 0xffffffffu : of_word <= 0 ? 0u : (1u << of_word) - 1u;
+        }
+      } else {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int of_word = left - 32 * w;
-            ranks.words[w] = of_word >= 32 ? 0xffffffffu : of_word <= 0 ? 0u : (1u << of_word) - 1u;
-          }
+        for (int w = 0; w < 4; ++w) ranks.words[w] = __ballot_sync(0xffffffffu, (ahead >> w) & 1u);
+        if (ranks.whole() && was_whole) return;
+      }
+      was_whole = ranks.whole();
+      ranks.count();
+      total = ranks.total;
+      if (!kPlain) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) words[w] = ranks.words[w];
+      }
+      live = ranks.live(q, lane);
+      live_token = ranks.live(warp & 3, lane);
+      // tokens to be cleared: masked ones (behind the last token there are zeros)
+      dead_tokens = a.mask != nullptr && !was_whole;
+      const int rho = ranks.rho(q, lane, reverse);
+      const float row_rho = static_cast<float>(rho);
+      if (n > 0) named_barrier(7, kWorkers);  // the tables have been read
+      if (group == 0) {
+        sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : 0.0f;
+      } else if (group == 1 && !kStateOnly && !kPlain) {
+        sh.col[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.last_rho(q, reverse) - rho)) : 0.0f;
+      }
+      if (n > 0) named_barrier(7, kWorkers);
+      if (!kStateOnly) {
+        if (kPlain) {
+          lambda = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.total - 1)));
+          kappa = exp2f(l2 * (static_cast<float>(ranks.total) - late)) / p.from;
         } else {
+          lambda = p.into * exp2f(l2 * (row_rho + 1.0f - late));
 #pragma unroll
-          for (int w = 0; w < 4; ++w) ranks.words[w] = __ballot_sync(0xffffffffu, (ahead >> w) & 1u);
-          if (ranks.whole() && was_whole) return;
+          for (int i = 0; i < kBlocks; ++i)
+            block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(group + kGroups * i, reverse))));
         }
-        was_whole = ranks.whole();
-        ranks.count();
-        live = ranks.live(q, lane);
-        live_token = ranks.live(warp & 3, lane);
-        // tokens to be cleared: masked ones (behind the last token there are zeros)
-        dead_tokens = a.mask != nullptr && !was_whole;
-        const int rho = ranks.rho(q, lane, reverse);
-        const float row_rho = static_cast<float>(rho);
-        if (n > 0) named_barrier(7, kWorkers);  // the tables have been read
-        if (group == 0) {
-          sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : 0.0f;
-        } else if (group == 1 && !kStateOnly && !kPlain) {
-          sh.col[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.last_rho(q, reverse) - rho)) : 0.0f;
-        }
-        if (n > 0) named_barrier(7, kWorkers);
-        if (!kStateOnly) {
-          if (kPlain) {
-            lambda = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.total - 1)));
-            kappa = exp2f(l2 * (static_cast<float>(ranks.total) - late)) / p.from;
-          } else {
-            lambda = p.into * exp2f(l2 * (row_rho + 1.0f - late));
-#pragma unroll
-            for (int i = 0; i < kBlocks; ++i)
-              block_factor[i] = inside * exp2f(l2 * (row_rho - static_cast<float>(ranks.last_rho(group + kGroups * i, reverse))));
-          }
-        }
-      };
+      }
+    };
 
-      if (!kOwnIssuer || warp < kWarps) {
-        {
-          const bool transposed = p.transposed != 0;
-          const float* src = p.state_in == nullptr || kStateOnly
-                                 ? nullptr
-                                 : p.state_in + (static_cast<int64_t>(item) * a.segments + segment) * ny * nz;
+    if (warp < kWarps) {
+      {
+        const bool transposed = p.transposed != 0;
+        const float* src = p.state_in == nullptr || kStateOnly
+                               ? nullptr
+                               : p.state_in + (static_cast<int64_t>(item) * a.segments + segment) * ny * nz;
 #pragma unroll
-          for (int i = 0; i < kOwn; ++i) {
-            m[i] = 0.0f;
-            const int c = mc + i;
-            if (src != nullptr && mv < nz && c < ny) m[i] = src[transposed ? mv * ny + c : c * nz + mv];
-          }
+        for (int i = 0; i < kOwn; ++i) {
+          m[i] = 0.0f;
+          const int c = mc + i;
+          if (src != nullptr && mv < nz && c < ny) m[i] = src[transposed ? mv * ny + c : c * nz + mv];
         }
-        fetch_mask(0);
-        prepare(0);
-        if (!kStateOnly) write_state(0);
-        fence_proxy_async();
       }
-      tc_fence_before();
-      __syncthreads();
+      fetch_mask(0);
+      prepare(0);
+      if (!kStateOnly) write_state(0);
+      fence_proxy_async();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    int tokens_seen = 0;
+    const uint32_t tmem = sh.tmem;
+    // the products of a chunk, by warp 0
+    const int y_steps = (ny + 15) / 16;
+    const uint32_t i_scores = idesc<kHalf>(128, false, false), i_xm = idesc<kHalf>((nz + 15) & ~15, false, false),
+                   i_change = idesc<kHalf>((ny + 15) & ~15, true, true), i_out = idesc<kHalf>((nz + 15) & ~15, false, true);
+    auto stage_at = [&](int n) { return base + stage_of(n) * kStage; };
+    auto issue_scores = [&](int n) {
+      const uint64_t xd = make_desc_sw128(stage_at(n), 16, 1024), yd = make_desc_sw128(stage_at(n) + kXBytes, 16, 1024);
+#pragma unroll
+      for (int k = 0; k < 4 * kKB; ++k) {
+        const int step = (k >> 2) * (kBox / 16) + (k & 3) * 2;
+        if (k < y_steps) mma_led(leader, tmem + kColP, xd + step, yd + step, i_scores, k > 0);
+      }
+      mma_led_commit(leader, scores_bar);
+    };
+    auto issue_state = [&](int n) {  // X M
+      const uint64_t xd = make_desc_sw128(stage_at(n), 16, 1024), md = make_desc_sw128(smem_u32(state_tile), 16, 1024);
+#pragma unroll
+      for (int k = 0; k < 4 * kKB; ++k) {
+        if (k < y_steps) {
+          mma_led(leader, tmem + kColOut, xd + (k >> 2) * (kBox / 16) + (k & 3) * 2,
+                  md + (k >> 2) * (kStateBox / 16) + (k & 3) * 2, i_xm, k > 0);
+        }
+      }
+      if (kHalf || !kPlain) mma_led_commit(leader, xm_bar);
+    };
+    auto issue_change = [&](int n) {
+      const uint32_t y_at = stage_at(n) + kXBytes;
+      const uint64_t zd = make_desc_sw128(y_at + kKB * kBox, kVB == 2 ? kBox : 0, 1024);  // one box: lanes 64-127 repeat 0-63
+      const uint64_t yd = make_desc_sw128(y_at, kBox, 1024);
+      if (kExact) {  // the smaller parts first
+        const uint64_t small = make_desc_sw128(smem_u32(third), kBox, 1024);
+#pragma unroll
+        for (int t = 0; t < (kHalf ? 1 : 2); ++t) {
+#pragma unroll
+          for (int k = 0; k < kChunk / 16; ++k)
+            mma_led(leader, tmem + kColChange, zd + k * 128, small + t * kKB * (kBox / 16) + k * 128, i_change, t + k > 0);
+        }
+      }
+      if (kHalf && kExact) {
+        mma_led_scaled_d(leader, tmem + kColChange, zd, yd, i_change);  // the part so far is 2^11 times too large
+      } else {
+        mma_led(leader, tmem + kColChange, zd, yd, i_change, kExact);
+      }
+#pragma unroll
+      for (int k = 1; k < kChunk / 16; ++k) mma_led(leader, tmem + kColChange, zd + k * 128, yd + k * 128, i_change, 1);
+      mma_led_commit(leader, change_bar);
+    };
+    auto issue_out = [&](int n) {
+      const uint64_t zd = make_desc_sw128(stage_at(n) + kXBytes + kKB * kBox, kBox, 1024);
+#pragma unroll
+      for (int k = 0; k < kChunk / 16; ++k)
+        mma_led_tmem_a(leader, tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), zd + k * 128, i_out, 1);
+      mma_led_commit(leader, out_bar);
+    };
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      ok = wait_warp(bar, parity, sh, a.status) && ok;
       tc_fence_after();
-      int tokens_seen = 0;
-      const uint32_t tmem = sh.tmem;
-      // the products of a chunk, by warp 0
-      const int y_steps = (ny + 15) / 16;
-      const uint32_t i_scores = idesc<kHalf>(128, false, false), i_xm = idesc<kHalf>((nz + 15) & ~15, false, false),
-                     i_change = idesc<kHalf>((ny + 15) & ~15, true, true), i_out = idesc<kHalf>((nz + 15) & ~15, false, true);
-      auto stage_at = [&](int n) { return base + stage_of(n) * kStage; };
-      auto issue_scores = [&](int n) {
-        const uint64_t xd = make_desc_sw128(stage_at(n), 16, 1024), yd = make_desc_sw128(stage_at(n) + kXBytes, 16, 1024);
-#pragma unroll
-        for (int k = 0; k < 4 * kKB; ++k) {
-          const int step = (k >> 2) * (kBox / 16) + (k & 3) * 2;
-          if (k < y_steps) mma_led(leader, tmem + kColP, xd + step, yd + step, i_scores, k > 0);
-        }
-        mma_led_commit(leader, scores_bar);
-      };
-      auto issue_state = [&](int n) {  // X M
-        const uint64_t xd = make_desc_sw128(stage_at(n), 16, 1024), md = make_desc_sw128(smem_u32(state_tile), 16, 1024);
-#pragma unroll
-        for (int k = 0; k < 4 * kKB; ++k) {
-          if (k < y_steps) {
-            mma_led(leader, tmem + kColOut, xd + (k >> 2) * (kBox / 16) + (k & 3) * 2,
-                    md + (k >> 2) * (kStateBox / 16) + (k & 3) * 2, i_xm, k > 0);
-          }
-        }
-        if (kHalf || !kPlain) mma_led_commit(leader, xm_bar);
-      };
-      auto issue_change = [&](int n) {
-        const uint32_t y_at = stage_at(n) + kXBytes;
-        const uint64_t zd = make_desc_sw128(y_at + kKB * kBox, kVB == 2 ? kBox : 0, 1024);  // one box: lanes 64-127 repeat 0-63
-        const uint64_t yd = make_desc_sw128(y_at, kBox, 1024);
-        if (kExact) {  // the smaller parts first
-          const uint64_t small = make_desc_sw128(smem_u32(third), kBox, 1024);
-#pragma unroll
-          for (int t = 0; t < (kHalf ? 1 : 2); ++t) {
-#pragma unroll
-            for (int k = 0; k < kChunk / 16; ++k)
-              mma_led(leader, tmem + kColChange, zd + k * 128, small + t * kKB * (kBox / 16) + k * 128, i_change, t + k > 0);
-          }
-        }
-        if (kHalf && kExact) {
-          mma_led_scaled_d(leader, tmem + kColChange, zd, yd, i_change);  // the part so far is 2^11 times too large
-        } else {
-          mma_led(leader, tmem + kColChange, zd, yd, i_change, kExact);
-        }
-#pragma unroll
-        for (int k = 1; k < kChunk / 16; ++k) mma_led(leader, tmem + kColChange, zd + k * 128, yd + k * 128, i_change, 1);
-        mma_led_commit(leader, change_bar);
-      };
-      auto issue_out = [&](int n) {
-        const uint64_t zd = make_desc_sw128(stage_at(n) + kXBytes + kKB * kBox, kBox, 1024);
-#pragma unroll
-        for (int k = 0; k < kChunk / 16; ++k)
-          mma_led_tmem_a(leader, tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), zd + k * 128, i_out, 1);
-        mma_led_commit(leader, out_bar);
-      };
-      auto wait = [&](uint32_t bar, uint32_t parity) {
-        ok = wait_warp(bar, parity, sh, a.status) && ok;
-        tc_fence_after();
-      };
-      const bool issuer = warp == (kOwnIssuer ? kWarps : 0);
-      if (issuer) {
-        while (loaded < min(stages, count)) load();
-      }
-      // The issuing warp's part of chunk n, up to its weighing, after it, before its scores' use, and after that.
-      // The next load goes out once the chunk before is done with its stage (and its scores).
-      auto move_on = [&](int n) {
+    };
+    if (warp == kWarps) {
+      while (loaded < min(stages, count)) load();
+      for (int n = 0; n < count; ++n) {
+        // the next load and the scores once the chunk before is done with its stage and its scores
         if (n > 0) {
           wait(kStateOnly ? change_bar : out_bar, (n & 1) ^ 1);
           if (loaded < count) load();
         }
-      };
-      auto issue_first = [&](int n) {
-        if (!kStateOnly && !kPlain) {
-          move_on(n);
-          wait(full_bar + 8 * stage_of(n), full_parity(n));
-          if (ok) issue_scores(n);
-        } else if (stages == 1) {
-          move_on(n);
-        }
-      };
-      auto issue_weighed = [&](int n) {
         if (kStateOnly || kPlain) {
-          if (stages == 2) move_on(n);
           wait(weighed_bar, n & 1);
-          if (!kStateOnly && ok) issue_scores(n);
+        } else {
+          wait(full_bar + 8 * stage_of(n), full_parity(n));
         }
-      };
-      auto issue_taken = [&](int n) {
+        if (!kStateOnly && ok) issue_scores(n);
         if (n > 0) wait(taken_bar, (n & 1) ^ 1);
         if (!kStateOnly && !kPlain) wait(weighed_bar, n & 1);
         if (!kStateOnly && ok) issue_state(n);
         if (ok) issue_change(n);
-      };
-      auto issue_decayed = [&](int n) {
-        wait(decayed_bar, n & 1);
-        if (ok) issue_out(n);
-      };
-      if (kOwnIssuer && issuer) {
-        for (int n = 0; n < count; ++n) {
-          issue_first(n);
-          issue_weighed(n);
-          issue_taken(n);
-          if (!kStateOnly) issue_decayed(n);
+        if (!kStateOnly) {
+          wait(decayed_bar, n & 1);
+          if (ok) issue_out(n);
         }
-        return;
       }
-      const uint32_t quadrant = tmem + (static_cast<uint32_t>(q) << 21);  // this warp's lanes
-      auto arrive = [&](uint32_t bar) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-      };
-      // what the products of chunk n - 1 left to do while those of chunk n run: its state, its output
-      float row_out = 0.0f;
-      bool row_live = false;
-      auto take = [&](int n, bool more) {
-        // (the output's product is issued after the change's and completes after it)
-        wait(kStateOnly ? change_bar : out_bar, (n - 1) & 1);
+      return;
+    }
+    const uint32_t quadrant = tmem + (static_cast<uint32_t>(q) << 21);  // this warp's lanes
+    auto arrive = [&](uint32_t bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    // what the products of chunk n - 1 left to do while those of chunk n run: its state, its output
+    float row_out = 0.0f;
+    bool row_live = false;
+    auto take = [&](int n, bool more) {
+      // (the output's product is issued after the change's and completes after it)
+      wait(kStateOnly ? change_bar : out_bar, (n - 1) & 1);
 #pragma unroll
-        for (int i = 0; i < kOwn; i += 16) {
-          if (mc + i >= ny) break;  // no product wrote these columns
-          float d[16];
-          tmem_ld16(quadrant + kColChange + mc + i, d);
-          tmem_ld_wait();
+      for (int i = 0; i < kOwn; i += 16) {
+        if (mc + i >= ny) break;  // no product wrote these columns
+        float d[16];
+        tmem_ld16(quadrant + kColChange + mc + i, d);
+        tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            const float2 old = make_float2(m[i + j], m[i + j + 1]);
-            const float2 now = fma2(make_float2(d[j], d[j + 1]), make_float2(join, join),
-                                    fma2(old, make_float2(decay_factor, decay_factor), mul2(old, make_float2(decay_keep, decay_keep))));
-            m[i + j] = now.x;
-            m[i + j + 1] = now.y;
-          }
+        for (int j = 0; j < 16; j += 2) {
+          const float2 old = make_float2(m[i + j], m[i + j + 1]);
+          const float2 now = fma2(make_float2(d[j], d[j + 1]), make_float2(join, join),
+                                  fma2(old, make_float2(decay_factor, decay_factor), mul2(old, make_float2(decay_keep, decay_keep))));
+          m[i + j] = now.x;
+          m[i + j + 1] = now.y;
         }
-        if (!kStateOnly && more) {
-          write_state(n);
-          fence_proxy_async();
-        }
-        if (kStateOnly) {
-          tc_fence_before();
-          arrive(taken_bar);
-          return;
-        }
-        const int col0 = 32 * group, t = chunk_at(n - 1) * kChunk + 32 * q + lane;
-        uint32_t w[16];
-        if (col0 < nz) {
-#pragma unroll
-          for (int i = 0; i < 32; i += kPiece) {
-            float o[kPiece];
-            tmem_ld(quadrant + kColOut + col0 + i, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < kPiece / 2; ++j) {
-              const float2 v = mul2(make_float2(o[2 * j], o[2 * j + 1]), make_float2(row_out, row_out));
-              w[i / 2 + j] = pack2<kHalf>(v.x, v.y);
-            }
-            if (!row_live) {
-#pragma unroll
-              for (int j = 0; j < kPiece / 2; ++j) w[i / 2 + j] = 0u;
-            }
-          }
-        }
+      }
+      if (!kStateOnly && more) {
+        write_state(n);
+        fence_proxy_async();
+      }
+      if (kStateOnly) {
         tc_fence_before();
         arrive(taken_bar);
-        if (col0 < nz && ok && t < a.length) {
-          uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(p.w.ptr)) + sample * p.w.stride_batch +
-                          t * p.w.stride_token + head * p.w.stride_head + col0;
+        return;
+      }
+      const int col0 = 32 * group, t = chunk_at(n - 1) * kChunk + 32 * q + lane;
+      uint32_t w[16];
+      if (col0 < nz) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (p.wide && col0 + 16 * c + 16 <= nz) {
-              store_32(dst + 16 * c, &w[8 * c]);
-            } else {
+        for (int i = 0; i < 32; i += 16) {
+          float o[16];
+          tmem_ld16(quadrant + kColOut + col0 + i, o);
+          tmem_ld_wait();
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                if (col0 + 16 * c + 8 * h < nz)
-                  *reinterpret_cast<uint4*>(dst + 16 * c + 8 * h) =
-                      make_uint4(w[8 * c + 4 * h], w[8 * c + 4 * h + 1], w[8 * c + 4 * h + 2], w[8 * c + 4 * h + 3]);
-            }
+          for (int j = 0; j < 8; ++j) {
+            const float2 v = mul2(make_float2(o[2 * j], o[2 * j + 1]), make_float2(row_out, row_out));
+            w[i / 2 + j] = pack2<kHalf>(v.x, v.y);
+          }
+          if (!row_live) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[i / 2 + j] = 0u;
           }
         }
-      };
-      for (int n = 0; n < count; ++n) {
-        const uint32_t parity = n & 1;
-        uint8_t* const y_tile = smem + stage_of(n) * kStage + kXBytes;
-        uint8_t* const z_tile = y_tile + kKB * kBox;
-        if (n + 1 < count) fetch_mask(n + 1);
-        tokens_seen += ranks.total;
-        if (!kOwnIssuer && issuer) issue_first(n);
-        if (!kStateOnly && !kPlain) wait(scores_bar, parity);  // y's rows have been read
-        if (kExact && n > 0) wait(change_bar, parity ^ 1);     // the small parts have been, too
-        wait(full_bar + 8 * stage_of(n), full_parity(n));
-
-        // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
-        {
-          const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;  // 16-byte pieces of a row (of each box) that hold features
-          // Loads of up to kAtOnce pieces in flight, then their products.
-          auto weigh = [&](auto masked) {
-            constexpr bool kMasked = decltype(masked)::value;
-            constexpr int kAll = kKB * kChunk * 8 / kWorkers, kAtOnce = kExact ? 1 : kAll < 4 ? kAll : 4;
-#pragma unroll 1
-            for (int first_piece = 0; first_piece < kAll; first_piece += kAtOnce) {
-              uint4 v[kAtOnce];
-              float f[kAtOnce];
-              const uint32_t start = tid + first_piece * kWorkers;
-              auto place = [&](int i) {
-                const uint32_t index = start + i * kWorkers, in_box = kKB == 1 ? index : index & 1023;
-                const uint32_t row = in_box >> shift, piece = in_box & (pieces - 1);
-                return (kKB == 1 ? 0 : (index >> 10) * kBox) + row * 128 + ((piece ^ (row & 7)) << 4);
-              };
-              auto row_of = [&](int i) { return (kKB == 1 ? start + i * kWorkers : (start + i * kWorkers) & 1023) >> shift; };
+      }
+      tc_fence_before();
+      arrive(taken_bar);
+      if (col0 < nz && ok && t < a.length) {
+        uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(p.w.ptr)) + sample * p.w.stride_batch +
+                        t * p.w.stride_token + head * p.w.stride_head + col0;
 #pragma unroll
-              for (int i = 0; i < kAtOnce; ++i) {
-                if (kKB == 2 || row_of(i) < kChunk) {
-                  f[i] = sh.from[row_of(i)];
-                  v[i] = *reinterpret_cast<const uint4*>(y_tile + place(i));
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < kAtOnce; ++i) {
-                if (kKB == 2 || row_of(i) < kChunk) {
-                  const uint32_t in[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                  uint32_t hi[4], mid[4], lo[4];
-                  const float2 ff = make_float2(f[i], f[i]);
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    float2 e = mul2(unpack2<kHalf>(in[j]), ff);
-                    if (kMasked && f[i] == 0.0f) e = make_float2(0.0f, 0.0f);  // whatever a masked token holds
-                    hi[j] = pack2<kHalf>(e.x, e.y);
-                    if (kExact) {
-                      const float2 h = unpack2<kHalf>(hi[j]);
-                      const float rx = e.x - h.x, ry = e.y - h.y;
-                      mid[j] = kHalf ? pack2<kHalf>(rx * 2048.0f, ry * 2048.0f) : pack2<kHalf>(rx, ry);
-                      const float2 g = unpack2<kHalf>(mid[j]);
-                      lo[j] = pack2<kHalf>(rx - g.x, ry - g.y);
-                    }
-                  }
-                  uint8_t* const at = y_tile + place(i);
-                  *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                  if (kExact) {
-                    uint8_t* const small = third + place(i);
-                    *reinterpret_cast<uint4*>(small + (kHalf ? 0 : kKB * kBox)) = make_uint4(mid[0], mid[1], mid[2], mid[3]);
-                    if (!kHalf) *reinterpret_cast<uint4*>(small) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                  }
-                }
-              }
-            }
-          };
-          if (dead_tokens) {
-            weigh(std::true_type());
+        for (int c = 0; c < 2; ++c) {
+          if (p.wide && col0 + 16 * c + 16 <= nz) {
+            store_32(dst + 16 * c, &w[8 * c]);
           } else {
-            weigh(std::false_type());
-          }
-          if (dead_tokens && tid < kChunk && !live_token) {
 #pragma unroll
-            for (int b = 0; b < kVB; ++b)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(z_tile + b * kBox + tid * 128 + 16 * j) = make_uint4(0, 0, 0, 0);
+            for (int h = 0; h < 2; ++h)
+              if (col0 + 16 * c + 8 * h < nz)
+                *reinterpret_cast<uint4*>(dst + 16 * c + 8 * h) =
+                    make_uint4(w[8 * c + 4 * h], w[8 * c + 4 * h + 1], w[8 * c + 4 * h + 2], w[8 * c + 4 * h + 3]);
           }
         }
-        fence_proxy_async();
-        arrive(weighed_bar);
-        if (!kOwnIssuer && issuer) issue_weighed(n);
-        if (n > 0) take(n, true);
-        if (!kOwnIssuer && issuer) issue_taken(n);
-        if (ranks.total != decay_total) {  // of this chunk, for its state
-          decay_total = ranks.total;
-          const Decay d(l * static_cast<float>(decay_total));
-          decay_factor = d.factor;
-          decay_keep = d.near_one ? 1.0f : 0.0f;
-        }
+      }
+    };
+    for (int n = 0; n < count; ++n) {
+      const uint32_t parity = n & 1;
+      uint8_t* const y_tile = smem + stage_of(n) * kStage + kXBytes;
+      uint8_t* const z_tile = y_tile + kKB * kBox;
+      if (n + 1 < count) fetch_mask(n + 1);
+      tokens_seen += total;
+      if (!kStateOnly && !kPlain) wait(scores_bar, parity);  // y's rows have been read
+      if (kExact && n > 0) wait(change_bar, parity ^ 1);     // the small parts have been, too
+      wait(full_bar + 8 * stage_of(n), full_parity(n));
 
-        float down = 1.0f;
-        if (!kStateOnly) {
-          // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns (a short loop: the chunk's code has
-          // to stay close to the instruction cache).  FP16 goes over them twice, first for the largest of a row.
-          constexpr int kPieces = kBlocks * 32 / kPiece;
-          float up = 1.0f, most = 0.0f;
-          if (kPlain) wait(scores_bar, parity);
+      // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
+      {
+        const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;  // 16-byte pieces of a row (of each box) that hold features
+        auto weigh = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll 1
-          for (int it = kHalf ? -kPieces : 0; it < kPieces; ++it) {
-            const int i = (it & (kPieces - 1)) * kPiece / 32, half = ((it & (kPieces - 1)) * kPiece) & 31;
-            const int block = group + kGroups * i;
-            const uint32_t whole = kPlain ? 0xffffffffu : ranks.word(block);  // plain: masked rows of y are zero
-            // this row's columns: all before its block, those up to its own in it (from it on), valid ones
-            const bool on_diagonal = block == q;
-            const uint32_t seen = on_diagonal ? whole & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane))
-                                              : (reverse ? block > q : block < q) ? whole : 0u;
-            float v[kPiece];
-            if (!on_diagonal && seen == 0u) {
+          for (int i = tid; i < kKB * kChunk << shift; i += kWorkers) {
+            const int row = (i >> shift) & (kChunk - 1), piece = i & (pieces - 1);
+            uint8_t* const at = y_tile + (kKB == 1 ? 0 : (i >> 10) * kBox) + row * 128 + ((piece ^ (row & 7)) << 4);
+            const float f = sh.from[row];
+            const uint4 v = *reinterpret_cast<const uint4*>(at);
+            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+            uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
-              for (int j = 0; j < kPiece; ++j) v[j] = 0.0f;
-            } else {
-              tmem_ld(quadrant + kColP + 32 * block + half, v);
-              tmem_ld_wait();
-              if (!kPlain) {
-                const float f = kBlocks > 1 && i == 1 ? block_factor[kBlocks - 1] : block_factor[0];
-                const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block + half);
-                if (gentle || !on_diagonal) {
+            for (int j = 0; j < 4; ++j) {
+              float2 e = mul2(unpack2<kHalf>(in[j]), make_float2(f, f));
+              if (kMasked && f == 0.0f) e = make_float2(0.0f, 0.0f);  // whatever a masked token holds
+              hi[j] = pack2<kHalf>(e.x, e.y);
+              if (kExact) {
+                const float2 h = unpack2<kHalf>(hi[j]);
+                const float rx = e.x - h.x, ry = e.y - h.y;
+                mid[j] = kHalf ? pack2<kHalf>(rx * 2048.0f, ry * 2048.0f) : pack2<kHalf>(rx, ry);
+                const float2 g = unpack2<kHalf>(mid[j]);
+                lo[j] = pack2<kHalf>(rx - g.x, ry - g.y);
+              }
+            }
+            *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (kExact) {
+              uint8_t* const small = third + (at - y_tile);
+              *reinterpret_cast<uint4*>(small + (kHalf ? 0 : kKB * kBox)) = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+              if (!kHalf) *reinterpret_cast<uint4*>(small) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+          }
+        };
+        if (dead_tokens) {
+          weigh(std::true_type());
+        } else {
+          weigh(std::false_type());
+        }
+        if (dead_tokens && tid < kChunk && !live_token) {
 #pragma unroll
-                  for (int j = 0; j < kPiece; j += 4) {
-                    const float4 c = col[j / 4];
-                    v[j] *= f * c.x;
-                    v[j + 1] *= f * c.y;
-                    v[j + 2] *= f * c.z;
-                    v[j + 3] *= f * c.w;
-                  }
-                } else {
+          for (int b = 0; b < kVB; ++b)
 #pragma unroll
-                  for (int j = 0; j < kPiece; ++j) {
-                    // rank distance: valid tokens seen by the row that lie on its side of token half + j
-                    const uint32_t side = reverse ? (1u << (half + j)) - 1u : ~(0xffffffffu >> (31 - half - j));
-                    v[j] *= inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)));
-                  }
+            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(z_tile + b * kBox + tid * 128 + 16 * j) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async();
+      arrive(weighed_bar);
+      if (n > 0) take(n, true);
+      if (total != decay_total) {  // of this chunk, for its state
+        decay_total = total;
+        const Decay d(l * static_cast<float>(decay_total));
+        decay_factor = d.factor;
+        decay_keep = d.near_one ? 1.0f : 0.0f;
+      }
+
+      float down = 1.0f;
+      if (!kStateOnly) {
+        // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns (a short loop: the chunk's code has
+        // to stay close to the instruction cache).  FP16 goes over them twice, first for the largest of a row.
+        constexpr int kPieces = kBlocks * 2;  // of sixteen columns
+        float up = 1.0f, most = 0.0f;
+        if (kPlain) wait(scores_bar, parity);
+#pragma unroll 1
+        for (int it = kHalf ? -kPieces : 0; it < kPieces; ++it) {
+          const int i = (it & (kPieces - 1)) >> 1, half = (it & 1) * 16;
+          const int block = group + kGroups * i;
+          const uint32_t whole = kPlain ? 0xffffffffu : block < 2 ? (block == 0 ? words[0] : words[1]) : (block == 2 ? words[2] : words[3]);  // plain: masked rows of y are zero
+          // this row's columns: all before its block, those up to its own in it (from it on), valid ones
+          const bool on_diagonal = block == q;
+          const uint32_t seen = on_diagonal ? whole & (reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane))
+                                            : (reverse ? block > q : block < q) ? whole : 0u;
+          float v[16];
+          if (!on_diagonal && seen == 0u) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+          } else {
+            tmem_ld16(quadrant + kColP + 32 * block + half, v);
+            tmem_ld_wait();
+            if (!kPlain) {
+              const float f = kBlocks > 1 && i == 1 ? block_factor[kBlocks - 1] : block_factor[0];
+              const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block + half);
+              if (gentle || !on_diagonal) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 c = col[j / 4];
+                  v[j] *= f * c.x;
+                  v[j + 1] *= f * c.y;
+                  v[j + 2] *= f * c.z;
+                  v[j + 3] *= f * c.w;
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  // rank distance: valid tokens seen by the row that lie on its side of token half + j
+                  const uint32_t side = reverse ? (1u << (half + j)) - 1u : ~(0xffffffffu >> (31 - half - j));
+                  v[j] *= inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)));
                 }
               }
-              if (on_diagonal || seen != 0xffffffffu) {
-                const uint32_t bits = seen >> half;
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.0f;
-              }
             }
-            if (kHalf && it < 0) {
+            if (on_diagonal || seen != 0xffffffffu) {
+              const uint32_t bits = seen >> half;
 #pragma unroll
-              for (int j = 0; j < kPiece; ++j) most = fmaxf(most, fabsf(v[j]));
-              if (it == -1) {
-                sh.row_top[group * kChunk + 32 * q + lane] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
-                named_barrier(1 + q, 32 * kGroups);
-                uint32_t e = 0;
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) e = max(e, static_cast<uint32_t>(sh.row_top[g * kChunk + 32 * q + lane]));
-                const PowerScale sc(e);
-                up = sc.up;
-                down = sc.down;
-              }
-              continue;
+              for (int j = 0; j < 16; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.0f;
             }
-            uint32_t w[kPiece / 2];
-#pragma unroll
-            for (int j = 0; j < kPiece / 2; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
-            tmem_st(quadrant + kColP + 32 * block + half / 2, w);
           }
-          // ---- the state's part, which P' Z is added to, by the row's factor (plain chunks have it in M already) and, in
-          // FP16, those of P' and of M's rows
-          if (kHalf || !kPlain) {
-            wait(xm_bar, parity);
-            const float row_factor = kPlain ? up * kappa : lambda * up;
+          if (kHalf && it < 0) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[j]));
+            if (it == -1) {
+              sh.row_top[group * kChunk + 32 * q + lane] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
+              named_barrier(1 + q, 32 * kGroups);
+              uint32_t e = 0;
+#pragma unroll
+              for (int g = 0; g < kGroups; ++g) e = max(e, static_cast<uint32_t>(sh.row_top[g * kChunk + 32 * q + lane]));
+              const PowerScale sc(e);
+              up = sc.up;
+              down = sc.down;
+            }
+            continue;
+          }
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
+          tmem_st8(quadrant + kColP + 32 * block + half / 2, w);
+        }
+        // ---- the state's part, which P' Z is added to, by the row's factor (plain chunks have it in M already) and, in
+        // FP16, those of P' and of M's rows
+        if (kHalf || !kPlain) {
+          wait(xm_bar, parity);
+          const float row_factor = kPlain ? up * kappa : lambda * up;
 #pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-              const int col0 = 32 * group + 16 * c;
-              if (col0 >= nz) break;
-              float x[16];
-              tmem_ld16(quadrant + kColOut + col0, x);
-              tmem_ld_wait();
-              uint32_t w[16];
+          for (int c = 0; c < 2; ++c) {
+            const int col0 = 32 * group + 16 * c;
+            if (col0 >= nz) break;
+            float x[16];
+            tmem_ld16(quadrant + kColOut + col0, x);
+            tmem_ld_wait();
+            uint32_t w[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                float f = row_factor;
-                if (kHalf) f *= PowerScale(sh.state_exponent[parity][col0 + j]).down;
-                w[j] = __float_as_uint(x[j] * f);
-              }
-              tmem_st16(quadrant + kColOut + col0, w);
+            for (int j = 0; j < 16; ++j) {
+              float f = row_factor;
+              if (kHalf) f *= PowerScale(sh.state_exponent[parity][col0 + j]).down;
+              w[j] = __float_as_uint(x[j] * f);
             }
+            tmem_st16(quadrant + kColOut + col0, w);
           }
-          tmem_st_wait();
-          tc_fence_before();
-          arrive(decayed_bar);
-          if (!kOwnIssuer && issuer) issue_decayed(n);
         }
-        row_out = kPlain ? lambda * down : down;
-        row_live = live;
-        if (n + 1 < count) prepare(n + 1);
+        tmem_st_wait();
+        tc_fence_before();
+        arrive(decayed_bar);
       }
-      take(count, false);
-      if (ok && p.state_out != nullptr && mv < nz) {
-        // a whole scan's state is the caller's; a segment's belongs to its segment
-        const bool end = reverse ? segment == 0 : segment == a.segments - 1;
-        if (kStateOnly || end) {
-          float* dst = p.state_out + (kStateOnly ? static_cast<int64_t>(item) * a.segments + segment : item) * ny * nz;
+      row_out = kPlain ? lambda * down : down;
+      row_live = live;
+      if (n + 1 < count) prepare(n + 1);
+    }
+    take(count, false);
+    if (ok && p.state_out != nullptr && mv < nz) {
+      // a whole scan's state is the caller's; a segment's belongs to its segment
+      const bool end = reverse ? segment == 0 : segment == a.segments - 1;
+      if (kStateOnly || end) {
+        float* dst = p.state_out + (kStateOnly ? static_cast<int64_t>(item) * a.segments + segment : item) * ny * nz;
 #pragma unroll
-          for (int i = 0; i < kOwn; ++i)
-            if (mc + i < ny) dst[(mc + i) * nz + mv] = m[i];
-        }
+        for (int i = 0; i < kOwn; ++i)
+          if (mc + i < ny) dst[(mc + i) * nz + mv] = m[i];
       }
-      if (kStateOnly && tid == 0 && pass_index == 0) a.counts[item * a.segments + segment] = tokens_seen;
+    }
+    if (kStateOnly && tid == 0 && pass_index == 0) a.counts[item * a.segments + segment] = tokens_seen;
     };
+  const bool all_parts = kMayExact && exact;
   if (kStateOnly || plain) {
-    if (exact) {
-      work(std::true_type(), std::true_type());
+    if (all_parts) {
+      work(std::true_type(), std::bool_constant<kMayExact>());
     } else {
       work(std::true_type(), std::false_type());
     }
-  } else if (exact) {
-    work(std::false_type(), std::true_type());
-  } else {
-    work(std::false_type(), std::false_type());
+  } else if constexpr (!kStateOnly) {
+    if (all_parts) {
+      work(std::false_type(), std::bool_constant<kMayExact>());
+    } else {
+      work(std::false_type(), std::false_type());
+    }
   }
   // nothing may be in flight when the CTA ends
-  if (warp == (kOwnIssuer ? kWarps : 0) && leader) {
+  if (warp == kWarps && leader) {
     if (!ok) {
       for (int n = max(0, loaded - stages); n < loaded; ++n)
         mbar_wait_bounded(full_bar + 8 * stage_of(n), full_parity(n), nullptr, a.status);
@@ -937,7 +894,7 @@ cudaError_t launch_one(ScanArgs& a, int64_t items, const char* name, cudaStream_
   // Two stages where they fit (beside a second CTA, where its TMEM leaves room for one).
   const size_t most = kKB + kVB == 2 ? 113 * 1024 - 4096 : 232448 - 2560;
   a.stages = 2 * stage + rest <= most ? 2 : 1;
-  auto kernel = &decay_scan_kernel<kHalf, kKB, kVB, kStateOnly>;
+  auto kernel = exact ? &decay_scan_kernel<kHalf, kKB, kVB, kStateOnly, true> : &decay_scan_kernel<kHalf, kKB, kVB, kStateOnly, false>;
   const size_t smem = a.stages * stage + rest;
   const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (e != cudaSuccess) return e;
