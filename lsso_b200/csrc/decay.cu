@@ -53,7 +53,7 @@ struct ScanPass {
   TokenTensor w;
   int wide;               // w's rows start on 32 bytes
   const float* state_in;  // nullable; per sample and head [key][value], of the segment where there are several
-  float* state_out;       // nullable; likewise
+  float* state_out;       // nullable; likewise, after the last chunk
   int ny, nz;             // widths of x and y, and of z and w
   int transposed;         // the state's axes are (z, y)
   int reverse;            // from the last token to the first; the state then is that of before the decay
@@ -75,11 +75,13 @@ struct ScanShared {
   float from[kChunk], col[kChunk];
   uint8_t row_top[4 * kChunk], state_top[4 * kChunk];  // FP16: largest exponents of score rows and of state rows
   uint8_t state_exponent[2][kChunk];                   // FP16: of the state rows as the product has them
+  uint32_t warp_top[16];                               // FP16: the largest magnitude of a chunk's rows, by warps
   // full: a stage has landed.  scores, xm, change, out: products done.  weighed, decayed, taken: all workers have written
   // Y', written P' (and scaled the state's part), and read the products of a chunk and written the next one's state.
   uint64_t full[2], scores, xm, change, out, weighed, decayed, taken, drain;
   uint32_t tmem;
   int abort_flag;
+  int first_live, last_live;  // chunks of this CTA that hold valid tokens
 };
 
 template <bool kHalf>
@@ -215,7 +217,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   const int unit = blockIdx.x / a.passes, segment = unit % a.segments, item = unit / a.segments;
   const int head = item % a.heads, sample = item / a.heads;
   const bool reverse = p.reverse != 0, exact = p.exact != 0;
-  const int first = segment * a.segment_chunks, count = min(a.segment_chunks, a.chunks - first);
+  int first = segment * a.segment_chunks, count = min(a.segment_chunks, a.chunks - first);
   const int ny = p.ny, nz = p.nz, stages = a.stages;
   uint8_t* const state_tile = smem + stages * kStage;                      // M^T: [kKB][64 kVB rows][128 bytes]
   uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kStateBox);  // exact: the smaller parts of weighted rows
@@ -228,11 +230,56 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
     for (uint32_t bar : {full_bar, full_bar + 8, scores_bar, xm_bar, change_bar, out_bar, smem_u32(&sh.drain)}) mbar_init(bar, 1);
     for (uint32_t bar : {weighed_bar, decayed_bar, taken_bar}) mbar_init(bar, kWarps);
     sh.abort_flag = 0;
+    sh.first_live = a.chunks;
+    sh.last_live = -1;
     fence_mbar_init();
   }
   // Before the allocation, so that no block of an earlier kernel finds its TMEM taken by one that waits for it.
   pdl_wait();
   if (warp == 0) tmem_alloc(smem_u32(&sh.tmem), kCols);
+  if (a.mask != nullptr) {
+    // Chunks without a valid token, before the first and behind the last one that has some, change no state and give
+    // zeros (padding: a third of the chunks of a batch whose lengths are spread evenly from a quarter to all of it).
+    // The warps look at chunks from both ends, until each end has met a valid token.
+    const uint8_t* of_sample = a.mask + static_cast<int64_t>(sample) * a.length;
+    auto any_live = [&](int chunk) {
+      bool some = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int t = chunk * kChunk + 32 * w + lane;
+        some = some || (t < a.length && of_sample[t] != 0);
+      }
+      return __any_sync(0xffffffffu, some);
+    };
+    __syncthreads();
+    for (int step = 0; step * kWarps < count; ++step) {
+      const int c = step * kWarps + warp;
+      if (warp < kWarps && c < count) {
+        if (any_live(first + c) && lane == 0) atomicMin(&sh.first_live, first + c);
+        if (any_live(first + count - 1 - c) && lane == 0) atomicMax(&sh.last_live, first + count - 1 - c);
+      }
+      __syncthreads();
+      const bool found = sh.last_live >= 0 && sh.first_live < a.chunks;
+      __syncthreads();
+      if (found) break;
+    }
+    const int end = first + count;
+    int from = sh.first_live, to = sh.last_live + 1;
+    if (to <= from) from = first, to = first + 1;  // none: one chunk of masked tokens
+    if (!kStateOnly) {
+      const int pieces = nz / 8;
+      uint16_t* w = static_cast<uint16_t*>(const_cast<void*>(p.w.ptr)) + sample * p.w.stride_batch + head * p.w.stride_head;
+      auto clear = [&](int chunk0, int chunk1) {
+        const int t0 = chunk0 * kChunk, rows = min(chunk1 * kChunk, a.length) - t0;
+        for (int i = tid; i < rows * pieces; i += kWorkers + 32)
+          *reinterpret_cast<uint4*>(w + (t0 + i / pieces) * p.w.stride_token + (i % pieces) * 8) = make_uint4(0, 0, 0, 0);
+      };
+      clear(first, from);
+      clear(to, end);
+    }
+    first = from;
+    count = to - from;
+  }
 
   auto chunk_at = [&](int n) { return reverse ? first + count - 1 - n : first + n; };
   auto stage_of = [&](int n) { return stages == 2 ? n & 1 : 0; };
@@ -252,9 +299,10 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   //   kappa = e^(l (n - late)) / from,
   // the scores need no factor of their own (only the mask of their diagonal), and the state's part and the scores' share
   // an accumulator.  Rounding is relative, so nothing is lost while the weights stay within the type's range: e^(127 |l|)
-  // up to 2^96 in FP32 and BF16, up to 2^4 in FP16, whose small weights would become subnormal.  Other heads take the
-  // scores of raw rows and weigh every score.
-  const bool plain = l2 * 127.0f > (kHalf ? -4.0f : -96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
+  // up to 2^96 in FP32 and BF16, up to 2^26 in
+  // FP16, whose rows are brought up to 2^15 first (the smallest weights then leave a chunk's largest values 2^11, of whose
+  // size FP16 keeps 11 bits).  Other heads take the scores of raw rows and weigh every score.
+  const bool plain = l2 * 127.0f > (kHalf ? -26.0f : -96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
   bool ok = true;
   // Weights, decays, states, outputs by the workers; loads and products by a warp of its own, which walks them together
@@ -495,7 +543,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
       if (lane == 0) mbar_arrive(bar);
     };
     // what the products of chunk n - 1 left to do while those of chunk n run: its state, its output
-    float row_out = 0.0f;
+    float row_out = 0.0f, join_out = 0.0f;
     bool row_live = false;
     auto take = [&](int n, bool more) {
       // (the output's product is issued after the change's and completes after it)
@@ -509,7 +557,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
           const float2 old = make_float2(m[i + j], m[i + j + 1]);
-          const float2 now = fma2(make_float2(d[j], d[j + 1]), make_float2(join, join),
+          const float2 now = fma2(make_float2(d[j], d[j + 1]), make_float2(join_out, join_out),
                                   fma2(old, make_float2(decay_factor, decay_factor), mul2(old, make_float2(decay_keep, decay_keep))));
           m[i + j] = now.x;
           m[i + j + 1] = now.y;
@@ -572,6 +620,28 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
       if (kExact && n > 0) wait(change_bar, parity ^ 1);     // the small parts have been, too
       wait(full_bar + 8 * stage_of(n), full_parity(n));
 
+      // ---- FP16: the power of two that brings the chunk's rows into range
+      PowerScale lift(255u);
+      if (kHalf) {
+        const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;
+        uint32_t top = 0;  // pairs of magnitudes, as integers
+#pragma unroll 1
+        for (int i = tid; i < kKB * kChunk << shift; i += kWorkers) {
+          const int row = (i >> shift) & (kChunk - 1), piece = i & (pieces - 1);
+          const uint4 v = *reinterpret_cast<const uint4*>(y_tile + (kKB == 1 ? 0 : (i >> 10) * kBox) + row * 128 + ((piece ^ (row & 7)) << 4));
+          if (sh.from[row] != 0.0f) {
+            top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+            top = __vmaxu2(__vmaxu2(top, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+          }
+        }
+        top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+        if (lane == 0) sh.warp_top[warp] = top;
+        named_barrier(7, kWorkers);
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) top = max(top, sh.warp_top[i]);
+        lift = PowerScale(top >= 0x7c00u ? 255u : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top)))) >> 23);
+      }
+
       // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
       {
         const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;  // 16-byte pieces of a row (of each box) that hold features
@@ -581,7 +651,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
           for (int i = tid; i < kKB * kChunk << shift; i += kWorkers) {
             const int row = (i >> shift) & (kChunk - 1), piece = i & (pieces - 1);
             uint8_t* const at = y_tile + (kKB == 1 ? 0 : (i >> 10) * kBox) + row * 128 + ((piece ^ (row & 7)) << 4);
-            const float f = sh.from[row];
+            const float f = kHalf ? sh.from[row] * lift.up : sh.from[row];
             const uint4 v = *reinterpret_cast<const uint4*>(at);
             const uint32_t in[4] = {v.x, v.y, v.z, v.w};
             uint32_t hi[4], mid[4], lo[4];
@@ -702,7 +772,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         // FP16, those of P' and of M's rows
         if (kHalf || !kPlain) {
           wait(xm_bar, parity);
-          const float row_factor = kPlain ? up * kappa : lambda * up;
+          const float row_factor = kPlain ? up * kappa * lift.up : lambda * up;
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
             const int col0 = 32 * group + 16 * c;
@@ -724,20 +794,17 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         tc_fence_before();
         arrive(decayed_bar);
       }
-      row_out = kPlain ? lambda * down : down;
+      row_out = kPlain ? lambda * down * lift.down : down;
+      join_out = join * lift.down;
       row_live = live;
       if (n + 1 < count) prepare(n + 1);
     }
     take(count, false);
     if (ok && p.state_out != nullptr && mv < nz) {
-      // a whole scan's state is the caller's; a segment's belongs to its segment
-      const bool end = reverse ? segment == 0 : segment == a.segments - 1;
-      if (kStateOnly || end) {
-        float* dst = p.state_out + (kStateOnly ? static_cast<int64_t>(item) * a.segments + segment : item) * ny * nz;
+      float* dst = p.state_out + (static_cast<int64_t>(item) * a.segments + segment) * ny * nz;
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i)
-          if (mc + i < ny) dst[(mc + i) * nz + mv] = m[i];
-      }
+      for (int i = 0; i < kOwn; ++i)
+        if (mc + i < ny) dst[(mc + i) * nz + mv] = m[i];
     }
     if (kStateOnly && tid == 0 && pass_index == 0) a.counts[item * a.segments + segment] = tokens_seen;
     };
@@ -773,6 +840,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
 struct JoinSet {
   float* states;         // [item][segment][values]: a segment's own part in, the state before it out
   const float* initial;  // nullable [item][values]
+  float* final;          // nullable [item][values]: the state after the last segment
   int reverse;
 };
 struct JoinArgs {
@@ -818,6 +886,7 @@ __global__ void __launch_bounds__(kJoinThreads) decay_join_kernel(const JoinArgs
       m = fmaf(m, factor[s], m * keep[s]) + own[i];
     }
   }
+  if (set.final != nullptr) set.final[static_cast<int64_t>(item) * a.values + e] = m;
 }
 
 cudaError_t launch_join(const JoinArgs& j, int64_t items, int sets, cudaStream_t stream) {
@@ -941,13 +1010,15 @@ cudaError_t launch_decay_forward(const DecayCall& c, uint8_t* workspace, int sm_
   const int exact = c.last != nullptr ? 1 : 0;
   float* states = reinterpret_cast<float*>(workspace);
   a.passes = 1;
-  const ScanPass pass{{}, 0, p.segments > 1 ? states : c.state, c.last, c.key, c.value, 0, 0, exact, c.scale, 1.0f};
-  if (p.segments > 1) {
+  // the last state comes from the scan itself, or where it is cut from joining its segments
+  const bool cut = p.segments > 1;
+  const ScanPass pass{{}, 0, cut ? states : c.state, cut ? nullptr : c.last, c.key, c.value, 0, 0, cut ? 0 : exact, c.scale, 1.0f};
+  if (cut) {
     const ScanPass own{{}, 0, nullptr, states, c.key, c.value, 0, 0, exact, 1.0f, 1.0f};
     if (!set_pass(&a, 0, c, nullptr, c.k, c.v, nullptr, own)) return cudaErrorInvalidValue;
     cudaError_t e = launch_scans<true>(a, items, c.type, c.key, c.value, "decay_states", stream);
     if (e != cudaSuccess) return e;
-    e = launch_join(JoinArgs{{JoinSet{states, c.state, 0}, JoinSet{}}, c.log_decay, a.counts, c.heads, p.segments, c.key * c.value},
+    e = launch_join(JoinArgs{{JoinSet{states, c.state, c.last, 0}, JoinSet{}}, c.log_decay, a.counts, c.heads, p.segments, c.key * c.value},
                     items, 1, stream);
     if (e != cudaSuccess) return e;
   }
@@ -961,7 +1032,8 @@ cudaError_t launch_decay_backward(const DecayCall& c, uint8_t* workspace, int sm
   const TokenTensor& dy = c.y;
   const int exact = c.dstate != nullptr ? 1 : 0;
   const float *before = c.state, *after = c.dlast;
-  if (p.segments > 1) {
+  const bool cut = p.segments > 1;
+  if (cut) {
     float* sums[2] = {reinterpret_cast<float*>(workspace), reinterpret_cast<float*>(workspace + p.states[1])};
     ScanArgs a = common(c, p, workspace);
     a.passes = 2;
@@ -972,7 +1044,7 @@ cudaError_t launch_decay_backward(const DecayCall& c, uint8_t* workspace, int sm
     }
     cudaError_t e = launch_scans<true>(a, items, c.type, c.key, c.value, "decay_states", stream);
     if (e != cudaSuccess) return e;
-    e = launch_join(JoinArgs{{JoinSet{sums[0], c.state, 0}, JoinSet{sums[1], c.dlast, 1}}, c.log_decay, a.counts, c.heads,
+    e = launch_join(JoinArgs{{JoinSet{sums[0], c.state, nullptr, 0}, JoinSet{sums[1], c.dlast, c.dstate, 1}}, c.log_decay, a.counts, c.heads,
                              p.segments, c.key * c.value},
                     items, 2, stream);
     if (e != cudaSuccess) return e;
@@ -981,7 +1053,7 @@ cudaError_t launch_decay_backward(const DecayCall& c, uint8_t* workspace, int sm
   }
   const ScanPass passes[3] = {ScanPass{{}, 0, before, nullptr, c.value, c.key, 1, 0, 0, c.scale, 1.0f},
                               ScanPass{{}, 0, after, nullptr, c.value, c.key, 1, 1, 0, 1.0f, c.scale},
-                              ScanPass{{}, 0, after, c.dstate, c.key, c.value, 0, 1, exact, 1.0f, c.scale}};
+                              ScanPass{{}, 0, after, cut ? nullptr : c.dstate, c.key, c.value, 0, 1, cut ? 0 : exact, 1.0f, c.scale}};
   const TokenTensor* tensors[3][4] = {{&dy, &c.v, &c.k, &c.dq}, {&c.v, &dy, &c.q, &c.dk}, {&c.k, &c.q, &dy, &c.dv}};
   // All three in one launch where they run the same kernel: those of a sample and head stand side by side and share
   // their inputs in L2.
