@@ -908,8 +908,10 @@ DecayPlan make_plan(int64_t batch, int64_t length, int heads, int key, int value
   const int64_t items = batch * heads, units = items * (backward ? 3 : 1);
   const int per_sm = key <= 64 && value <= 64 ? 2 : 1;
   const int64_t room = static_cast<int64_t>(per_sm) * sm_count / units;  // segments that fit in one wave
-  p.segments = 1;
-  if (room > 1 && p.chunks >= 8) p.segments = static_cast<int>(std::min<int64_t>({room, p.chunks / 2, kMostSegments}));
+  // Cutting costs two more launches (about 6.5 us) and a pass for the states (1.2 us per chunk and segment beside the
+  // scan's 1.6), so it has to save more than that: n chunks in s segments, 1.6 n > 6.5 + 2.8 n / s.
+  const int64_t s = std::min<int64_t>({room, p.chunks / 2, kMostSegments});
+  p.segments = s > 1 && static_cast<int64_t>(p.chunks) * (8 * s - 14) > 33 * s ? static_cast<int>(s) : 1;
   p.segment_chunks = (p.chunks + p.segments - 1) / p.segments;
   p.segments = (p.chunks + p.segment_chunks - 1) / p.segment_chunks;
   p.total = 16;

@@ -68,61 +68,75 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryCall c, in
   head -= t * heads;
   const int step_run = kThreads % runs, step_row = kThreads / runs, step_t = step_row / heads, step_head = step_row % heads;
   int64_t sample = (first + t) / c.length, token = first + t - sample * c.length;
+  // Two items' loads are in flight at a time.  An item is a run of pairs (their first and second features, or both in
+  // turn) or, behind the turned features, a copy of as many values.
+  constexpr int kItems = 2;
   while (t < tokens) {
-    const int64_t flat = first + t;
-    const T* src = in + sample * c.stride_batch + token * c.stride_token + (head0 + head) * c.stride_head;
-    T* dst = out + (flat * c.heads + head0 + head) * c.dim;
-    if (run < turned) {
-      const int p = run * kRun;
-      const float2* cs = table + t * f + p;
-      if (kInterleaved) {
-        Run<T, 2 * kRun> r = load_run<T, 2 * kRun>(src + 2 * p);
-        float v[2 * kRun];
-        run_to_float(r, v);
+    Run<T, kRun> one[kItems], two[kItems];
+    T* dst[kItems];
+    int pair[kItems];  // the first pair of the run; -1: a copy of one run, -2: of two
+    int second[kItems];
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          const float a = v[2 * j], b = v[2 * j + 1];
-          v[2 * j] = a * cs[j].x - b * cs[j].y;
-          v[2 * j + 1] = b * cs[j].x + a * cs[j].y;
+    for (int i = 0; i < kItems; ++i) {
+      pair[i] = -3;
+      if (t < tokens) {
+        const T* src = in + sample * c.stride_batch + token * c.stride_token + (head0 + head) * c.stride_head;
+        dst[i] = out + ((first + t) * c.heads + head0 + head) * c.dim;
+        int at;
+        if (run < turned) {
+          at = run * kRun * (kInterleaved ? 2 : 1);
+          second[i] = kInterleaved ? kRun : f;
+          pair[i] = t * f + run * kRun;
+        } else {
+          at = 2 * f + (run - turned) * 2 * kRun;
+          second[i] = kRun;
+          pair[i] = at + kRun < c.dim ? -2 : -1;
         }
-        store_run(dst + 2 * p, v);
-      } else {
-        Run<T, kRun> ra = load_run<T, kRun>(src + p), rb = load_run<T, kRun>(src + f + p);
-        float a[kRun], b[kRun];
-        run_to_float(ra, a);
-        run_to_float(rb, b);
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          const float x = a[j];
-          a[j] = x * cs[j].x - b[j] * cs[j].y;
-          b[j] = b[j] * cs[j].x + x * cs[j].y;
+        dst[i] += at;
+        one[i] = load_run<T, kRun>(src + at);
+        if (pair[i] != -1) two[i] = load_run<T, kRun>(src + at + second[i]);
+        run += step_run;
+        head += step_head;
+        int ahead = step_t;
+        if (run >= runs) {
+          run -= runs;
+          ++head;
         }
-        store_run(dst + p, a);
-        store_run(dst + f + p, b);
+        if (head >= heads) {
+          head -= heads;
+          ++ahead;
+        }
+        t += ahead;
+        token += ahead;
+        while (token >= c.length) {
+          token -= c.length;
+          ++sample;
+        }
       }
-    } else {
-      const int at = 2 * f + (run - turned) * 2 * kRun;
-      // copied as they are, whatever they hold
+    }
 #pragma unroll
-      for (int j = 0; j < 2 * kRun; j += kRun)
-        if (at + j < c.dim) *reinterpret_cast<Run<T, kRun>*>(dst + at + j) = load_run<T, kRun>(src + at + j);
-    }
-    run += step_run;
-    head += step_head;
-    int ahead = step_t;
-    if (run >= runs) {
-      run -= runs;
-      ++head;
-    }
-    if (head >= heads) {
-      head -= heads;
-      ++ahead;
-    }
-    t += ahead;
-    token += ahead;
-    while (token >= c.length) {
-      token -= c.length;
-      ++sample;
+    for (int i = 0; i < kItems; ++i) {
+      if (pair[i] >= 0) {
+        const float2* cs = table + pair[i];
+        float a[kRun], b[kRun];
+        run_to_float(one[i], a);
+        run_to_float(two[i], b);
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          // pair j: (a, b)[2j, 2j + 1] of both runs together, or a[j] and b[j]
+          float& x = kInterleaved ? (2 * j < kRun ? a[(2 * j) % kRun] : b[(2 * j) % kRun]) : a[j];
+          float& y = kInterleaved ? (2 * j + 1 < kRun ? a[(2 * j + 1) % kRun] : b[(2 * j + 1) % kRun]) : b[j];
+          const float x0 = x, y0 = y;
+          x = x0 * cs[j].x - y0 * cs[j].y;
+          y = y0 * cs[j].x + x0 * cs[j].y;
+        }
+        store_run(dst[i], a);
+        store_run(dst[i] + second[i], b);
+      } else if (pair[i] != -3) {
+        // copied as they are, whatever they hold
+        *reinterpret_cast<Run<T, kRun>*>(dst[i]) = one[i];
+        if (pair[i] == -2) *reinterpret_cast<Run<T, kRun>*>(dst[i] + kRun) = two[i];
+      }
     }
   }
 }
@@ -131,9 +145,9 @@ template <typename T, int kRun>
 cudaError_t launch_run(const RotaryCall& c, int sm_count, cudaStream_t stream) {
   const int64_t total = c.batch * c.length;
   const int64_t items = static_cast<int64_t>(c.heads) * (c.dim / 2 / kRun + 1);  // of a token, about
-  // Tokens per block: sixteen items per thread where there are many tokens (the table is then shared by as many heads
+  // Tokens per block: eight items per thread where there are many tokens (the table is then shared by as many heads
   // as there are), fewer where that leaves SMs idle, and no more than the table holds.
-  int64_t tokens = std::max<int64_t>(1, kThreads * 16 / items);
+  int64_t tokens = std::max<int64_t>(1, kThreads * 8 / items);
   tokens = std::min<int64_t>(tokens, std::max<int64_t>(1, total / (4 * sm_count)));
   tokens = std::min<int64_t>(tokens, std::max(1, kMaxTable / c.pairs));
   const int64_t blocks = (total + tokens - 1) / tokens;
@@ -148,19 +162,17 @@ cudaError_t launch_run(const RotaryCall& c, int sm_count, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-// The longest run that divides every offset a run starts at, up to 16 bytes.  Interleaved runs hold both features of
-// their pairs, so they take half as many pairs.
+// The longest run that divides every offset a run starts at, up to 16 bytes.
 template <typename T>
 cudaError_t launch_type(const RotaryCall& c, int sm_count, cudaStream_t stream) {
   const uint64_t elements = static_cast<uint64_t>(c.stride_batch) | static_cast<uint64_t>(c.stride_token) |
                             static_cast<uint64_t>(c.stride_head) | static_cast<uint64_t>(c.dim) |
                             (reinterpret_cast<uintptr_t>(c.x) | reinterpret_cast<uintptr_t>(c.y)) / sizeof(T);
-  const uint64_t starts = static_cast<uint64_t>(c.pairs) | (c.interleaved ? elements / 2 : elements);
-  const uint64_t most = 16 / sizeof(T) / (c.interleaved ? 2 : 1);
+  const uint64_t starts = elements | static_cast<uint64_t>(c.pairs);
   if constexpr (sizeof(T) == 2) {
-    if (most >= 8 && starts % 8 == 0) return launch_run<T, 8>(c, sm_count, stream);
+    if (starts % 8 == 0) return launch_run<T, 8>(c, sm_count, stream);
   }
-  if (most >= 4 && starts % 4 == 0) return launch_run<T, 4>(c, sm_count, stream);
+  if (starts % 4 == 0) return launch_run<T, 4>(c, sm_count, stream);
   if (starts % 2 == 0) return launch_run<T, 2>(c, sm_count, stream);
   return launch_run<T, 1>(c, sm_count, stream);
 }
