@@ -18,6 +18,7 @@ import ctypes
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _native
 
@@ -171,6 +172,11 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
     raise RuntimeError("a fresh tensor was not aligned to 16 bytes")
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def _workspace(device: torch.device, sizes: tuple, backward: bool) -> tuple[int | None, int, torch.Tensor | None]:
     """Pointer, bytes and owner of a call's scratch (none where the sequences are not cut)."""
     key = (device.index, *sizes, backward)
@@ -236,7 +242,7 @@ class _DecayAttention(torch.autograd.Function):
             return dq, dk, dv, None, None, dstate, None, None
         if dy is None:
             dy = torch.zeros_like(v, memory_format=torch.contiguous_format)
-        dlast = None if dlast is None else dlast.contiguous()
+        dlast = None if dlast is None else _aligned(dlast)
         (q, qs), (k, ks), (v, vs), (dy, ys) = _rows(q), _rows(k), _rows(v), _rows(dy)
         (dq, dqs), (dk, dks), (dv, dvs) = _rows(dq), _rows(dk), _rows(dv)
         sizes = (batch, length, heads, key, value)
@@ -274,18 +280,13 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         raise TypeError(f"state must use torch.float32, got {state.dtype}")
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     log_decay = log_decay.contiguous()
-    state = None if state is None else _native_aligned(state)
+    state = None if state is None else _aligned(state)
     mask = None if valid_mask is None else valid_mask.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (state is not None and state.requires_grad)):
         return _DecayAttention.apply(q, k, v, log_decay, scale, state, mask, return_state)
     y, last = _forward(q, k, v, log_decay, scale, state, mask, return_state)
     return (y, last) if return_state else y
-
-
-def _native_aligned(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
 
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
@@ -333,6 +334,8 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
                 _array(vs[:2]), _native.ELEMENT_TYPES[kind], log_decay.data_ptr(), _native._ptr(valid_mask), batch, heads,
                 key, value, key ** -0.5 if scale is None else scale, at, at if new_state is None else new_state.data_ptr(),
                 y.data_ptr())
+    if not target.is_inference():
+        increment_version(target)  # a graph that kept it for its backward says so
     return y
 
 

@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   // up to 2^96 in FP32 and BF16, up to 2^26 in
   // FP16, whose rows are brought up to 2^15 first (the smallest weights then leave a chunk's largest values 2^11, of whose
   // size FP16 keeps 11 bits).  Other heads take the scores of raw rows and weigh every score.
-  const bool plain = l2 * 127.0f > (kHalf ? -26.0f : -96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
+  const bool plain = fabsf(l2) * 127.0f < (kHalf ? 26.0f : 96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
   bool ok = true;
   // Weights, decays, states, outputs by the workers; loads and products by a warp of its own, which walks them together

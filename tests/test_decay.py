@@ -166,7 +166,7 @@ def compare(q, k, v, l, s0, valid, *, scale=None, seed=9) -> None:
     sides = []
     for sign in (False, True):
         x = [t.detach().abs().requires_grad_() if sign else t for t in wide]
-        w, wl = exact(*x[:3], l, scale, x[3] if carried else None, valid)
+        w, wl = exact(*x[:3], l, abs(scale) if sign else scale, x[3] if carried else None, valid)
         up = [t.double().abs() if sign else t.double() for t in ((dy, dlast) if carried else (dy,))]
         sides.append((w, wl, torch.autograd.grad((w, wl) if carried else (w,), x, up)))
     (w, wl, wg), (m, ml, mg) = sides
