@@ -309,12 +309,11 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   // while one lane issues (warp 0 doing both had a third more registers and took 196 against 174 us, forward of 64 x 4096
   // tokens, 8 heads of 32).  A wait that runs out does not leave the loop (other warps may be at a barrier with this one):
   // the rest runs through without waiting, issuing or storing.
-  const bool leader = elect_leader();
   int loaded = 0;
   auto load = [&]() {
     if (!ok) return;
     const int n = loaded++, t0 = chunk_at(n) * kChunk;
-    if (leader) {
+    if (elect_leader()) {
       const uint32_t bar = full_bar + 8 * stage_of(n);
       uint32_t dst = base + stage_of(n) * kStage;
       mbar_arrive_expect_tx(bar, kStage);
@@ -464,20 +463,20 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
 #pragma unroll
       for (int k = 0; k < 4 * kKB; ++k) {
         const int step = (k >> 2) * (kBox / 16) + (k & 3) * 2;
-        if (k < y_steps) mma_led(leader, tmem + kColP, xd + step, yd + step, i_scores, k > 0);
+        if (k < y_steps) mma_bf16(tmem + kColP, xd + step, yd + step, i_scores, k > 0);
       }
-      mma_led_commit(leader, scores_bar);
+      mma_commit(scores_bar);
     };
     auto issue_state = [&](int n) {  // X M
       const uint64_t xd = make_desc_sw128(stage_at(n), 16, 1024), md = make_desc_sw128(smem_u32(state_tile), 16, 1024);
 #pragma unroll
       for (int k = 0; k < 4 * kKB; ++k) {
         if (k < y_steps) {
-          mma_led(leader, tmem + kColOut, xd + (k >> 2) * (kBox / 16) + (k & 3) * 2,
+          mma_bf16(tmem + kColOut, xd + (k >> 2) * (kBox / 16) + (k & 3) * 2,
                   md + (k >> 2) * (kStateBox / 16) + (k & 3) * 2, i_xm, k > 0);
         }
       }
-      if (kHalf || !kPlain) mma_led_commit(leader, xm_bar);
+      if (kHalf || !kPlain) mma_commit(xm_bar);
     };
     auto issue_change = [&](int n) {
       const uint32_t y_at = stage_at(n) + kXBytes;
@@ -489,24 +488,24 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         for (int t = 0; t < (kHalf ? 1 : 2); ++t) {
 #pragma unroll
           for (int k = 0; k < kChunk / 16; ++k)
-            mma_led(leader, tmem + kColChange, zd + k * 128, small + t * kKB * (kBox / 16) + k * 128, i_change, t + k > 0);
+            mma_bf16(tmem + kColChange, zd + k * 128, small + t * kKB * (kBox / 16) + k * 128, i_change, t + k > 0);
         }
       }
       if (kHalf && kExact) {
-        mma_led_scaled_d(leader, tmem + kColChange, zd, yd, i_change);  // the part so far is 2^11 times too large
+        mma_scaled_d(tmem + kColChange, zd, yd, i_change);  // the part so far is 2^11 times too large
       } else {
-        mma_led(leader, tmem + kColChange, zd, yd, i_change, kExact);
+        mma_bf16(tmem + kColChange, zd, yd, i_change, kExact);
       }
 #pragma unroll
-      for (int k = 1; k < kChunk / 16; ++k) mma_led(leader, tmem + kColChange, zd + k * 128, yd + k * 128, i_change, 1);
-      mma_led_commit(leader, change_bar);
+      for (int k = 1; k < kChunk / 16; ++k) mma_bf16(tmem + kColChange, zd + k * 128, yd + k * 128, i_change, 1);
+      mma_commit(change_bar);
     };
     auto issue_out = [&](int n) {
       const uint64_t zd = make_desc_sw128(stage_at(n) + kXBytes + kKB * kBox, kBox, 1024);
 #pragma unroll
       for (int k = 0; k < kChunk / 16; ++k)
-        mma_led_tmem_a(leader, tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), zd + k * 128, i_out, 1);
-      mma_led_commit(leader, out_bar);
+        mma_tmem_a(tmem + kColOut, tmem + kColP + 32 * (k >> 1) + 8 * (k & 1), zd + k * 128, i_out, 1);
+      mma_commit(out_bar);
     };
     auto wait = [&](uint32_t bar, uint32_t parity) {
       ok = wait_warp(bar, parity, sh, a.status) && ok;
@@ -525,14 +524,19 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         } else {
           wait(full_bar + 8 * stage_of(n), full_parity(n));
         }
-        if (!kStateOnly && ok) issue_scores(n);
+        if (!kStateOnly && ok && elect_leader()) issue_scores(n);
+        __syncwarp();
         if (n > 0) wait(taken_bar, (n & 1) ^ 1);
         if (!kStateOnly && !kPlain) wait(weighed_bar, n & 1);
-        if (!kStateOnly && ok) issue_state(n);
-        if (ok) issue_change(n);
+        if (ok && elect_leader()) {
+          if (!kStateOnly) issue_state(n);
+          issue_change(n);
+        }
+        __syncwarp();
         if (!kStateOnly) {
           wait(decayed_bar, n & 1);
-          if (ok) issue_out(n);
+          if (ok && elect_leader()) issue_out(n);
+          __syncwarp();
         }
       }
       return;
@@ -823,7 +827,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
     }
   }
   // nothing may be in flight when the CTA ends
-  if (warp == kWarps && leader) {
+  if (warp == kWarps && elect_leader()) {
     if (!ok) {
       for (int n = max(0, loaded - stages); n < loaded; ++n)
         mbar_wait_bounded(full_bar + 8 * stage_of(n), full_parity(n), nullptr, a.status);

@@ -307,8 +307,9 @@ __device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t adesc, uint64
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Forms for a whole warp that walks its products together (every operand is uniform, so descriptors are formed on the
-// uniform datapath): the lane with `leader` issues.
+// One lane of a converged warp, the same one every time.  Products issued under `if (elect_leader())` take 71 cycles
+// each (M = 128, N = 32, operands in shared memory: the time of reading A), under `if (lane == 0)` or a lane's own
+// predicate 105-109, whatever their size: the compiler then cannot know that one thread alone is active.
 __device__ __forceinline__ bool elect_leader() {
   uint32_t e;
   asm volatile(
@@ -318,44 +319,23 @@ __device__ __forceinline__ bool elect_leader() {
       : "=r"(e));
   return e != 0;
 }
-__device__ __forceinline__ void mma_led(bool leader, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
+// mma_bf16 with A in TMEM: row i in lane i, two adjacent 16-bit elements of K per 32-bit column.
+__device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
+      "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 e, %5, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(static_cast<uint32_t>(leader))
-      : "memory");
-}
-// A in TMEM: row i in lane i, two adjacent 16-bit elements of K per 32-bit column.
-__device__ __forceinline__ void mma_led_tmem_a(bool leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
-                                               uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 e, %5, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(static_cast<uint32_t>(leader))
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // D = A * B^T + 2^-11 D.
-__device__ __forceinline__ void mma_led_scaled_d(bool leader, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                                 uint32_t idesc) {
+__device__ __forceinline__ void mma_scaled_d(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
+      "{\n\t.reg .pred p;\n\t"
       "setp.eq.b32 p, 0, 0;\n\t"
-      "setp.ne.b32 e, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(static_cast<uint32_t>(leader))
-      : "memory");
-}
-__device__ __forceinline__ void mma_led_commit(bool leader, uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "setp.ne.b32 e, %1, 0;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar),
-      "r"(static_cast<uint32_t>(leader))
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, 11;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc)
       : "memory");
 }
 // Arrive once on the mbarrier when every MMA issued so far by this thread completes.
