@@ -73,9 +73,9 @@ struct ScanArgs {
 
 struct ScanShared {
   float from[kChunk], col[kChunk];
-  uint8_t row_top[4 * kChunk], state_top[4 * kChunk];  // FP16: largest exponents of score rows and of state rows
+  uint8_t state_top[4 * kChunk];                       // FP16: largest exponents of state rows
   uint8_t state_exponent[2][kChunk];                   // FP16: of the state rows as the product has them
-  uint32_t warp_top[16];                               // FP16: the largest magnitude of a chunk's rows, by warps
+  uint32_t warp_top[2][16];                            // FP16: the largest magnitudes of a chunk's x and y, by warps
   // full: a stage has landed.  scores, xm, change, out: products done.  weighed, decayed, taken: all workers have written
   // Y', written P' (and scaled the state's part), and read the products of a chunk and written the next one's state.
   uint64_t full[2], scores, xm, change, out, weighed, decayed, taken, drain;
@@ -614,6 +614,11 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         }
       }
     };
+    // This thread's 16-byte pieces of a tile of x or y, of those that hold features: of rows a multiple of eight apart, so
+    // that the swizzle is the same, and of both boxes in one sequence.
+    const int shift = ny <= 32 ? 2 : 3;  // pieces of a row (of each box)
+    const uint32_t piece0 = (tid >> shift) * 128 + (((tid & ((1 << shift) - 1)) ^ ((tid >> shift) & 7)) << 4);
+    const uint32_t piece_step = (kWorkers >> shift) * 128, piece_end = kKB * kBox;
     for (int n = 0; n < count; ++n) {
       const uint32_t parity = n & 1;
       uint8_t* const y_tile = smem + stage_of(n) * kStage + kXBytes;
@@ -624,37 +629,58 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
       if (kExact && n > 0) wait(change_bar, parity ^ 1);     // the small parts have been, too
       wait(full_bar + 8 * stage_of(n), full_parity(n));
 
-      // ---- FP16: the power of two that brings the chunk's rows into range
+      // ---- FP16: powers of two that bring the chunk's weighted rows and its scores into range.  Scores by their bound,
+      // ny |x| |y| in largest magnitudes: what it overestimates costs exponents, of which FP16 has more than the scores
+      // of a chunk need, not bits.
       PowerScale lift(255u);
+      float up = 1.0f, down = 1.0f;
       if (kHalf) {
-        const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;
-        uint32_t top = 0;  // pairs of magnitudes, as integers
+        uint32_t top[2];
+#pragma unroll
+        for (int which = kStateOnly ? 1 : 0; which < 2; ++which) {
+          const uint8_t* tile = y_tile - (which == 0 ? kXBytes : 0);
+          uint32_t most = 0;  // pairs of magnitudes, as integers
 #pragma unroll 1
-        for (int i = tid; i < kKB * kChunk << shift; i += kWorkers) {
-          const int row = (i >> shift) & (kChunk - 1), piece = i & (pieces - 1);
-          const uint4 v = *reinterpret_cast<const uint4*>(y_tile + (kKB == 1 ? 0 : (i >> 10) * kBox) + row * 128 + ((piece ^ (row & 7)) << 4));
-          if (sh.from[row] != 0.0f) {
-            top = __vmaxu2(__vmaxu2(top, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
-            top = __vmaxu2(__vmaxu2(top, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+          for (uint32_t at = piece0; at < piece_end; at += piece_step) {
+            const uint4 v = *reinterpret_cast<const uint4*>(tile + at);
+            if (sh.from[(at >> 7) & (kChunk - 1)] != 0.0f) {
+              most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
+              most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
+            }
           }
+          most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+          if (lane == 0) sh.warp_top[which][warp] = most;
         }
-        top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-        if (lane == 0) sh.warp_top[warp] = top;
         named_barrier(7, kWorkers);
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) top = max(top, sh.warp_top[i]);
-        lift = PowerScale(top >= 0x7c00u ? 255u : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top)))) >> 23);
+        for (int which = kStateOnly ? 1 : 0; which < 2; ++which) {
+          top[which] = 0;
+#pragma unroll
+          for (int i = 0; i < kWarps; ++i) top[which] = max(top[which], sh.warp_top[which][i]);
+          // as a biased FP32 exponent; 255 for infinities and NaN
+          top[which] = top[which] >= 0x7c00u ? 255u
+                                             : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top[which])))) >> 23;
+        }
+        lift = PowerScale(top[1]);
+        if (!kStateOnly) {
+          const int of_y = kPlain ? 15 : static_cast<int>(top[1]) - 126 + static_cast<int>(__float_as_uint(fabsf(inside)) >> 23) - 126;
+          const int bound = static_cast<int>(top[0]) - 126 + (32 - __clz(ny - 1)) + of_y;  // scores stay below 2^bound
+          if (top[0] < 255u && top[1] < 255u) {
+            const int e = min(max(15 - bound, -100), 100);
+            up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+          }
+        }
       }
 
       // ---- weighted rows of y (in parts that sum to 2^-24 of the product where a state goes back to the caller)
       {
-        const int shift = ny <= 32 ? 2 : 3, pieces = 1 << shift;  // 16-byte pieces of a row (of each box) that hold features
         auto weigh = [&](auto masked) {
           constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll 1
-          for (int i = tid; i < kKB * kChunk << shift; i += kWorkers) {
-            const int row = (i >> shift) & (kChunk - 1), piece = i & (pieces - 1);
-            uint8_t* const at = y_tile + (kKB == 1 ? 0 : (i >> 10) * kBox) + row * 128 + ((piece ^ (row & 7)) << 4);
+          for (uint32_t offset = piece0; offset < piece_end; offset += piece_step) {
+            uint8_t* const at = y_tile + offset;
+            const int row = (offset >> 7) & (kChunk - 1);
             const float f = kHalf ? sh.from[row] * lift.up : sh.from[row];
             const uint4 v = *reinterpret_cast<const uint4*>(at);
             const uint32_t in[4] = {v.x, v.y, v.z, v.w};
@@ -674,7 +700,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
             }
             *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             if (kExact) {
-              uint8_t* const small = third + (at - y_tile);
+              uint8_t* const small = third + offset;
               *reinterpret_cast<uint4*>(small + (kHalf ? 0 : kKB * kBox)) = make_uint4(mid[0], mid[1], mid[2], mid[3]);
               if (!kHalf) *reinterpret_cast<uint4*>(small) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
@@ -702,16 +728,14 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         decay_keep = d.near_one ? 1.0f : 0.0f;
       }
 
-      float down = 1.0f;
       if (!kStateOnly) {
         // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns (a short loop: the chunk's code has
-        // to stay close to the instruction cache).  FP16 goes over them twice, first for the largest of a row.
+        // to stay close to the instruction cache).
         constexpr int kPieces = kBlocks * 2;  // of sixteen columns
-        float up = 1.0f, most = 0.0f;
         if (kPlain) wait(scores_bar, parity);
 #pragma unroll 1
-        for (int it = kHalf ? -kPieces : 0; it < kPieces; ++it) {
-          const int i = (it & (kPieces - 1)) >> 1, half = (it & 1) * 16;
+        for (int it = 0; it < kPieces; ++it) {
+          const int i = it >> 1, half = (it & 1) * 16;
           const int block = group + kGroups * i;
           const uint32_t whole = kPlain ? 0xffffffffu : block < 2 ? (block == 0 ? words[0] : words[1]) : (block == 2 ? words[2] : words[3]);  // plain: masked rows of y are zero
           // this row's columns: all before its block, those up to its own in it (from it on), valid ones
@@ -751,21 +775,6 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
 #pragma unroll
               for (int j = 0; j < 16; ++j) v[j] = (bits >> j) & 1u ? v[j] : 0.0f;
             }
-          }
-          if (kHalf && it < 0) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) most = fmaxf(most, fabsf(v[j]));
-            if (it == -1) {
-              sh.row_top[group * kChunk + 32 * q + lane] = static_cast<uint8_t>(__float_as_uint(most) >> 23);
-              named_barrier(1 + q, 32 * kGroups);
-              uint32_t e = 0;
-#pragma unroll
-              for (int g = 0; g < kGroups; ++g) e = max(e, static_cast<uint32_t>(sh.row_top[g * kChunk + 32 * q + lane]));
-              const PowerScale sc(e);
-              up = sc.up;
-              down = sc.down;
-            }
-            continue;
           }
           uint32_t w[8];
 #pragma unroll
