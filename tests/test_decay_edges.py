@@ -60,6 +60,29 @@ def test_long_sequences_equal_their_parts(dtype) -> None:
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_tokens_of_very_different_sizes(dtype) -> None:
+    """Tokens whose values differ by up to 2^8 keep each its own precision: every row within 3 u of its magnitude (the
+    definition with absolute values), for decays that leave all but nothing of a chunk's first token at its last."""
+    q, k, v, l, _, _ = inputs(2, 400, 6, 64, 64, dtype, decays=[-0.001, -0.03, -0.07, -0.08, -0.13, -0.5])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    sized = lambda t: (t * 2.0 ** -torch.randint(0, 9, (*t.shape[:2], 1, 1), device="cuda", generator=g)).to(dtype)  # noqa: E731
+    leaves = [sized(t).requires_grad_() for t in (q, k, v)]
+    dy = sized(torch.randn(v.shape, device="cuda", generator=g))
+    y = decay_attention(*leaves, l)
+    grads = torch.autograd.grad(y, leaves, dy)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    want, _ = exact(*wide, l, 0.125)
+    wants = (want, *torch.autograd.grad(want, wide, dy.double()))
+    sizes = [t.detach().abs().requires_grad_() for t in wide]
+    size, _ = exact(*sizes, l, 0.125)
+    sizes = (size, *torch.autograd.grad(size, sizes, dy.double().abs()))
+    for a, b, m in zip((y, *grads), wants, sizes):
+        error = (a.double() - b).norm(dim=-1)
+        floor = 2.0 ** -25 * 8 if dtype == torch.float16 else 0.0  # a row of 64 results' own smallest steps
+        assert (error <= 3 * U[dtype] * m.detach().norm(dim=-1) + floor).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_padding_at_both_ends(dtype) -> None:
     """Whole chunks of masked tokens before, behind and between valid ones, a single valid token, none."""
     q, k, v, l, s0, _ = inputs(5, 1500, 2, 64, 32, dtype, state=True, seed=6)
