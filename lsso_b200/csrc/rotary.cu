@@ -11,6 +11,8 @@
 // memory order with 16-byte runs.  Angles of far positions need more bits than
 // FP32 has (position 2^20 leaves 2^-4 of a radian), so position * frequency is
 // formed in 64 bits and reduced to a fraction of a turn there; the rest is FP32.
+// Measured: 64 x 4096 tokens, 16 heads of 32, BF16, 91 us (5.9 TB/s); 3 x 20011
+// tokens, 10 heads of 80, 48 of them turned, interleaved, FP32, 65 us (5.9 TB/s).
 #include <algorithm>
 
 #include "elements.cuh"
