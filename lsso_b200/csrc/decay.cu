@@ -75,7 +75,7 @@ struct ScanArgs {
 };
 
 struct ScanShared {
-  float from[kChunk], col[kChunk];
+  float from[kChunk], col[kChunk];  // from: -0 for a masked token, so that a weight too small for FP32 differs from it
   uint8_t state_top[4 * kChunk];                       // FP16: largest exponents of state rows
   uint8_t state_exponent[2][kChunk];                   // FP16: of the state rows as the product has them
   uint32_t warp_top[2][16];                            // FP16: the largest magnitudes of a chunk's x and y, by warps
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
       const float row_rho = static_cast<float>(rho);
       if (n > 0) named_barrier(7, kWorkers);  // the tables have been read
       if (group == 0) {
-        sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : 0.0f;
+        sh.from[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.total - 1 - rho)) : -0.0f;
       } else if (group == 1 && !kStateOnly && !kPlain) {
         sh.col[32 * q + lane] = live ? exp2f(l2 * static_cast<float>(ranks.last_rho(q, reverse) - rho)) : 0.0f;
       }
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
 #pragma unroll 1
           for (uint32_t at = piece0; at < piece_end; at += piece_step) {
             const uint4 v = *reinterpret_cast<const uint4*>(tile + at);
-            if (sh.from[(at >> 7) & (kChunk - 1)] != 0.0f) {
+            if (__float_as_uint(sh.from[(at >> 7) & (kChunk - 1)]) != 0x80000000u) {
               most = __vmaxu2(__vmaxu2(most, v.x & 0x7fff7fffu), v.y & 0x7fff7fffu);
               most = __vmaxu2(__vmaxu2(most, v.z & 0x7fff7fffu), v.w & 0x7fff7fffu);
             }

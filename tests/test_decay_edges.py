@@ -82,6 +82,33 @@ def test_tokens_of_very_different_sizes(dtype) -> None:
         assert (error <= 3 * U[dtype] * m.detach().norm(dim=-1) + floor).all()
 
 
+@pytest.mark.parametrize("large", ["first", "last"])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_tokens_that_nothing_is_left_of(dtype, masked, large) -> None:
+    """Strong decays leave nothing of one half of a chunk at its end (in time, and against it), but its tokens' own
+    scores remain, here 2^18 times those of the other half: each row within 3 u of its magnitude, as above."""
+    q, k, v, l, _, _ = inputs(2, 300, 5, 64, 64, dtype, decays=[-2.0, -4.0, -20.0, -60.0, -100.0])
+    g = torch.Generator(device="cuda").manual_seed(4)
+    half = torch.arange(300, device="cuda") % 128 < 64
+    size = torch.where(half == (large == "first"), 2.0, 2.0 ** -8)[None, :, None, None]
+    mask = torch.rand(2, 300, device="cuda", generator=g) < 0.8 if masked else None
+    leaves = [(t * size).to(dtype).requires_grad_() for t in (q, k, v)]
+    dy = (torch.randn(v.shape, device="cuda", generator=g) * size).to(dtype)
+    y = decay_attention(*leaves, l, valid_mask=mask)
+    grads = torch.autograd.grad(y, leaves, dy)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    want, _ = exact(*wide, l, 0.125, mask=mask)
+    wants = (want, *torch.autograd.grad(want, wide, dy.double()))
+    sizes = [t.detach().abs().requires_grad_() for t in wide]
+    size, _ = exact(*sizes, l, 0.125, mask=mask)
+    sizes = (size, *torch.autograd.grad(size, sizes, dy.double().abs()))
+    for a, b, m in zip((y, *grads), wants, sizes):
+        error = (a.double() - b).norm(dim=-1)
+        floor = 2.0 ** -25 * 8 if dtype == torch.float16 else 0.0  # a row of 64 results' own smallest steps
+        assert (error <= 3 * U[dtype] * m.detach().norm(dim=-1) + floor).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_padding_at_both_ends(dtype) -> None:
     """Whole chunks of masked tokens before, behind and between valid ones, a single valid token, none."""
