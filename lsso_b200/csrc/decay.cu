@@ -664,11 +664,11 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
           top[which] = top[which] >= 0x7c00u ? 255u
                                              : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top[which])))) >> 23;
         }
-        lift = PowerScale(top[1]);
+        if (top[1] != 0u) lift = PowerScale(top[1]);  // rows of zeros as they are
         if (!kStateOnly) {
           const int of_y = kPlain ? 15 : static_cast<int>(top[1]) - 126 + static_cast<int>(__float_as_uint(fabsf(inside)) >> 23) - 126;
           const int bound = static_cast<int>(top[0]) - 126 + (32 - __clz(ny - 1)) + of_y;  // scores stay below 2^bound
-          if (top[0] < 255u && top[1] < 255u) {
+          if (top[0] < 255u && top[1] < 255u && top[0] != 0u && top[1] != 0u) {
             const int e = min(max(15 - bound, -100), 100);
             up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
@@ -799,9 +799,9 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              float f = row_factor;
-              if (kHalf) f *= PowerScale(sh.state_exponent[parity][col0 + j]).down;
-              w[j] = __float_as_uint(x[j] * f);
+              // (this order: the factors' product may leave FP32's range)
+              const float f = kHalf ? x[j] * PowerScale(sh.state_exponent[parity][col0 + j]).down : x[j];
+              w[j] = __float_as_uint(f * row_factor);
             }
             tmem_st16(quadrant + kColOut + col0, w);
           }

@@ -109,6 +109,38 @@ def test_large_tokens_that_nothing_is_left_of(dtype, masked, large) -> None:
         assert (error <= 3 * U[dtype] * m.detach().norm(dim=-1) + floor).all()
 
 
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("decay", [-0.01, -0.5, -30.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_chunks_of_zeros_and_of_tiny_values(dtype, decay, given) -> None:
+    """Every chunk's q, k, v and dy are zero, tiny or ordinary, each for itself: rows within 3 u of their magnitude."""
+    q, k, v, l, state, _ = inputs(4, 640, 4, 64, 64, dtype, decays=[decay] * 4, state=given)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    kinds = torch.tensor([0.0, 2.0 ** -18, 2.0 ** -3, 1.0], device="cuda")
+
+    def sized(t):
+        kind = torch.randint(0, 4, (t.shape[0], 5, t.shape[2], 1), device="cuda", generator=g)
+        return (t * kinds[kind].repeat_interleave(128, 1)).to(dtype)
+
+    leaves = [sized(t).requires_grad_() for t in (q, k, v)]
+    dy = sized(torch.randn(v.shape, device="cuda", generator=g))
+    y = decay_attention(*leaves, l, state=state)
+    grads = torch.autograd.grad(y, leaves, dy)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    want, _ = exact(*wide, l, 0.125, state)
+    wants = (want, *torch.autograd.grad(want, wide, dy.double()))
+    sizes = [t.detach().abs().requires_grad_() for t in wide]
+    size, _ = exact(*sizes, l, 0.125, None if state is None else state.abs())
+    sizes = (size, *torch.autograd.grad(size, sizes, dy.double().abs()))
+    for a, b, m in zip((y, *grads), wants, sizes):
+        error = (a.double() - b).norm(dim=-1)
+        # FP16: a row of 64 results' own smallest steps.  BF16: parts of the sums below 2^-126 (results here reach down to
+        # 1e-160) vanish, and the rows' factors bring back up to 2^32: 2^-94, times two values below 2^3, 64 features and
+        # 128 tokens, over a row of 64.
+        floor = 2.0 ** -25 * 8 if dtype == torch.float16 else 2.0 ** (-94 + 6 + 6 + 7 + 3)
+        assert (error <= 3 * U[dtype] * m.detach().norm(dim=-1) + floor).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_padding_at_both_ends(dtype) -> None:
     """Whole chunks of masked tokens before, behind and between valid ones, a single valid token, none."""
