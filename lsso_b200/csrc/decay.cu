@@ -301,11 +301,10 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   //   w_i = a_i [ sum over j of (x_i . y'_j) z_j + kappa x_i M ],   a_i = into from e^(l (r_i - n + 1)),
   //   kappa = e^(l (n - late)) / from,
   // the scores need no factor of their own (only the mask of their diagonal), and the state's part and the scores' share
-  // an accumulator.  Rounding is relative, so nothing is lost while the weights stay within the type's range: e^(127 |l|)
-  // up to 2^96 in FP32 and BF16, up to 2^14 in FP16, whose rows are brought up to 2^15 first (values down to 2^-15 of the
-  // chunk's largest then keep their bits at the smallest weight).  Other heads take the scores of raw rows and weigh every
-  // score.
-  const bool plain = fabsf(l2) * 127.0f < (kHalf ? 14.0f : 96.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
+  // an accumulator.  Rounding is relative, so nothing is lost while weighted values stay within the type's range: e^(127 |l|)
+  // up to 2^64 in BF16 (half of its range below one; values down to 2^-62 keep their bits at the smallest weight), up to
+  // 2^14 in FP16, whose rows are brought up to 2^15 first (values down to 2^-15 of the chunk's largest keep theirs).  Other heads take the scores of raw rows and weigh every score.
+  const bool plain = fabsf(l2) * 127.0f < (kHalf ? 14.0f : 64.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
   const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
   bool ok = true;
   // Weights, decays, states, outputs by the workers; loads and products by a warp of its own, which walks them together

@@ -135,10 +135,34 @@ def test_chunks_of_zeros_and_of_tiny_values(dtype, decay, given) -> None:
     for a, b, m in zip((y, *grads), wants, sizes):
         error = (a.double() - b).norm(dim=-1)
         # FP16: a row of 64 results' own smallest steps.  BF16: parts of the sums below 2^-126 (results here reach down to
-        # 1e-160) vanish, and the rows' factors bring back up to 2^32: 2^-94, times two values below 2^3, 64 features and
+        # 1e-160) vanish, and the rows' factors, e^(128 |l|) where they are applied after the sums (l = -0.01 here), bring
+        # back at most 2^2, with room 2^32: 2^-94, times two values below 2^3, 64 features and
         # 128 tokens, over a row of 64.
         floor = 2.0 ** -25 * 8 if dtype == torch.float16 else 2.0 ** (-94 + 6 + 6 + 7 + 3)
         assert (error <= 3 * U[dtype] * m.detach().norm(dim=-1) + floor).all()
+
+
+@pytest.mark.parametrize("small", ["q", "k", "v", "dy", "state"])
+def test_one_tensor_of_small_values(small) -> None:
+    """BF16 values of 1e-12 (a loss's mean over many tokens) under decays of windows down to two tokens."""
+    tiny = 2.0 ** -40
+    q, k, v, l, state, _ = inputs(2, 300, 6, 64, 64, torch.bfloat16, decays=[-0.03, -0.17, -0.18, -0.3, -0.5, -0.52], state=True)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    size = lambda name: tiny if small == name else 1.0  # noqa: E731
+    leaves = [(t * size(n)).requires_grad_() for n, t in zip("qkv", (q, k, v))]
+    state = state * (tiny if small in ("k", "v", "state") else 1.0)
+    dy = (torch.randn(v.shape, device="cuda", generator=g) * size("dy")).to(v.dtype)
+    y = decay_attention(*leaves, l, state=state)
+    grads = torch.autograd.grad(y, leaves, dy)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    want, _ = exact(*wide, l, 0.125, state)
+    wants = (want, *torch.autograd.grad(want, wide, dy.double()))
+    sizes = [t.detach().abs().requires_grad_() for t in wide]
+    magnitude, _ = exact(*sizes, l, 0.125, state.abs())
+    magnitudes = (magnitude, *torch.autograd.grad(magnitude, sizes, dy.double().abs()))
+    for a, b, m in zip((y, *grads), wants, magnitudes):
+        error = (a.double() - b).norm(dim=-1)
+        assert (error <= 3 * U[torch.bfloat16] * m.detach().norm(dim=-1) + 2.0 ** -72).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
