@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         }
         if (top[1] != 0u) lift = PowerScale(top[1]);  // rows of zeros as they are
         if (!kStateOnly) {
-          const int of_y = kPlain ? 15 : static_cast<int>(top[1]) - 126 + static_cast<int>(__float_as_uint(fabsf(inside)) >> 23) - 126;
+          const int of_y = static_cast<int>(top[1]) - 126 + static_cast<int>(__float_as_uint(fabsf(inside)) >> 23) - 126;
           const int bound = static_cast<int>(top[0]) - 126 + (32 - __clz(ny - 1)) + of_y;  // scores stay below 2^bound
           if (top[0] < 255u && top[1] < 255u && top[0] != 0u && top[1] != 0u) {
             const int e = min(max(15 - bound, -100), 100);
@@ -734,6 +734,9 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         // ---- scores with their decay, rounded: rows 32 q + lane, blocks of 32 columns (a short loop: the chunk's code has
         // to stay close to the instruction cache).
         constexpr int kPieces = kBlocks * 2;  // of sixteen columns
+        // (plain FP16 heads have the row's factor in P' already: the first rows' scores would else be up to 2^14 smaller
+        // than the last ones' and lose their bits)
+        const float of_scores = kHalf && kPlain ? lambda * lift.down * up : up;
         if (kPlain) wait(scores_bar, parity);
 #pragma unroll 1
         for (int it = 0; it < kPieces; ++it) {
@@ -780,14 +783,14 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
           }
           uint32_t w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * up, v[2 * j + 1] * up) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
+          for (int j = 0; j < 8; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * of_scores, v[2 * j + 1] * of_scores) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
           tmem_st8(quadrant + kColP + 32 * block + half / 2, w);
         }
         // ---- the state's part, which P' Z is added to, by the row's factor (plain chunks have it in M already) and, in
         // FP16, those of P' and of M's rows
         if (kHalf || !kPlain) {
           wait(xm_bar, parity);
-          const float row_factor = kPlain ? up * kappa * lift.up : lambda * up;
+          const float row_factor = kPlain ? lambda * kappa * up : lambda * up;
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {
             const int col0 = 32 * group + 16 * c;
@@ -809,7 +812,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         tc_fence_before();
         arrive(decayed_bar);
       }
-      row_out = kPlain ? lambda * down * lift.down : down;
+      row_out = kPlain && !kHalf ? lambda : down;
       join_out = join * lift.down;
       row_live = live;
       if (n + 1 < count) prepare(n + 1);

@@ -165,6 +165,30 @@ def test_one_tensor_of_small_values(small) -> None:
         assert (error <= 3 * U[torch.bfloat16] * m.detach().norm(dim=-1) + 2.0 ** -72).all()
 
 
+@pytest.mark.parametrize("where", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_small_scores_of_tokens_far_from_their_chunks_end(dtype, where) -> None:
+    """The first (or last) 16 tokens of a chunk have queries and keys of 2^-8, the others of one; values are ordinary."""
+    q, k, v, l, _, _ = inputs(2, 128, 4, 64, 64, dtype, decays=[-0.02, -0.05, -0.07, -0.076])
+    g = torch.Generator(device="cuda").manual_seed(7)
+    t = torch.arange(128, device="cuda")
+    small = torch.where(t < 16 if where == "first" else t >= 112, 2.0 ** -8, 1.0)[None, :, None, None]
+    leaves = [(a * b).to(dtype).requires_grad_() for a, b in ((q, small), (k, small), (v, 1.0))]
+    dy = torch.randn(v.shape, device="cuda", generator=g).to(dtype)
+    y = decay_attention(*leaves, l)
+    grads = torch.autograd.grad(y, leaves, dy)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    want, _ = exact(*wide, l, 0.125)
+    wants = (want, *torch.autograd.grad(want, wide, dy.double()))
+    sizes = [t.detach().abs().requires_grad_() for t in wide]
+    size, _ = exact(*sizes, l, 0.125)
+    sizes = (size, *torch.autograd.grad(size, sizes, dy.double().abs()))
+    for a, b, m in zip((y, *grads), wants, sizes):
+        error = (a.double() - b).norm(dim=-1)
+        floor = 2.0 ** -25 * 8 if dtype == torch.float16 else 0.0  # a row of 64 results' own smallest steps
+        assert (error <= 3 * U[dtype] * m.detach().norm(dim=-1) + floor).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_padding_at_both_ends(dtype) -> None:
     """Whole chunks of masked tokens before, behind and between valid ones, a single valid token, none."""
