@@ -13,9 +13,9 @@
 //
 // One CTA runs a scan of one sample and head (or a segment of it) with the state on chip, so every input is read once
 // and every output written once: 4 d values of 2 bytes per token and head in the forward, against 4 products of 128 x d
-// per token; HBM is the bound that is aimed at (heads of 128: 5.0 TB/s, forward of 8 x 8192 tokens, 16 heads, 214 us;
-// heads of 64: 4.3 TB/s, 32 x 2048, 8 heads, 63 us).  Heads of 32 are bound by issue slots, 54 % used with two CTAs per
-// SM (64 x 4096, 8 heads: 158 us, 3.4 TB/s).  Chunks of 128 because a product has 128 rows whatever is in them.  The
+// per token; HBM is the bound that is aimed at (heads of 128: 4.9 TB/s, forward of 8 x 8192 tokens, 16 heads, 217 us;
+// heads of 64: 4.4 TB/s, 32 x 2048, 8 heads, 61 us).  Heads of 32 are bound by issue slots, 54 % used with two CTAs per
+// SM (64 x 4096, 8 heads: 149 us, 3.6 TB/s).  Chunks of 128 because a product has 128 rows whatever is in them.  The
 // tokens come by TMA from wherever the caller keeps them (strides of
 // a packed projection).  A token axis that is long for the number of heads is cut into segments: their states first
 // (products of y and z alone), joined in order, then all segments at once.
@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         constexpr int kPieces = kBlocks * 2;  // of sixteen columns
         // (plain FP16 heads have the row's factor in P' already: the first rows' scores would else be up to 2^14 smaller
         // than the last ones' and lose their bits)
-        const float of_scores = kHalf && kPlain ? lambda * lift.down * up : up;
+        const float of_scores = lambda * lift.down * up;
         if (kPlain) wait(scores_bar, parity);
 #pragma unroll 1
         for (int it = 0; it < kPieces; ++it) {
@@ -755,23 +755,32 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
             tmem_ld16(quadrant + kColP + 32 * block + half, v);
             tmem_ld_wait();
             if (!kPlain) {
-              const float f = kBlocks > 1 && i == 1 ? block_factor[kBlocks - 1] : block_factor[0];
+              const float f = (kBlocks > 1 && i == 1 ? block_factor[kBlocks - 1] : block_factor[0]) * up;
               const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block + half);
               if (gentle || !on_diagonal) {
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
                   const float4 c = col[j / 4];
-                  v[j] *= f * c.x;
-                  v[j + 1] *= f * c.y;
-                  v[j + 2] *= f * c.z;
-                  v[j + 3] *= f * c.w;
+                  if (!kSmall && !kHalf) {  // (in pairs the wide heads' other code takes more registers: 215 -> 231 us)
+                    v[j] *= f * c.x;
+                    v[j + 1] *= f * c.y;
+                    v[j + 2] *= f * c.z;
+                    v[j + 3] *= f * c.w;
+                    continue;
+                  }
+                  const float2 lo = mul2(make_float2(v[j], v[j + 1]), mul2(make_float2(c.x, c.y), make_float2(f, f)));
+                  const float2 hi = mul2(make_float2(v[j + 2], v[j + 3]), mul2(make_float2(c.z, c.w), make_float2(f, f)));
+                  v[j] = lo.x;
+                  v[j + 1] = lo.y;
+                  v[j + 2] = hi.x;
+                  v[j + 3] = hi.y;
                 }
               } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                   // rank distance: valid tokens seen by the row that lie on its side of token half + j
                   const uint32_t side = reverse ? (1u << (half + j)) - 1u : ~(0xffffffffu >> (31 - half - j));
-                  v[j] *= inside * exp2_approx(l2 * static_cast<float>(__popc(seen & side)));
+                  v[j] *= inside * up * exp2_approx(l2 * static_cast<float>(__popc(seen & side)));
                 }
               }
             }
@@ -783,7 +792,11 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
           }
           uint32_t w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = kHalf ? pack2<kHalf>(v[2 * j] * of_scores, v[2 * j + 1] * of_scores) : pack2<kHalf>(v[2 * j], v[2 * j + 1]);
+          for (int j = 0; j < 8; ++j) {
+            const float2 s = make_float2(v[2 * j], v[2 * j + 1]);
+            const float2 r = kHalf && kPlain ? mul2(s, make_float2(of_scores, of_scores)) : s;
+            w[j] = pack2<kHalf>(r.x, r.y);
+          }
           tmem_st8(quadrant + kColP + 32 * block + half / 2, w);
         }
         // ---- the state's part, which P' Z is added to, by the row's factor (plain chunks have it in M already) and, in
