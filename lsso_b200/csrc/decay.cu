@@ -81,7 +81,8 @@ struct ScanShared {
   uint32_t warp_top[2][16];                            // FP16: the largest magnitudes of a chunk's x and y, by warps
   // full: a stage has landed.  scores, xm, change, out: products done.  weighed, decayed, taken: all workers have written
   // Y', written P' (and scaled the state's part), and read the products of a chunk and written the next one's state.
-  uint64_t full[2], scores, xm, change, out, weighed, decayed, taken, drain;
+  // weighed: [n & 1] in the states pass, else [0] alone (see weighed_of).
+  uint64_t full[2], scores, xm, change, out, weighed[2], decayed, taken, drain;
   uint32_t tmem;
   int abort_flag;
   int first_live, last_live;  // chunks of this CTA that hold valid tokens
@@ -226,12 +227,12 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   uint8_t* const third = state_tile + (kStateOnly ? 0 : kKB * kStateBox);  // exact: the smaller parts of weighted rows
   const uint32_t base = smem_u32(smem), full_bar = smem_u32(sh.full);
   const uint32_t scores_bar = smem_u32(&sh.scores), xm_bar = smem_u32(&sh.xm), change_bar = smem_u32(&sh.change),
-                 out_bar = smem_u32(&sh.out), weighed_bar = smem_u32(&sh.weighed), decayed_bar = smem_u32(&sh.decayed),
+                 out_bar = smem_u32(&sh.out), weighed_bar = smem_u32(sh.weighed), decayed_bar = smem_u32(&sh.decayed),
                  taken_bar = smem_u32(&sh.taken);
 
   if (tid == 0) {
     for (uint32_t bar : {full_bar, full_bar + 8, scores_bar, xm_bar, change_bar, out_bar, smem_u32(&sh.drain)}) mbar_init(bar, 1);
-    for (uint32_t bar : {weighed_bar, decayed_bar, taken_bar}) mbar_init(bar, kWarps);
+    for (uint32_t bar : {weighed_bar, weighed_bar + 8, decayed_bar, taken_bar}) mbar_init(bar, kWarps);
     sh.abort_flag = 0;
     sh.first_live = a.chunks;
     sh.last_live = -1;
@@ -287,6 +288,12 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   auto chunk_at = [&](int n) { return reverse ? first + count - 1 - n : first + n; };
   auto stage_of = [&](int n) { return stages == 2 ? n & 1 : 0; };
   auto full_parity = [&](int n) { return static_cast<uint32_t>(stages == 2 ? (n >> 1) & 1 : n & 1); };
+  // Where there are outputs every warp waits for the scores of chunk n, which all warps' weighing of it precedes, before
+  // it weighs the next.  In the states pass a warp may weigh chunk n + 1 while another still weighs n (it waits for the
+  // change of n - 1 alone): with one barrier its second arrival would stand for the other's first.  With two, none runs
+  // a phase ahead: between a warp's arrivals for n and n + 2 lies the change of n, which has all arrivals for n.
+  auto weighed_of = [&](int n) { return kStateOnly ? weighed_bar + 8 * (n & 1) : weighed_bar; };
+  auto weighed_parity = [&](int n) { return static_cast<uint32_t>(kStateOnly ? (n >> 1) & 1 : n & 1); };
 
   // ---- the head's decay; valid tokens of a chunk
   float l = a.log_decay[head];
@@ -522,14 +529,14 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
           if (loaded < count) load();
         }
         if (kStateOnly || kPlain) {
-          wait(weighed_bar, n & 1);
+          wait(weighed_of(n), weighed_parity(n));
         } else {
           wait(full_bar + 8 * stage_of(n), full_parity(n));
         }
         if (!kStateOnly && ok && elect_leader()) issue_scores(n);
         __syncwarp();
         if (n > 0) wait(taken_bar, (n & 1) ^ 1);
-        if (!kStateOnly && !kPlain) wait(weighed_bar, n & 1);
+        if (!kStateOnly && !kPlain) wait(weighed_of(n), weighed_parity(n));
         if (ok && elect_leader()) {
           if (!kStateOnly) issue_state(n);
           issue_change(n);
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         }
       }
       fence_proxy_async();
-      arrive(weighed_bar);
+      arrive(weighed_of(n));
       if (n > 0) take(n, true);
       if (total != decay_total) {  // of this chunk, for its state
         decay_total = total;
