@@ -74,11 +74,11 @@ struct ScanArgs {
   int* status;
 };
 
-struct ScanShared {
+struct ScanShared {  // with the stages it has to fit an SM's shared memory: 2 KB at most
   float from[kChunk], col[kChunk];  // from: -0 for a masked token, so that a weight too small for FP32 differs from it
   uint8_t state_top[4 * kChunk];                       // FP16: largest exponents of state rows
   uint8_t state_exponent[2][kChunk];                   // FP16: of the state rows as the product has them
-  uint32_t warp_top[2][16];                            // FP16: the largest magnitudes of a chunk's x and y, by warps
+  uint32_t warp_top[2][16];  // FP16: the largest magnitudes of a chunk's x and y, by warps; states pass: of its y, by n & 1
   // full: a stage has landed.  scores, xm, change, out: products done.  weighed, decayed, taken: all workers have written
   // Y', written P' (and scaled the state's part), and read the products of a chunk and written the next one's state.
   // weighed: [n & 1] in the states pass, else [0] alone (see weighed_of).
@@ -87,6 +87,7 @@ struct ScanShared {
   int abort_flag;
   int first_live, last_live;  // chunks of this CTA that hold valid tokens
 };
+static_assert(sizeof(ScanShared) <= 2048, "the widest stages leave 3 KB beside them");
 
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -644,6 +645,9 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
       PowerScale lift(255u);
       float up = 1.0f, down = 1.0f;
       if (kHalf) {
+        // In the states pass a warp may be at chunk n + 1 while another still reads n's: a slot each (the barrier of n + 1
+        // lies between those reads and the writes of n + 2).  With outputs the scores of n lie between (see weighed_of).
+        auto top_slot = [&](int which) { return kStateOnly ? n & 1 : which; };
         uint32_t top[2];
 #pragma unroll
         for (int which = kStateOnly ? 1 : 0; which < 2; ++which) {
@@ -658,14 +662,14 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
             }
           }
           most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
-          if (lane == 0) sh.warp_top[which][warp] = most;
+          if (lane == 0) sh.warp_top[top_slot(which)][warp] = most;
         }
         named_barrier(7, kWorkers);
 #pragma unroll
         for (int which = kStateOnly ? 1 : 0; which < 2; ++which) {
           top[which] = 0;
 #pragma unroll
-          for (int i = 0; i < kWarps; ++i) top[which] = max(top[which], sh.warp_top[which][i]);
+          for (int i = 0; i < kWarps; ++i) top[which] = max(top[which], sh.warp_top[top_slot(which)][i]);
           // as a biased FP32 exponent; 255 for infinities and NaN
           top[which] = top[which] >= 0x7c00u ? 255u
                                              : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top[which])))) >> 23;

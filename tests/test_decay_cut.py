@@ -16,7 +16,7 @@ from tests.test_decay import U, check, exact, inputs
 
 pytestmark = pytest.mark.gpu
 
-DTYPES = [torch.bfloat16]
+DTYPES = [torch.bfloat16, torch.float16]
 
 
 @pytest.fixture(scope="module", autouse=True)
