@@ -313,7 +313,9 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   // up to 2^64 in BF16 (half of its range below one; values down to 2^-62 keep their bits at the smallest weight), up to
   // 2^14 in FP16, whose rows are brought up to 2^15 first (values down to 2^-15 of the chunk's largest keep theirs).  Other heads take the scores of raw rows and weigh every score.
   const bool plain = fabsf(l2) * 127.0f < (kHalf ? 14.0f : 64.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
-  const bool gentle = l2 > -3.2f;  // e^(31 |l|) < 2^100: powers of both signs within a block
+  // Weighed scores of a block of 32 tokens by a factor of the row times one of the column, powers of both signs up to
+  // e^(31 |l|) < 2^100, while the row's factor, scale and FP16's power of two in it, stays below this.
+  const float gentle = fabsf(l2) < 3.2f ? exp2f(126.0f - 31.0f * fabsf(l2)) : 0.0f;
   bool ok = true;
   // Weights, decays, states, outputs by the workers; loads and products by a warp of its own, which walks them together
   // while one lane issues (warp 0 doing both had a third more registers and took 196 against 174 us, forward of 64 x 4096
@@ -748,6 +750,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         // (plain FP16 heads have the row's factor in P' already: the first rows' scores would else be up to 2^14 smaller
         // than the last ones' and lose their bits)
         const float of_scores = lambda * lift.down * up;
+        const bool by_columns = fabsf(inside * up) < gentle;
         if (kPlain) wait(scores_bar, parity);
 #pragma unroll 1
         for (int it = 0; it < kPieces; ++it) {
@@ -768,7 +771,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
             if (!kPlain) {
               const float f = (kBlocks > 1 && i == 1 ? block_factor[kBlocks - 1] : block_factor[0]) * up;
               const float4* col = reinterpret_cast<const float4*>(sh.col + 32 * block + half);
-              if (gentle || !on_diagonal) {
+              if (by_columns || !on_diagonal) {
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
                   const float4 c = col[j / 4];
