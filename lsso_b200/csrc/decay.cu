@@ -312,7 +312,8 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   // an accumulator.  Rounding is relative, so nothing is lost while weighted values stay within the type's range: e^(127 |l|)
   // up to 2^64 in BF16 (half of its range below one; values down to 2^-62 keep their bits at the smallest weight), up to
   // 2^14 in FP16, whose rows are brought up to 2^15 first (values down to 2^-15 of the chunk's largest keep theirs).  Other heads take the scores of raw rows and weigh every score.
-  const bool plain = fabsf(l2) * 127.0f < (kHalf ? 14.0f : 64.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f;
+  const bool plain = fabsf(l2) * 127.0f < (kHalf ? 14.0f : 64.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f &&
+                     fabsf(p.into) < 1e6f;  // (a row's factor, the scale in it, stays within FP32)
   // Weighed scores of a block of 32 tokens by a factor of the row times one of the column, powers of both signs up to
   // e^(31 |l|) < 2^100, while the row's factor, scale and FP16's power of two in it, stays below this.
   const float gentle = fabsf(l2) < 3.2f ? exp2f(126.0f - 31.0f * fabsf(l2)) : 0.0f;

@@ -67,3 +67,12 @@ def test_large_scales_under_steep_decays(decay, scale) -> None:
     q, k, v, l, state, mask = inputs(2, 300, 2, 32, 32, torch.bfloat16, decays=[decay], state=True, mask="holes", seed=23)
     dy = torch.randn(v.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(24)).bfloat16()
     rows_are_within_three_roundings(q, k, v, dy, l, scale, state, mask)
+
+
+@pytest.mark.parametrize("decay", [-0.01, -0.3, -0.34])
+@pytest.mark.parametrize("scale", [2.0 ** 19, 2.0 ** 80, 2.0 ** 100])
+def test_large_scales_of_weighted_rows(decay, scale) -> None:
+    """Heads that weigh their rows once, whose first rows' factor is up to 2^64 times the scale."""
+    q, k, v, l, state, mask = inputs(2, 300, 2, 32, 32, torch.bfloat16, decays=[decay], state=True, mask="holes", seed=25)
+    dy = torch.randn(v.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(26)).bfloat16()
+    rows_are_within_three_roundings(q, k, v, dy, l, scale, state, mask)
