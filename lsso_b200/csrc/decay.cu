@@ -652,6 +652,9 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         // lies between those reads and the writes of n + 2).  With outputs the scores of n lie between (see weighed_of).
         auto top_slot = [&](int which) { return kStateOnly ? n & 1 : which; };
         uint32_t top[2];
+        // A growing state (l > 0) has weights above one, up to 2^grow in this chunk, that its rows and scores leave room for.
+        int grow = 0;
+        if (l2 > 0.0f) grow = static_cast<int>(fminf(ceilf(l2 * static_cast<float>(total)), 112.0f));
 #pragma unroll
         for (int which = kStateOnly ? 1 : 0; which < 2; ++which) {
           const uint8_t* tile = y_tile - (which == 0 ? kXBytes : 0);
@@ -677,10 +680,14 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
           top[which] = top[which] >= 0x7c00u ? 255u
                                              : __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top[which])))) >> 23;
         }
-        if (top[1] != 0u) lift = PowerScale(top[1]);  // rows of zeros as they are
+        if (top[1] != 0u) lift = PowerScale(top[1] < 255u ? top[1] + grow : 255u);  // rows of zeros as they are
         if (!kStateOnly) {
           const int of_y = static_cast<int>(top[1]) - 126 + static_cast<int>(__float_as_uint(fabsf(inside)) >> 23) - 126;
-          const int bound = static_cast<int>(top[0]) - 126 + (32 - __clz(ny - 1)) + of_y;  // scores stay below 2^bound
+          int bound = static_cast<int>(top[0]) - 126 + (32 - __clz(ny - 1)) + of_y;  // scores stay below 2^bound
+          if (grow > 0) {  // weighed scores by their row's own weights, the largest of which is about lambda / into
+            const int of_row = static_cast<int>(__float_as_uint(fabsf(lambda)) >> 23) - static_cast<int>(__float_as_uint(fabsf(p.into)) >> 23) + 1;
+            bound += kPlain ? grow : min(max(of_row, 0), grow);
+          }
           if (top[0] < 255u && top[1] < 255u && top[0] != 0u && top[1] != 0u) {
             const int e = min(max(15 - bound, -100), 100);
             up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);

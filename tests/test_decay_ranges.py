@@ -36,8 +36,9 @@ def rows_are_within_three_roundings(q, k, v, dy, l, scale, state=None, mask=None
         sides.append((w, *torch.autograd.grad(w, wide, size(dy.double()))))
     for name, got, want, magnitude in zip(("y", "dq", "dk", "dv"), (y, *grads), *sides):
         error = (got.double() - want).norm(dim=-1)
-        assert torch.isfinite(got).all(), name
-        assert (error <= 3 * U[q.dtype] * magnitude.norm(dim=-1) + floor).all(), name
+        within = want.abs().amax(-1) <= 0.99 * torch.finfo(q.dtype).max  # the others are infinite in the type
+        assert torch.isfinite(got)[within].all(), name
+        assert (error <= 3 * U[q.dtype] * magnitude.norm(dim=-1) + floor)[within].all(), name
 
 
 @pytest.mark.parametrize("given", [False, True])
@@ -76,3 +77,16 @@ def test_large_scales_of_weighted_rows(decay, scale) -> None:
     q, k, v, l, state, mask = inputs(2, 300, 2, 32, 32, torch.bfloat16, decays=[decay], state=True, mask="holes", seed=25)
     dy = torch.randn(v.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(26)).bfloat16()
     rows_are_within_three_roundings(q, k, v, dy, l, scale, state, mask)
+
+
+@pytest.mark.parametrize(("growth", "length"), [(1e-4, 5000), (0.01, 400), (0.05, 150), (0.075, 150), (0.2, 64)])
+@pytest.mark.parametrize(("given", "masked"), [(False, False), (True, False), (True, True)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_states_that_grow(dtype, growth, length, given, masked) -> None:
+    """A positive log decay: weights above one, for sequences whose outputs stay within FP16 (but a few rows of the last
+    case, whose definition gives up to 6.8e6)."""
+    q, k, v, l, state, mask = inputs(1, length, 2, 32, 64, dtype, decays=[growth], state=given, mask="holes" if masked else "none", seed=27)
+    g = torch.Generator(device="cuda").manual_seed(28)
+    dy = (2.0 ** -8 * torch.randn(v.shape, device="cuda", generator=g)).to(dtype)
+    floor = 2.0 ** -25 * 8 if dtype == torch.float16 else 0.0  # a row of 64 results' own smallest steps
+    rows_are_within_three_roundings(q, k, 2.0 ** -5 * v, dy, l, 0.25, state, mask, floor=floor)
