@@ -52,19 +52,37 @@ class CausalMixer(nn.Module):
         self.widths = (2 * heads * config.rank, heads * config.head_dim)
         self.w_qkv = nn.Linear(config.dim, sum(self.widths), bias=config.bias)
         self.w_o = nn.Linear(config.dim, config.dim, bias=config.bias)
+        self._windows, self._rotary = tuple(windows), dict(rotary or {})
+        _, self.magnitude = rotary_frequencies(config.rank, **self._rotary)
+        for name, value in self._constants().items():
+            self.register_buffer(name, value, persistent=name == "log_decay")
+
+    def _constants(self) -> dict[str, torch.Tensor]:
+        heads, windows = self.config.num_heads, self._windows
         spread = torch.arange(heads, dtype=torch.float64) / max(1, heads - 1)
         window = windows[0] * (windows[1] / windows[0]) ** spread
-        self.register_buffer("log_decay", torch.log1p(-1 / window).float())
-        frequencies, self.magnitude = rotary_frequencies(config.rank, **(rotary or {}))
-        self.register_buffer("frequencies", frequencies, persistent=False)
+        frequencies, _ = rotary_frequencies(self.config.rank, **self._rotary)
+        return {"log_decay": torch.log1p(-1 / window).float(), "frequencies": frequencies}
+
+    def _constant(self, name: str, device: torch.device) -> torch.Tensor:
+        with torch.device("cpu"):
+            return self._constants()[name].to(device=device)
 
     def _apply(self, fn, recurse=True):
-        # module-wide dtype changes leave the constants in their precision
+        # module-wide dtype changes leave the constants in their precision, and what to_empty() gives a module that was
+        # made on the meta device is filled in
         constants = {name: getattr(self, name) for name in ("log_decay", "frequencies")}
         super()._apply(fn, recurse)
         for name, value in constants.items():
-            setattr(self, name, value.to(device=getattr(self, name).device))
+            device = getattr(self, name).device
+            empty = value.is_meta and device.type != "meta"
+            setattr(self, name, self._constant(name, device) if empty else value.to(device=device))
         return self
+
+    def _load_from_state_dict(self, *args, **kwargs) -> None:
+        super()._load_from_state_dict(*args, **kwargs)
+        if self.frequencies.is_meta and not self.log_decay.is_meta:  # assigned to a module on the meta device
+            self.frequencies = self._constant("frequencies", self.log_decay.device)
 
     def new_state(self, batch: int) -> CausalState:
         """The state before any token."""

@@ -1,0 +1,53 @@
+"""The causal mixer as a module: made without memory, moved and loaded, and the configurations that it refuses."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from lsso import LSSOConfig
+from lsso_b200.ball.causal import CausalMixer
+from lsso_b200.ball.shell import SequenceShell
+
+CONFIG = LSSOConfig(32, 2, 16)
+OPTIONS = dict(windows=(4.0, 64.0), rotary=dict(base=500.0, scaling="blend", factor=4.0))
+
+
+@pytest.mark.parametrize("assign", [False, True])
+def test_made_on_the_meta_device(assign) -> None:
+    """``to_empty`` and a loaded checkpoint, or a checkpoint that is assigned, give the mixer that was saved."""
+    torch.manual_seed(0)
+    ready = CausalMixer(CONFIG, **OPTIONS)
+    with torch.device("meta"):
+        mixer = CausalMixer(CONFIG, **OPTIONS)
+    assert mixer.log_decay.is_meta and mixer.frequencies.is_meta
+    if not assign:
+        mixer = mixer.to_empty(device="cpu")
+        assert torch.equal(mixer.log_decay, ready.log_decay)
+    mixer.load_state_dict(ready.state_dict(), assign=assign)
+    assert torch.equal(mixer.log_decay, ready.log_decay) and torch.equal(mixer.frequencies, ready.frequencies)
+    assert mixer.log_decay.dtype == torch.float32 and mixer.frequencies.dtype == torch.float64
+    x = torch.randn(2, 9, 32)
+    assert torch.equal(mixer(x), ready(x))
+
+
+def test_a_shell_made_on_the_meta_device() -> None:
+    options = dict(depth=2, vocab=11, gated="silu", hidden=40, embedding_scale=4.0, mixer="causal", mixer_options=OPTIONS)
+    torch.manual_seed(0)
+    ready = SequenceShell(CONFIG, **options)
+    with torch.device("meta"):
+        shell = SequenceShell(CONFIG, **options)
+    shell = shell.to_empty(device="cpu")
+    shell.load_state_dict(ready.state_dict())
+    ids = torch.randint(0, 11, (2, 7))
+    assert torch.equal(shell(ids), ready(ids))
+
+
+def test_casts_and_moves_leave_the_constants() -> None:
+    mixer = CausalMixer(CONFIG, **OPTIONS)
+    decay, frequencies = mixer.log_decay.clone(), mixer.frequencies.clone()
+    for change in (lambda m: m.half(), lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.to_empty(device="cpu")):
+        mixer = change(mixer)
+        assert torch.equal(mixer.log_decay, decay) and torch.equal(mixer.frequencies, frequencies)
+        assert mixer.log_decay.dtype == torch.float32 and mixer.frequencies.dtype == torch.float64
+    assert mixer.to("meta").log_decay.is_meta
