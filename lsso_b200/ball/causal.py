@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from .config import LSSOConfig
+from .config import CoreMode, LSSOConfig
 from .decay import decay_attention, decay_attention_reference, decay_attention_step
 from .rotary import rotary, rotary_frequencies, rotary_reference
 
@@ -38,11 +38,16 @@ class CausalMixer(nn.Module):
     ``windows``: the first and the last head's decay window in tokens, the
     heads between spaced evenly over its logarithm (``decay = 1 - 1 /
     window``, a constant of the model).  ``rotary``: arguments of
-    ``rotary_frequencies`` (base, scaling, ...) beside the width.
+    ``rotary_frequencies`` (base, scaling, ...) beside the width.  The
+    configuration's ablations (``core_mode``, ``rank_rotary``) are LSSO's and
+    refused here.
     """
 
     def __init__(self, config: LSSOConfig, *, windows: tuple[float, float] = (8.0, 512.0), rotary: dict | None = None) -> None:
         super().__init__()
+        if config.core_mode is not CoreMode.DYNAMIC or not config.rank_rotary:
+            raise ValueError("CausalMixer has no compact core and always rotates queries and keys: core_mode must be 'dynamic' and "
+                             f"rank_rotary True, got {config.core_mode.value!r} and {config.rank_rotary}")
         if config.rank % 2:
             raise ValueError(f"rotary positions require an even rank, got rank={config.rank}")
         if not all(w >= 1 for w in windows) or len(windows) != 2:

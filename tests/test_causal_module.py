@@ -51,3 +51,13 @@ def test_casts_and_moves_leave_the_constants() -> None:
         assert torch.equal(mixer.log_decay, decay) and torch.equal(mixer.frequencies, frequencies)
         assert mixer.log_decay.dtype == torch.float32 and mixer.frequencies.dtype == torch.float64
     assert mixer.to("meta").log_decay.is_meta
+
+
+@pytest.mark.parametrize("change", [dict(core_mode="static"), dict(core_mode="zero"), dict(rank_rotary=False)])
+def test_ablations_of_the_other_mixer_are_refused(change) -> None:
+    config = LSSOConfig(32, 2, 16, **change)
+    SequenceShell(config, depth=1)
+    with pytest.raises(ValueError, match="core_mode must be 'dynamic' and rank_rotary True"):
+        CausalMixer(config)
+    with pytest.raises(ValueError, match="core_mode must be 'dynamic' and rank_rotary True"):
+        SequenceShell(config, depth=1, mixer="causal")
