@@ -117,11 +117,17 @@ class CausalMixer(nn.Module):
             if torch.is_grad_enabled():
                 raise RuntimeError("a state is updated in place: run with it under torch.no_grad()")
         if implementation == "cuda":
+            for label, width in (("rank", c.rank), ("dim // num_heads", c.head_dim)):
+                if width % 8 or not 8 <= width <= 128:
+                    raise ValueError(f"implementation='cuda' supports {label} of multiples of 8 from 8 to 128, got {width}")
             if x.dtype not in (torch.float16, torch.bfloat16) or not x.is_cuda:
                 raise TypeError(f"implementation='cuda' supports CUDA tensors of torch.float16 or torch.bfloat16, got {x.dtype} on {x.device}")
             for name, parameter in self.named_parameters():
                 if parameter.dtype != torch.float32 or parameter.device != x.device:
                     raise TypeError(f"implementation='cuda' requires {name} to use torch.float32 on {x.device}")
+            if state is not None and (state.memory.dtype != torch.float32 or state.memory.device != x.device):
+                raise TypeError(f"implementation='cuda' requires a state of torch.float32 on {x.device}, got "
+                                f"{state.memory.dtype} on {state.memory.device}")
 
     def _positions(self, x, valid_mask, position_ids, state):
         """Rotary positions: of valid tokens in order (where nothing else is given, None for 0, 1, ..)."""

@@ -61,3 +61,33 @@ def test_ablations_of_the_other_mixer_are_refused(change) -> None:
         CausalMixer(config)
     with pytest.raises(ValueError, match="core_mode must be 'dynamic' and rank_rotary True"):
         SequenceShell(config, depth=1, mixer="causal")
+
+
+@pytest.mark.parametrize(("dim", "heads", "rank", "label"), [(32, 2, 12, "rank"), (48, 4, 16, "dim // num_heads"), (32, 2, 136, "rank"), (272, 2, 16, "dim // num_heads")])
+def test_widths_that_the_kernels_lack_are_refused_before_any_work(dim, heads, rank, label, monkeypatch) -> None:
+    from lsso_b200.ball import projection
+
+    monkeypatch.setattr(projection, "layer_images", lambda *_: pytest.fail("work was done"))
+    mixer = CausalMixer(LSSOConfig(dim, heads, rank))
+    assert mixer(torch.randn(1, 3, dim)).shape == (1, 3, dim)
+    with pytest.raises(ValueError, match=f"{label} of multiples of 8"):
+        mixer(torch.randn(1, 3, dim), implementation="cuda")
+
+
+@pytest.mark.gpu
+def test_states_that_the_kernels_lack_are_refused_before_any_work(monkeypatch) -> None:
+    from lsso_b200.ball import projection
+    from tests.gpu_util import require_native
+
+    require_native()
+    mixer = CausalMixer(CONFIG).cuda()
+    x = torch.randn(2, 3, 32, device="cuda").bfloat16()
+    good = mixer.new_state(2)
+    with torch.no_grad():
+        mixer(x, state=good, implementation="cuda")
+        monkeypatch.setattr(projection, "layer_images", lambda *_: pytest.fail("work was done"))
+        for memory in (good.memory.double(), good.memory.cpu(), good.memory.bfloat16()):
+            kept = memory.clone()
+            with pytest.raises(TypeError, match="state of torch.float32"):
+                mixer(x, state=good._replace(memory=memory), implementation="cuda")
+            assert torch.equal(memory, kept)
