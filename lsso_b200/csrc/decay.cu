@@ -875,12 +875,11 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
       work(std::false_type(), std::false_type());
     }
   }
-  // nothing may be in flight when the CTA ends
+  // Nothing may be in flight when the CTA ends.  (Loads too: a worker whose wait for one ran out arrives all the same, and
+  // this warp then sees its own waits through.  Where they have landed these waits return at once.)
   if (warp == kWarps && elect_leader()) {
-    if (!ok) {
-      for (int n = max(0, loaded - stages); n < loaded; ++n)
-        mbar_wait_bounded(full_bar + 8 * stage_of(n), full_parity(n), nullptr, a.status);
-    }
+    for (int n = max(0, loaded - stages); n < loaded; ++n)
+      mbar_wait_bounded(full_bar + 8 * stage_of(n), full_parity(n), nullptr, a.status);
     mma_drain(smem_u32(&sh.drain), a.status);
   }
   tc_fence_before();
