@@ -40,7 +40,7 @@ class CausalMixer(nn.Module):
     window``, a constant of the model).  ``rotary``: arguments of
     ``rotary_frequencies`` (base, scaling, ...) beside the width.  The
     configuration's ablations (``core_mode``, ``rank_rotary``) are LSSO's and
-    refused here.
+    refused here.  The CUDA path projects to BF16 whatever the input's type.
     """
 
     def __init__(self, config: LSSOConfig, *, windows: tuple[float, float] = (8.0, 512.0), rotary: dict | None = None) -> None:

@@ -28,7 +28,14 @@
 //   X M + P' Z                          tcgen05, A from TMEM
 //   M in registers, w                   worker warps, while the next chunk's scores are formed
 // Strong decays take the scores of raw rows and weigh every score instead.  No barrier joins all warps (but where masks
-// change): each product waits for the warps that prepare its operands, and each warp for the products that it reads.
+// change, and in FP16): each product waits for the warps that prepare its operands, and each warp for the products that it
+// reads.
+//
+// Sums, states and what joins them are FP32.  Rounded to the type, each once: Y', P' and M as a product reads it (its
+// operands have 16 bits), and w.  Two of the first three meet in every pair of tokens: 2.9e-3 against 64 bits in BF16
+// (3.6e-4 in FP16), of which the rounding of w alone is 1.7e-3 (2.1e-4).  A second part of P' and M would take twice the
+// products that read them and both passes through TMEM again.  States that go back to the caller are summed from Y' in
+// parts (24 bits); those of segments, where no state does, are rounded where X meets them and their Y' is not split.
 #include <cuda.h>
 
 #include <algorithm>
@@ -311,7 +318,8 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   // the scores need no factor of their own (only the mask of their diagonal), and the state's part and the scores' share
   // an accumulator.  Rounding is relative, so nothing is lost while weighted values stay within the type's range: e^(127 |l|)
   // up to 2^64 in BF16 (half of its range below one; values down to 2^-62 keep their bits at the smallest weight), up to
-  // 2^14 in FP16, whose rows are brought up to 2^15 first (values down to 2^-15 of the chunk's largest keep theirs).  Other heads take the scores of raw rows and weigh every score.
+  // 2^14 in FP16, whose rows are brought up to 2^15 first (values down to 2^-15 of the chunk's largest keep theirs).  Other
+  // heads take the scores of raw rows and weigh every score.
   const bool plain = fabsf(l2) * 127.0f < (kHalf ? 14.0f : 64.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f &&
                      fabsf(p.into) < 1e6f;  // (a row's factor, the scale in it, stays within FP32)
   // Weighed scores of a block of 32 tokens by a factor of the row times one of the column, powers of both signs up to
@@ -466,7 +474,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
     tc_fence_after();
     int tokens_seen = 0;
     const uint32_t tmem = sh.tmem;
-    // the products of a chunk, by warp 0
+    // the products of a chunk, by the issuing warp
     const int y_steps = (ny + 15) / 16;
     const uint32_t i_scores = idesc<kHalf>(128, false, false), i_xm = idesc<kHalf>((nz + 15) & ~15, false, false),
                    i_change = idesc<kHalf>((ny + 15) & ~15, true, true), i_out = idesc<kHalf>((nz + 15) & ~15, false, true);
