@@ -263,8 +263,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     BF16 or FP16 with widths that are multiples of 8 from 8 to 128;
     ``log_decay`` ``[heads]`` FP32, at most zero in use (``-inf``: a token sees
     itself alone; above zero the state grows, as far as the types reach; FP16
-    heads below -0.076 take the slower of two paths); ``scale`` defaults to ``key ** -0.5``; ``state`` FP32
-    ``[batch, heads, key, value]`` precedes the first token (default zero);
+    heads below -0.076 take the slower of two paths); ``scale`` defaults to
+    ``key ** -0.5``; ``state`` FP32 ``[batch, heads, key, value]`` precedes the first token (default zero);
     ``valid_mask`` is bool ``[batch, length]``.  What masked tokens hold does
     not matter; a valid token that is not finite may spoil the outputs of its
     128-token chunk before it, too.  Views whose strides are multiples of 8

@@ -323,8 +323,9 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
   const bool plain = fabsf(l2) * 127.0f < (kHalf ? 14.0f : 64.0f) && fabsf(p.from) > 1e-6f && fabsf(p.from) < 1e6f &&
                      fabsf(p.into) < 1e6f;  // (a row's factor, the scale in it, stays within FP32)
   // Weighed scores of a block of 32 tokens by a factor of the row times one of the column, powers of both signs up to
-  // e^(31 |l|) < 2^100, while the row's factor, scale and FP16's power of two in it, stays below this.
-  const float gentle = fabsf(l2) < 3.2f ? exp2f(126.0f - 31.0f * fabsf(l2)) : 0.0f;
+  // e^(31 |l|) < 2^100, while the row's factor, scale and FP16's power of two in it, stays below this.  (Where the state
+  // grows that power is the row's own, but the rest of its factor is the scale and less, and all of it below 2^126.)
+  const float gentle = l2 > 0.0f ? __int_as_float(0x7f800000) : l2 > -3.2f ? exp2f(126.0f + 31.0f * l2) : 0.0f;
   bool ok = true;
   // Weights, decays, states, outputs by the workers; loads and products by a warp of its own, which walks them together
   // while one lane issues (warp 0 doing both had a third more registers and took 196 against 174 us, forward of 64 x 4096
@@ -766,7 +767,7 @@ __global__ void __launch_bounds__(kScanThreads<kKB, kVB>, kKB + kVB == 2 ? 2 : 1
         // (plain FP16 heads have the row's factor in P' already: the first rows' scores would else be up to 2^14 smaller
         // than the last ones' and lose their bits)
         const float of_scores = lambda * lift.down * up;
-        const bool by_columns = fabsf(inside * up) < gentle;
+        const bool by_columns = fabsf(inside * up) < gentle;  // for all rows of a warp alike: its stores below are collective
         if (kPlain) wait(scores_bar, parity);
 #pragma unroll 1
         for (int it = 0; it < kPieces; ++it) {

@@ -79,6 +79,20 @@ def test_large_scales_of_weighted_rows(decay, scale) -> None:
     rows_are_within_three_roundings(q, k, v, dy, l, scale, state, mask)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_states_that_grow_out_of_the_type(dtype) -> None:
+    """Growth by up to e^2.2 per token: rows are right until the definition leaves the type, whichever way they are weighed."""
+    q, k, v, l, _, _ = inputs(1, 128, 4, 32, 32, dtype, decays=[0.5, 1.0, 2.1, 2.2], seed=29)
+    with torch.no_grad():
+        y = decay_attention(q[:, :8], 2.0 ** -9 * k[:, :8], v[:, :8], l, scale=2.0 ** -9)
+        want, _ = exact(q[:, :8], 2.0 ** -9 * k[:, :8], v[:, :8], l, 2.0 ** -9)
+        size, _ = exact(q[:, :8].abs(), 2.0 ** -9 * k[:, :8].abs(), v[:, :8].abs(), l, 2.0 ** -9)
+        error = (y.double() - want).norm(dim=-1)
+        floor = 2.0 ** -25 * 32 ** 0.5 if dtype == torch.float16 else 0.0  # a row of 32 results' own smallest steps
+        assert (error <= 3 * U[dtype] * size.norm(dim=-1) + floor).all()
+        assert decay_attention(q, k, v, l).shape == v.shape  # whatever it holds then
+
+
 @pytest.mark.parametrize(("growth", "length"), [(1e-4, 5000), (0.01, 400), (0.05, 150), (0.075, 150), (0.2, 64)])
 @pytest.mark.parametrize(("given", "masked"), [(False, False), (True, False), (True, True)])
 @pytest.mark.parametrize("dtype", DTYPES)
